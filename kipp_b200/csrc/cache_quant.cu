@@ -1,0 +1,390 @@
+// Writing the quantised cache (quant_format.cuh) and reading it back.
+//
+// Writing: what rope_cache.cu does for a cache in the compute type (per-head RMSNorm of queries and
+// keys, rotation, queries to an activation buffer, src/kipp.c:2480-2500, 2368-2382), with keys and
+// values rounded to codes on the way into the pages (the reference's Q8_0 cache, src/kipp.c:2757-2805).
+//
+// Which code an element gets turns on which side of a border it falls, so the arithmetic before it is
+// spelled out, and two kernels (and a plain implementation) that see the same head get the same codes:
+// the sum of squares is formed in 64 bits and its mean rounded once to 32 (any order of that sum then
+// gives the same mean, short of a tie in the 29 bits that are dropped), and the norm and the rotation
+// are single operations in 32 bits, each rounded, none fused.  Keys are coded from 32 bits, not
+// from a bfloat16 copy.
+//
+// Reading back: codes -> bfloat16 or float32 rows in pages of the same shape, for a list of pages, or
+// for the entries of a step with the block table of the pages made (prompt attention reads those).
+#include "quant_format.cuh"
+#include "head_math.cuh"
+
+namespace {
+
+struct QuantPages {
+    uint8_t* k_codes; bf16* k_scales; uint8_t* v_codes; bf16* v_scales;
+    int n_pages, page_size, n_kv;
+};
+
+struct WriteParams {
+    const void* qkv; long long ld;
+    void* q_out;
+    QuantPages pages;
+    const void* q_norm_w; const void* k_norm_w; int norm_dtype; float eps;
+    const float2* cos_sin; int rotary_dim;
+    const int* positions; const int* entry_of_token; const int* block_table; int table_width;
+    int tokens, n_q, head_dim, write_cache;
+    int* status;
+};
+
+// The cache row (page, kv head, slot) of kv head g of a token, or -1: an unmapped page is refused.
+__device__ __forceinline__ long long cache_row(const WriteParams& p, int t, int g) {
+    const int pos = p.positions[t], slot = pos / p.pages.page_size;
+    const int page = pos >= 0 && slot < p.table_width ? p.block_table[(size_t)p.entry_of_token[t] * p.table_width + slot] : -1;
+    if (page < 0 || page >= p.pages.n_pages) return -1;
+    return ((long long)page * p.pages.n_kv + g) * p.pages.page_size + (pos - slot * p.pages.page_size);
+}
+
+__device__ __forceinline__ float mean_square(double sum, int n) { return (float)(sum / (double)n); }
+__device__ __forceinline__ float norm_factor(float mean, float eps) {
+    return __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(mean, eps)));
+}
+__device__ __forceinline__ void turn(float& a, float& b, float2 cs) {
+    const float a0 = a, b0 = b;
+    a = __fsub_rn(__fmul_rn(a0, cs.x), __fmul_rn(b0, cs.y));
+    b = __fadd_rn(__fmul_rn(b0, cs.x), __fmul_rn(a0, cs.y));
+}
+
+// Any head size (a multiple of 32), any rotary size, any alignment: one warp per (token, head), the
+// head in shared memory.  A group is a lane per channel.
+template <typename T, int BITS>
+__global__ void __launch_bounds__(128) quant_write_any_kernel(const WriteParams p) {
+    __shared__ float rows[4][512];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, D = p.head_dim, heads = p.n_q + 2 * p.pages.n_kv;
+    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (item >= (long long)p.tokens * heads) return;
+    const int t = (int)(item / heads), h = (int)(item - (long long)t * heads);
+    const bool is_q = h < p.n_q, is_v = h >= p.n_q + p.pages.n_kv;
+    if (!is_q && !p.write_cache) return;
+    float* row = rows[threadIdx.x >> 5];
+    const T* src = static_cast<const T*>(p.qkv) + (size_t)t * p.ld + (size_t)h * D;
+    for (int i = lane; i < D; i += 32) row[i] = to_f32(src[i]);
+    __syncwarp();
+    if (!is_v) {
+        const void* nw = is_q ? p.q_norm_w : p.k_norm_w;
+        if (nw != nullptr) {
+            double ss = 0.0;
+            for (int i = lane; i < D; i += 32) ss += (double)row[i] * (double)row[i];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float r = norm_factor(mean_square(ss, D), p.eps);
+            for (int i = lane; i < D; i += 32) row[i] = __fmul_rn(__fmul_rn(row[i], r), load_w(nw, p.norm_dtype, i));
+            __syncwarp();
+        }
+        if (p.cos_sin != nullptr) {
+            const int half = p.rotary_dim / 2;
+            for (int i = lane; i < half; i += 32) turn(row[i], row[i + half], p.cos_sin[(size_t)t * half + i]);
+            __syncwarp();
+        }
+    }
+    if (is_q) {
+        T* dst = static_cast<T*>(p.q_out) + ((size_t)t * p.n_q + h) * D;
+        for (int i = lane; i < D; i += 32) dst[i] = from_f32<T>(row[i]);
+        return;
+    }
+    const long long at = cache_row(p, t, is_v ? h - p.n_q - p.pages.n_kv : h - p.n_q);
+    if (at < 0) {
+        if (lane == 0) atomicExch(p.status, 2);
+        return;
+    }
+    uint8_t* codes = (is_v ? p.pages.v_codes : p.pages.k_codes) + (size_t)at * (D * BITS / 8);
+    bf16* scales = (is_v ? p.pages.v_scales : p.pages.k_scales) + (size_t)at * (D / 32);
+    const int G = D / 32;
+    for (int g = 0; g < G; ++g) {
+        const int c = (lane >> 2) * 4 * G + g * 4 + (lane & 3);
+        const float x = quant_input(row[c]);
+        const float hi = warp_max(x), lo = -warp_max(-x);
+        const uint16_t sb = quant_scale<BITS>(hi, lo);
+        const uint32_t code = quant_code<BITS>(x, quant_scale_value(sb));
+        if (BITS == 8) {
+            codes[c] = (uint8_t)code;
+        } else {
+            const uint32_t high = __shfl_down_sync(0xffffffffu, code, 1);
+            if ((lane & 1) == 0) codes[c >> 1] = (uint8_t)(code | (high << 4));
+        }
+        if (lane == 0) reinterpret_cast<uint16_t*>(scales)[g] = sb;
+    }
+}
+
+__device__ __forceinline__ void take8(float (&x)[8], const bf16* p) { unpack8(x, *reinterpret_cast<const uint4*>(p)); }
+__device__ __forceinline__ void take8(float (&x)[8], const float* p) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+__device__ __forceinline__ void put8(bf16* p, const float (&x)[8]) { *reinterpret_cast<uint4*>(p) = pack8(x); }
+__device__ __forceinline__ void put8(float* p, const float (&x)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+template <int BITS> __device__ __forceinline__ void put_codes(uint8_t* p, const float (&x)[8], float s0, float s1) {
+    uint32_t c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = quant_code<BITS>(x[i], i < 4 ? s0 : s1);
+    if (BITS == 4) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w |= c[i] << (4 * i);
+        *reinterpret_cast<uint32_t*>(p) = w;
+    } else {
+        *reinterpret_cast<uint2*>(p) = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+    }
+}
+
+// Heads of 64, 128 or 256 channels, rotated whole or not at all, 16-byte aligned: HEAD_DIM / 16 lanes
+// share a (token, head), a lane holds 8 channels of the first half and their rotation partners, as
+// in rope_cache.cu.  Those are four runs of two groups; the four lanes whose numbers agree modulo
+// HEAD_DIM / 64 hold the same two groups, so a group's extremes are two exchanges away.
+constexpr int WRITE_THREADS = 128;
+template <typename T, int BITS, int HEAD_DIM>
+__global__ void __launch_bounds__(WRITE_THREADS) quant_write_kernel(const WriteParams p) {
+    constexpr int LPH = HEAD_DIM / 16, HALF = HEAD_DIM / 2, G = HEAD_DIM / 32;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int t = blockIdx.y, h = blockIdx.x * (WRITE_THREADS / LPH) + threadIdx.x / LPH, sub = threadIdx.x % LPH;
+    const int n_kv = p.pages.n_kv;
+    const bool is_q = h < p.n_q, is_k = !is_q && h < p.n_q + n_kv;
+    const bool active = h < p.n_q + 2 * n_kv && (is_q || p.write_cache);
+    long long at = -1;
+    if (active && !is_q) {
+        at = cache_row(p, t, is_k ? h - p.n_q : h - p.n_q - n_kv);
+        if (at < 0 && sub == 0) atomicExch(p.status, 2);
+    }
+    // No lane leaves early: a warp holds several heads and all lanes take part in the exchanges.
+    float a[8], b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+    if (active) {
+        const T* src = static_cast<const T*>(p.qkv) + (size_t)t * p.ld + (size_t)h * HEAD_DIM + sub * 8;
+        take8(a, src);
+        take8(b, src + HALF);
+    }
+    if (p.q_norm_w != nullptr) {                  // both weights or neither (checked by the host)
+        double ss = 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss += (double)a[i] * (double)a[i] + (double)b[i] * (double)b[i];
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (active && (is_q || is_k)) {
+            const float r = norm_factor(mean_square(ss, HEAD_DIM), p.eps);
+            const void* nw = is_q ? p.q_norm_w : p.k_norm_w;
+            float w[8];
+            load_w8(w, nw, p.norm_dtype, sub * 8);
+            head_scale8(a, r, w);
+            load_w8(w, nw, p.norm_dtype, HALF + sub * 8);
+            head_scale8(b, r, w);
+        }
+    }
+    if (p.cos_sin != nullptr && active && (is_q || is_k)) {
+        const float4* cs = reinterpret_cast<const float4*>(p.cos_sin + (size_t)t * HALF + sub * 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 c = cs[i];
+            turn(a[2 * i], b[2 * i], make_float2(c.x, c.y));
+            turn(a[2 * i + 1], b[2 * i + 1], make_float2(c.z, c.w));
+        }
+    }
+    if (active && is_q) {
+        T* dst = static_cast<T*>(p.q_out) + ((size_t)t * p.n_q + h) * HEAD_DIM + sub * 8;
+        put8(dst, a);
+        put8(dst + HALF, b);
+    }
+    float hi[2], lo[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        hi[r] = -INFINITY; lo[r] = INFINITY;
+#pragma unroll
+        for (int i = 4 * r; i < 4 * r + 4; ++i) {
+            a[i] = quant_input(a[i]); b[i] = quant_input(b[i]);
+            hi[r] = fmaxf(hi[r], fmaxf(a[i], b[i]));
+            lo[r] = fminf(lo[r], fminf(a[i], b[i]));
+        }
+#pragma unroll
+        for (int o = G / 2; o <= G; o <<= 1) {
+            hi[r] = fmaxf(hi[r], __shfl_xor_sync(0xffffffffu, hi[r], o));
+            lo[r] = fminf(lo[r], __shfl_xor_sync(0xffffffffu, lo[r], o));
+        }
+    }
+    if (at < 0) return;
+    const uint16_t s0 = quant_scale<BITS>(hi[0], lo[0]), s1 = quant_scale<BITS>(hi[1], lo[1]);
+    uint8_t* codes = (is_k ? p.pages.k_codes : p.pages.v_codes) + (size_t)at * (HEAD_DIM * BITS / 8) + sub * BITS;
+    put_codes<BITS>(codes, a, quant_scale_value(s0), quant_scale_value(s1));
+    put_codes<BITS>(codes + HALF * BITS / 8, b, quant_scale_value(s0), quant_scale_value(s1));
+    if (sub < G / 2)
+        reinterpret_cast<uint32_t*>((is_k ? p.pages.k_scales : p.pages.v_scales) + (size_t)at * G)[sub] = (uint32_t)s0 | (uint32_t)s1 << 16;
+}
+
+template <typename T, int BITS> int launch_write(const WriteParams& p, cudaStream_t s) {
+    const int heads = p.n_q + 2 * p.pages.n_kv, D = p.head_dim;
+    const uintptr_t bits = (uintptr_t)p.qkv | (uintptr_t)p.q_out | (uintptr_t)p.q_norm_w | (uintptr_t)p.k_norm_w | (uintptr_t)p.cos_sin |
+                           (uintptr_t)p.pages.k_codes | (uintptr_t)p.pages.v_codes | (uintptr_t)p.pages.k_scales | (uintptr_t)p.pages.v_scales;
+    const bool aligned = (bits & 15) == 0 && p.ld * (long long)sizeof(T) % 16 == 0;
+    if (aligned && (p.cos_sin == nullptr || p.rotary_dim == D) && p.tokens <= 65535 && (D == 64 || D == 128 || D == 256)) {
+        const int per = WRITE_THREADS / (D / 16);
+        const dim3 grid((unsigned)((heads + per - 1) / per), (unsigned)p.tokens);
+        auto kernel = D == 64 ? quant_write_kernel<T, BITS, 64> : D == 128 ? quant_write_kernel<T, BITS, 128> : quant_write_kernel<T, BITS, 256>;
+        return kipp_launch(kernel, grid, dim3(WRITE_THREADS), 0, s, 1, p);
+    }
+    const long long blocks = ((long long)p.tokens * heads + 3) / 4;
+    if (blocks > 0x7fffffffLL) return KIPP_ERR_ARG;
+    return kipp_launch(quant_write_any_kernel<T, BITS>, dim3((unsigned)blocks), dim3(128), 0, s, 1, p);
+}
+
+// ------------------------------------------------------------------------------------- reading back
+struct ReadParams {
+    void* k_out; void* v_out;
+    QuantPages pages;
+    const int* list;                // [n] pages, or the step's block table
+    int n, head_dim;
+    int* status;
+    // the entries' form: pages of entries that bring more than one token, and the table of those made
+    int* table_out; const int* q_start; const int* context_len;
+    int table_width, first_entry, window;
+};
+
+__device__ __forceinline__ void put_out(float* p, const float (&x)[8]) { put8(p, x); }
+__device__ __forceinline__ void put_out(bf16* p, const float (&x)[8]) { put8(p, x); }
+
+// eight channels from channel c on (a multiple of 8): two runs
+template <int BITS> __device__ __forceinline__ void values8(float (&x)[8], const uint8_t* codes, const uint16_t* scales, int c, int G) {
+    constexpr float L = BITS == 4 ? 8.f : 128.f;
+    const int g0 = (c >> 2) % G, g1 = g0 + 1 == G ? 0 : g0 + 1;
+    const float s0 = quant_scale_value(scales[g0]), s1 = quant_scale_value(scales[g1]);
+    if (BITS == 4) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + c / 2);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = ((float)((w >> (4 * i)) & 15) - L) * (i < 4 ? s0 : s1);
+    } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(codes + c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = ((float)(((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 255) - L) * (i < 4 ? s0 : s1);
+    }
+}
+
+// One block per (share of a page, page).  A page whose number is negative (unmapped) or past the pool
+// becomes zeros; past the pool is also reported.
+constexpr int READ_THREADS = 256;
+template <typename T, int BITS, bool ENTRIES>
+__global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const ReadParams p) {
+    if constexpr (!ENTRIES) pdl_launch_dependents();      // (a step's table is read before a kernel's wait: this one lets none start early)
+    pdl_wait();
+    const int i = blockIdx.y, D = p.head_dim, G = D / 32;
+    const int page = p.list[ENTRIES ? (size_t)(p.first_entry + i / p.table_width) * p.table_width + i % p.table_width : (size_t)i];
+    if constexpr (ENTRIES) {
+        const int e = p.first_entry + i / p.table_width, slot = i % p.table_width;
+        const int tokens = p.q_start[e + 1] - p.q_start[e], first = p.context_len[e], len = first + tokens;
+        const int seen = p.window > 0 ? max(0, first - p.window + 1) : 0;
+        const bool used = tokens > 0 && page >= 0 && (long long)slot * p.pages.page_size < len &&
+                          (long long)(slot + 1) * p.pages.page_size > seen;
+        if (blockIdx.x == 0 && threadIdx.x == 0) p.table_out[(size_t)e * p.table_width + slot] = used ? i : -1;
+        if (!used) return;
+    }
+    const bool ok = page >= 0 && page < p.pages.n_pages;
+    if (page >= p.pages.n_pages && threadIdx.x == 0) atomicExch(p.status, 3);
+    const int per_row = D / 8, rows = p.pages.n_kv * p.pages.page_size;
+    const size_t in = (size_t)(ok ? page : 0) * rows, out = (size_t)i * rows;
+    for (long long u = (long long)blockIdx.x * READ_THREADS + threadIdx.x; u < (long long)rows * per_row; u += (long long)gridDim.x * READ_THREADS) {
+        const int row = (int)(u / per_row), c = (int)(u - (long long)row * per_row) * 8;
+        float k[8], v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) k[j] = v[j] = 0.f;
+        if (ok) {
+            values8<BITS>(k, p.pages.k_codes + (in + row) * (D * BITS / 8), reinterpret_cast<const uint16_t*>(p.pages.k_scales) + (in + row) * G, c, G);
+            values8<BITS>(v, p.pages.v_codes + (in + row) * (D * BITS / 8), reinterpret_cast<const uint16_t*>(p.pages.v_scales) + (in + row) * G, c, G);
+        }
+        put_out(static_cast<T*>(p.k_out) + (out + row) * D + c, k);
+        put_out(static_cast<T*>(p.v_out) + (out + row) * D + c, v);
+    }
+}
+
+template <bool ENTRIES> int launch_read(const ReadParams& p, int bits, int out_dtype, cudaStream_t s) {
+    const long long units = (long long)p.pages.n_kv * p.pages.page_size * (p.head_dim / 8);
+    const unsigned x = (unsigned)((units + READ_THREADS * 4 - 1) / (READ_THREADS * 4));
+    auto kernel = out_dtype == KIPP_DT_F32 ? (bits == 4 ? quant_read_kernel<float, 4, ENTRIES> : quant_read_kernel<float, 8, ENTRIES>)
+                                           : (bits == 4 ? quant_read_kernel<bf16, 4, ENTRIES> : quant_read_kernel<bf16, 8, ENTRIES>);
+    // (a grid's second dimension ends at 65,535)
+    for (int done = 0; done < p.n; done += 65535) {
+        ReadParams q = p;
+        if (ENTRIES && done > 0) return KIPP_ERR_ARG;
+        q.n = p.n - done < 65535 ? p.n - done : 65535;
+        q.list = p.list + (ENTRIES ? 0 : done);
+        const size_t skip = (size_t)done * p.pages.n_kv * p.pages.page_size * p.head_dim * (out_dtype == KIPP_DT_F32 ? 4 : 2);
+        q.k_out = static_cast<char*>(p.k_out) + skip;
+        q.v_out = static_cast<char*>(p.v_out) + skip;
+        if (const int e = kipp_launch(kernel, dim3(x, (unsigned)q.n), dim3(READ_THREADS), 0, s, 1, q)) return e;
+    }
+    return 0;
+}
+
+bool pages_ok(const QuantPages& g, int bits, int head_dim) {
+    return (bits == 4 || bits == 8) && quant_head_ok(head_dim) && g.n_pages > 0 && g.page_size > 0 && g.n_kv > 0 &&
+           g.k_codes && g.k_scales && g.v_codes && g.v_scales;
+}
+}  // namespace
+
+// Norm, rotation and the write of a step's keys and values as codes; queries to q_out
+// [tokens][n_q][head_dim] in the projection's type.  write_cache 0: queries only.
+extern "C" int kipp_quant_cache_write(const void* qkv, long long ld_qkv, void* q_out, void* k_codes, void* k_scales, void* v_codes,
+                                      void* v_scales, int bits, int n_pages, int page_size, int dtype, const void* q_norm_w,
+                                      const void* k_norm_w, int norm_dtype, float eps, const void* cos_sin, int rotary_dim,
+                                      const int* positions, const int* entry_of_token, const int* block_table, int table_width,
+                                      int tokens, int n_q, int n_kv, int head_dim, int write_cache, int* status, void* stream) {
+    if (tokens <= 0) return 0;
+    const QuantPages pages = {(uint8_t*)k_codes, (bf16*)k_scales, (uint8_t*)v_codes, (bf16*)v_scales, n_pages, page_size, n_kv};
+    if (!pages_ok(pages, bits, head_dim) || n_q <= 0 || (q_norm_w == nullptr) != (k_norm_w == nullptr) || rotary_dim < 0 ||
+        rotary_dim > head_dim || (rotary_dim & 1) || table_width <= 0 || status == nullptr || ld_qkv < (long long)(n_q + 2 * n_kv) * head_dim)
+        return KIPP_ERR_ARG;
+    if ((dtype != KIPP_DT_F32 && dtype != KIPP_DT_BF16) || (norm_dtype != KIPP_DT_F32 && norm_dtype != KIPP_DT_BF16)) return KIPP_ERR_DTYPE;
+    const WriteParams p = {qkv, ld_qkv, q_out, pages, q_norm_w, k_norm_w, norm_dtype, eps, rotary_dim > 0 ? (const float2*)cos_sin : nullptr,
+                           rotary_dim, positions, entry_of_token, block_table, table_width, tokens, n_q, head_dim, write_cache & 1, status};
+    cudaStream_t s = (cudaStream_t)stream;
+    if (dtype == KIPP_DT_F32) return bits == 4 ? launch_write<float, 4>(p, s) : launch_write<float, 8>(p, s);
+    return bits == 4 ? launch_write<bf16, 4>(p, s) : launch_write<bf16, 8>(p, s);
+}
+
+static bool read_aligned(const QuantPages& g, const void* k_out, const void* v_out) {
+    return (((uintptr_t)g.k_codes | (uintptr_t)g.v_codes) & 7) == 0 && (((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0;
+}
+
+// k_out and v_out [n][n_kv][page_size][head_dim] of out_dtype: what pages list[0 .. n) stand for.  A
+// negative number gives zeros.
+extern "C" int kipp_quant_cache_read(void* k_out, void* v_out, int out_dtype, const void* k_codes, const void* k_scales,
+                                     const void* v_codes, const void* v_scales, int bits, int n_pages, int page_size, const int* list,
+                                     int n, int n_kv, int head_dim, int* status, void* stream) {
+    if (n <= 0) return 0;
+    const QuantPages pages = {(uint8_t*)k_codes, (bf16*)k_scales, (uint8_t*)v_codes, (bf16*)v_scales, n_pages, page_size, n_kv};
+    if (!pages_ok(pages, bits, head_dim) || k_out == nullptr || v_out == nullptr || list == nullptr || status == nullptr) return KIPP_ERR_ARG;
+    if (out_dtype != KIPP_DT_F32 && out_dtype != KIPP_DT_BF16) return KIPP_ERR_DTYPE;
+    if (!read_aligned(pages, k_out, v_out)) return -3;
+    ReadParams p = {k_out, v_out, pages, list, n, head_dim, status, nullptr, nullptr, nullptr, 0, 0, 0};
+    return launch_read<false>(p, bits, out_dtype, (cudaStream_t)stream);
+}
+
+// The pages that the tokens of entries first_entry .. first_entry + entries - 1 see, read back into pages of
+// their own (entry by entry, table_width pages each), and the block table of those: table_out has the
+// step's shape and only those entries' rows are written.  The pages no token sees are neither read nor
+// written; their table entries are -1.
+extern "C" int kipp_quant_cache_read_entries(void* k_out, void* v_out, int* table_out, int out_dtype, const void* k_codes,
+                                             const void* k_scales, const void* v_codes, const void* v_scales, int bits, int n_pages,
+                                             int page_size, const int* q_start, const int* context_len, const int* block_table,
+                                             int table_width, int first_entry, int entries, int window, int n_kv, int head_dim,
+                                             int* status, void* stream) {
+    if (entries <= 0) return 0;
+    const QuantPages pages = {(uint8_t*)k_codes, (bf16*)k_scales, (uint8_t*)v_codes, (bf16*)v_scales, n_pages, page_size, n_kv};
+    if (!pages_ok(pages, bits, head_dim) || k_out == nullptr || v_out == nullptr || table_out == nullptr || status == nullptr ||
+        table_width <= 0 || first_entry < 0 || window < 0 || (long long)entries * table_width > 65535)
+        return KIPP_ERR_ARG;
+    if (out_dtype != KIPP_DT_F32 && out_dtype != KIPP_DT_BF16) return KIPP_ERR_DTYPE;
+    if (!read_aligned(pages, k_out, v_out)) return -3;
+    ReadParams p = {k_out, v_out, pages, block_table, entries * table_width, head_dim, status, table_out, q_start, context_len, table_width,
+                    first_entry, window};
+    return launch_read<true>(p, bits, out_dtype, (cudaStream_t)stream);
+}
