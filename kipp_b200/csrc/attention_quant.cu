@@ -1,0 +1,692 @@
+// Attention over the quantised cache (quant_format.cuh) for single tokens and short portions, in
+// bfloat16: codes go from memory to the tensor cores without ever being written out as numbers.
+//
+// For a key j and its group scales a[j, g], a query's score is
+//     s_j = scale * sum_g a[j, g] * (sum_{c in g} q_c code[j, c]  -  L sum_{c in g} q_c)
+// and the result, with weights p_j = exp(s_j - max) and value scales b[j, g],
+//     o_c = sum_j (p_j b[j, g(c)]) code[j, c]  -  L sum_j p_j b[j, g(c)],      out = o / sum_j p_j
+// so that both products run over bare codes; the scales multiply a score's parts (a number per key, query
+// and group) and the weights, and the offset L costs one start value per query and group, and one more
+// product of the weights with ones.
+//
+// A code is a bfloat16 operand as it stands: an integer n of up to 8 bits in the low bits of a 16-bit word
+// is the number n * 2^-133 (subnormal up to 127; the exponent's first step goes on in the same line), and
+// mma.sync takes subnormals exactly.  Two codes then become an operand register by one mask.  Four-bit
+// codes in bits 4 to 7 count sixteenfold: their queries are divided by 16, the results at the end.  Queries
+// and weights carry a factor of 2^60 so that the sums stay clear of float32's lower end; all of these are
+// powers of two.
+//
+// Products are made the other way round from the kernels of attention_mma.cu, keys (then channels) as
+// rows, queries as columns, 8 at a time: mma.m16n8k16 with S^T = K Q^T, O^T = V^T P^T.  The codes are then the
+// register operand, and a warp that serves the few queries of a kv head (the heads of its group times
+// the tokens) wastes fewer columns.  P^T turns from result to operand by movmatrix.
+//
+// What bounds it: at 4 bits a 16-byte load holds 32 keys' channels, so the instructions that take codes apart
+// (about 1.4 a code pair, keys and values together) and the softmax stand against HBM's rate; each warp works on
+// its own 32 keys of a step of 128 with its own maximum, fetches its own rows by cp.async, and meets the
+// other three warps only at the end of a piece.  A maximum is raised only when a score passes it by 2^8.
+//
+// How the work is cut: every (entry, kv head, block of columns) is a row of steps of 128 keys; all rows
+// one behind the other are dealt out in equal runs to one wave of CTAs, whatever the lengths.  A CTA may so
+// have the end of one row, some whole ones and the start of another; parts of a row go through
+// scratch and are added in order by a second kernel.  Both compute the cut from the step's lists, on
+// the device, so a captured graph follows the lengths.
+#include "quant_format.cuh"
+#include <math.h>
+
+namespace {
+
+constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr int WARP_KEYS = 32, STEP = WARPS * WARP_KEYS;
+constexpr int MERGE_THREADS = 512;
+constexpr int MOST_CTAS = 148 * 8, MOST_COLUMNS = 16;          // what the scratch has room for
+
+struct Params {
+    bf16* out; const bf16* q;
+    const uint8_t* k_codes; const uint8_t* k_scales; const uint8_t* v_codes; const uint8_t* v_scales;
+    const int* q_start; const int* context_len; const int* block_table;
+    int entries, table_width, page_size, page_shift, n_pages, most, n_q, n_kv, window;
+    float score_scale;               // scale * log2(e) * 2^73
+    float* part_o; float* part_ml;   // [2 ctas][columns][D], [2 ctas][columns][2]
+    int ctas;
+    int* status;
+};
+
+// One entry's share of the work.
+struct Entry {
+    int q_len, context, first_step, n_steps, column_blocks, blocks;
+    __device__ __forceinline__ int steps() const { return blocks * n_steps; }
+};
+template <int COLS> __device__ __forceinline__ Entry entry_of(const Params& p, int e) {
+    Entry r;
+    r.q_len = p.q_start[e + 1] - p.q_start[e];
+    r.context = p.context_len[e];
+    if (r.q_len <= 0 || r.q_len > p.most || r.context < 0) { r.blocks = r.n_steps = 0; return r; }
+    const int room = p.table_width * p.page_size;
+    const int hi = min(r.context + r.q_len, room) - 1;
+    const int lo = p.window > 0 ? max(0, r.context - p.window + 1) : 0;
+    r.first_step = min(lo, hi) / STEP;
+    r.n_steps = hi / STEP - r.first_step + 1;
+    r.column_blocks = (r.q_len * (p.n_q / p.n_kv) + COLS - 1) / COLS;
+    r.blocks = r.column_blocks * p.n_kv;
+    return r;
+}
+
+// Sum of v over the block, and over the threads before this one.
+template <int N> __device__ __forceinline__ int block_scan(int v, int& before, int* scratch) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) scratch[warp] = x;
+    __syncthreads();
+    int total = 0, ahead = 0;
+#pragma unroll
+    for (int w = 0; w < N / 32; ++w) {
+        if (w < warp) ahead += scratch[w];
+        total += scratch[w];
+    }
+    before = ahead + x - v;
+    return total;
+}
+
+__device__ __forceinline__ int steps_per_cta(int total, int ctas) { return max(1, (total + ctas - 1) / ctas); }
+
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float low_f32(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high_f32(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ void cp_async_row(uint32_t dst, const void* src, int bytes, int kept) {
+    if (bytes == 16) asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(kept) : "memory");
+    else if (bytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(kept) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(kept) : "memory");
+}
+template <int BYTES> __device__ __forceinline__ void take(uint32_t (&w)[BYTES / 4], const uint8_t* p) {
+    if constexpr (BYTES == 4) w[0] = *reinterpret_cast<const uint32_t*>(p);
+    else if constexpr (BYTES == 8) { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
+    else { const uint4 v = *reinterpret_cast<const uint4*>(p); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+}
+
+template <int D, int BITS> struct Shape {
+    static constexpr int G = D / 32;                         // groups
+    static constexpr int RB = D * BITS / 8;                  // bytes of a row of codes
+    static constexpr int SB = 2 * G;                         // bytes of its scales
+    static constexpr int CHUNKS = RB / 16;
+    static constexpr int K_BYTES = RB / 4, V_BYTES = RB / 8; // a lane's stretch of a key's row and of a value's
+    static constexpr int WARP_STAGE = WARP_KEYS * 2 * (RB + SB);
+    static constexpr int STAGES = WARP_STAGE <= 2560 ? 4 : 3;
+    static constexpr float L = BITS == 4 ? 8.f : 128.f;
+};
+
+// Where a tile of 16 keys lies.  Row r of the products (S^T's rows, P^T's and V's inner dimension) is key
+// 4 (2 h + e) + t for r = 2 t + e + 8 h: a lane (g, t) then meets the values of keys t, 4 + t, 8 + t, 12 + t,
+// which are neighbours of its neighbours' in memory.  Keys lie in product order, values in memory order, both with
+// their 16-byte chunks exchanged so that what 8 (16, 32) lanes load at once falls into different banks.
+__device__ __forceinline__ int product_row(int key) { return 2 * (key & 3) + ((key >> 2) & 1) + (key & 8); }
+__device__ __forceinline__ int key_of_row(int r) { return 4 * (r & 1) + ((r & 7) >> 1) + (r & 8); }
+template <int RB> __device__ __forceinline__ int k_chunk(int row, int c) {
+    if constexpr (RB == 128) return c ^ (row & 1);
+    if constexpr (RB == 256) return c ^ ((c >> 2) & 2) ^ (row & 1);
+    return c;
+}
+template <int RB> __device__ __forceinline__ int v_chunk(int key, int c) {
+    if constexpr (RB == 64) return c ^ (key & 2);
+    if constexpr (RB == 128) return c ^ ((key & 3) << 1);
+    if constexpr (RB == 256) return c ^ ((key & 1) | ((key & 2) << 1));
+    return c;
+}
+
+// Two runs of four codes as four operand registers: x[i] holds code i of the first run in its low half and of
+// the second in its high half.  4 bits: `first` and `second` are words, HALF which half of them the run is;
+// codes 1 and 3 count sixteenfold.  8 bits: a run is a word.
+template <int BITS> __device__ __forceinline__ void spread(uint32_t (&x)[4], uint32_t first, uint32_t second, int half) {
+    if constexpr (BITS == 4) {
+        const uint32_t w = __byte_perm(first, second, half ? 0x7632 : 0x5410), u = w >> 8;
+        x[0] = w & 0x000f000fu; x[1] = w & 0x00f000f0u; x[2] = u & 0x000f000fu; x[3] = u & 0x00f000f0u;
+    } else {
+        const uint32_t w = __byte_perm(first, second, 0x5410), u = __byte_perm(first, second, 0x7632);
+        x[0] = w & 0x00ff00ffu; x[1] = (w >> 8) & 0x00ff00ffu; x[2] = u & 0x00ff00ffu; x[3] = (u >> 8) & 0x00ff00ffu;
+    }
+}
+
+template <int D, int BITS, int NT>
+__global__ void __launch_bounds__(THREADS) attn_quant_kernel(const Params p) {
+    using S = Shape<D, BITS>;
+    constexpr int G = S::G, RB = S::RB, SB = S::SB, COLS = 8 * NT, WO = D + 4;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int scan[WARPS + 2];
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, t4 = lane & 3;
+    const int group = p.n_q / p.n_kv;
+
+    // -- the run of this CTA: from the step's lists, which may be read before the wait
+    int total = 0;
+    for (int base = 0; base < p.entries; base += THREADS) {
+        const int e = base + threadIdx.x;
+        int before;
+        total += block_scan<THREADS>(e < p.entries ? entry_of<COLS>(p, e).steps() : 0, before, scan);
+    }
+    const int per = steps_per_cta(total, p.ctas);
+    const int run_first = (int)min((long long)blockIdx.x * per, (long long)total), run_end = min(total, run_first + per);
+    if (run_first >= run_end) {
+        pdl_wait();
+        return;
+    }
+    for (int base = 0, passed = 0; base < p.entries; base += THREADS) {
+        const int e = base + threadIdx.x, mine = e < p.entries ? entry_of<COLS>(p, e).steps() : 0;
+        int before;
+        const int sum = block_scan<THREADS>(mine, before, scan);
+        if (mine > 0 && passed + before <= run_first && run_first < passed + before + mine) { scan[WARPS] = e; scan[WARPS + 1] = passed + before; }
+        passed += sum;
+        if (run_first < passed) break;
+    }
+    __syncthreads();
+    int entry = scan[WARPS], at = run_first - scan[WARPS + 1];
+    pdl_wait();
+
+    uint8_t* const my = smem + warp * (S::STAGES * S::WARP_STAGE);
+    const uint32_t my_s = smem_address(my);
+    constexpr int V_AT = WARP_KEYS * RB, KS_AT = 2 * WARP_KEYS * RB, VS_AT = KS_AT + WARP_KEYS * SB;
+
+    for (int x = run_first; x < run_end;) {
+        Entry en = entry_of<COLS>(p, entry);
+        while (at >= en.steps()) { at -= en.steps(); en = entry_of<COLS>(p, ++entry); }
+        const int block = at / en.n_steps, from = at - block * en.n_steps, n = min(run_end - x, en.n_steps - from);
+        const int g = block / en.column_blocks, column0 = (block - g * en.column_blocks) * COLS;
+        const int qs = p.q_start[entry], columns = en.q_len * group;
+        const int* table = p.block_table + (size_t)entry * p.table_width;
+        // the keys that this block's columns see, and what this lane's columns see of them
+        const int tok0 = column0 / group, tok1 = min(column0 + COLS - 1, columns - 1) / group;
+        const int see_hi = min(en.context + tok1, p.table_width * p.page_size - 1);
+        const int see_lo = p.window > 0 ? max(0, en.context + tok0 - p.window + 1) : 0;
+        int col_hi[NT][2], col_lo[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int pos = en.context + min(column0 + nt * 8 + 2 * t4 + i, columns - 1) / group;
+                col_hi[nt][i] = min(pos, see_hi);
+                col_lo[nt][i] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+            }
+        // keys all columns see (a table that ends before a token's position is reported)
+        if (en.context + tok1 > see_hi && threadIdx.x == 0) atomicExch(p.status, 3);
+        const int all_hi = min(en.context + tok0, see_hi), all_lo = p.window > 0 ? max(0, en.context + tok1 - p.window + 1) : 0;
+
+        // the row of pages that holds key j, -1 outside what is seen
+        auto row_of = [&](int j) {
+            int row = -1;
+            if (j >= see_lo && j <= see_hi) {
+                const int slot = p.page_shift >= 0 ? j >> p.page_shift : j / p.page_size;
+                const int page = table[slot];
+                if (page >= 0 && page < p.n_pages) row = (page * p.n_kv + g) * p.page_size + (j - slot * p.page_size);
+                else atomicExch(p.status, 3);
+            }
+            return row;
+        };
+        const int j_first = (en.first_step + from) * STEP + warp * WARP_KEYS;
+        auto fetch = [&](int stage, int row) {
+            const uint32_t to = my_s + stage * S::WARP_STAGE;
+            constexpr int ROWS = 32 / S::CHUNKS;               // rows of a pass
+            const int c = lane % S::CHUNKS;
+#pragma unroll
+            for (int i = 0; i < S::CHUNKS; ++i) {
+                const int key = i * ROWS + lane / S::CHUNKS, src = __shfl_sync(0xffffffffu, row, key);
+                const size_t off = (size_t)max(src, 0) * RB + c * 16;
+                const int pr = (key & 16) + product_row(key & 15), kept = src >= 0 ? 16 : 0;
+                cp_async16(to + pr * RB + k_chunk<RB>(pr, c) * 16, p.k_codes + off, kept);
+                cp_async16(to + V_AT + key * RB + v_chunk<RB>(key, c) * 16, p.v_codes + off, kept);
+            }
+            const int pr = (lane & 16) + product_row(lane & 15);
+            const size_t off = (size_t)max(row, 0) * SB;
+            cp_async_row(to + KS_AT + pr * SB, p.k_scales + off, SB, row >= 0 ? SB : 0);
+            cp_async_row(to + VS_AT + pr * SB, p.v_scales + off, SB, row >= 0 ? SB : 0);
+        };
+        int ahead = row_of(j_first + lane);
+#pragma unroll
+        for (int s = 0; s < S::STAGES - 1; ++s) {
+            if (s < n) {
+                fetch(s, ahead);
+                ahead = s + 1 < n ? row_of(j_first + (s + 1) * STEP + lane) : -1;
+            }
+            cp_async_commit();
+        }
+
+        // -- queries as operands, and what the offset of their codes comes to
+        uint32_t qf[NT][G][4];
+        float offset[NT][G][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int c = column0 + nt * 8 + g4;
+            const bool live = c < columns;
+            const int tok = live ? c / group : 0, h = live ? c - tok * group : 0;
+            const bf16* src = p.q + ((size_t)(qs + tok) * p.n_q + g * group + h) * D + t4 * (D / 4);
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi) {
+                uint2 a = make_uint2(0u, 0u), b = a;
+                if (live) {
+                    a = *reinterpret_cast<const uint2*>(src + 4 * gi);
+                    b = *reinterpret_cast<const uint2*>(src + 4 * (gi + G));
+                }
+                float sum = (low_f32(a.x) + high_f32(a.x)) + (low_f32(a.y) + high_f32(a.y)) + (low_f32(b.x) + high_f32(b.x)) + (low_f32(b.y) + high_f32(b.y));
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                sum *= -S::L * 0x1p-73f;
+                offset[nt][gi][0] = __shfl_sync(0xffffffffu, sum, 8 * t4);
+                offset[nt][gi][1] = __shfl_sync(0xffffffffu, sum, 8 * t4 + 4);
+                const uint32_t raw[4] = {__byte_perm(a.x, b.x, 0x5410), __byte_perm(a.x, b.x, 0x7632), __byte_perm(a.y, b.y, 0x5410),
+                                         __byte_perm(a.y, b.y, 0x7632)};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float f = BITS == 4 && (i & 1) ? 0x1p56f : 0x1p60f;
+                    qf[nt][gi][i] = pack2(low_f32(raw[i]) * f, high_f32(raw[i]) * f);
+                }
+            }
+        }
+
+        float o[NT][2 * G][4], ones[NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[nt][i][k] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) ones[nt][k] = 0.f;
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+        }
+
+        for (int i = 0, stage = 0; i < n; ++i) {
+            {
+                const int s = i + S::STAGES - 1;
+                if (s < n) {
+                    fetch(stage == 0 ? S::STAGES - 1 : stage - 1, ahead);
+                    ahead = s + 1 < n ? row_of(j_first + (s + 1) * STEP + lane) : -1;
+                }
+                cp_async_commit();
+                cp_async_wait<S::STAGES - 1>();
+                __syncwarp();
+            }
+            const uint8_t* tile = my + stage * S::WARP_STAGE;
+            const int j0 = j_first + i * STEP;
+            // (the warps of a step may all be outside what is seen, but for one)
+            if (j0 <= see_hi && j0 + WARP_KEYS > see_lo) {
+                // -- scores, in units of log2
+                float s[NT][2][4];
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt) {
+                    uint32_t w0[S::K_BYTES / 4], w1[S::K_BYTES / 4];
+                    const int r0 = mt * 16 + g4, r1 = r0 + 8;
+                    if constexpr (S::K_BYTES <= 16) {
+                        take<S::K_BYTES>(w0, tile + r0 * RB + t4 * S::K_BYTES);
+                        take<S::K_BYTES>(w1, tile + r1 * RB + t4 * S::K_BYTES);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < S::K_BYTES / 16; ++c) {
+                            uint32_t v[4];
+                            take<16>(v, tile + r0 * RB + k_chunk<RB>(r0, t4 * (S::K_BYTES / 16) + c) * 16);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) w0[4 * c + k] = v[k];
+                            take<16>(v, tile + r1 * RB + k_chunk<RB>(r1, t4 * (S::K_BYTES / 16) + c) * 16);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) w1[4 * c + k] = v[k];
+                        }
+                    }
+                    uint32_t a0[(SB + 3) / 4], a1[(SB + 3) / 4];
+                    take<SB>(a0, tile + KS_AT + r0 * SB);
+                    take<SB>(a1, tile + KS_AT + r1 * SB);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.f;
+#pragma unroll
+                    for (int gi = 0; gi < G; ++gi) {
+                        uint32_t x0[4], x1[4];
+                        if constexpr (BITS == 4) {
+                            spread<4>(x0, w0[gi >> 1], w0[(gi + G) >> 1], gi & 1);
+                            spread<4>(x1, w1[gi >> 1], w1[(gi + G) >> 1], gi & 1);
+                        } else {
+                            spread<8>(x0, w0[gi], w0[gi + G], 0);
+                            spread<8>(x1, w1[gi], w1[gi + G], 0);
+                        }
+                        const float f0 = gi & 1 ? high_f32(a0[gi >> 1]) : low_f32(a0[gi >> 1]);
+                        const float f1 = gi & 1 ? high_f32(a1[gi >> 1]) : low_f32(a1[gi >> 1]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            float c[4] = {offset[nt][gi][0], offset[nt][gi][1], offset[nt][gi][0], offset[nt][gi][1]};
+                            mma(c, x0[0], x1[0], x0[1], x1[1], qf[nt][gi][0], qf[nt][gi][1]);
+                            mma(c, x0[2], x1[2], x0[3], x1[3], qf[nt][gi][2], qf[nt][gi][3]);
+                            s[nt][mt][0] = fmaf(f0, c[0], s[nt][mt][0]);
+                            s[nt][mt][1] = fmaf(f0, c[1], s[nt][mt][1]);
+                            s[nt][mt][2] = fmaf(f1, c[2], s[nt][mt][2]);
+                            s[nt][mt][3] = fmaf(f1, c[3], s[nt][mt][3]);
+                        }
+                    }
+                }
+                const bool cut = j0 + WARP_KEYS - 1 > all_hi || j0 < all_lo;
+                bool raise = false;
+                float top[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            s[nt][mt][k] *= p.score_scale;
+                            if (cut) {
+                                const int j = j0 + mt * 16 + key_of_row(g4 + (k >> 1) * 8);
+                                if (j > col_hi[nt][k & 1] || j < col_lo[nt][k & 1]) s[nt][mt][k] = -INFINITY;
+                            }
+                        }
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        top[nt][c] = fmaxf(fmaxf(s[nt][0][c], s[nt][0][2 + c]), fmaxf(s[nt][1][c], s[nt][1][2 + c]));
+                        raise |= top[nt][c] > m[nt][c] + 8.f;
+                    }
+                }
+                if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float f[2];
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float mx = fmaxf(m[nt][c], top[nt][c]);
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                            f[c] = m[nt][c] == -INFINITY ? 0.f : exp2_fast(m[nt][c] - mx);
+                            m[nt][c] = mx;
+                            l[nt][c] *= f[c];
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            ones[nt][k] *= f[k & 1];
+#pragma unroll
+                            for (int d = 0; d < 2 * G; ++d) o[nt][d][k] *= f[k & 1];
+                        }
+                    }
+                }
+                // -- weights (times 2^60), and the weighted sums
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const float back = (m[nt][c] == -INFINITY ? 0.f : m[nt][c]) - 60.f;
+#pragma unroll
+                        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float w = exp2_fast(s[nt][mt][2 * h + c] - back);
+                                s[nt][mt][2 * h + c] = w;
+                                l[nt][c] += w;
+                            }
+                    }
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt) {
+                    uint32_t a0[(SB + 3) / 4], a1[(SB + 3) / 4];
+                    take<SB>(a0, tile + VS_AT + (mt * 16 + g4) * SB);
+                    take<SB>(a1, tile + VS_AT + (mt * 16 + g4 + 8) * SB);
+                    uint32_t v[4][S::V_BYTES / 4];                     // keys t, 4 + t, 8 + t, 12 + t
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int key = mt * 16 + 4 * k + t4;
+                        if constexpr (S::V_BYTES <= 16) {
+                            constexpr int PER = 16 / S::V_BYTES;        // stretches of a chunk
+                            take<S::V_BYTES>(v[k], tile + V_AT + key * RB + v_chunk<RB>(key, g4 / PER) * 16 + (g4 % PER) * S::V_BYTES);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < S::V_BYTES / 16; ++c) {
+                                uint32_t u[4];
+                                take<16>(u, tile + V_AT + key * RB + v_chunk<RB>(key, g4 * (S::V_BYTES / 16) + c) * 16);
+#pragma unroll
+                                for (int b = 0; b < 4; ++b) v[k][4 * c + b] = u[b];
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int gi = 0; gi < G; ++gi) {
+                        uint32_t x0[4], x1[4];                         // keys of the first and the second half of the rows
+                        constexpr int W = BITS == 4 ? 1 : 0;
+                        spread<BITS>(x0, v[0][gi >> W], v[1][gi >> W], gi & 1);
+                        spread<BITS>(x1, v[2][gi >> W], v[3][gi >> W], gi & 1);
+                        const float f0 = gi & 1 ? high_f32(a0[gi >> 1]) : low_f32(a0[gi >> 1]);
+                        const float f1 = gi & 1 ? high_f32(a1[gi >> 1]) : low_f32(a1[gi >> 1]);
+                        const uint32_t one = g4 == gi ? 0x3f803f80u : 0u;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const uint32_t b0 = transposed(pack2(s[nt][mt][0] * f0, s[nt][mt][1] * f0));
+                            const uint32_t b1 = transposed(pack2(s[nt][mt][2] * f1, s[nt][mt][3] * f1));
+                            mma(o[nt][2 * gi], x0[0], x0[1], x1[0], x1[1], b0, b1);
+                            mma(o[nt][2 * gi + 1], x0[2], x0[3], x1[2], x1[3], b0, b1);
+                            mma(ones[nt], one, 0u, one, 0u, b0, b1);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+        }
+        cp_async_wait<0>();
+
+        // -- the four warps' parts together, through shared memory
+        __syncthreads();
+        float* w_m = reinterpret_cast<float*>(smem);                   // [WARPS][COLS]
+        float* w_l = w_m + WARPS * COLS;                               // [WARPS][COLS]
+        float* w_o = w_l + WARPS * COLS;                               // [WARPS][COLS][WO]
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float sum = l[nt][c];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                const int col = nt * 8 + 2 * t4 + c;
+                if (g4 == 0) {
+                    w_m[warp * COLS + col] = m[nt][c];
+                    w_l[warp * COLS + col] = sum * 0x1p-60f;
+                }
+            }
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi) {
+                // (row gi of the product with ones lies with lane 4 gi + t)
+                const float less[2] = {__shfl_sync(0xffffffffu, ones[nt][0], 4 * gi + t4) * (S::L * 0x1p-60f),
+                                       __shfl_sync(0xffffffffu, ones[nt][1], 4 * gi + t4) * (S::L * 0x1p-60f)};
+                constexpr float EVEN = 0x1p73f, ODD = BITS == 4 ? 0x1p69f : 0x1p73f;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float4 r;
+                    r.x = fmaf(o[nt][2 * gi][c], EVEN, -less[c]);
+                    r.y = fmaf(o[nt][2 * gi][2 + c], ODD, -less[c]);
+                    r.z = fmaf(o[nt][2 * gi + 1][c], EVEN, -less[c]);
+                    r.w = fmaf(o[nt][2 * gi + 1][2 + c], ODD, -less[c]);
+                    *reinterpret_cast<float4*>(w_o + (size_t)(warp * COLS + nt * 8 + 2 * t4 + c) * WO + g4 * (D / 8) + 4 * gi) = r;
+                }
+            }
+        }
+        __syncthreads();
+        const bool whole = n == en.n_steps;
+        const int slot = 2 * blockIdx.x + (x == run_first ? 0 : 1);
+        const int live = min(COLS, columns - column0);
+        for (int i = threadIdx.x; i < live * D; i += THREADS) {
+            const int col = i / D, d = i % D;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) mx = fmaxf(mx, w_m[w * COLS + col]);
+            float sum = 0.f, acc = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float wm = w_m[w * COLS + col], f = wm == -INFINITY ? 0.f : exp2_fast(wm - mx);
+                sum += w_l[w * COLS + col] * f;
+                acc += w_o[(size_t)(w * COLS + col) * WO + d] * f;
+            }
+            if (whole) {
+                const int c = column0 + col, tok = c / group;
+                p.out[((size_t)(qs + tok) * p.n_q + g * group + (c - tok * group)) * D + d] = __float2bfloat16_rn(sum > 0.f ? acc / sum : 0.f);
+            } else {
+                p.part_o[((size_t)slot * COLS + col) * D + d] = acc;
+                if (d == 0) {
+                    p.part_ml[((size_t)slot * COLS + col) * 2] = mx;
+                    p.part_ml[((size_t)slot * COLS + col) * 2 + 1] = sum;
+                }
+            }
+        }
+        __syncthreads();
+        x += n;
+        at += n;
+    }
+}
+
+// Adds the parts of one head of one token, in the order of the keys: MERGE_THREADS / D threads an element, each
+// a share of the parts.
+template <int D, int NT>
+__global__ void __launch_bounds__(MERGE_THREADS) attn_quant_merge_kernel(const Params p) {
+    constexpr int COLS = 8 * NT, SHARES = MERGE_THREADS / D;
+    __shared__ int scan[MERGE_THREADS / 32];
+    __shared__ float sh_o[SHARES][D], sh_l[SHARES];
+    __shared__ float sh_m[MERGE_THREADS / 32];
+    const int e = blockIdx.y, tok = blockIdx.x / p.n_q, head = blockIdx.x - tok * p.n_q;
+    const Entry en = entry_of<COLS>(p, e);
+    if (en.blocks == 0 || tok >= en.q_len) { pdl_wait(); return; }
+    int total = 0, start = 0;
+    for (int base = 0; base < p.entries; base += MERGE_THREADS) {
+        const int i = base + threadIdx.x, steps = i < p.entries ? entry_of<COLS>(p, i).steps() : 0;
+        int before;
+        total += block_scan<MERGE_THREADS>(steps, before, scan);
+        start += block_scan<MERGE_THREADS>(i < e ? steps : 0, before, scan);
+    }
+    const int group = p.n_q / p.n_kv, g = head / group, c = tok * group + head - g * group, col = c % COLS;
+    start += (g * en.column_blocks + c / COLS) * en.n_steps;
+    const int per = steps_per_cta(total, p.ctas), c0 = start / per, c1 = (start + en.n_steps - 1) / per, parts = c1 - c0 + 1;
+    pdl_wait();
+    if (parts == 1) return;
+    auto slot = [&](int part) { return 2 * (c0 + part) + ((c0 + part) * (long long)per >= start ? 0 : 1); };
+    float mx = -INFINITY;
+    for (int i = threadIdx.x; i < parts; i += MERGE_THREADS) mx = fmaxf(mx, p.part_ml[((size_t)slot(i) * COLS + col) * 2]);
+    mx = warp_max(mx);
+    if ((threadIdx.x & 31) == 0) sh_m[threadIdx.x >> 5] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < MERGE_THREADS / 32; ++w) mx = fmaxf(mx, sh_m[w]);
+    const int d = threadIdx.x % D, share = threadIdx.x / D;
+    const int many = (parts + SHARES - 1) / SHARES, end = min(parts, (share + 1) * many);
+    float acc = 0.f, sum = 0.f;
+#pragma unroll 8
+    for (int i = share * many; i < end; ++i) {
+        const size_t at = (size_t)slot(i) * COLS + col;
+        const float pm = p.part_ml[at * 2], f = pm == -INFINITY ? 0.f : exp2_fast(pm - mx);
+        sum += p.part_ml[at * 2 + 1] * f;
+        acc += p.part_o[at * D + d] * f;
+    }
+    sh_o[share][d] = acc;
+    if (d == 0) sh_l[share] = sum;
+    __syncthreads();
+    if (share == 0) {
+        acc = sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < SHARES; ++i) { acc += sh_o[i][d]; sum += sh_l[i]; }
+        p.out[((size_t)(p.q_start[e] + tok) * p.n_q + head) * D + d] = __float2bfloat16_rn(sum > 0.f ? acc / sum : 0.f);
+    }
+}
+
+template <int D, int BITS, int NT> constexpr size_t smem_bytes() {
+    using S = Shape<D, BITS>;
+    constexpr size_t ring = (size_t)WARPS * S::STAGES * S::WARP_STAGE, merge = (size_t)WARPS * 8 * NT * (D + 4 + 2) * 4;
+    return ring > merge ? ring : merge;
+}
+// CTAs of one wave.
+template <int D, int BITS, int NT> int wave() {
+    static const int ctas = [] {
+        int per = 0;
+        const size_t smem = smem_bytes<D, BITS, NT>();
+        if (kipp_allow_smem(attn_quant_kernel<D, BITS, NT>, smem) != 0 ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attn_quant_kernel<D, BITS, NT>, THREADS, smem) != cudaSuccess || per < 1) {
+            cudaGetLastError();
+            per = 1;
+        }
+        return per * kipp_sm_count();
+    }();
+    return ctas;
+}
+template <int D, int BITS, int NT> int launch(Params p, long long most_steps, cudaStream_t s) {
+    constexpr size_t smem = smem_bytes<D, BITS, NT>();
+    const int most_ctas = wave<D, BITS, NT>() < MOST_CTAS ? wave<D, BITS, NT>() : MOST_CTAS;
+    p.ctas = (int)(most_steps < most_ctas ? most_steps : most_ctas);
+    if (const int e = kipp_allow_smem(attn_quant_kernel<D, BITS, NT>, smem)) return e;
+    if (const int e = kipp_launch(attn_quant_kernel<D, BITS, NT>, dim3((unsigned)p.ctas), dim3(THREADS), smem, s, 1, p)) return e;
+    return kipp_launch(attn_quant_merge_kernel<D, NT>, dim3((unsigned)(p.n_q * p.most), (unsigned)p.entries), dim3(MERGE_THREADS), 0, s, 1, p);
+}
+
+// 8 columns where they hold every query of a kv head, else 16 (heads of 256 have no room for their sums: always 8)
+int columns_of(int head_dim, long long queries) { return head_dim == 256 || queries <= 8 ? 8 : 16; }
+}  // namespace
+
+// Whether the kernel takes these heads.
+extern "C" int kipp_attn_quant_supported(int bits, int head_dim, int n_q, int n_kv) {
+    return (bits == 4 || bits == 8) && (head_dim == 64 || head_dim == 128 || head_dim == 256) && n_kv > 0 && n_q > 0 && n_q % n_kv == 0;
+}
+// Bytes of scratch of a launch (the parts of rows that several CTAs share), whatever the step.
+extern "C" long long kipp_attn_quant_scratch_bytes(int head_dim) { return 2LL * MOST_CTAS * MOST_COLUMNS * (head_dim + 2) * 4; }
+
+// out, q: bf16 [tokens][n_q][head_dim].  The entries that bring 1 to `most` tokens; the others are left alone.
+extern "C" int kipp_attn_quant(void* out, const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
+                               const void* v_scales, int bits, int n_pages, int page_size, const int* q_start, const int* context_len,
+                               const int* block_table, int table_width, int entries, int most, int n_q, int n_kv, int head_dim,
+                               float scale, int window, void* scratch, long long scratch_bytes, int* status, void* stream) {
+    if (entries <= 0 || most <= 0) return 0;
+    if (!kipp_attn_quant_supported(bits, head_dim, n_q, n_kv) || page_size <= 0 || n_pages <= 0 || table_width <= 0 || window < 0 ||
+        status == nullptr || scratch == nullptr || entries > 65535)
+        return KIPP_ERR_ARG;
+    if (scratch_bytes < kipp_attn_quant_scratch_bytes(head_dim)) return -4;
+    if ((((uintptr_t)q | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scales | (uintptr_t)v_scales | (uintptr_t)scratch) & 15) != 0) return -3;
+    // (row numbers of pages, steps of all rows and blocks of the second kernel are 32-bit)
+    const long long cols = columns_of(head_dim, (long long)most * (n_q / n_kv));
+    const long long room = (long long)table_width * page_size, steps = (room + STEP - 1) / STEP;
+    const long long rows = (long long)entries * n_kv * (((long long)most * (n_q / n_kv) + cols - 1) / cols);
+    if ((long long)n_pages * n_kv * page_size > 0x7fffffffLL || room > 0x7fffffffLL || rows > 0x3fffffffLL / steps ||
+        (long long)most * n_q > 0x7fffffffLL)
+        return KIPP_ERR_ARG;
+    Params p = {};
+    p.out = (bf16*)out; p.q = (const bf16*)q;
+    p.k_codes = (const uint8_t*)k_codes; p.k_scales = (const uint8_t*)k_scales;
+    p.v_codes = (const uint8_t*)v_codes; p.v_scales = (const uint8_t*)v_scales;
+    p.q_start = q_start; p.context_len = context_len; p.block_table = block_table;
+    p.entries = entries; p.table_width = table_width; p.page_size = page_size; p.n_pages = n_pages; p.most = most;
+    p.page_shift = -1;
+    for (int i = 0; i < 31; ++i) if (page_size == 1 << i) p.page_shift = i;
+    p.n_q = n_q; p.n_kv = n_kv; p.window = window;
+    p.score_scale = scale * 1.4426950408889634f * 0x1p73f;
+    p.part_o = (float*)scratch;
+    p.part_ml = p.part_o + 2LL * MOST_CTAS * MOST_COLUMNS * head_dim;
+    p.status = status;
+    cudaStream_t s = (cudaStream_t)stream;
+    const long long steps_at_most = rows * steps;
+#define KIPP_CASE(d, b)                                                                             \
+    if (head_dim == d && bits == b) {                                                               \
+        if (cols == 8) return launch<d, b, 1>(p, steps_at_most, s);                                 \
+        if constexpr (d != 256) return launch<d, b, 2>(p, steps_at_most, s);                        \
+    }
+    KIPP_CASE(64, 4) KIPP_CASE(64, 8) KIPP_CASE(128, 4) KIPP_CASE(128, 8) KIPP_CASE(256, 4) KIPP_CASE(256, 8)
+#undef KIPP_CASE
+    return KIPP_ERR_ARG;
+}

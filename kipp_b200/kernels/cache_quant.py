@@ -151,13 +151,40 @@ def _entries_at_once(pages: QuantizedPages, dtype: torch.dtype, width: int) -> i
     return max(1, min(READ_BYTES // per, 65535 // width))
 
 
+PORTION_MIN = 64              # an entry of as many tokens is read back for the prompt kernel of 128-token tiles
+
+
+def _direct_ok(q: torch.Tensor, pages: QuantizedPages, n_q: int) -> bool:
+    f = _fn("attention_quant", "kipp_attn_quant_supported", [c_int, c_int, c_int, c_int])
+    return (q.dtype == torch.bfloat16 and bool(f(pages.bits, pages.head_dim, n_q, pages.n_kv))
+            and all(t.data_ptr() % 16 == 0 for t in (q, pages.k_codes, pages.v_codes, pages.k_scales, pages.v_scales)))
+
+
+def _plan(out, q, pages, meta, block_table, n_q):
+    """(form of the entries of one token, form of the others, the entries of more than one token from the first to the last):
+    forms "direct" (the kernel over codes), "portion" (read back, tcgen05 prompt kernel) and "read" (read back, CUDA cores).
+    The prompt kernel reads a key and a value once for 128 tokens, the kernel over codes once for 8 or 16 columns."""
+    if not _direct_ok(q, pages, n_q):
+        return "read", "read", None
+    several = [e for e, n in enumerate(meta.q_lens) if n > 1]
+    if several and max(meta.q_lens) >= PORTION_MIN and getattr(meta, "prefill_work128", None) is not None:
+        from . import attention_bf16
+        span = (several[0], several[-1] + 1)
+        if attention_bf16.prefill_tc_supported(pages.head_dim, n_q, pages.n_kv, pages.page_size) and out.data_ptr() % 16 == 0 and \
+                span[1] - span[0] <= _entries_at_once(pages, q.dtype, block_table.shape[1]):
+            return "direct", "portion", span
+    return "direct", "direct", None
+
+
 def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPages, meta, block_table: torch.Tensor, n_q: int,
                         scale: float, window: Optional[int], status: torch.Tensor, impl: Optional[str] = None) -> None:
     """Causal grouped-query attention of the step's tokens over a quantised cache.
 
     ``meta`` is the step's metadata as for ``attention`` (``tokens``, ``q_lens``, ``positions``, ``entry_of_token``,
-    ``q_start``, ``context_len``).  ``impl`` forces a form: "read" brings the entries' pages back into q's type and takes
-    the attention over those."""
+    ``q_start``, ``context_len``, and where entries bring 64 tokens or more the list of their 128-token tiles,
+    ``prefill_work128`` and ``n_prefill_items128``).  bfloat16 with heads of 64, 128 or 256 runs on the codes themselves; longer
+    portions of prompts, other heads and float32 on pages that are read back.  ``impl`` forces a form for the whole step:
+    "direct" or "read"."""
     what, D, n_kv, window = "attention_quantized", pages.head_dim, pages.n_kv, int(window or 0)
     dtype_code(q.dtype)
     if q.dim() != 3 or tuple(q.shape[1:]) != (n_q, D) or q.shape[0] < meta.tokens or not q.is_contiguous() or n_q % n_kv:
@@ -166,18 +193,50 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
         raise KernelError(f"{what}: out must be contiguous, of q's dtype and shape")
     if window < 0:
         raise KernelError(f"{what}: a window must not be negative")
-    if block_table.dim() != 2 or block_table.shape[0] < len(meta.q_lens) or sum(meta.q_lens) != meta.tokens:
+    if block_table.dim() != 2 or block_table.shape[0] < len(meta.q_lens) or block_table.shape[1] == 0 or sum(meta.q_lens) != meta.tokens:
         raise KernelError(f"{what}: a row of block_table for every entry, and as many tokens as the entries bring")
     for t, name in ((block_table, "block_table"), (meta.positions, "positions"), (meta.entry_of_token, "entry_of_token"),
                     (meta.q_start, "q_start"), (meta.context_len, "context_len")):
         _int32(t, name)
+    if meta.q_start.numel() <= len(meta.q_lens) or meta.context_len.numel() < len(meta.q_lens) or \
+            min(meta.positions.numel(), meta.entry_of_token.numel()) < meta.tokens:
+        raise KernelError(f"{what}: the step's lists are shorter than the step")
     _status(status, what)
     _on(q.device, what, out, pages.k_codes, block_table, meta.q_start, meta.context_len, meta.positions, meta.entry_of_token, status)
-    if impl not in (None, "read"):
+    if impl not in (None, "direct", "read"):
         raise KernelError(f"unknown attention implementation {impl!r}")
+    if impl == "direct" and not _direct_ok(q, pages, n_q):
+        raise KernelError(f"{what}: the kernel over codes takes bfloat16 heads of 64, 128 or 256, 16-byte aligned")
     if meta.tokens == 0:
         return
-    _by_reading(out, q, pages, meta, block_table, n_q, scale, window, status)
+    single, several, span = _plan(out, q, pages, meta, block_table, n_q) if impl is None else (impl, impl, None)
+    if single == "read":
+        _by_reading(out, q, pages, meta, block_table, n_q, scale, window, status)
+        return
+    if several == "direct" or 1 in meta.q_lens:
+        _direct(out, q, pages, meta, block_table, n_q, scale, window, status, max(meta.q_lens) if several == "direct" else 1)
+    if several == "portion":
+        _portions(out, q, pages, meta, block_table, n_q, scale, window, status, span)
+
+
+def _direct(out, q, pages, meta, block_table, n_q, scale, window, status, most: int) -> None:
+    """The entries of up to ``most`` tokens, over the codes."""
+    need = _fn("attention_quant", "kipp_attn_quant_scratch_bytes", [c_int], restype=c_ll)(pages.head_dim)
+    scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+    f = _fn("attention_quant", "kipp_attn_quant",
+            [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
+             c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_ll, c_void_p, c_void_p])
+    _check(f(_ptr(out), _ptr(q), *pages.pointers(), _ptr(meta.q_start), _ptr(meta.context_len), _ptr(block_table), block_table.shape[1],
+             len(meta.q_lens), most, n_q, pages.n_kv, pages.head_dim, float(scale), window, _ptr(scratch), need, _ptr(status), _stream()),
+           "attn_quant")
+
+
+def _portions(out, q, pages, meta, block_table, n_q, scale, window, status, span) -> None:
+    """The entries of more than one token: their pages read back, and the prompt kernel over those."""
+    table = torch.empty_like(block_table)
+    k, v = _read_entries(pages, q.dtype, meta, block_table, span[0], span[1] - span[0], window, status, table)
+    from . import attention_bf16
+    attention_bf16.prefill_tc(out, q, k, v, meta, table, pages.page_size, n_q, pages.n_kv, pages.head_dim, scale, window, status)
 
 
 def _by_reading(out, q, pages, meta, block_table, n_q, scale, window, status) -> None:
