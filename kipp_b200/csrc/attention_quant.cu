@@ -23,22 +23,26 @@
 //
 // What bounds it: at 4 bits a 16-byte load holds 32 keys' channels, so the instructions that take codes apart
 // (about 1.4 a code pair, keys and values together) and the softmax stand against HBM's rate; each warp works on
-// its own 32 keys of a step of 128 with its own maximum, fetches its own rows by cp.async, and meets the
-// other three warps only at the end of a piece.  A maximum is raised only when a score passes it by 2^8.
+// its own 32 keys of a step of 128 with its own maximum, fetches its own rows, and meets the other three
+// warps only at the end of a piece.  A maximum is raised only when a score passes it by 2^8.
+//
+// Rows come by bulk copies into a ring per warp: 16 keys of one kv head lie in one piece where the page size is
+// a multiple of 16, and eight lanes ask for the codes and scales of 32 keys and values with one instruction.
+// Other page sizes take cp.async row by row.
 //
 // How the work is cut: every (entry, kv head, block of columns) is a row of steps of 128 keys; all rows
 // one behind the other are dealt out in equal runs to one wave of CTAs, whatever the lengths.  A CTA may so
 // have the end of one row, some whole ones and the start of another; parts of a row go through
-// scratch and are added in order by a second kernel.  Both compute the cut from the step's lists, on
+// scratch and are added in order by a second kernel.  The cut is made from the step's lists, on
 // the device, so a captured graph follows the lengths.
 #include "quant_format.cuh"
+#include "mbarrier.cuh"
 #include <math.h>
 
 namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int WARP_KEYS = 32, STEP = WARPS * WARP_KEYS;
-constexpr int MERGE_THREADS = 512;
 constexpr int MOST_CTAS = 148 * 8, MOST_COLUMNS = 16;          // what the scratch has room for
 
 struct Params {
@@ -48,7 +52,10 @@ struct Params {
     int entries, table_width, page_size, page_shift, n_pages, most, n_q, n_kv, window;
     float score_scale;               // scale * log2(e) * 2^73
     float* part_o; float* part_ml;   // [2 ctas][columns][D], [2 ctas][columns][2]
-    int ctas;
+    // rows that several CTAs share, by the row's number (by_row) or by the first CTA: (entry, kv head, 2 first column + the first
+    // part's slot, first CTA << 16 | CTAs); 0 CTAs: nothing to add
+    int4* shared_rows;
+    int ctas, by_row, most_blocks;   // most_blocks: rows of an entry of `most` tokens
     int* status;
 };
 
@@ -94,7 +101,9 @@ template <int N> __device__ __forceinline__ int block_scan(int v, int& before, i
     return total;
 }
 
-__device__ __forceinline__ int steps_per_cta(int total, int ctas) { return max(1, (total + ctas - 1) / ctas); }
+// Runs differ by one step at most: CTA c has steps [total c / ctas, total (c + 1) / ctas).
+__device__ __forceinline__ int run_start(int total, int ctas, int c) { return (int)((long long)total * c / ctas); }
+__device__ __forceinline__ int cta_of_step(int total, int ctas, int x) { return (int)(((long long)(x + 1) * ctas - 1) / total); }
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -126,7 +135,13 @@ __device__ __forceinline__ void cp_async_row(uint32_t dst, const void* src, int 
 template <int BYTES> __device__ __forceinline__ void take(uint32_t (&w)[BYTES / 4], const uint8_t* p) {
     if constexpr (BYTES == 4) w[0] = *reinterpret_cast<const uint32_t*>(p);
     else if constexpr (BYTES == 8) { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
-    else { const uint4 v = *reinterpret_cast<const uint4*>(p); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+    else {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) {
+            const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+        }
+    }
 }
 
 template <int D, int BITS> struct Shape {
@@ -136,27 +151,17 @@ template <int D, int BITS> struct Shape {
     static constexpr int CHUNKS = RB / 16;
     static constexpr int K_BYTES = RB / 4, V_BYTES = RB / 8; // a lane's stretch of a key's row and of a value's
     static constexpr int WARP_STAGE = WARP_KEYS * 2 * (RB + SB);
-    static constexpr int STAGES = WARP_STAGE <= 2560 ? 4 : 3;
+    // steps in the ring, and CTAs an SM: 228 KB hold four of three steps of 4.5 KB a warp (heads of 128 in 4 bits)
+    static constexpr int STAGES = WARP_STAGE <= 2560 ? 4 : RB == 128 && D == 128 ? 2 : 3;
     static constexpr float L = BITS == 4 ? 8.f : 128.f;
 };
+template <int D, int BITS, int NT> constexpr int ctas_per_sm() {
+    return D == 256 ? (BITS == 4 ? 2 : 1) : NT == 2 ? (D == 64 ? 3 : 2) : D == 128 && BITS == 8 ? 3 : 4;
+}
 
-// Where a tile of 16 keys lies.  Row r of the products (S^T's rows, P^T's and V's inner dimension) is key
-// 4 (2 h + e) + t for r = 2 t + e + 8 h: a lane (g, t) then meets the values of keys t, 4 + t, 8 + t, 12 + t,
-// which are neighbours of its neighbours' in memory.  Keys lie in product order, values in memory order, both with
-// their 16-byte chunks exchanged so that what 8 (16, 32) lanes load at once falls into different banks.
-__device__ __forceinline__ int product_row(int key) { return 2 * (key & 3) + ((key >> 2) & 1) + (key & 8); }
+// Row r of the products (S^T's rows, P^T's and V's inner dimension) is key 4 (2 h + e) + t of a tile of 16, for
+// r = 2 t + e + 8 h: a lane (g, t) then meets the values of keys t, 4 + t, 8 + t, 12 + t.
 __device__ __forceinline__ int key_of_row(int r) { return 4 * (r & 1) + ((r & 7) >> 1) + (r & 8); }
-template <int RB> __device__ __forceinline__ int k_chunk(int row, int c) {
-    if constexpr (RB == 128) return c ^ (row & 1);
-    if constexpr (RB == 256) return c ^ ((c >> 2) & 2) ^ (row & 1);
-    return c;
-}
-template <int RB> __device__ __forceinline__ int v_chunk(int key, int c) {
-    if constexpr (RB == 64) return c ^ (key & 2);
-    if constexpr (RB == 128) return c ^ ((key & 3) << 1);
-    if constexpr (RB == 256) return c ^ ((key & 1) | ((key & 2) << 1));
-    return c;
-}
 
 // Two runs of four codes as four operand registers: x[i] holds code i of the first run in its low half and of
 // the second in its high half.  4 bits: `first` and `second` are words, HALF which half of them the run is;
@@ -171,15 +176,32 @@ template <int BITS> __device__ __forceinline__ void spread(uint32_t (&x)[4], uin
     }
 }
 
-template <int D, int BITS, int NT>
-__global__ void __launch_bounds__(THREADS) attn_quant_kernel(const Params p) {
+__device__ __forceinline__ void expect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(kipp_smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(kipp_smem_u32(bar)) : "memory");
+}
+
+// BULK: the page size is a multiple of 16.
+template <int D, int BITS, int NT, bool BULK>
+__global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quant_kernel(const Params p) {
     using S = Shape<D, BITS>;
-    constexpr int G = S::G, RB = S::RB, SB = S::SB, COLS = 8 * NT, WO = D + 4;
+    constexpr int G = S::G, RB = S::RB, SB = S::SB, COLS = 8 * NT, WO = D + 4, STAGES = S::STAGES;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int scan[WARPS + 2];
+    __shared__ uint64_t full[WARPS][STAGES];
+    __shared__ int gave_up;
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, t4 = lane & 3;
     const int group = p.n_q / p.n_kv;
+    if constexpr (BULK) {
+        if (threadIdx.x < WARPS * STAGES)
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(kipp_smem_u32(&full[0][0] + threadIdx.x)) : "memory");
+        if (threadIdx.x == 0) gave_up = 0;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
 
     // -- the run of this CTA: from the step's lists, which may be read before the wait
     int total = 0;
@@ -188,10 +210,12 @@ __global__ void __launch_bounds__(THREADS) attn_quant_kernel(const Params p) {
         int before;
         total += block_scan<THREADS>(e < p.entries ? entry_of<COLS>(p, e).steps() : 0, before, scan);
     }
-    const int per = steps_per_cta(total, p.ctas);
-    const int run_first = (int)min((long long)blockIdx.x * per, (long long)total), run_end = min(total, run_first + per);
+    const int ctas = min(p.ctas, total);                   // (so that none between two others is empty)
+    const int run_first = (int)blockIdx.x < ctas ? run_start(total, ctas, blockIdx.x) : total;
+    const int run_end = (int)blockIdx.x < ctas ? run_start(total, ctas, blockIdx.x + 1) : total;
     if (run_first >= run_end) {
         pdl_wait();
+        if (!p.by_row && threadIdx.x == 0) p.shared_rows[blockIdx.x] = make_int4(0, 0, 0, 0);
         return;
     }
     for (int base = 0, passed = 0; base < p.entries; base += THREADS) {
@@ -205,10 +229,18 @@ __global__ void __launch_bounds__(THREADS) attn_quant_kernel(const Params p) {
     __syncthreads();
     int entry = scan[WARPS], at = run_first - scan[WARPS + 1];
     pdl_wait();
+    if (!p.by_row && threadIdx.x == 0) p.shared_rows[blockIdx.x] = make_int4(0, 0, 0, 0);
 
-    uint8_t* const my = smem + warp * (S::STAGES * S::WARP_STAGE);
+    uint8_t* const my = smem + warp * (STAGES * S::WARP_STAGE);
     const uint32_t my_s = smem_address(my);
     constexpr int V_AT = WARP_KEYS * RB, KS_AT = 2 * WARP_KEYS * RB, VS_AT = KS_AT + WARP_KEYS * SB;
+    // bulk copies: lane 4 tile + array asks for array (keys, values, their scales) of tile (16 keys)
+    const int b_array = lane & 3, b_bytes = b_array < 2 ? RB : SB;
+    const uint8_t* const b_from = b_array == 0 ? p.k_codes : b_array == 1 ? p.v_codes : b_array == 2 ? p.k_scales : p.v_scales;
+    const uint32_t b_to = my_s + (b_array == 0 ? 0 : b_array == 1 ? V_AT : b_array == 2 ? KS_AT : VS_AT) + ((lane >> 2) & 1) * 16 * b_bytes;
+    uint32_t parity = 0;                                       // of each stage's next arrival
+    int stage = 0;
+    bool failed = false;
 
     for (int x = run_first; x < run_end;) {
         Entry en = entry_of<COLS>(p, entry);
@@ -221,23 +253,15 @@ __global__ void __launch_bounds__(THREADS) attn_quant_kernel(const Params p) {
         const int tok0 = column0 / group, tok1 = min(column0 + COLS - 1, columns - 1) / group;
         const int see_hi = min(en.context + tok1, p.table_width * p.page_size - 1);
         const int see_lo = p.window > 0 ? max(0, en.context + tok0 - p.window + 1) : 0;
-        int col_hi[NT][2], col_lo[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int pos = en.context + min(column0 + nt * 8 + 2 * t4 + i, columns - 1) / group;
-                col_hi[nt][i] = min(pos, see_hi);
-                col_lo[nt][i] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-            }
         // keys all columns see (a table that ends before a token's position is reported)
         if (en.context + tok1 > see_hi && threadIdx.x == 0) atomicExch(p.status, 3);
         const int all_hi = min(en.context + tok0, see_hi), all_lo = p.window > 0 ? max(0, en.context + tok1 - p.window + 1) : 0;
+        const int j_first = (en.first_step + from) * STEP + warp * WARP_KEYS;
 
-        // the row of pages that holds key j, -1 outside what is seen
+        // the row of pages that holds key j (BULK: key j and the 15 behind it); -1: none of it is seen
         auto row_of = [&](int j) {
             int row = -1;
-            if (j >= see_lo && j <= see_hi) {
+            if (j + (BULK ? 15 : 0) >= see_lo && j <= see_hi) {
                 const int slot = p.page_shift >= 0 ? j >> p.page_shift : j / p.page_size;
                 const int page = table[slot];
                 if (page >= 0 && page < p.n_pages) row = (page * p.n_kv + g) * p.page_size + (j - slot * p.page_size);
@@ -245,32 +269,37 @@ __global__ void __launch_bounds__(THREADS) attn_quant_kernel(const Params p) {
             }
             return row;
         };
-        const int j_first = (en.first_step + from) * STEP + warp * WARP_KEYS;
         auto fetch = [&](int stage, int row) {
-            const uint32_t to = my_s + stage * S::WARP_STAGE;
-            constexpr int ROWS = 32 / S::CHUNKS;               // rows of a pass
-            const int c = lane % S::CHUNKS;
+            if constexpr (BULK) {
+                const unsigned tiles = __ballot_sync(0xffffffffu, row >= 0) & 0x11u;
+                if (lane == 0) expect(&full[warp][stage], __popc(tiles) * (32 * (RB + SB)));
+                __syncwarp();
+                if (lane < 8 && row >= 0) bulk_copy(b_to + stage * S::WARP_STAGE, b_from + (size_t)row * b_bytes, 16 * b_bytes, &full[warp][stage]);
+            } else {
+                const uint32_t to = my_s + stage * S::WARP_STAGE;
+                constexpr int ROWS = 32 / S::CHUNKS;               // rows of a pass
+                const int c = lane % S::CHUNKS;
 #pragma unroll
-            for (int i = 0; i < S::CHUNKS; ++i) {
-                const int key = i * ROWS + lane / S::CHUNKS, src = __shfl_sync(0xffffffffu, row, key);
-                const size_t off = (size_t)max(src, 0) * RB + c * 16;
-                const int pr = (key & 16) + product_row(key & 15), kept = src >= 0 ? 16 : 0;
-                cp_async16(to + pr * RB + k_chunk<RB>(pr, c) * 16, p.k_codes + off, kept);
-                cp_async16(to + V_AT + key * RB + v_chunk<RB>(key, c) * 16, p.v_codes + off, kept);
+                for (int i = 0; i < S::CHUNKS; ++i) {
+                    const int key = i * ROWS + lane / S::CHUNKS, src = __shfl_sync(0xffffffffu, row, key);
+                    const size_t off = (size_t)max(src, 0) * RB + c * 16;
+                    cp_async16(to + key * RB + c * 16, p.k_codes + off, src >= 0 ? 16 : 0);
+                    cp_async16(to + V_AT + key * RB + c * 16, p.v_codes + off, src >= 0 ? 16 : 0);
+                }
+                const size_t off = (size_t)max(row, 0) * SB;
+                cp_async_row(to + KS_AT + lane * SB, p.k_scales + off, SB, row >= 0 ? SB : 0);
+                cp_async_row(to + VS_AT + lane * SB, p.v_scales + off, SB, row >= 0 ? SB : 0);
             }
-            const int pr = (lane & 16) + product_row(lane & 15);
-            const size_t off = (size_t)max(row, 0) * SB;
-            cp_async_row(to + KS_AT + pr * SB, p.k_scales + off, SB, row >= 0 ? SB : 0);
-            cp_async_row(to + VS_AT + pr * SB, p.v_scales + off, SB, row >= 0 ? SB : 0);
         };
-        int ahead = row_of(j_first + lane);
+        const int j_mine = j_first + (BULK ? (lane & 4) * 4 : lane);     // the key whose row this lane looks up
+        int ahead = row_of(j_mine);
 #pragma unroll
-        for (int s = 0; s < S::STAGES - 1; ++s) {
-            if (s < n) {
-                fetch(s, ahead);
-                ahead = s + 1 < n ? row_of(j_first + (s + 1) * STEP + lane) : -1;
+        for (int s = 0; s < STAGES - 1; ++s) {
+            if (s < n && !failed) {
+                fetch((stage + s) % STAGES, ahead);
+                ahead = s + 1 < n ? row_of(j_mine + (s + 1) * STEP) : -1;
             }
-            cp_async_commit();
+            if constexpr (!BULK) cp_async_commit();
         }
 
         // -- queries as operands, and what the offset of their codes comes to
@@ -318,45 +347,60 @@ __global__ void __launch_bounds__(THREADS) attn_quant_kernel(const Params p) {
             l[nt][0] = l[nt][1] = 0.f;
         }
 
-        for (int i = 0, stage = 0; i < n; ++i) {
+        // (the ring goes on where the last piece left it: its barriers' phases do)
+        for (int i = 0; i < n && !failed; ++i) {
             {
-                const int s = i + S::STAGES - 1;
+                const int s = i + STAGES - 1;
                 if (s < n) {
-                    fetch(stage == 0 ? S::STAGES - 1 : stage - 1, ahead);
-                    ahead = s + 1 < n ? row_of(j_first + (s + 1) * STEP + lane) : -1;
+                    fetch(stage == 0 ? STAGES - 1 : stage - 1, ahead);
+                    ahead = s + 1 < n ? row_of(j_mine + (s + 1) * STEP) : -1;
                 }
-                cp_async_commit();
-                cp_async_wait<S::STAGES - 1>();
-                __syncwarp();
+                if constexpr (BULK) {
+                    const bool here = kipp_mbar_wait_limited(&full[warp][stage], (parity >> stage) & 1u, &gave_up, KIPP_WAIT_LIMIT_CYCLES);
+                    if (!__all_sync(0xffffffffu, here)) {
+                        // gave up: nothing more is asked for, and what was is waited for, within the limit
+                        failed = true;
+                        int alone = 0;
+                        for (int k = 0, q = stage; k < STAGES && i + k < n; ++k, q = q + 1 == STAGES ? 0 : q + 1)
+                            kipp_mbar_wait_limited(&full[warp][q], (parity >> q) & 1u, &alone, KIPP_WAIT_LIMIT_CYCLES);
+                        break;
+                    }
+                    parity ^= 1u << stage;
+                } else {
+                    cp_async_commit();
+                    cp_async_wait<STAGES - 1>();
+                    __syncwarp();
+                }
             }
-            const uint8_t* tile = my + stage * S::WARP_STAGE;
+            uint8_t* const tile = my + stage * S::WARP_STAGE;
             const int j0 = j_first + i * STEP;
             // (the warps of a step may all be outside what is seen, but for one)
             if (j0 <= see_hi && j0 + WARP_KEYS > see_lo) {
+                const bool cut = j0 + WARP_KEYS - 1 > all_hi || j0 < all_lo;
+                if (cut) {
+                    // rows that no column sees may hold anything: their scales become 0 (their codes are numbers anyhow)
+                    const int j = j0 + lane;
+                    if (j > see_hi || j < see_lo) {
+#pragma unroll
+                        for (int k = 0; k < SB / 4; ++k) {
+                            *reinterpret_cast<uint32_t*>(tile + KS_AT + lane * SB + 4 * k) = 0u;
+                            *reinterpret_cast<uint32_t*>(tile + VS_AT + lane * SB + 4 * k) = 0u;
+                        }
+                        if constexpr (BULK) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                    __syncwarp();
+                }
                 // -- scores, in units of log2
                 float s[NT][2][4];
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt) {
                     uint32_t w0[S::K_BYTES / 4], w1[S::K_BYTES / 4];
-                    const int r0 = mt * 16 + g4, r1 = r0 + 8;
-                    if constexpr (S::K_BYTES <= 16) {
-                        take<S::K_BYTES>(w0, tile + r0 * RB + t4 * S::K_BYTES);
-                        take<S::K_BYTES>(w1, tile + r1 * RB + t4 * S::K_BYTES);
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < S::K_BYTES / 16; ++c) {
-                            uint32_t v[4];
-                            take<16>(v, tile + r0 * RB + k_chunk<RB>(r0, t4 * (S::K_BYTES / 16) + c) * 16);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) w0[4 * c + k] = v[k];
-                            take<16>(v, tile + r1 * RB + k_chunk<RB>(r1, t4 * (S::K_BYTES / 16) + c) * 16);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) w1[4 * c + k] = v[k];
-                        }
-                    }
-                    uint32_t a0[(SB + 3) / 4], a1[(SB + 3) / 4];
-                    take<SB>(a0, tile + KS_AT + r0 * SB);
-                    take<SB>(a1, tile + KS_AT + r1 * SB);
+                    const uint8_t* r0 = tile + (mt * 16 + key_of_row(g4)) * RB + t4 * S::K_BYTES;
+                    take<S::K_BYTES>(w0, r0);
+                    take<S::K_BYTES>(w1, r0 + 8 * RB);
+                    uint32_t a0[SB / 4], a1[SB / 4];
+                    take<SB>(a0, tile + KS_AT + (mt * 16 + key_of_row(g4)) * SB);
+                    take<SB>(a1, tile + KS_AT + (mt * 16 + key_of_row(g4) + 8) * SB);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.f;
 #pragma unroll
@@ -383,7 +427,6 @@ __global__ void __launch_bounds__(THREADS) attn_quant_kernel(const Params p) {
                         }
                     }
                 }
-                const bool cut = j0 + WARP_KEYS - 1 > all_hi || j0 < all_lo;
                 bool raise = false;
                 float top[NT][2];
 #pragma unroll
@@ -391,13 +434,21 @@ __global__ void __launch_bounds__(THREADS) attn_quant_kernel(const Params p) {
 #pragma unroll
                     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            s[nt][mt][k] *= p.score_scale;
-                            if (cut) {
-                                const int j = j0 + mt * 16 + key_of_row(g4 + (k >> 1) * 8);
-                                if (j > col_hi[nt][k & 1] || j < col_lo[nt][k & 1]) s[nt][mt][k] = -INFINITY;
-                            }
+                        for (int k = 0; k < 4; ++k) s[nt][mt][k] *= p.score_scale;
+                    if (cut) {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int pos = en.context + min(column0 + nt * 8 + 2 * t4 + c, columns - 1) / group;
+                            const int hi = min(pos, see_hi), lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+#pragma unroll
+                            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const int j = j0 + mt * 16 + key_of_row(g4) + h * 8;
+                                    if (j > hi || j < lo) s[nt][mt][2 * h + c] = -INFINITY;
+                                }
                         }
+                    }
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         top[nt][c] = fmaxf(fmaxf(s[nt][0][c], s[nt][0][2 + c]), fmaxf(s[nt][1][c], s[nt][1][2 + c]));
@@ -443,26 +494,12 @@ __global__ void __launch_bounds__(THREADS) attn_quant_kernel(const Params p) {
                     }
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt) {
-                    uint32_t a0[(SB + 3) / 4], a1[(SB + 3) / 4];
-                    take<SB>(a0, tile + VS_AT + (mt * 16 + g4) * SB);
-                    take<SB>(a1, tile + VS_AT + (mt * 16 + g4 + 8) * SB);
+                    uint32_t a0[SB / 4], a1[SB / 4];
+                    take<SB>(a0, tile + VS_AT + (mt * 16 + key_of_row(g4)) * SB);
+                    take<SB>(a1, tile + VS_AT + (mt * 16 + key_of_row(g4) + 8) * SB);
                     uint32_t v[4][S::V_BYTES / 4];                     // keys t, 4 + t, 8 + t, 12 + t
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int key = mt * 16 + 4 * k + t4;
-                        if constexpr (S::V_BYTES <= 16) {
-                            constexpr int PER = 16 / S::V_BYTES;        // stretches of a chunk
-                            take<S::V_BYTES>(v[k], tile + V_AT + key * RB + v_chunk<RB>(key, g4 / PER) * 16 + (g4 % PER) * S::V_BYTES);
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < S::V_BYTES / 16; ++c) {
-                                uint32_t u[4];
-                                take<16>(u, tile + V_AT + key * RB + v_chunk<RB>(key, g4 * (S::V_BYTES / 16) + c) * 16);
-#pragma unroll
-                                for (int b = 0; b < 4; ++b) v[k][4 * c + b] = u[b];
-                            }
-                        }
-                    }
+                    for (int k = 0; k < 4; ++k) take<S::V_BYTES>(v[k], tile + V_AT + (mt * 16 + 4 * k + t4) * RB + g4 * S::V_BYTES);
 #pragma unroll
                     for (int gi = 0; gi < G; ++gi) {
                         uint32_t x0[4], x1[4];                         // keys of the first and the second half of the rows
@@ -484,9 +521,9 @@ __global__ void __launch_bounds__(THREADS) attn_quant_kernel(const Params p) {
                 }
             }
             __syncwarp();
-            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
         }
-        cp_async_wait<0>();
+        if constexpr (!BULK) cp_async_wait<0>();
 
         // -- the four warps' parts together, through shared memory
         __syncthreads();
@@ -528,6 +565,11 @@ __global__ void __launch_bounds__(THREADS) attn_quant_kernel(const Params p) {
         const bool whole = n == en.n_steps;
         const int slot = 2 * blockIdx.x + (x == run_first ? 0 : 1);
         const int live = min(COLS, columns - column0);
+        if (threadIdx.x == 0 && from == 0 && (p.by_row || !whole)) {
+            const int parts = whole ? 0 : cta_of_step(total, ctas, x + en.n_steps - 1) - (int)blockIdx.x + 1;
+            p.shared_rows[p.by_row ? entry * p.most_blocks + block : blockIdx.x] =
+                make_int4(entry, g, 2 * column0 + (x == run_first ? 0 : 1), (int)blockIdx.x << 16 | parts);
+        }
         for (int i = threadIdx.x; i < live * D; i += THREADS) {
             const int col = i / D, d = i % D;
             float mx = -INFINITY;
@@ -551,62 +593,58 @@ __global__ void __launch_bounds__(THREADS) attn_quant_kernel(const Params p) {
                 }
             }
         }
+        if constexpr (BULK) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // (the ring takes copies again)
         __syncthreads();
         x += n;
         at += n;
     }
+    if (BULK && threadIdx.x == 0 && gave_up) atomicExch(p.status + 1, 1);
 }
 
-// Adds the parts of one head of one token, in the order of the keys: MERGE_THREADS / D threads an element, each
-// a share of the parts.
-template <int D, int NT>
-__global__ void __launch_bounds__(MERGE_THREADS) attn_quant_merge_kernel(const Params p) {
-    constexpr int COLS = 8 * NT, SHARES = MERGE_THREADS / D;
-    __shared__ int scan[MERGE_THREADS / 32];
-    __shared__ float sh_o[SHARES][D], sh_l[SHARES];
-    __shared__ float sh_m[MERGE_THREADS / 32];
-    const int e = blockIdx.y, tok = blockIdx.x / p.n_q, head = blockIdx.x - tok * p.n_q;
-    const Entry en = entry_of<COLS>(p, e);
-    if (en.blocks == 0 || tok >= en.q_len) { pdl_wait(); return; }
-    int total = 0, start = 0;
-    for (int base = 0; base < p.entries; base += MERGE_THREADS) {
-        const int i = base + threadIdx.x, steps = i < p.entries ? entry_of<COLS>(p, i).steps() : 0;
-        int before;
-        total += block_scan<MERGE_THREADS>(steps, before, scan);
-        start += block_scan<MERGE_THREADS>(i < e ? steps : 0, before, scan);
+// Adds the parts of one head of one token of a row that CTAs shared, in the order of the keys: SHARES threads an
+// element, each with a run of the parts.
+template <int D, int NT, int SHARES>
+__global__ void __launch_bounds__(D * SHARES) attn_quant_merge_kernel(const Params p) {
+    constexpr int COLS = 8 * NT, WARPS_M = D * SHARES / 32;
+    __shared__ float sh_o[SHARES][D], sh_l[SHARES], sh_m[WARPS_M];
+    if (p.by_row) {                                    // (only rows that exist have left word of themselves)
+        const int e = blockIdx.x / p.most_blocks;
+        if ((int)blockIdx.x - e * p.most_blocks >= entry_of<COLS>(p, e).blocks) { pdl_wait(); return; }
     }
-    const int group = p.n_q / p.n_kv, g = head / group, c = tok * group + head - g * group, col = c % COLS;
-    start += (g * en.column_blocks + c / COLS) * en.n_steps;
-    const int per = steps_per_cta(total, p.ctas), c0 = start / per, c1 = (start + en.n_steps - 1) / per, parts = c1 - c0 + 1;
     pdl_wait();
-    if (parts == 1) return;
-    auto slot = [&](int part) { return 2 * (c0 + part) + ((c0 + part) * (long long)per >= start ? 0 : 1); };
+    const int4 row = p.shared_rows[blockIdx.x];
+    const int parts = row.w & 0xffff, c0 = row.w >> 16, e = row.x, group = p.n_q / p.n_kv, c = (row.z >> 1) + blockIdx.y;
+    if (parts == 0) return;
+    const int qs = p.q_start[e];
+    if (c >= (p.q_start[e + 1] - qs) * group) return;
+    auto at = [&](int part) { return (size_t)(2 * (c0 + part) + (part == 0 ? row.z & 1 : 0)) * COLS + blockIdx.y; };
     float mx = -INFINITY;
-    for (int i = threadIdx.x; i < parts; i += MERGE_THREADS) mx = fmaxf(mx, p.part_ml[((size_t)slot(i) * COLS + col) * 2]);
+    for (int i = threadIdx.x; i < parts; i += D * SHARES) mx = fmaxf(mx, p.part_ml[at(i) * 2]);
     mx = warp_max(mx);
     if ((threadIdx.x & 31) == 0) sh_m[threadIdx.x >> 5] = mx;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < MERGE_THREADS / 32; ++w) mx = fmaxf(mx, sh_m[w]);
+    for (int w = 0; w < WARPS_M; ++w) mx = fmaxf(mx, sh_m[w]);
     const int d = threadIdx.x % D, share = threadIdx.x / D;
     const int many = (parts + SHARES - 1) / SHARES, end = min(parts, (share + 1) * many);
     float acc = 0.f, sum = 0.f;
 #pragma unroll 8
     for (int i = share * many; i < end; ++i) {
-        const size_t at = (size_t)slot(i) * COLS + col;
-        const float pm = p.part_ml[at * 2], f = pm == -INFINITY ? 0.f : exp2_fast(pm - mx);
-        sum += p.part_ml[at * 2 + 1] * f;
-        acc += p.part_o[at * D + d] * f;
+        const float pm = p.part_ml[at(i) * 2], f = pm == -INFINITY ? 0.f : exp2_fast(pm - mx);
+        sum += p.part_ml[at(i) * 2 + 1] * f;
+        acc += p.part_o[at(i) * D + d] * f;
     }
-    sh_o[share][d] = acc;
-    if (d == 0) sh_l[share] = sum;
-    __syncthreads();
-    if (share == 0) {
+    if constexpr (SHARES > 1) {
+        sh_o[share][d] = acc;
+        if (d == 0) sh_l[share] = sum;
+        __syncthreads();
+        if (share != 0) return;
         acc = sum = 0.f;
 #pragma unroll
         for (int i = 0; i < SHARES; ++i) { acc += sh_o[i][d]; sum += sh_l[i]; }
-        p.out[((size_t)(p.q_start[e] + tok) * p.n_q + head) * D + d] = __float2bfloat16_rn(sum > 0.f ? acc / sum : 0.f);
     }
+    const int tok = c / group;
+    p.out[((size_t)(qs + tok) * p.n_q + row.y * group + (c - tok * group)) * D + d] = __float2bfloat16_rn(sum > 0.f ? acc / sum : 0.f);
 }
 
 template <int D, int BITS, int NT> constexpr size_t smem_bytes() {
@@ -615,26 +653,35 @@ template <int D, int BITS, int NT> constexpr size_t smem_bytes() {
     return ring > merge ? ring : merge;
 }
 // CTAs of one wave.
-template <int D, int BITS, int NT> int wave() {
+template <int D, int BITS, int NT, bool BULK> int wave() {
     static const int ctas = [] {
         int per = 0;
         const size_t smem = smem_bytes<D, BITS, NT>();
-        if (kipp_allow_smem(attn_quant_kernel<D, BITS, NT>, smem) != 0 ||
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attn_quant_kernel<D, BITS, NT>, THREADS, smem) != cudaSuccess || per < 1) {
+        if (kipp_allow_smem(attn_quant_kernel<D, BITS, NT, BULK>, smem) != 0 ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attn_quant_kernel<D, BITS, NT, BULK>, THREADS, smem) != cudaSuccess || per < 1) {
             cudaGetLastError();
             per = 1;
         }
-        return per * kipp_sm_count();
+        const int all = per * kipp_sm_count();
+        return all < MOST_CTAS ? all : MOST_CTAS;
     }();
     return ctas;
 }
-template <int D, int BITS, int NT> int launch(Params p, long long most_steps, cudaStream_t s) {
+template <int D, int BITS, int NT, bool BULK> int launch(Params p, long long steps_of_row, cudaStream_t s) {
     constexpr size_t smem = smem_bytes<D, BITS, NT>();
-    const int most_ctas = wave<D, BITS, NT>() < MOST_CTAS ? wave<D, BITS, NT>() : MOST_CTAS;
-    p.ctas = (int)(most_steps < most_ctas ? most_steps : most_ctas);
-    if (const int e = kipp_allow_smem(attn_quant_kernel<D, BITS, NT>, smem)) return e;
-    if (const int e = kipp_launch(attn_quant_kernel<D, BITS, NT>, dim3((unsigned)p.ctas), dim3(THREADS), smem, s, 1, p)) return e;
-    return kipp_launch(attn_quant_merge_kernel<D, NT>, dim3((unsigned)(p.n_q * p.most), (unsigned)p.entries), dim3(MERGE_THREADS), 0, s, 1, p);
+    constexpr int COLS = 8 * NT, FEW = D < 128 ? 128 / D : 1, MANY = 512 / D;
+    const int wave_ctas = wave<D, BITS, NT, BULK>();
+    const long long rows = (long long)p.entries * p.most_blocks, steps = rows * steps_of_row;
+    p.ctas = (int)(steps < wave_ctas ? steps : wave_ctas);
+    p.by_row = rows <= p.ctas ? 1 : 0;
+    if (const int e = kipp_allow_smem(attn_quant_kernel<D, BITS, NT, BULK>, smem)) return e;
+    if (const int e = kipp_launch(attn_quant_kernel<D, BITS, NT, BULK>, dim3((unsigned)p.ctas), dim3(THREADS), smem, s, 1, p)) return e;
+    if (steps_of_row <= 1) return 0;                   // every row is one step: none is shared
+    const int columns = p.most * (p.n_q / p.n_kv);
+    const dim3 grid((unsigned)(p.by_row ? rows : p.ctas), (unsigned)(columns < COLS ? columns : COLS));
+    // (a row of few is cut into many parts)
+    if (rows * 8 <= p.ctas) return kipp_launch(attn_quant_merge_kernel<D, NT, MANY>, grid, dim3(D * MANY), 0, s, 1, p);
+    return kipp_launch(attn_quant_merge_kernel<D, NT, FEW>, grid, dim3(D * FEW), 0, s, 1, p);
 }
 
 // 8 columns where they hold every query of a kv head, else 16 (heads of 256 have no room for their sums: always 8)
@@ -646,7 +693,9 @@ extern "C" int kipp_attn_quant_supported(int bits, int head_dim, int n_q, int n_
     return (bits == 4 || bits == 8) && (head_dim == 64 || head_dim == 128 || head_dim == 256) && n_kv > 0 && n_q > 0 && n_q % n_kv == 0;
 }
 // Bytes of scratch of a launch (the parts of rows that several CTAs share), whatever the step.
-extern "C" long long kipp_attn_quant_scratch_bytes(int head_dim) { return 2LL * MOST_CTAS * MOST_COLUMNS * (head_dim + 2) * 4; }
+extern "C" long long kipp_attn_quant_scratch_bytes(int head_dim) {
+    return 2LL * MOST_CTAS * MOST_COLUMNS * (head_dim + 2) * 4 + MOST_CTAS * 16LL;
+}
 
 // out, q: bf16 [tokens][n_q][head_dim].  The entries that bring 1 to `most` tokens; the others are left alone.
 extern "C" int kipp_attn_quant(void* out, const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
@@ -655,16 +704,16 @@ extern "C" int kipp_attn_quant(void* out, const void* q, const void* k_codes, co
                                float scale, int window, void* scratch, long long scratch_bytes, int* status, void* stream) {
     if (entries <= 0 || most <= 0) return 0;
     if (!kipp_attn_quant_supported(bits, head_dim, n_q, n_kv) || page_size <= 0 || n_pages <= 0 || table_width <= 0 || window < 0 ||
-        status == nullptr || scratch == nullptr || entries > 65535)
+        status == nullptr || scratch == nullptr)
         return KIPP_ERR_ARG;
     if (scratch_bytes < kipp_attn_quant_scratch_bytes(head_dim)) return -4;
     if ((((uintptr_t)q | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scales | (uintptr_t)v_scales | (uintptr_t)scratch) & 15) != 0) return -3;
-    // (row numbers of pages, steps of all rows and blocks of the second kernel are 32-bit)
+    // (row numbers of pages and steps of all rows are 32-bit)
     const long long cols = columns_of(head_dim, (long long)most * (n_q / n_kv));
     const long long room = (long long)table_width * page_size, steps = (room + STEP - 1) / STEP;
-    const long long rows = (long long)entries * n_kv * (((long long)most * (n_q / n_kv) + cols - 1) / cols);
-    if ((long long)n_pages * n_kv * page_size > 0x7fffffffLL || room > 0x7fffffffLL || rows > 0x3fffffffLL / steps ||
-        (long long)most * n_q > 0x7fffffffLL)
+    const long long blocks = n_kv * (((long long)most * (n_q / n_kv) + cols - 1) / cols);
+    if ((long long)n_pages * n_kv * page_size > 0x7fffffffLL || room > 0x7fffffffLL || blocks > 0x3fffffffLL / entries / steps ||
+        (long long)most * n_q > 0x3fffffffLL)
         return KIPP_ERR_ARG;
     Params p = {};
     p.out = (bf16*)out; p.q = (const bf16*)q;
@@ -678,13 +727,14 @@ extern "C" int kipp_attn_quant(void* out, const void* q, const void* k_codes, co
     p.score_scale = scale * 1.4426950408889634f * 0x1p73f;
     p.part_o = (float*)scratch;
     p.part_ml = p.part_o + 2LL * MOST_CTAS * MOST_COLUMNS * head_dim;
+    p.shared_rows = (int4*)(p.part_ml + 2LL * MOST_CTAS * MOST_COLUMNS * 2);
+    p.most_blocks = (int)blocks;
     p.status = status;
     cudaStream_t s = (cudaStream_t)stream;
-    const long long steps_at_most = rows * steps;
-#define KIPP_CASE(d, b)                                                                             \
-    if (head_dim == d && bits == b) {                                                               \
-        if (cols == 8) return launch<d, b, 1>(p, steps_at_most, s);                                 \
-        if constexpr (d != 256) return launch<d, b, 2>(p, steps_at_most, s);                        \
+#define KIPP_CASE(d, b)                                                                                            \
+    if (head_dim == d && bits == b) {                                                                              \
+        if (cols == 8) return page_size % 16 == 0 ? launch<d, b, 1, true>(p, steps, s) : launch<d, b, 1, false>(p, steps, s);        \
+        if constexpr (d != 256) return page_size % 16 == 0 ? launch<d, b, 2, true>(p, steps, s) : launch<d, b, 2, false>(p, steps, s); \
     }
     KIPP_CASE(64, 4) KIPP_CASE(64, 8) KIPP_CASE(128, 4) KIPP_CASE(128, 8) KIPP_CASE(256, 4) KIPP_CASE(256, 8)
 #undef KIPP_CASE

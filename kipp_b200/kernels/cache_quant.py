@@ -9,7 +9,7 @@ from typing import Optional
 
 import torch
 
-from .ops import KernelError, _check, _fn, _int32, _ptr, _stream, c_float, c_int, c_void_p, dtype_code, rope_table
+from .ops import KernelError, _check, _fn, _ptr, c_float, c_int, c_void_p, dtype_code, rope_table
 
 c_ll = ctypes.c_longlong
 READ_BYTES = 1 << 30          # most bytes of keys and values that attention reads back at a time
@@ -22,22 +22,27 @@ class QuantizedPages:
     def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor, bits: int):
         if bits not in (4, 8):
             raise KernelError(f"a quantised cache holds 8 or 4 bits, not {bits}")
-        for codes, scales in ((k_codes, k_scales), (v_codes, v_scales)):
-            if codes.dtype != torch.uint8 or scales.dtype != torch.bfloat16 or codes.dim() != 4 or scales.dim() != 4:
-                raise KernelError("QuantizedPages: codes are uint8 and scales bfloat16, [pages, n_kv, page_size, ..] each")
-            if not codes.is_contiguous() or not scales.is_contiguous() or codes.shape[:3] != scales.shape[:3] or \
-                    codes.device != scales.device:
-                raise KernelError("QuantizedPages: codes and scales must be contiguous, of the same pages and on one device")
-        if k_codes.shape != v_codes.shape or k_scales.shape != v_scales.shape or k_codes.device != v_codes.device:
-            raise KernelError("QuantizedPages: keys and values must be alike")
+        if k_codes.dtype != torch.uint8 or v_codes.dtype != torch.uint8 or k_scales.dtype != torch.bfloat16 or v_scales.dtype != torch.bfloat16:
+            raise KernelError("QuantizedPages: codes are uint8 and scales bfloat16")
+        shape, s_shape, device = k_codes.shape, k_scales.shape, k_codes.get_device()
+        if len(shape) != 4 or len(s_shape) != 4 or shape[:3] != s_shape[:3] or v_codes.shape != shape or v_scales.shape != s_shape:
+            raise KernelError("QuantizedPages: codes and scales are [pages, n_kv, page_size, ..], keys and values alike")
+        if not (k_codes.is_contiguous() and k_scales.is_contiguous() and v_codes.is_contiguous() and v_scales.is_contiguous()):
+            raise KernelError("QuantizedPages: codes and scales must be contiguous")
+        if k_scales.get_device() != device or v_codes.get_device() != device or v_scales.get_device() != device:
+            raise KernelError("QuantizedPages: codes and scales must be on one device")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales, self.bits = k_codes, k_scales, v_codes, v_scales, bits
-        self.n_pages, self.n_kv, self.page_size = k_codes.shape[:3]
-        self.head_dim = k_codes.shape[3] * 8 // bits
-        if self.head_dim % 32 or self.head_dim > 512 or self.head_dim == 0 or k_scales.shape[3] * 32 != self.head_dim:
-            raise KernelError(f"QuantizedPages: {self.head_dim} channels and {k_scales.shape[3]} scales a head; heads are a multiple of "
+        self.n_pages, self.n_kv, self.page_size, row = shape
+        self.head_dim = D = row * 8 // bits
+        if D % 32 or D > 512 or s_shape[3] * 32 != D:
+            raise KernelError(f"QuantizedPages: {D} channels and {s_shape[3]} scales a head; heads are a multiple of "
                               "32 channels, at most 512, with a scale for every 32")
-        if min(self.n_pages, self.n_kv, self.page_size) <= 0:
+        if min(shape) <= 0:
             raise KernelError("QuantizedPages: no pages")
+        self.device_index = device
+        # (what a launch is given: the tensors are held, so the addresses stay)
+        self.addresses = (k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr())
+        self.aligned = all(a % 16 == 0 for a in self.addresses)
 
     @classmethod
     def zeros(cls, n_pages: int, n_kv: int, page_size: int, head_dim: int, bits: int, device) -> "QuantizedPages":
@@ -47,23 +52,38 @@ class QuantizedPages:
         scales = lambda: torch.zeros(n_pages, n_kv, page_size, head_dim // 32, dtype=torch.bfloat16, device=device)     # noqa: E731
         return cls(codes(), scales(), codes(), scales(), bits)
 
-    def pointers(self) -> tuple:
-        return _ptr(self.k_codes), _ptr(self.k_scales), _ptr(self.v_codes), _ptr(self.v_scales), self.bits, self.n_pages, self.page_size
 
-
-def _on(device: torch.device, what: str, *tensors: Optional[torch.Tensor]) -> None:
-    """Everything lies on the current device: a launch goes there, whatever the tensors' own."""
-    if device.type != "cuda":
+def _launch_stream(what: str, device: int, *tensors: torch.Tensor) -> int:
+    """The current stream; every tensor must lie on the current device, where a launch goes whatever the tensors' own."""
+    if device < 0:
         raise KernelError("kernels need CUDA tensors; there is no CPU path")
-    if any(t is not None and t.device != device for t in tensors):
-        raise KernelError(f"{what}: the tensors are on several devices")
-    if device.index != torch.cuda.current_device():
-        raise KernelError(f"{what}: the tensors are on {device} and the current device is cuda:{torch.cuda.current_device()}")
+    for t in tensors:
+        if t.get_device() != device:
+            raise KernelError(f"{what}: the tensors are on several devices")
+    if device != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: the tensors are on cuda:{device} and the current device is cuda:{torch._C._cuda_getDevice()}")
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _status(status: torch.Tensor, what: str) -> None:
     if status.dtype != torch.int32 or status.numel() < 4 or not status.is_contiguous():
         raise KernelError(f"{what}: status must be a contiguous int32 tensor of 4 words")
+
+
+def _lists(what: str, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise KernelError(f"{what}: {name} must be a contiguous int32 tensor")
+
+
+_PAGES = [c_void_p] * 4 + [c_int] * 3                     # addresses, bits, pages, page size
+_WRITE = [c_void_p, c_ll, c_void_p, *_PAGES, c_int, c_void_p, c_void_p, c_int, c_float, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+          c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]
+_READ = [c_void_p, c_void_p, c_int, *_PAGES, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]
+_READ_ENTRIES = [c_void_p, c_void_p, c_void_p, c_int, *_PAGES, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
+                 c_void_p, c_void_p]
+_ATTEND = [c_void_p, c_void_p, *_PAGES, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p,
+           c_ll, c_void_p, c_void_p]
 
 
 def qk_norm_rope_write_quantized(qkv: torch.Tensor, q_out: torch.Tensor, pages: QuantizedPages, q_norm_w: Optional[torch.Tensor],
@@ -75,40 +95,41 @@ def qk_norm_rope_write_quantized(qkv: torch.Tensor, q_out: torch.Tensor, pages: 
     ``block_table`` [entries, width].  ``cos_sin`` is the step's ``rope_table``; without it the table is made here.
     A position whose page is not mapped is not written: status word 0 becomes 2."""
     what, D, n_kv = "qk_norm_rope_write_quantized", pages.head_dim, pages.n_kv
-    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != (n_q + 2 * n_kv) * D or qkv.shape[0] < tokens:
+    shape, dtype, q_norm, k_norm, table, norm_dtype = qkv.shape, qkv.dtype, None, None, None, 0
+    if len(shape) != 2 or shape[1] != (n_q + 2 * n_kv) * D or shape[0] < tokens or qkv.stride(1) != 1:
         raise KernelError(f"{what}: qkv has the wrong shape")
-    if q_out.dtype != qkv.dtype or not q_out.is_contiguous() or q_out.numel() < tokens * n_q * D:
+    if q_out.dtype != dtype or not q_out.is_contiguous() or q_out.numel() < tokens * n_q * D:
         raise KernelError(f"{what}: q_out must be contiguous, of qkv's dtype and hold every query")
-    for t, name in ((positions, "positions"), (entry_of_token, "entry_of_token"), (block_table, "block_table")):
-        _int32(t, name)
+    _lists(what, positions=positions, entry_of_token=entry_of_token, block_table=block_table)
     if positions.numel() < tokens or entry_of_token.numel() < tokens or block_table.dim() != 2:
         raise KernelError(f"{what}: a position and an entry for every token, and a table [entries, width]")
-    norm_dtype = 0
     if (q_norm_w is None) != (k_norm_w is None):
         raise KernelError(f"{what}: q and k norm weights must come together")
+    stream = _launch_stream(what, qkv.get_device(), q_out, pages.k_codes, positions, entry_of_token, block_table, status)
     if q_norm_w is not None:
         if q_norm_w.dtype != k_norm_w.dtype or q_norm_w.numel() != D or k_norm_w.numel() != D or \
                 not (q_norm_w.is_contiguous() and k_norm_w.is_contiguous()):
             raise KernelError(f"{what}: norm weights must be contiguous, alike and of the head's size")
-        norm_dtype = dtype_code(q_norm_w.dtype)
+        norm_dtype, q_norm, k_norm = dtype_code(q_norm_w.dtype), _ptr(q_norm_w), _ptr(k_norm_w)
+        _launch_stream(what, pages.device_index, q_norm_w, k_norm_w)
     if rotary_dim < 0 or rotary_dim % 2 or rotary_dim > D:
         raise KernelError(f"{what}: rotary_dim must be even and at most the head's size")
     if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() * 2 != rotary_dim):
         raise KernelError(f"{what}: inv_freq must be float32 [rotary_dim / 2]")
-    if rotary_dim > 0 and cos_sin is None:
-        if inv_freq is None:
-            raise KernelError(f"{what}: a rotation needs cos_sin or inv_freq")
-        cos_sin = rope_table(positions, inv_freq, tokens)
-    if rotary_dim > 0 and (cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or cos_sin.numel() < tokens * rotary_dim):
-        raise KernelError(f"{what}: cos_sin must be contiguous float32 [tokens, rotary_dim / 2, 2]")
+    if rotary_dim > 0:
+        if cos_sin is None:
+            if inv_freq is None:
+                raise KernelError(f"{what}: a rotation needs cos_sin or inv_freq")
+            cos_sin = rope_table(positions, inv_freq, tokens)
+        if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or cos_sin.numel() < tokens * rotary_dim or \
+                cos_sin.get_device() != pages.device_index:
+            raise KernelError(f"{what}: cos_sin must be contiguous float32 [tokens, rotary_dim / 2, 2] on the step's device")
+        table = cos_sin.data_ptr()
     _status(status, what)
-    _on(qkv.device, what, q_out, pages.k_codes, q_norm_w, k_norm_w, positions, entry_of_token, block_table, cos_sin, status)
-    f = _fn("cache_quant", "kipp_quant_cache_write",
-            [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int,
-             c_float, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p])
-    _check(f(_ptr(qkv), qkv.stride(0), _ptr(q_out), *pages.pointers(), dtype_code(qkv.dtype), _ptr(q_norm_w), _ptr(k_norm_w), norm_dtype,
-             float(eps), _ptr(cos_sin) if rotary_dim else None, rotary_dim, _ptr(positions), _ptr(entry_of_token), _ptr(block_table),
-             block_table.shape[1], tokens, n_q, n_kv, D, 1 if write_cache else 0, _ptr(status), _stream()), what)
+    f = _fn("cache_quant", "kipp_quant_cache_write", _WRITE)
+    _check(f(qkv.data_ptr(), qkv.stride(0), q_out.data_ptr(), *pages.addresses, pages.bits, pages.n_pages, pages.page_size, dtype_code(dtype),
+             q_norm, k_norm, norm_dtype, eps, table, rotary_dim, positions.data_ptr(), entry_of_token.data_ptr(), block_table.data_ptr(),
+             block_table.shape[1], tokens, n_q, n_kv, D, 1 if write_cache else 0, status.data_ptr(), stream), what)
 
 
 def read_quantized_pages(k_out: torch.Tensor, v_out: torch.Tensor, pages: QuantizedPages, page_list: torch.Tensor,
@@ -117,31 +138,27 @@ def read_quantized_pages(k_out: torch.Tensor, v_out: torch.Tensor, pages: Quanti
     ``k_out``, ``v_out`` [len(page_list), n_kv, page_size, D].  A negative number gives zeros, one past the
     pool zeros and status word 0 = 3."""
     what, n = "read_quantized_pages", page_list.numel()
-    _int32(page_list, "page_list")
+    _lists(what, page_list=page_list)
     shape = (n, pages.n_kv, pages.page_size, pages.head_dim)
-    if tuple(k_out.shape) != shape or tuple(v_out.shape) != shape or k_out.dtype != v_out.dtype or \
-            not (k_out.is_contiguous() and v_out.is_contiguous()):
+    if k_out.shape != shape or v_out.shape != shape or k_out.dtype != v_out.dtype or not (k_out.is_contiguous() and v_out.is_contiguous()):
         raise KernelError(f"{what}: k_out and v_out must be contiguous, of one dtype and {shape}")
     _status(status, what)
-    _on(pages.k_codes.device, what, k_out, v_out, page_list, status)
-    f = _fn("cache_quant", "kipp_quant_cache_read",
-            [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_int, c_int,
-             c_void_p, c_void_p])
-    _check(f(_ptr(k_out), _ptr(v_out), dtype_code(k_out.dtype), *pages.pointers(), _ptr(page_list), n, pages.n_kv, pages.head_dim,
-             _ptr(status), _stream()), what)
+    stream = _launch_stream(what, pages.device_index, k_out, v_out, page_list, status)
+    f = _fn("cache_quant", "kipp_quant_cache_read", _READ)
+    _check(f(k_out.data_ptr(), v_out.data_ptr(), dtype_code(k_out.dtype), *pages.addresses, pages.bits, pages.n_pages, pages.page_size,
+             page_list.data_ptr(), n, pages.n_kv, pages.head_dim, status.data_ptr(), stream), what)
 
 
 def _read_entries(pages: QuantizedPages, dtype: torch.dtype, meta, block_table: torch.Tensor, first: int, entries: int, window: int,
-                  status: torch.Tensor, table: torch.Tensor):
+                  status: torch.Tensor, table: torch.Tensor, stream: int):
     """Pages of what ``entries`` entries from ``first`` on see, in ``dtype``, and their rows of ``table``."""
-    shape = (entries * block_table.shape[1], pages.n_kv, pages.page_size, pages.head_dim)
-    k, v = (torch.empty(shape, dtype=dtype, device=table.device) for _ in range(2))
-    f = _fn("cache_quant", "kipp_quant_cache_read_entries",
-            [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
-             c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p])
-    _check(f(_ptr(k), _ptr(v), _ptr(table), dtype_code(dtype), *pages.pointers(), _ptr(meta.q_start), _ptr(meta.context_len),
-             _ptr(block_table), block_table.shape[1], first, entries, window, pages.n_kv, pages.head_dim, _ptr(status), _stream()),
-           "read_entries")
+    width = block_table.shape[1]
+    k = torch.empty((entries * width, pages.n_kv, pages.page_size, pages.head_dim), dtype=dtype, device=table.device)
+    v = torch.empty_like(k)
+    f = _fn("cache_quant", "kipp_quant_cache_read_entries", _READ_ENTRIES)
+    _check(f(k.data_ptr(), v.data_ptr(), table.data_ptr(), dtype_code(dtype), *pages.addresses, pages.bits, pages.n_pages, pages.page_size,
+             meta.q_start.data_ptr(), meta.context_len.data_ptr(), block_table.data_ptr(), width, first, entries, window, pages.n_kv,
+             pages.head_dim, status.data_ptr(), stream), "read_entries")
     return k, v
 
 
@@ -154,10 +171,15 @@ def _entries_at_once(pages: QuantizedPages, dtype: torch.dtype, width: int) -> i
 PORTION_MIN = 64              # an entry of as many tokens is read back for the prompt kernel of 128-token tiles
 
 
+_supported: dict = {}
+_scratch_bytes: dict = {}
+
+
 def _direct_ok(q: torch.Tensor, pages: QuantizedPages, n_q: int) -> bool:
-    f = _fn("attention_quant", "kipp_attn_quant_supported", [c_int, c_int, c_int, c_int])
-    return (q.dtype == torch.bfloat16 and bool(f(pages.bits, pages.head_dim, n_q, pages.n_kv))
-            and all(t.data_ptr() % 16 == 0 for t in (q, pages.k_codes, pages.v_codes, pages.k_scales, pages.v_scales)))
+    key = (pages.bits, pages.head_dim, n_q, pages.n_kv)
+    if key not in _supported:
+        _supported[key] = bool(_fn("attention_quant", "kipp_attn_quant_supported", [c_int] * 4)(*key))
+    return q.dtype == torch.bfloat16 and _supported[key] and pages.aligned and q.data_ptr() % 16 == 0
 
 
 def _plan(out, q, pages, meta, block_table, n_q):
@@ -166,9 +188,9 @@ def _plan(out, q, pages, meta, block_table, n_q):
     The prompt kernel reads a key and a value once for 128 tokens, the kernel over codes once for 8 or 16 columns."""
     if not _direct_ok(q, pages, n_q):
         return "read", "read", None
-    several = [e for e, n in enumerate(meta.q_lens) if n > 1]
-    if several and max(meta.q_lens) >= PORTION_MIN and getattr(meta, "prefill_work128", None) is not None:
+    if max(meta.q_lens) >= PORTION_MIN and getattr(meta, "prefill_work128", None) is not None:
         from . import attention_bf16
+        several = [e for e, n in enumerate(meta.q_lens) if n > 1]
         span = (several[0], several[-1] + 1)
         if attention_bf16.prefill_tc_supported(pages.head_dim, n_q, pages.n_kv, pages.page_size) and out.data_ptr() % 16 == 0 and \
                 span[1] - span[0] <= _entries_at_once(pages, q.dtype, block_table.shape[1]):
@@ -185,62 +207,72 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
     ``prefill_work128`` and ``n_prefill_items128``).  bfloat16 with heads of 64, 128 or 256 runs on the codes themselves; longer
     portions of prompts, other heads and float32 on pages that are read back.  ``impl`` forces a form for the whole step:
     "direct" or "read"."""
-    what, D, n_kv, window = "attention_quantized", pages.head_dim, pages.n_kv, int(window or 0)
+    what, D, n_kv, q_lens, tokens = "attention_quantized", pages.head_dim, pages.n_kv, meta.q_lens, meta.tokens
+    window = int(window or 0)
     dtype_code(q.dtype)
-    if q.dim() != 3 or tuple(q.shape[1:]) != (n_q, D) or q.shape[0] < meta.tokens or not q.is_contiguous() or n_q % n_kv:
+    shape, entries = q.shape, len(q_lens)
+    if len(shape) != 3 or shape[1] != n_q or shape[2] != D or shape[0] < tokens or n_q % n_kv or not q.is_contiguous():
         raise KernelError(f"{what}: q must be contiguous [tokens, n_q, head_dim] with n_q a multiple of the cache's heads")
-    if out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous():
+    if out.dtype != q.dtype or out.shape != shape or not out.is_contiguous():
         raise KernelError(f"{what}: out must be contiguous, of q's dtype and shape")
     if window < 0:
         raise KernelError(f"{what}: a window must not be negative")
-    if block_table.dim() != 2 or block_table.shape[0] < len(meta.q_lens) or block_table.shape[1] == 0 or sum(meta.q_lens) != meta.tokens:
+    t_shape = block_table.shape
+    if len(t_shape) != 2 or t_shape[0] < entries or t_shape[1] == 0 or sum(q_lens) != tokens:
         raise KernelError(f"{what}: a row of block_table for every entry, and as many tokens as the entries bring")
-    for t, name in ((block_table, "block_table"), (meta.positions, "positions"), (meta.entry_of_token, "entry_of_token"),
-                    (meta.q_start, "q_start"), (meta.context_len, "context_len")):
-        _int32(t, name)
-    if meta.q_start.numel() <= len(meta.q_lens) or meta.context_len.numel() < len(meta.q_lens) or \
-            min(meta.positions.numel(), meta.entry_of_token.numel()) < meta.tokens:
+    _lists(what, block_table=block_table, q_start=meta.q_start, context_len=meta.context_len)
+    if meta.q_start.numel() <= entries or meta.context_len.numel() < entries:
         raise KernelError(f"{what}: the step's lists are shorter than the step")
     _status(status, what)
-    _on(q.device, what, out, pages.k_codes, block_table, meta.q_start, meta.context_len, meta.positions, meta.entry_of_token, status)
-    if impl not in (None, "direct", "read"):
+    stream = _launch_stream(what, pages.device_index, q, out, block_table, meta.q_start, meta.context_len, status)
+    if tokens == 0:
+        return
+    if impl is None:
+        single, several, span = _plan(out, q, pages, meta, block_table, n_q)
+    elif impl in ("direct", "read"):
+        single, several, span = impl, impl, None
+        if impl == "direct" and not _direct_ok(q, pages, n_q):
+            raise KernelError(f"{what}: the kernel over codes takes bfloat16 heads of 64, 128 or 256, 16-byte aligned")
+    else:
         raise KernelError(f"unknown attention implementation {impl!r}")
-    if impl == "direct" and not _direct_ok(q, pages, n_q):
-        raise KernelError(f"{what}: the kernel over codes takes bfloat16 heads of 64, 128 or 256, 16-byte aligned")
-    if meta.tokens == 0:
-        return
-    single, several, span = _plan(out, q, pages, meta, block_table, n_q) if impl is None else (impl, impl, None)
     if single == "read":
-        _by_reading(out, q, pages, meta, block_table, n_q, scale, window, status)
+        _by_reading(out, q, pages, meta, block_table, n_q, scale, window, status, stream)
         return
-    if several == "direct" or 1 in meta.q_lens:
-        _direct(out, q, pages, meta, block_table, n_q, scale, window, status, max(meta.q_lens) if several == "direct" else 1)
-    if several == "portion":
-        _portions(out, q, pages, meta, block_table, n_q, scale, window, status, span)
+    if several == "direct":
+        _direct(out, q, pages, meta, block_table, n_q, scale, window, status, max(q_lens), stream)
+        return
+    if 1 in q_lens:
+        _direct(out, q, pages, meta, block_table, n_q, scale, window, status, 1, stream)
+    _portions(out, q, pages, meta, block_table, n_q, scale, window, status, span, stream)
 
 
-def _direct(out, q, pages, meta, block_table, n_q, scale, window, status, most: int) -> None:
+def _direct(out, q, pages, meta, block_table, n_q, scale, window, status, most: int, stream: int) -> None:
     """The entries of up to ``most`` tokens, over the codes."""
-    need = _fn("attention_quant", "kipp_attn_quant_scratch_bytes", [c_int], restype=c_ll)(pages.head_dim)
+    D = pages.head_dim
+    need = _scratch_bytes.get(D)
+    if need is None:
+        need = _scratch_bytes[D] = _fn("attention_quant", "kipp_attn_quant_scratch_bytes", [c_int], restype=c_ll)(D)
     scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
-    f = _fn("attention_quant", "kipp_attn_quant",
-            [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
-             c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_ll, c_void_p, c_void_p])
-    _check(f(_ptr(out), _ptr(q), *pages.pointers(), _ptr(meta.q_start), _ptr(meta.context_len), _ptr(block_table), block_table.shape[1],
-             len(meta.q_lens), most, n_q, pages.n_kv, pages.head_dim, float(scale), window, _ptr(scratch), need, _ptr(status), _stream()),
-           "attn_quant")
+    f = _fn("attention_quant", "kipp_attn_quant", _ATTEND)
+    _check(f(out.data_ptr(), q.data_ptr(), *pages.addresses, pages.bits, pages.n_pages, pages.page_size, meta.q_start.data_ptr(),
+             meta.context_len.data_ptr(), block_table.data_ptr(), block_table.shape[1], len(meta.q_lens), most, n_q, pages.n_kv, D, scale,
+             window, scratch.data_ptr(), need, status.data_ptr(), stream), "attn_quant")
 
 
-def _portions(out, q, pages, meta, block_table, n_q, scale, window, status, span) -> None:
+def _portions(out, q, pages, meta, block_table, n_q, scale, window, status, span, stream: int) -> None:
     """The entries of more than one token: their pages read back, and the prompt kernel over those."""
     table = torch.empty_like(block_table)
-    k, v = _read_entries(pages, q.dtype, meta, block_table, span[0], span[1] - span[0], window, status, table)
+    k, v = _read_entries(pages, q.dtype, meta, block_table, span[0], span[1] - span[0], window, status, table, stream)
     from . import attention_bf16
     attention_bf16.prefill_tc(out, q, k, v, meta, table, pages.page_size, n_q, pages.n_kv, pages.head_dim, scale, window, status)
 
 
-def _by_reading(out, q, pages, meta, block_table, n_q, scale, window, status) -> None:
+def _by_reading(out, q, pages, meta, block_table, n_q, scale, window, status, stream: int) -> None:
     """Every entry's pages read back, as many entries at a time as READ_BYTES allow, and the attention over them."""
+    _lists("attention_quantized", positions=meta.positions, entry_of_token=meta.entry_of_token)
+    if min(meta.positions.numel(), meta.entry_of_token.numel()) < meta.tokens:
+        raise KernelError("attention_quantized: the step's lists are shorter than the step")
+    _launch_stream("attention_quantized", pages.device_index, meta.positions, meta.entry_of_token)
     D, n_kv, width = pages.head_dim, pages.n_kv, block_table.shape[1]
     table = torch.empty_like(block_table)
     step, at = _entries_at_once(pages, q.dtype, width), 0
@@ -249,10 +281,10 @@ def _by_reading(out, q, pages, meta, block_table, n_q, scale, window, status) ->
         n = sum(lens)
         if n == 0:
             continue
-        k, v = _read_entries(pages, q.dtype, meta, block_table, first, len(lens), window, status, table)
+        k, v = _read_entries(pages, q.dtype, meta, block_table, first, len(lens), window, status, table, stream)
         f = _fn("attention_simt", "kipp_paged_attention_simt",
                 [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                  c_float, c_int, c_void_p, c_void_p])
         _check(f(_ptr(out[at:]), _ptr(q[at:]), _ptr(k), _ptr(v), dtype_code(q.dtype), _ptr(meta.positions[at:]), _ptr(meta.entry_of_token[at:]),
-                 _ptr(table), width, pages.page_size, n, n_q, n_kv, D, float(scale), window, _ptr(status), _stream()), "attention_simt")
+                 _ptr(table), width, pages.page_size, n, n_q, n_kv, D, float(scale), window, _ptr(status), stream), "attention_simt")
         at += n
