@@ -49,8 +49,8 @@ struct Params {
     bf16* out; const bf16* q;
     const uint8_t* k_codes; const uint8_t* k_scales; const uint8_t* v_codes; const uint8_t* v_scales;
     const int* q_start; const int* context_len; const int* block_table;
-    int entries, table_width, page_size, page_shift, n_pages, most, n_q, n_kv, window;
-    float score_scale;               // scale * log2(e) * 2^73
+    int entries, table_width, page_size, page_shift, n_pages, most, n_q, n_kv, group, window;
+    float score_scale, query_scale;  // |scale| * log2(e) * 2^73; 2^60 with the scale's sign
     float* part_o; float* part_ml;   // [2 ctas][columns][D], [2 ctas][columns][2]
     // rows that several CTAs share, by the row's number (by_row) or by the first CTA: (entry, kv head, 2 first column + the first
     // part's slot, first CTA << 16 | CTAs); 0 CTAs: nothing to add
@@ -74,46 +74,52 @@ template <int COLS> __device__ __forceinline__ Entry entry_of(const Params& p, i
     const int lo = p.window > 0 ? max(0, r.context - p.window + 1) : 0;
     r.first_step = min(lo, hi) / STEP;
     r.n_steps = hi / STEP - r.first_step + 1;
-    r.column_blocks = (r.q_len * (p.n_q / p.n_kv) + COLS - 1) / COLS;
+    r.column_blocks = (r.q_len * p.group + COLS - 1) / COLS;
     r.blocks = r.column_blocks * p.n_kv;
     return r;
 }
 
-// Sum of v over the block, and over the threads before this one.
-template <int N> __device__ __forceinline__ int block_scan(int v, int& before, int* scratch) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Sum of v over the warp, and over the lanes before this one.
+__device__ __forceinline__ int warp_scan(int v, int& before) {
     int x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+        if ((int)(threadIdx.x & 31) >= o) x += y;
     }
-    __syncthreads();
-    if (lane == 31) scratch[warp] = x;
-    __syncthreads();
-    int total = 0, ahead = 0;
-#pragma unroll
-    for (int w = 0; w < N / 32; ++w) {
-        if (w < warp) ahead += scratch[w];
-        total += scratch[w];
-    }
-    before = ahead + x - v;
-    return total;
+    before = x - v;
+    return __shfl_sync(0xffffffffu, x, 31);
 }
 
-// Runs differ by one step at most: CTA c has steps [total c / ctas, total (c + 1) / ctas).
-__device__ __forceinline__ int run_start(int total, int ctas, int c) { return (int)((long long)total * c / ctas); }
-__device__ __forceinline__ int cta_of_step(int total, int ctas, int x) { return (int)(((long long)(x + 1) * ctas - 1) / total); }
+// The cut: the first `more` CTAs have `per` + 1 steps, the others `per`.
+struct Cut {
+    int per, more;
+    Cut() = default;
+    __device__ __forceinline__ Cut(int total, int ctas) { per = total / ctas; more = total - per * ctas; }
+    __device__ __forceinline__ int start(int cta) const { return per * cta + min(cta, more); }
+    __device__ __forceinline__ int cta_of(int step) const {
+        const int first = more * (per + 1);
+        return step < first ? step / (per + 1) : more + (step - first) / per;
+    }
+};
 
+// d = a b + c
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0,
+                                    float c1, float c2, float c3) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    mma(c, a0, a1, a2, a3, b0, b1, c[0], c[1], c[2], c[3]);
+}
+__device__ __forceinline__ uint32_t times2(uint32_t a, uint32_t b) {                 // two bfloat16 products
+    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -163,6 +169,9 @@ template <int D, int BITS, int NT> constexpr int ctas_per_sm() {
 // r = 2 t + e + 8 h: a lane (g, t) then meets the values of keys t, 4 + t, 8 + t, 12 + t.
 __device__ __forceinline__ int key_of_row(int r) { return 4 * (r & 1) + ((r & 7) >> 1) + (r & 8); }
 
+// The steps of a CTA, and where the first of them is.
+struct Run { int first, end, entry, at; Cut cuts; };
+
 // Two runs of four codes as four operand registers: x[i] holds code i of the first run in its low half and of
 // the second in its high half.  4 bits: `first` and `second` are words, HALF which half of them the run is;
 // codes 1 and 3 count sixteenfold.  8 bits: a run is a word.
@@ -190,12 +199,15 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
     using S = Shape<D, BITS>;
     constexpr int G = S::G, RB = S::RB, SB = S::SB, COLS = 8 * NT, WO = D + 4, STAGES = S::STAGES;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int scan[WARPS + 2];
+    __shared__ Run run;
+    __shared__ uint4 q_operands[NT][G][32];                    // of a piece, by lane
+    __shared__ float2 q_offsets[NT][G][32];
+    __shared__ float part_f[WARPS][COLS];
     __shared__ uint64_t full[WARPS][STAGES];
     __shared__ int gave_up;
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, t4 = lane & 3;
-    const int group = p.n_q / p.n_kv;
+    const int group = p.group;
     if constexpr (BULK) {
         if (threadIdx.x < WARPS * STAGES)
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(kipp_smem_u32(&full[0][0] + threadIdx.x)) : "memory");
@@ -204,32 +216,29 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
     }
 
     // -- the run of this CTA: from the step's lists, which may be read before the wait
-    int total = 0;
-    for (int base = 0; base < p.entries; base += THREADS) {
-        const int e = base + threadIdx.x;
-        int before;
-        total += block_scan<THREADS>(e < p.entries ? entry_of<COLS>(p, e).steps() : 0, before, scan);
-    }
-    const int ctas = min(p.ctas, total);                   // (so that none between two others is empty)
-    const int run_first = (int)blockIdx.x < ctas ? run_start(total, ctas, blockIdx.x) : total;
-    const int run_end = (int)blockIdx.x < ctas ? run_start(total, ctas, blockIdx.x + 1) : total;
-    if (run_first >= run_end) {
-        pdl_wait();
-        if (!p.by_row && threadIdx.x == 0) p.shared_rows[blockIdx.x] = make_int4(0, 0, 0, 0);
-        return;
-    }
-    for (int base = 0, passed = 0; base < p.entries; base += THREADS) {
-        const int e = base + threadIdx.x, mine = e < p.entries ? entry_of<COLS>(p, e).steps() : 0;
-        int before;
-        const int sum = block_scan<THREADS>(mine, before, scan);
-        if (mine > 0 && passed + before <= run_first && run_first < passed + before + mine) { scan[WARPS] = e; scan[WARPS + 1] = passed + before; }
-        passed += sum;
-        if (run_first < passed) break;
+    if (warp == 0) {
+        int total = 0, before;
+        for (int base = 0; base < p.entries; base += 32) {
+            const int e = base + lane;
+            total += warp_scan(e < p.entries ? entry_of<COLS>(p, e).steps() : 0, before);
+        }
+        const int ctas = min(p.ctas, total);               // (so that none between two others is empty)
+        const Cut cuts(total, max(ctas, 1));
+        const int first = (int)blockIdx.x < ctas ? cuts.start(blockIdx.x) : total, end = (int)blockIdx.x < ctas ? cuts.start(blockIdx.x + 1) : total;
+        for (int base = 0, passed = 0; first < end && passed <= first; base += 32) {
+            const int e = base + lane, mine = e < p.entries ? entry_of<COLS>(p, e).steps() : 0;
+            const int sum = warp_scan(mine, before);
+            if (mine > 0 && passed + before <= first && first < passed + before + mine) { run.entry = e; run.at = first - passed - before; }
+            passed += sum;
+        }
+        if (lane == 0) { run.first = first; run.end = end; run.cuts = cuts; }
     }
     __syncthreads();
-    int entry = scan[WARPS], at = run_first - scan[WARPS + 1];
+    const int run_first = run.first, run_end = run.end;
+    int entry = run.entry, at = run.at;
     pdl_wait();
     if (!p.by_row && threadIdx.x == 0) p.shared_rows[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (run_first >= run_end) return;
 
     uint8_t* const my = smem + warp * (STAGES * S::WARP_STAGE);
     const uint32_t my_s = smem_address(my);
@@ -302,37 +311,43 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             if constexpr (!BULK) cp_async_commit();
         }
 
-        // -- queries as operands, and what the offset of their codes comes to
+        // -- queries as operands, and what the offset of their codes comes to: a warp makes every fourth group's
+        for (int k = warp; k < NT * G; k += WARPS) {
+            const int nt = k / G, gi = k % G, c = column0 + nt * 8 + g4;
+            uint2 a = make_uint2(0u, 0u), b = a;
+            if (c < columns) {
+                const int tok = c / group;
+                const bf16* src = p.q + ((size_t)(qs + tok) * p.n_q + g * group + (c - tok * group)) * D + t4 * (D / 4) + 4 * gi;
+                a = *reinterpret_cast<const uint2*>(src);
+                b = *reinterpret_cast<const uint2*>(src + 4 * G);
+            }
+            float sum = (low_f32(a.x) + high_f32(a.x)) + (low_f32(a.y) + high_f32(a.y)) + (low_f32(b.x) + high_f32(b.x)) + (low_f32(b.y) + high_f32(b.y));
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            sum *= -S::L * 0x1p-133f * p.query_scale;
+            q_offsets[nt][gi][lane] = make_float2(__shfl_sync(0xffffffffu, sum, 8 * t4), __shfl_sync(0xffffffffu, sum, 8 * t4 + 4));
+            const uint32_t raw[4] = {__byte_perm(a.x, b.x, 0x5410), __byte_perm(a.x, b.x, 0x7632), __byte_perm(a.y, b.y, 0x5410),
+                                     __byte_perm(a.y, b.y, 0x7632)};
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float f = BITS == 4 && (i & 1) ? p.query_scale * 0.0625f : p.query_scale;
+                w[i] = pack2(low_f32(raw[i]) * f, high_f32(raw[i]) * f);
+            }
+            q_operands[nt][gi][lane] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        __syncthreads();
         uint32_t qf[NT][G][4];
         float offset[NT][G][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int c = column0 + nt * 8 + g4;
-            const bool live = c < columns;
-            const int tok = live ? c / group : 0, h = live ? c - tok * group : 0;
-            const bf16* src = p.q + ((size_t)(qs + tok) * p.n_q + g * group + h) * D + t4 * (D / 4);
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int gi = 0; gi < G; ++gi) {
-                uint2 a = make_uint2(0u, 0u), b = a;
-                if (live) {
-                    a = *reinterpret_cast<const uint2*>(src + 4 * gi);
-                    b = *reinterpret_cast<const uint2*>(src + 4 * (gi + G));
-                }
-                float sum = (low_f32(a.x) + high_f32(a.x)) + (low_f32(a.y) + high_f32(a.y)) + (low_f32(b.x) + high_f32(b.x)) + (low_f32(b.y) + high_f32(b.y));
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                sum *= -S::L * 0x1p-73f;
-                offset[nt][gi][0] = __shfl_sync(0xffffffffu, sum, 8 * t4);
-                offset[nt][gi][1] = __shfl_sync(0xffffffffu, sum, 8 * t4 + 4);
-                const uint32_t raw[4] = {__byte_perm(a.x, b.x, 0x5410), __byte_perm(a.x, b.x, 0x7632), __byte_perm(a.y, b.y, 0x5410),
-                                         __byte_perm(a.y, b.y, 0x7632)};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float f = BITS == 4 && (i & 1) ? 0x1p56f : 0x1p60f;
-                    qf[nt][gi][i] = pack2(low_f32(raw[i]) * f, high_f32(raw[i]) * f);
-                }
+                const uint4 w = q_operands[nt][gi][lane];
+                const float2 f = q_offsets[nt][gi][lane];
+                qf[nt][gi][0] = w.x; qf[nt][gi][1] = w.y; qf[nt][gi][2] = w.z; qf[nt][gi][3] = w.w;
+                offset[nt][gi][0] = f.x; offset[nt][gi][1] = f.y;
             }
-        }
 
         float o[NT][2 * G][4], ones[NT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -390,7 +405,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                     }
                     __syncwarp();
                 }
-                // -- scores, in units of log2
+                // -- scores, to be multiplied by score_scale for units of log2
                 float s[NT][2][4];
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt) {
@@ -417,8 +432,9 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                         const float f1 = gi & 1 ? high_f32(a1[gi >> 1]) : low_f32(a1[gi >> 1]);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            float c[4] = {offset[nt][gi][0], offset[nt][gi][1], offset[nt][gi][0], offset[nt][gi][1]};
-                            mma(c, x0[0], x1[0], x0[1], x1[1], qf[nt][gi][0], qf[nt][gi][1]);
+                            float c[4];
+                            mma(c, x0[0], x1[0], x0[1], x1[1], qf[nt][gi][0], qf[nt][gi][1], offset[nt][gi][0], offset[nt][gi][1],
+                                offset[nt][gi][0], offset[nt][gi][1]);
                             mma(c, x0[2], x1[2], x0[3], x1[3], qf[nt][gi][2], qf[nt][gi][3]);
                             s[nt][mt][0] = fmaf(f0, c[0], s[nt][mt][0]);
                             s[nt][mt][1] = fmaf(f0, c[1], s[nt][mt][1]);
@@ -431,10 +447,6 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                 float top[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) s[nt][mt][k] *= p.score_scale;
                     if (cut) {
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
@@ -451,7 +463,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                     }
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        top[nt][c] = fmaxf(fmaxf(s[nt][0][c], s[nt][0][2 + c]), fmaxf(s[nt][1][c], s[nt][1][2 + c]));
+                        top[nt][c] = fmaxf(fmaxf(s[nt][0][c], s[nt][0][2 + c]), fmaxf(s[nt][1][c], s[nt][1][2 + c])) * p.score_scale;
                         raise |= top[nt][c] > m[nt][c] + 8.f;
                     }
                 }
@@ -487,32 +499,37 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const float w = exp2_fast(s[nt][mt][2 * h + c] - back);
+                                const float w = exp2_fast(fmaf(s[nt][mt][2 * h + c], p.score_scale, -back));
                                 s[nt][mt][2 * h + c] = w;
                                 l[nt][c] += w;
                             }
                     }
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt) {
-                    uint32_t a0[SB / 4], a1[SB / 4];
-                    take<SB>(a0, tile + VS_AT + (mt * 16 + key_of_row(g4)) * SB);
-                    take<SB>(a1, tile + VS_AT + (mt * 16 + key_of_row(g4) + 8) * SB);
-                    uint32_t v[4][S::V_BYTES / 4];                     // keys t, 4 + t, 8 + t, 12 + t
+                    uint32_t v[4][S::V_BYTES / 4], f[4][SB / 4];       // keys t, 4 + t, 8 + t, 12 + t
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) take<S::V_BYTES>(v[k], tile + V_AT + (mt * 16 + 4 * k + t4) * RB + g4 * S::V_BYTES);
+                    for (int k = 0; k < 4; ++k) {
+                        take<S::V_BYTES>(v[k], tile + V_AT + (mt * 16 + 4 * k + t4) * RB + g4 * S::V_BYTES);
+                        take<SB>(f[k], tile + VS_AT + (mt * 16 + 4 * k + t4) * SB);
+                    }
+                    uint32_t w[NT][2];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        w[nt][0] = transposed(pack2(s[nt][mt][0], s[nt][mt][1]));
+                        w[nt][1] = transposed(pack2(s[nt][mt][2], s[nt][mt][3]));
+                    }
 #pragma unroll
                     for (int gi = 0; gi < G; ++gi) {
                         uint32_t x0[4], x1[4];                         // keys of the first and the second half of the rows
                         constexpr int W = BITS == 4 ? 1 : 0;
                         spread<BITS>(x0, v[0][gi >> W], v[1][gi >> W], gi & 1);
                         spread<BITS>(x1, v[2][gi >> W], v[3][gi >> W], gi & 1);
-                        const float f0 = gi & 1 ? high_f32(a0[gi >> 1]) : low_f32(a0[gi >> 1]);
-                        const float f1 = gi & 1 ? high_f32(a1[gi >> 1]) : low_f32(a1[gi >> 1]);
+                        const uint32_t f0 = __byte_perm(f[0][gi >> 1], f[1][gi >> 1], gi & 1 ? 0x7632 : 0x5410);
+                        const uint32_t f1 = __byte_perm(f[2][gi >> 1], f[3][gi >> 1], gi & 1 ? 0x7632 : 0x5410);
                         const uint32_t one = g4 == gi ? 0x3f803f80u : 0u;
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            const uint32_t b0 = transposed(pack2(s[nt][mt][0] * f0, s[nt][mt][1] * f0));
-                            const uint32_t b1 = transposed(pack2(s[nt][mt][2] * f1, s[nt][mt][3] * f1));
+                            const uint32_t b0 = times2(w[nt][0], f0), b1 = times2(w[nt][1], f1);
                             mma(o[nt][2 * gi], x0[0], x0[1], x1[0], x1[1], b0, b1);
                             mma(o[nt][2 * gi + 1], x0[2], x0[3], x1[2], x1[3], b0, b1);
                             mma(ones[nt], one, 0u, one, 0u, b0, b1);
@@ -565,32 +582,45 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
         const bool whole = n == en.n_steps;
         const int slot = 2 * blockIdx.x + (x == run_first ? 0 : 1);
         const int live = min(COLS, columns - column0);
-        if (threadIdx.x == 0 && from == 0 && (p.by_row || !whole)) {
-            const int parts = whole ? 0 : cta_of_step(total, ctas, x + en.n_steps - 1) - (int)blockIdx.x + 1;
-            p.shared_rows[p.by_row ? entry * p.most_blocks + block : blockIdx.x] =
-                make_int4(entry, g, 2 * column0 + (x == run_first ? 0 : 1), (int)blockIdx.x << 16 | parts);
-        }
-        for (int i = threadIdx.x; i < live * D; i += THREADS) {
-            const int col = i / D, d = i % D;
-            float mx = -INFINITY;
+        if (threadIdx.x < COLS) {
+            const int col = threadIdx.x;
+            float mx = -INFINITY, sum = 0.f;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) mx = fmaxf(mx, w_m[w * COLS + col]);
-            float sum = 0.f, acc = 0.f;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
                 const float wm = w_m[w * COLS + col], f = wm == -INFINITY ? 0.f : exp2_fast(wm - mx);
                 sum += w_l[w * COLS + col] * f;
-                acc += w_o[(size_t)(w * COLS + col) * WO + d] * f;
+                part_f[w][col] = f;
+            }
+            if (whole) {
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) part_f[w][col] = sum > 0.f ? part_f[w][col] / sum : 0.f;
+            } else if (col < live) {
+                *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * COLS + col) * 2) = make_float2(mx, sum);
+            }
+        }
+        if (threadIdx.x == THREADS - 1 && from == 0 && (p.by_row || !whole)) {
+            const int parts = whole ? 0 : run.cuts.cta_of(x + en.n_steps - 1) - (int)blockIdx.x + 1;
+            p.shared_rows[p.by_row ? entry * p.most_blocks + block : blockIdx.x] =
+                make_int4(entry, g, 2 * column0 + (x == run_first ? 0 : 1), (int)blockIdx.x << 16 | parts);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x * 4; i < live * D; i += THREADS * 4) {
+            const int col = i / D, d = i % D;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float f = part_f[w][col];
+                const float4 r = *reinterpret_cast<const float4*>(w_o + (size_t)(w * COLS + col) * WO + d);
+                acc.x = fmaf(r.x, f, acc.x); acc.y = fmaf(r.y, f, acc.y); acc.z = fmaf(r.z, f, acc.z); acc.w = fmaf(r.w, f, acc.w);
             }
             if (whole) {
                 const int c = column0 + col, tok = c / group;
-                p.out[((size_t)(qs + tok) * p.n_q + g * group + (c - tok * group)) * D + d] = __float2bfloat16_rn(sum > 0.f ? acc / sum : 0.f);
+                *reinterpret_cast<uint2*>(p.out + ((size_t)(qs + tok) * p.n_q + g * group + (c - tok * group)) * D + d) =
+                    make_uint2(pack2(acc.x, acc.y), pack2(acc.z, acc.w));
             } else {
-                p.part_o[((size_t)slot * COLS + col) * D + d] = acc;
-                if (d == 0) {
-                    p.part_ml[((size_t)slot * COLS + col) * 2] = mx;
-                    p.part_ml[((size_t)slot * COLS + col) * 2 + 1] = sum;
-                }
+                *reinterpret_cast<float4*>(p.part_o + ((size_t)slot * COLS + col) * D + d) = acc;
             }
         }
         if constexpr (BULK) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // (the ring takes copies again)
@@ -613,7 +643,7 @@ __global__ void __launch_bounds__(D * SHARES) attn_quant_merge_kernel(const Para
     }
     pdl_wait();
     const int4 row = p.shared_rows[blockIdx.x];
-    const int parts = row.w & 0xffff, c0 = row.w >> 16, e = row.x, group = p.n_q / p.n_kv, c = (row.z >> 1) + blockIdx.y;
+    const int parts = row.w & 0xffff, c0 = row.w >> 16, e = row.x, group = p.group, c = (row.z >> 1) + blockIdx.y;
     if (parts == 0) return;
     const int qs = p.q_start[e];
     if (c >= (p.q_start[e + 1] - qs) * group) return;
@@ -707,7 +737,7 @@ extern "C" int kipp_attn_quant(void* out, const void* q, const void* k_codes, co
         status == nullptr || scratch == nullptr)
         return KIPP_ERR_ARG;
     if (scratch_bytes < kipp_attn_quant_scratch_bytes(head_dim)) return -4;
-    if ((((uintptr_t)q | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scales | (uintptr_t)v_scales | (uintptr_t)scratch) & 15) != 0) return -3;
+    if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scales | (uintptr_t)v_scales | (uintptr_t)scratch) & 15) != 0) return -3;
     // (row numbers of pages and steps of all rows are 32-bit)
     const long long cols = columns_of(head_dim, (long long)most * (n_q / n_kv));
     const long long room = (long long)table_width * page_size, steps = (room + STEP - 1) / STEP;
@@ -723,8 +753,9 @@ extern "C" int kipp_attn_quant(void* out, const void* q, const void* k_codes, co
     p.entries = entries; p.table_width = table_width; p.page_size = page_size; p.n_pages = n_pages; p.most = most;
     p.page_shift = -1;
     for (int i = 0; i < 31; ++i) if (page_size == 1 << i) p.page_shift = i;
-    p.n_q = n_q; p.n_kv = n_kv; p.window = window;
-    p.score_scale = scale * 1.4426950408889634f * 0x1p73f;
+    p.n_q = n_q; p.n_kv = n_kv; p.group = n_q / n_kv; p.window = window;
+    p.score_scale = fabsf(scale) * 1.4426950408889634f * 0x1p73f;
+    p.query_scale = scale < 0.f ? -0x1p60f : 0x1p60f;
     p.part_o = (float*)scratch;
     p.part_ml = p.part_o + 2LL * MOST_CTAS * MOST_COLUMNS * head_dim;
     p.shared_rows = (int4*)(p.part_ml + 2LL * MOST_CTAS * MOST_COLUMNS * 2);

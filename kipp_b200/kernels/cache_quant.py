@@ -175,24 +175,24 @@ _supported: dict = {}
 _scratch_bytes: dict = {}
 
 
-def _direct_ok(q: torch.Tensor, pages: QuantizedPages, n_q: int) -> bool:
+def _direct_ok(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPages, n_q: int) -> bool:
     key = (pages.bits, pages.head_dim, n_q, pages.n_kv)
     if key not in _supported:
         _supported[key] = bool(_fn("attention_quant", "kipp_attn_quant_supported", [c_int] * 4)(*key))
-    return q.dtype == torch.bfloat16 and _supported[key] and pages.aligned and q.data_ptr() % 16 == 0
+    return q.dtype == torch.bfloat16 and _supported[key] and pages.aligned and (q.data_ptr() | out.data_ptr()) % 16 == 0
 
 
 def _plan(out, q, pages, meta, block_table, n_q):
     """(form of the entries of one token, form of the others, the entries of more than one token from the first to the last):
     forms "direct" (the kernel over codes), "portion" (read back, tcgen05 prompt kernel) and "read" (read back, CUDA cores).
     The prompt kernel reads a key and a value once for 128 tokens, the kernel over codes once for 8 or 16 columns."""
-    if not _direct_ok(q, pages, n_q):
+    if not _direct_ok(out, q, pages, n_q):
         return "read", "read", None
     if max(meta.q_lens) >= PORTION_MIN and getattr(meta, "prefill_work128", None) is not None:
         from . import attention_bf16
         several = [e for e, n in enumerate(meta.q_lens) if n > 1]
         span = (several[0], several[-1] + 1)
-        if attention_bf16.prefill_tc_supported(pages.head_dim, n_q, pages.n_kv, pages.page_size) and out.data_ptr() % 16 == 0 and \
+        if attention_bf16.prefill_tc_supported(pages.head_dim, n_q, pages.n_kv, pages.page_size) and \
                 span[1] - span[0] <= _entries_at_once(pages, q.dtype, block_table.shape[1]):
             return "direct", "portion", span
     return "direct", "direct", None
@@ -231,7 +231,7 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
         single, several, span = _plan(out, q, pages, meta, block_table, n_q)
     elif impl in ("direct", "read"):
         single, several, span = impl, impl, None
-        if impl == "direct" and not _direct_ok(q, pages, n_q):
+        if impl == "direct" and not _direct_ok(out, q, pages, n_q):
             raise KernelError(f"{what}: the kernel over codes takes bfloat16 heads of 64, 128 or 256, 16-byte aligned")
     else:
         raise KernelError(f"unknown attention implementation {impl!r}")
