@@ -26,9 +26,10 @@
 // its own 32 keys of a step of 128 with its own maximum, fetches its own rows, and meets the other three
 // warps only at the end of a piece.  A maximum is raised only when a score passes it by 2^8.
 //
-// Rows come by bulk copies into a ring per warp: 16 keys of one kv head lie in one piece where the page size is
-// a multiple of 16, and eight lanes ask for the codes and scales of 32 keys and values with one instruction.
-// Other page sizes take cp.async row by row.
+// Rows come by cp.async into a ring per warp.  Where the page size is a multiple of 16, 16 keys of one kv head
+// lie in one piece and a warp fetches them from one address (bulk copies, eight of 128 to 1,024 bytes for 32 keys,
+// cost more: each takes its operands from uniform registers, some 20 instructions a copy); other page
+// sizes go row by row.
 //
 // How the work is cut: every (entry, kv head, block of columns) is a row of steps of 128 keys; all rows
 // one behind the other are dealt out in equal runs to one wave of CTAs, whatever the lengths.  A CTA may so
@@ -36,7 +37,6 @@
 // scratch and are added in order by a second kernel.  The cut is made from the step's lists, on
 // the device, so a captured graph follows the lengths.
 #include "quant_format.cuh"
-#include "mbarrier.cuh"
 #include <math.h>
 
 namespace {
@@ -161,6 +161,8 @@ template <int D, int BITS> struct Shape {
     static constexpr int STAGES = WARP_STAGE <= 2560 ? 4 : RB == 128 && D == 128 ? 2 : 3;
     static constexpr float L = BITS == 4 ? 8.f : 128.f;
 };
+template <int D, int NT> constexpr int q_bytes() { return NT * (D / 32) * 32 * 24; }          // the queries of a piece as operands
+template <int D, int BITS, int NT> constexpr bool q_in_ring() { return q_bytes<D, NT>() <= Shape<D, BITS>::WARP_STAGE; }
 template <int D, int BITS, int NT> constexpr int ctas_per_sm() {
     return D == 256 ? (BITS == 4 ? 2 : 1) : NT == 2 ? (D == 64 ? 3 : 2) : D == 128 && BITS == 8 ? 3 : 4;
 }
@@ -185,35 +187,19 @@ template <int BITS> __device__ __forceinline__ void spread(uint32_t (&x)[4], uin
     }
 }
 
-__device__ __forceinline__ void expect(uint64_t* bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(kipp_smem_u32(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(kipp_smem_u32(bar)) : "memory");
-}
-
-// BULK: the page size is a multiple of 16.
-template <int D, int BITS, int NT, bool BULK>
+// TILES: the page size is a multiple of 16.
+template <int D, int BITS, int NT, bool TILES>
 __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quant_kernel(const Params p) {
     using S = Shape<D, BITS>;
     constexpr int G = S::G, RB = S::RB, SB = S::SB, COLS = 8 * NT, WO = D + 4, STAGES = S::STAGES;
+    constexpr int RING = WARPS * STAGES * S::WARP_STAGE;
+    constexpr bool Q_IN_RING = q_in_ring<D, BITS, NT>();
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Run run;
-    __shared__ uint4 q_operands[NT][G][32];                    // of a piece, by lane
-    __shared__ float2 q_offsets[NT][G][32];
     __shared__ float part_f[WARPS][COLS];
-    __shared__ uint64_t full[WARPS][STAGES];
-    __shared__ int gave_up;
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, t4 = lane & 3;
     const int group = p.group;
-    if constexpr (BULK) {
-        if (threadIdx.x < WARPS * STAGES)
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(kipp_smem_u32(&full[0][0] + threadIdx.x)) : "memory");
-        if (threadIdx.x == 0) gave_up = 0;
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
 
     // -- the run of this CTA: from the step's lists, which may be read before the wait
     if (warp == 0) {
@@ -243,13 +229,11 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
     uint8_t* const my = smem + warp * (STAGES * S::WARP_STAGE);
     const uint32_t my_s = smem_address(my);
     constexpr int V_AT = WARP_KEYS * RB, KS_AT = 2 * WARP_KEYS * RB, VS_AT = KS_AT + WARP_KEYS * SB;
-    // bulk copies: lane 4 tile + array asks for array (keys, values, their scales) of tile (16 keys)
-    const int b_array = lane & 3, b_bytes = b_array < 2 ? RB : SB;
-    const uint8_t* const b_from = b_array == 0 ? p.k_codes : b_array == 1 ? p.v_codes : b_array == 2 ? p.k_scales : p.v_scales;
-    const uint32_t b_to = my_s + (b_array == 0 ? 0 : b_array == 1 ? V_AT : b_array == 2 ? KS_AT : VS_AT) + ((lane >> 2) & 1) * 16 * b_bytes;
-    uint32_t parity = 0;                                       // of each stage's next arrival
+    // a lane's 16 bytes of a tile's keys, values and scales (the first SB lanes those of the keys, the next SB of the values)
+    const uint8_t *const k_lane = p.k_codes + lane * 16, *const v_lane = p.v_codes + lane * 16;
+    const uint8_t* const s_lane = lane < SB ? p.k_scales + lane * 16 : p.v_scales + (lane - SB) * 16;
+    const int s_to = lane < SB ? KS_AT : VS_AT - 16 * SB;
     int stage = 0;
-    bool failed = false;
 
     for (int x = run_first; x < run_end;) {
         Entry en = entry_of<COLS>(p, entry);
@@ -267,10 +251,10 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
         const int all_hi = min(en.context + tok0, see_hi), all_lo = p.window > 0 ? max(0, en.context + tok1 - p.window + 1) : 0;
         const int j_first = (en.first_step + from) * STEP + warp * WARP_KEYS;
 
-        // the row of pages that holds key j (BULK: key j and the 15 behind it); -1: none of it is seen
+        // the row of pages that holds key j (TILES: key j and the 15 behind it); -1: none of it is seen
         auto row_of = [&](int j) {
             int row = -1;
-            if (j + (BULK ? 15 : 0) >= see_lo && j <= see_hi) {
+            if (j + (TILES ? 15 : 0) >= see_lo && j <= see_hi) {
                 const int slot = p.page_shift >= 0 ? j >> p.page_shift : j / p.page_size;
                 const int page = table[slot];
                 if (page >= 0 && page < p.n_pages) row = (page * p.n_kv + g) * p.page_size + (j - slot * p.page_size);
@@ -278,14 +262,35 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             }
             return row;
         };
-        auto fetch = [&](int stage, int row) {
-            if constexpr (BULK) {
-                const unsigned tiles = __ballot_sync(0xffffffffu, row >= 0) & 0x11u;
-                if (lane == 0) expect(&full[warp][stage], __popc(tiles) * (32 * (RB + SB)));
-                __syncwarp();
-                if (lane < 8 && row >= 0) bulk_copy(b_to + stage * S::WARP_STAGE, b_from + (size_t)row * b_bytes, 16 * b_bytes, &full[warp][stage]);
+        // TILES: the rows of the tiles of 16 steps are looked up at once, a tile a lane, and a batch ahead; otherwise each lane's
+        // own key, a step ahead.  (What is not seen keeps whatever lies in the ring.)
+        int rows = -1, rows_next;
+        auto look_up = [&](int step) {
+            if constexpr (TILES) rows_next = row_of(j_first + (step + (lane >> 1)) * STEP + (lane & 1) * 16);
+            else rows_next = row_of(j_first + step * STEP + lane);
+        };
+        auto fetch = [&](int step, int to_stage) {
+            const uint32_t to = my_s + to_stage * S::WARP_STAGE;
+            if constexpr (TILES) {
+                if ((step & 15) == 0) {
+                    rows = rows_next;
+                    if (step + 16 < n) look_up(step + 16);
+                }
+#pragma unroll
+                for (int tile = 0; tile < 2; ++tile) {
+                    const int row = __shfl_sync(0xffffffffu, rows, 2 * (step & 15) + tile);
+                    if (row < 0) continue;
+                    const uint8_t *k = k_lane + (size_t)row * RB, *v = v_lane + (size_t)row * RB;
+#pragma unroll
+                    for (int i = 0; i < RB / 32; ++i) {
+                        cp_async16(to + lane * 16 + tile * 16 * RB + i * 512, k + i * 512, 16);
+                        cp_async16(to + lane * 16 + V_AT + tile * 16 * RB + i * 512, v + i * 512, 16);
+                    }
+                    if (lane < 2 * SB) cp_async16(to + lane * 16 + s_to + tile * 16 * SB, s_lane + (size_t)row * SB, 16);
+                }
             } else {
-                const uint32_t to = my_s + stage * S::WARP_STAGE;
+                const int row = rows_next;
+                if (step + 1 < n) look_up(step + 1);
                 constexpr int ROWS = 32 / S::CHUNKS;               // rows of a pass
                 const int c = lane % S::CHUNKS;
 #pragma unroll
@@ -300,18 +305,17 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                 cp_async_row(to + VS_AT + lane * SB, p.v_scales + off, SB, row >= 0 ? SB : 0);
             }
         };
-        const int j_mine = j_first + (BULK ? (lane & 4) * 4 : lane);     // the key whose row this lane looks up
-        int ahead = row_of(j_mine);
+        look_up(0);
 #pragma unroll
         for (int s = 0; s < STAGES - 1; ++s) {
-            if (s < n && !failed) {
-                fetch((stage + s) % STAGES, ahead);
-                ahead = s + 1 < n ? row_of(j_mine + (s + 1) * STEP) : -1;
-            }
-            if constexpr (!BULK) cp_async_commit();
+            if (s < n) fetch(s, (stage + s) % STAGES);
+            cp_async_commit();
         }
 
-        // -- queries as operands, and what the offset of their codes comes to: a warp makes every fourth group's
+        // -- queries as operands, and what the offset of their codes comes to: a warp makes every fourth group's (through the
+        // first warp's free stage, where they have room)
+        uint4* const q_operands = reinterpret_cast<uint4*>(Q_IN_RING ? smem + (stage + STAGES - 1) % STAGES * S::WARP_STAGE : smem + RING);
+        float2* const q_offsets = reinterpret_cast<float2*>(q_operands + NT * G * 32);
         for (int k = warp; k < NT * G; k += WARPS) {
             const int nt = k / G, gi = k % G, c = column0 + nt * 8 + g4;
             uint2 a = make_uint2(0u, 0u), b = a;
@@ -325,7 +329,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             sum *= -S::L * 0x1p-133f * p.query_scale;
-            q_offsets[nt][gi][lane] = make_float2(__shfl_sync(0xffffffffu, sum, 8 * t4), __shfl_sync(0xffffffffu, sum, 8 * t4 + 4));
+            q_offsets[k * 32 + lane] = make_float2(__shfl_sync(0xffffffffu, sum, 8 * t4), __shfl_sync(0xffffffffu, sum, 8 * t4 + 4));
             const uint32_t raw[4] = {__byte_perm(a.x, b.x, 0x5410), __byte_perm(a.x, b.x, 0x7632), __byte_perm(a.y, b.y, 0x5410),
                                      __byte_perm(a.y, b.y, 0x7632)};
             uint32_t w[4];
@@ -334,7 +338,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                 const float f = BITS == 4 && (i & 1) ? p.query_scale * 0.0625f : p.query_scale;
                 w[i] = pack2(low_f32(raw[i]) * f, high_f32(raw[i]) * f);
             }
-            q_operands[nt][gi][lane] = make_uint4(w[0], w[1], w[2], w[3]);
+            q_operands[k * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
         }
         __syncthreads();
         uint32_t qf[NT][G][4];
@@ -343,11 +347,12 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int gi = 0; gi < G; ++gi) {
-                const uint4 w = q_operands[nt][gi][lane];
-                const float2 f = q_offsets[nt][gi][lane];
+                const uint4 w = q_operands[(nt * G + gi) * 32 + lane];
+                const float2 f = q_offsets[(nt * G + gi) * 32 + lane];
                 qf[nt][gi][0] = w.x; qf[nt][gi][1] = w.y; qf[nt][gi][2] = w.z; qf[nt][gi][3] = w.w;
                 offset[nt][gi][0] = f.x; offset[nt][gi][1] = f.y;
             }
+        if constexpr (Q_IN_RING) __syncthreads();
 
         float o[NT][2 * G][4], ones[NT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -362,31 +367,11 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             l[nt][0] = l[nt][1] = 0.f;
         }
 
-        // (the ring goes on where the last piece left it: its barriers' phases do)
-        for (int i = 0; i < n && !failed; ++i) {
-            {
-                const int s = i + STAGES - 1;
-                if (s < n) {
-                    fetch(stage == 0 ? STAGES - 1 : stage - 1, ahead);
-                    ahead = s + 1 < n ? row_of(j_mine + (s + 1) * STEP) : -1;
-                }
-                if constexpr (BULK) {
-                    const bool here = kipp_mbar_wait_limited(&full[warp][stage], (parity >> stage) & 1u, &gave_up, KIPP_WAIT_LIMIT_CYCLES);
-                    if (!__all_sync(0xffffffffu, here)) {
-                        // gave up: nothing more is asked for, and what was is waited for, within the limit
-                        failed = true;
-                        int alone = 0;
-                        for (int k = 0, q = stage; k < STAGES && i + k < n; ++k, q = q + 1 == STAGES ? 0 : q + 1)
-                            kipp_mbar_wait_limited(&full[warp][q], (parity >> q) & 1u, &alone, KIPP_WAIT_LIMIT_CYCLES);
-                        break;
-                    }
-                    parity ^= 1u << stage;
-                } else {
-                    cp_async_commit();
-                    cp_async_wait<STAGES - 1>();
-                    __syncwarp();
-                }
-            }
+        for (int i = 0; i < n; ++i) {
+            if (i + STAGES - 1 < n) fetch(i + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+            cp_async_commit();
+            cp_async_wait<STAGES - 1>();
+            __syncwarp();
             uint8_t* const tile = my + stage * S::WARP_STAGE;
             const int j0 = j_first + i * STEP;
             // (the warps of a step may all be outside what is seen, but for one)
@@ -401,7 +386,6 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                             *reinterpret_cast<uint32_t*>(tile + KS_AT + lane * SB + 4 * k) = 0u;
                             *reinterpret_cast<uint32_t*>(tile + VS_AT + lane * SB + 4 * k) = 0u;
                         }
-                        if constexpr (BULK) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     }
                     __syncwarp();
                 }
@@ -540,7 +524,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             __syncwarp();
             stage = stage + 1 == STAGES ? 0 : stage + 1;
         }
-        if constexpr (!BULK) cp_async_wait<0>();
+        cp_async_wait<0>();
 
         // -- the four warps' parts together, through shared memory
         __syncthreads();
@@ -623,12 +607,10 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                 *reinterpret_cast<float4*>(p.part_o + ((size_t)slot * COLS + col) * D + d) = acc;
             }
         }
-        if constexpr (BULK) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // (the ring takes copies again)
         __syncthreads();
         x += n;
         at += n;
     }
-    if (BULK && threadIdx.x == 0 && gave_up) atomicExch(p.status + 1, 1);
 }
 
 // Adds the parts of one head of one token of a row that CTAs shared, in the order of the keys: SHARES threads an
@@ -680,15 +662,16 @@ __global__ void __launch_bounds__(D * SHARES) attn_quant_merge_kernel(const Para
 template <int D, int BITS, int NT> constexpr size_t smem_bytes() {
     using S = Shape<D, BITS>;
     constexpr size_t ring = (size_t)WARPS * S::STAGES * S::WARP_STAGE, merge = (size_t)WARPS * 8 * NT * (D + 4 + 2) * 4;
-    return ring > merge ? ring : merge;
+    constexpr size_t all = ring + (q_in_ring<D, BITS, NT>() ? 0 : q_bytes<D, NT>());
+    return all > merge ? all : merge;
 }
 // CTAs of one wave.
-template <int D, int BITS, int NT, bool BULK> int wave() {
+template <int D, int BITS, int NT, bool TILES> int wave() {
     static const int ctas = [] {
         int per = 0;
         const size_t smem = smem_bytes<D, BITS, NT>();
-        if (kipp_allow_smem(attn_quant_kernel<D, BITS, NT, BULK>, smem) != 0 ||
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attn_quant_kernel<D, BITS, NT, BULK>, THREADS, smem) != cudaSuccess || per < 1) {
+        if (kipp_allow_smem(attn_quant_kernel<D, BITS, NT, TILES>, smem) != 0 ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attn_quant_kernel<D, BITS, NT, TILES>, THREADS, smem) != cudaSuccess || per < 1) {
             cudaGetLastError();
             per = 1;
         }
@@ -697,15 +680,15 @@ template <int D, int BITS, int NT, bool BULK> int wave() {
     }();
     return ctas;
 }
-template <int D, int BITS, int NT, bool BULK> int launch(Params p, long long steps_of_row, cudaStream_t s) {
+template <int D, int BITS, int NT, bool TILES> int launch(Params p, long long steps_of_row, cudaStream_t s) {
     constexpr size_t smem = smem_bytes<D, BITS, NT>();
     constexpr int COLS = 8 * NT, FEW = D < 128 ? 128 / D : 1, MANY = 512 / D;
-    const int wave_ctas = wave<D, BITS, NT, BULK>();
+    const int wave_ctas = wave<D, BITS, NT, TILES>();
     const long long rows = (long long)p.entries * p.most_blocks, steps = rows * steps_of_row;
     p.ctas = (int)(steps < wave_ctas ? steps : wave_ctas);
     p.by_row = rows <= p.ctas ? 1 : 0;
-    if (const int e = kipp_allow_smem(attn_quant_kernel<D, BITS, NT, BULK>, smem)) return e;
-    if (const int e = kipp_launch(attn_quant_kernel<D, BITS, NT, BULK>, dim3((unsigned)p.ctas), dim3(THREADS), smem, s, 1, p)) return e;
+    if (const int e = kipp_allow_smem(attn_quant_kernel<D, BITS, NT, TILES>, smem)) return e;
+    if (const int e = kipp_launch(attn_quant_kernel<D, BITS, NT, TILES>, dim3((unsigned)p.ctas), dim3(THREADS), smem, s, 1, p)) return e;
     if (steps_of_row <= 1) return 0;                   // every row is one step: none is shared
     const int columns = p.most * (p.n_q / p.n_kv);
     const dim3 grid((unsigned)(p.by_row ? rows : p.ctas), (unsigned)(columns < COLS ? columns : COLS));
