@@ -33,8 +33,9 @@
 //
 // How the work is cut: every (entry, kv head, block of columns) is a row of steps of 128 keys; all rows
 // one behind the other are dealt out in equal runs to one wave of CTAs, whatever the lengths.  A CTA may so
-// have the end of one row, some whole ones and the start of another; parts of a row go through
-// scratch and are added in order by a second kernel.  The cut is made from the step's lists, on
+// have the end of one row, some whole ones and the start of another, and each of those costs it a
+// queue that fills and drains and a sum over its warps: a row counts for some units more than it has steps.  Parts of a
+// row go through scratch and are added in order by a second kernel.  Both make the cut from the step's lists, on
 // the device, so a captured graph follows the lengths.
 #include "quant_format.cuh"
 #include <math.h>
@@ -52,23 +53,23 @@ struct Params {
     int entries, table_width, page_size, page_shift, n_pages, most, n_q, n_kv, group, window;
     float score_scale, query_scale;  // |scale| * log2(e) * 2^73; 2^60 with the scale's sign
     float* part_o; float* part_ml;   // [2 ctas][columns][D], [2 ctas][columns][2]
-    // rows that several CTAs share, by the row's number (by_row) or by the first CTA: (entry, kv head, 2 first column + the first
-    // part's slot, first CTA << 16 | CTAs); 0 CTAs: nothing to add
-    int4* shared_rows;
-    int ctas, by_row, most_blocks;   // most_blocks: rows of an entry of `most` tokens
+    int ctas, most_blocks;           // most_blocks: rows of an entry of `most` tokens
     int* status;
 };
+
+constexpr int ROW_COST = 1;          // units of a row beside its steps
 
 // One entry's share of the work.
 struct Entry {
     int q_len, context, first_step, n_steps, column_blocks, blocks;
-    __device__ __forceinline__ int steps() const { return blocks * n_steps; }
+    __device__ __forceinline__ int row_units() const { return n_steps + ROW_COST; }
+    __device__ __forceinline__ int units() const { return blocks * row_units(); }
 };
 template <int COLS> __device__ __forceinline__ Entry entry_of(const Params& p, int e) {
     Entry r;
     r.q_len = p.q_start[e + 1] - p.q_start[e];
     r.context = p.context_len[e];
-    if (r.q_len <= 0 || r.q_len > p.most || r.context < 0) { r.blocks = r.n_steps = 0; return r; }
+    if (r.q_len <= 0 || r.q_len > p.most || r.context < 0) { r.blocks = r.n_steps = r.column_blocks = 0; return r; }
     const int room = p.table_width * p.page_size;
     const int hi = min(r.context + r.q_len, room) - 1;
     const int lo = p.window > 0 ? max(0, r.context - p.window + 1) : 0;
@@ -79,29 +80,59 @@ template <int COLS> __device__ __forceinline__ Entry entry_of(const Params& p, i
     return r;
 }
 
-// Sum of v over the warp, and over the lanes before this one.
-__device__ __forceinline__ int warp_scan(int v, int& before) {
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if ((int)(threadIdx.x & 31) >= o) x += y;
-    }
-    before = x - v;
-    return __shfl_sync(0xffffffffu, x, 31);
-}
-
-// The cut: the first `more` CTAs have `per` + 1 steps, the others `per`.
+// The cut: the first `more` CTAs have `per` + 1 units, the others `per`; there are no more CTAs than units.
 struct Cut {
-    int per, more;
+    int ctas, per, more;
     Cut() = default;
-    __device__ __forceinline__ Cut(int total, int ctas) { per = total / ctas; more = total - per * ctas; }
+    __device__ __forceinline__ Cut(int total, int most_ctas) : ctas(max(min(most_ctas, total), 1)) { per = total / ctas; more = total - per * ctas; }
     __device__ __forceinline__ int start(int cta) const { return per * cta + min(cta, more); }
-    __device__ __forceinline__ int cta_of(int step) const {
+    __device__ __forceinline__ int cta_of(int unit) const {
         const int first = more * (per + 1);
-        return step < first ? step / (per + 1) : more + (step - first) / per;
+        return unit < first ? unit / (per + 1) : more + (unit - first) / per;
     }
 };
+
+// Where a unit is: the entry, and the units of it that lie before (entry -1: there is no such unit).  One warp, all lanes
+// together; `total` comes out as well.  unit_of makes the unit looked for out of the cut (once the total is known).
+struct Place { int entry, at; Cut cuts; };
+template <int COLS, typename UnitOf> __device__ __forceinline__ Place find_unit(const Params& p, UnitOf unit_of) {
+    const int lane = threadIdx.x & 31;
+    auto scan = [&](int base, int& mine, int& before) {
+        mine = base + lane < p.entries ? entry_of<COLS>(p, base + lane).units() : 0;
+        int x = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        before = x - mine;
+        return __shfl_sync(0xffffffffu, x, 31);
+    };
+    int mine, before;
+    const int first_sum = scan(0, mine, before);
+    int total = first_sum;
+    for (int base = 32; base < p.entries; base += 32) {
+        int m, b;
+        total += scan(base, m, b);
+    }
+    Place r;
+    r.cuts = Cut(total, p.ctas);
+    r.entry = -1;
+    r.at = 0;
+    const int unit = unit_of(total, r.cuts);
+    if (unit < 0 || unit >= total) return r;
+    int base = 0, passed = 0, sum = first_sum;
+    while (passed + sum <= unit) {
+        passed += sum;
+        base += 32;
+        sum = scan(base, mine, before);
+    }
+    const unsigned here = __ballot_sync(0xffffffffu, passed + before <= unit && unit < passed + before + mine);
+    const int who = __ffs(here) - 1;
+    r.entry = base + who;
+    r.at = unit - passed - __shfl_sync(0xffffffffu, before, who);
+    return r;
+}
 
 // d = a b + c
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0,
@@ -171,9 +202,6 @@ template <int D, int BITS, int NT> constexpr int ctas_per_sm() {
 // r = 2 t + e + 8 h: a lane (g, t) then meets the values of keys t, 4 + t, 8 + t, 12 + t.
 __device__ __forceinline__ int key_of_row(int r) { return 4 * (r & 1) + ((r & 7) >> 1) + (r & 8); }
 
-// The steps of a CTA, and where the first of them is.
-struct Run { int first, end, entry, at; Cut cuts; };
-
 // Two runs of four codes as four operand registers: x[i] holds code i of the first run in its low half and of
 // the second in its high half.  4 bits: `first` and `second` are words, HALF which half of them the run is;
 // codes 1 and 3 count sixteenfold.  8 bits: a run is a word.
@@ -195,7 +223,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
     constexpr int RING = WARPS * STAGES * S::WARP_STAGE;
     constexpr bool Q_IN_RING = q_in_ring<D, BITS, NT>();
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ Run run;
+    __shared__ Place place;
     __shared__ float part_f[WARPS][COLS];
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, t4 = lane & 3;
@@ -203,28 +231,14 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
 
     // -- the run of this CTA: from the step's lists, which may be read before the wait
     if (warp == 0) {
-        int total = 0, before;
-        for (int base = 0; base < p.entries; base += 32) {
-            const int e = base + lane;
-            total += warp_scan(e < p.entries ? entry_of<COLS>(p, e).steps() : 0, before);
-        }
-        const int ctas = min(p.ctas, total);               // (so that none between two others is empty)
-        const Cut cuts(total, max(ctas, 1));
-        const int first = (int)blockIdx.x < ctas ? cuts.start(blockIdx.x) : total, end = (int)blockIdx.x < ctas ? cuts.start(blockIdx.x + 1) : total;
-        for (int base = 0, passed = 0; first < end && passed <= first; base += 32) {
-            const int e = base + lane, mine = e < p.entries ? entry_of<COLS>(p, e).steps() : 0;
-            const int sum = warp_scan(mine, before);
-            if (mine > 0 && passed + before <= first && first < passed + before + mine) { run.entry = e; run.at = first - passed - before; }
-            passed += sum;
-        }
-        if (lane == 0) { run.first = first; run.end = end; run.cuts = cuts; }
+        const Place found = find_unit<COLS>(p, [&](int total, const Cut& c) { return (int)blockIdx.x < c.ctas && total > 0 ? c.start(blockIdx.x) : -1; });
+        if (lane == 0) place = found;
     }
     __syncthreads();
-    const int run_first = run.first, run_end = run.end;
-    int entry = run.entry, at = run.at;
+    int entry = place.entry, at = place.at;
     pdl_wait();
-    if (!p.by_row && threadIdx.x == 0) p.shared_rows[blockIdx.x] = make_int4(0, 0, 0, 0);
-    if (run_first >= run_end) return;
+    if (entry < 0) return;
+    const int run_first = place.cuts.start(blockIdx.x), run_end = place.cuts.start(blockIdx.x + 1);
 
     uint8_t* const my = smem + warp * (STAGES * S::WARP_STAGE);
     const uint32_t my_s = smem_address(my);
@@ -237,8 +251,13 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
 
     for (int x = run_first; x < run_end;) {
         Entry en = entry_of<COLS>(p, entry);
-        while (at >= en.steps()) { at -= en.steps(); en = entry_of<COLS>(p, ++entry); }
-        const int block = at / en.n_steps, from = at - block * en.n_steps, n = min(run_end - x, en.n_steps - from);
+        while (at >= en.units()) { at -= en.units(); en = entry_of<COLS>(p, ++entry); }
+        const int block = at / en.row_units(), unit = at - block * en.row_units(), units = min(run_end - x, en.row_units() - unit);
+        const int from = max(unit - ROW_COST, 0), n = unit + units - ROW_COST - from;      // steps of the row
+        const int slot = 2 * blockIdx.x + (x == run_first ? 0 : 1);
+        x += units;
+        at += units;
+        if (n <= 0) continue;
         const int g = block / en.column_blocks, column0 = (block - g * en.column_blocks) * COLS;
         const int qs = p.q_start[entry], columns = en.q_len * group;
         const int* table = p.block_table + (size_t)entry * p.table_width;
@@ -306,25 +325,34 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             }
         };
         look_up(0);
+        // -- the queries are asked for first: a warp makes operands of every fourth group's
+        constexpr int MINE = (NT * G + WARPS - 1) / WARPS;
+        uint2 q_raw[MINE][2];
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            const int k = warp + i * WARPS, c = column0 + k / G * 8 + g4;
+            q_raw[i][0] = q_raw[i][1] = make_uint2(0u, 0u);
+            if (k < NT * G && c < columns) {
+                const int tok = c / group;
+                const bf16* src = p.q + ((size_t)(qs + tok) * p.n_q + g * group + (c - tok * group)) * D + t4 * (D / 4) + 4 * (k % G);
+                q_raw[i][0] = *reinterpret_cast<const uint2*>(src);
+                q_raw[i][1] = *reinterpret_cast<const uint2*>(src + 4 * G);
+            }
+        }
 #pragma unroll
         for (int s = 0; s < STAGES - 1; ++s) {
             if (s < n) fetch(s, (stage + s) % STAGES);
             cp_async_commit();
         }
 
-        // -- queries as operands, and what the offset of their codes comes to: a warp makes every fourth group's (through the
-        // first warp's free stage, where they have room)
+        // -- as operands, with what the offset of their codes comes to (through the first warp's free stage, where they have room)
         uint4* const q_operands = reinterpret_cast<uint4*>(Q_IN_RING ? smem + (stage + STAGES - 1) % STAGES * S::WARP_STAGE : smem + RING);
         float2* const q_offsets = reinterpret_cast<float2*>(q_operands + NT * G * 32);
-        for (int k = warp; k < NT * G; k += WARPS) {
-            const int nt = k / G, gi = k % G, c = column0 + nt * 8 + g4;
-            uint2 a = make_uint2(0u, 0u), b = a;
-            if (c < columns) {
-                const int tok = c / group;
-                const bf16* src = p.q + ((size_t)(qs + tok) * p.n_q + g * group + (c - tok * group)) * D + t4 * (D / 4) + 4 * gi;
-                a = *reinterpret_cast<const uint2*>(src);
-                b = *reinterpret_cast<const uint2*>(src + 4 * G);
-            }
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            const int k = warp + i * WARPS;
+            if (k >= NT * G) break;
+            const uint2 a = q_raw[i][0], b = q_raw[i][1];
             float sum = (low_f32(a.x) + high_f32(a.x)) + (low_f32(a.y) + high_f32(a.y)) + (low_f32(b.x) + high_f32(b.x)) + (low_f32(b.y) + high_f32(b.y));
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -564,7 +592,6 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
         }
         __syncthreads();
         const bool whole = n == en.n_steps;
-        const int slot = 2 * blockIdx.x + (x == run_first ? 0 : 1);
         const int live = min(COLS, columns - column0);
         if (threadIdx.x < COLS) {
             const int col = threadIdx.x;
@@ -583,11 +610,6 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             } else if (col < live) {
                 *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * COLS + col) * 2) = make_float2(mx, sum);
             }
-        }
-        if (threadIdx.x == THREADS - 1 && from == 0 && (p.by_row || !whole)) {
-            const int parts = whole ? 0 : run.cuts.cta_of(x + en.n_steps - 1) - (int)blockIdx.x + 1;
-            p.shared_rows[p.by_row ? entry * p.most_blocks + block : blockIdx.x] =
-                make_int4(entry, g, 2 * column0 + (x == run_first ? 0 : 1), (int)blockIdx.x << 16 | parts);
         }
         __syncthreads();
         for (int i = threadIdx.x * 4; i < live * D; i += THREADS * 4) {
@@ -608,55 +630,89 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             }
         }
         __syncthreads();
-        x += n;
-        at += n;
     }
 }
 
-// Adds the parts of one head of one token of a row that CTAs shared, in the order of the keys: SHARES threads an
-// element, each with a run of the parts.
-template <int D, int NT, int SHARES>
-__global__ void __launch_bounds__(D * SHARES) attn_quant_merge_kernel(const Params p) {
-    constexpr int COLS = 8 * NT, WARPS_M = D * SHARES / 32;
-    __shared__ float sh_o[SHARES][D], sh_l[SHARES], sh_m[WARPS_M];
-    if (p.by_row) {                                    // (only rows that exist have left word of themselves)
-        const int e = blockIdx.x / p.most_blocks;
-        if ((int)blockIdx.x - e * p.most_blocks >= entry_of<COLS>(p, e).blocks) { pdl_wait(); return; }
+// Adds the parts of one head of one token of a row that CTAs shared, in an order that the cut alone sets.  Block x is
+// a row (BY_ROW) or the row that CTA x begins and the next one goes on with; y is the column.  A warp reads whole parts, D / 32
+// values a lane, every MERGE_WARPS-th of them.
+template <int D, int NT, int MERGE_WARPS, bool BY_ROW>
+__global__ void __launch_bounds__(MERGE_WARPS * 32) attn_quant_merge_kernel(const Params p) {
+    constexpr int COLS = 8 * NT, PER = D / 32, BATCH = 8;
+    __shared__ float sh_o[MERGE_WARPS][D], sh_l[MERGE_WARPS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y;
+    // (every warp for itself, from the step's lists)
+    int row_start = 0;
+    const Place at = find_unit<COLS>(p, [&](int total, const Cut& c) {
+        return BY_ROW ? -1 : (int)blockIdx.x + 1 < c.ctas ? c.start(blockIdx.x + 1) - 1 : -1;
+    });
+    int e = at.entry, block;
+    Entry en;
+    if constexpr (BY_ROW) {
+        e = blockIdx.x / p.most_blocks;
+        block = blockIdx.x - e * p.most_blocks;
+        en = entry_of<COLS>(p, e);
+        int before = 0;
+        for (int i = lane; i < e; i += 32) before += entry_of<COLS>(p, i).units();
+        row_start = (int)__reduce_add_sync(0xffffffffu, (unsigned)before) + block * en.row_units();
+        if (block >= en.blocks) e = -1;
+    } else if (e >= 0) {
+        en = entry_of<COLS>(p, e);
+        block = at.at / en.row_units();
+        row_start = at.cuts.start(blockIdx.x + 1) - 1 - (at.at - block * en.row_units());
     }
     pdl_wait();
-    const int4 row = p.shared_rows[blockIdx.x];
-    const int parts = row.w & 0xffff, c0 = row.w >> 16, e = row.x, group = p.group, c = (row.z >> 1) + blockIdx.y;
-    if (parts == 0) return;
-    const int qs = p.q_start[e];
-    if (c >= (p.q_start[e + 1] - qs) * group) return;
-    auto at = [&](int part) { return (size_t)(2 * (c0 + part) + (part == 0 ? row.z & 1 : 0)) * COLS + blockIdx.y; };
+    if (e < 0) return;
+    const int c0 = at.cuts.cta_of(row_start + ROW_COST), parts = at.cuts.cta_of(row_start + en.row_units() - 1) - c0 + 1;
+    const int g = block / en.column_blocks, c = (block - g * en.column_blocks) * COLS + col;
+    if (parts < 2 || (!BY_ROW && c0 != (int)blockIdx.x) || c >= en.q_len * p.group) return;
+    // (a CTA's first piece is in slot 0)
+    auto index = [&](int part) { return (size_t)(2 * (c0 + part) + (row_start > at.cuts.start(c0 + part) ? 1 : 0)) * COLS + col; };
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
     float mx = -INFINITY;
-    for (int i = threadIdx.x; i < parts; i += D * SHARES) mx = fmaxf(mx, p.part_ml[at(i) * 2]);
-    mx = warp_max(mx);
-    if ((threadIdx.x & 31) == 0) sh_m[threadIdx.x >> 5] = mx;
+    for (int i = lane; i < parts; i += 32) mx = fmaxf(mx, ml[index(i)].x);
+    float acc[PER], sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) acc[k] = 0.f;
+    for (int first = warp; first < parts; first += MERGE_WARPS * BATCH) {
+        float r[BATCH][PER];
+        float2 f[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int part = first + i * MERGE_WARPS;
+            f[i] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int k = 0; k < PER; ++k) r[i][k] = 0.f;
+            if (part < parts) {
+                f[i] = ml[index(part)];
+#pragma unroll
+                for (int k = 0; k < PER; ++k) r[i][k] = p.part_o[index(part) * D + k * 32 + lane];
+            }
+        }
+        if (first == warp) mx = warp_max(mx);
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const float w = f[i].x == -INFINITY ? 0.f : exp2_fast(f[i].x - mx);
+            sum = fmaf(f[i].y, w, sum);
+#pragma unroll
+            for (int k = 0; k < PER; ++k) acc[k] = fmaf(r[i][k], w, acc[k]);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) sh_o[warp][k * 32 + lane] = acc[k];
+    if (lane == 0) sh_l[warp] = sum;
     __syncthreads();
+    float total = 0.f;
 #pragma unroll
-    for (int w = 0; w < WARPS_M; ++w) mx = fmaxf(mx, sh_m[w]);
-    const int d = threadIdx.x % D, share = threadIdx.x / D;
-    const int many = (parts + SHARES - 1) / SHARES, end = min(parts, (share + 1) * many);
-    float acc = 0.f, sum = 0.f;
-#pragma unroll 8
-    for (int i = share * many; i < end; ++i) {
-        const float pm = p.part_ml[at(i) * 2], f = pm == -INFINITY ? 0.f : exp2_fast(pm - mx);
-        sum += p.part_ml[at(i) * 2 + 1] * f;
-        acc += p.part_o[at(i) * D + d] * f;
-    }
-    if constexpr (SHARES > 1) {
-        sh_o[share][d] = acc;
-        if (d == 0) sh_l[share] = sum;
-        __syncthreads();
-        if (share != 0) return;
-        acc = sum = 0.f;
+    for (int w = 0; w < MERGE_WARPS; ++w) total += sh_l[w];
+    const int tok = c / p.group;
+    bf16* out = p.out + ((size_t)(p.q_start[e] + tok) * p.n_q + g * p.group + (c - tok * p.group)) * D;
+    for (int d = threadIdx.x; d < D; d += MERGE_WARPS * 32) {
+        float v = 0.f;
 #pragma unroll
-        for (int i = 0; i < SHARES; ++i) { acc += sh_o[i][d]; sum += sh_l[i]; }
+        for (int w = 0; w < MERGE_WARPS; ++w) v += sh_o[w][d];
+        out[d] = __float2bfloat16_rn(total > 0.f ? v / total : 0.f);
     }
-    const int tok = c / group;
-    p.out[((size_t)(qs + tok) * p.n_q + row.y * group + (c - tok * group)) * D + d] = __float2bfloat16_rn(sum > 0.f ? acc / sum : 0.f);
 }
 
 template <int D, int BITS, int NT> constexpr size_t smem_bytes() {
@@ -682,19 +738,18 @@ template <int D, int BITS, int NT, bool TILES> int wave() {
 }
 template <int D, int BITS, int NT, bool TILES> int launch(Params p, long long steps_of_row, cudaStream_t s) {
     constexpr size_t smem = smem_bytes<D, BITS, NT>();
-    constexpr int COLS = 8 * NT, FEW = D < 128 ? 128 / D : 1, MANY = 512 / D;
+    constexpr int COLS = 8 * NT;
     const int wave_ctas = wave<D, BITS, NT, TILES>();
-    const long long rows = (long long)p.entries * p.most_blocks, steps = rows * steps_of_row;
-    p.ctas = (int)(steps < wave_ctas ? steps : wave_ctas);
-    p.by_row = rows <= p.ctas ? 1 : 0;
+    const long long rows = (long long)p.entries * p.most_blocks, units = rows * (steps_of_row + ROW_COST);
+    p.ctas = (int)(units < wave_ctas ? units : wave_ctas);
     if (const int e = kipp_allow_smem(attn_quant_kernel<D, BITS, NT, TILES>, smem)) return e;
     if (const int e = kipp_launch(attn_quant_kernel<D, BITS, NT, TILES>, dim3((unsigned)p.ctas), dim3(THREADS), smem, s, 1, p)) return e;
     if (steps_of_row <= 1) return 0;                   // every row is one step: none is shared
-    const int columns = p.most * (p.n_q / p.n_kv);
-    const dim3 grid((unsigned)(p.by_row ? rows : p.ctas), (unsigned)(columns < COLS ? columns : COLS));
-    // (a row of few is cut into many parts)
-    if (rows * 8 <= p.ctas) return kipp_launch(attn_quant_merge_kernel<D, NT, MANY>, grid, dim3(D * MANY), 0, s, 1, p);
-    return kipp_launch(attn_quant_merge_kernel<D, NT, FEW>, grid, dim3(D * FEW), 0, s, 1, p);
+    const int columns = p.most * p.group, y = columns < COLS ? columns : COLS;
+    // a block a row, or a CTA where those are fewer; rows of few are cut into many parts
+    if (rows > p.ctas) return kipp_launch(attn_quant_merge_kernel<D, NT, 2, false>, dim3((unsigned)p.ctas, (unsigned)y), dim3(64), 0, s, 1, p);
+    if (rows * 16 > p.ctas) return kipp_launch(attn_quant_merge_kernel<D, NT, 4, true>, dim3((unsigned)rows, (unsigned)y), dim3(128), 0, s, 1, p);
+    return kipp_launch(attn_quant_merge_kernel<D, NT, 16, true>, dim3((unsigned)rows, (unsigned)y), dim3(512), 0, s, 1, p);
 }
 
 // 8 columns where they hold every query of a kv head, else 16 (heads of 256 have no room for their sums: always 8)
@@ -707,7 +762,7 @@ extern "C" int kipp_attn_quant_supported(int bits, int head_dim, int n_q, int n_
 }
 // Bytes of scratch of a launch (the parts of rows that several CTAs share), whatever the step.
 extern "C" long long kipp_attn_quant_scratch_bytes(int head_dim) {
-    return 2LL * MOST_CTAS * MOST_COLUMNS * (head_dim + 2) * 4 + MOST_CTAS * 16LL;
+    return 2LL * MOST_CTAS * MOST_COLUMNS * (head_dim + 2) * 4;
 }
 
 // out, q: bf16 [tokens][n_q][head_dim].  The entries that bring 1 to `most` tokens; the others are left alone.
@@ -725,7 +780,7 @@ extern "C" int kipp_attn_quant(void* out, const void* q, const void* k_codes, co
     const long long cols = columns_of(head_dim, (long long)most * (n_q / n_kv));
     const long long room = (long long)table_width * page_size, steps = (room + STEP - 1) / STEP;
     const long long blocks = n_kv * (((long long)most * (n_q / n_kv) + cols - 1) / cols);
-    if ((long long)n_pages * n_kv * page_size > 0x7fffffffLL || room > 0x7fffffffLL || blocks > 0x3fffffffLL / entries / steps ||
+    if ((long long)n_pages * n_kv * page_size > 0x7fffffffLL || room > 0x7fffffffLL || blocks > 0x3fffffffLL / entries / (steps + ROW_COST) ||
         (long long)most * n_q > 0x3fffffffLL)
         return KIPP_ERR_ARG;
     Params p = {};
@@ -741,7 +796,6 @@ extern "C" int kipp_attn_quant(void* out, const void* q, const void* k_codes, co
     p.query_scale = scale < 0.f ? -0x1p60f : 0x1p60f;
     p.part_o = (float*)scratch;
     p.part_ml = p.part_o + 2LL * MOST_CTAS * MOST_COLUMNS * head_dim;
-    p.shared_rows = (int4*)(p.part_ml + 2LL * MOST_CTAS * MOST_COLUMNS * 2);
     p.most_blocks = (int)blocks;
     p.status = status;
     cudaStream_t s = (cudaStream_t)stream;
