@@ -188,14 +188,16 @@ template <int D, int BITS> struct Shape {
     static constexpr int CHUNKS = RB / 16;
     static constexpr int K_BYTES = RB / 4, V_BYTES = RB / 8; // a lane's stretch of a key's row and of a value's
     static constexpr int WARP_STAGE = WARP_KEYS * 2 * (RB + SB);
-    // steps in the ring, and CTAs an SM: 228 KB hold four of three steps of 4.5 KB a warp (heads of 128 in 4 bits)
-    static constexpr int STAGES = WARP_STAGE <= 2560 ? 4 : RB == 128 && D == 128 ? 2 : 3;
+    // Steps in the ring, and CTAs an SM (ctas_per_sm).  Heads of 128: three CTAs of 168 registers a thread and four steps (4 bits,
+    // 8 tokens of 8,100 keys 26.1 us; four CTAs of 128 registers and three steps 28.5).  A step's scores made beside the one before's
+    // values, two streams of instructions, gave nothing (26.1).
+    static constexpr int STAGES = RB == 128 && D == 128 ? 2 : D == 256 ? 3 : 4;
     static constexpr float L = BITS == 4 ? 8.f : 128.f;
 };
 template <int D, int NT> constexpr int q_bytes() { return NT * (D / 32) * 32 * 24; }          // the queries of a piece as operands
 template <int D, int BITS, int NT> constexpr bool q_in_ring() { return q_bytes<D, NT>() <= Shape<D, BITS>::WARP_STAGE; }
 template <int D, int BITS, int NT> constexpr int ctas_per_sm() {
-    return D == 256 ? (BITS == 4 ? 2 : 1) : NT == 2 ? (D == 64 ? 3 : 2) : D == 128 && BITS == 8 ? 3 : 4;
+    return D == 256 ? (BITS == 4 ? 2 : 1) : NT == 2 ? (D == 64 ? 3 : 2) : D == 128 ? 3 : 4;
 }
 
 // Row r of the products (S^T's rows, P^T's and V's inner dimension) is key 4 (2 h + e) + t of a tile of 16, for
@@ -395,6 +397,150 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             l[nt][0] = l[nt][1] = 0.f;
         }
 
+        float s[NT][2][4];                                     // scores of a step, to be multiplied by score_scale for units of log2
+        uint32_t w[NT][2][2];                                  // its weights as operands
+        // The rows of a step that no column sees may hold anything: their scales become 0 (their codes are numbers anyhow).
+        auto arrived = [&](int j0, uint8_t* tile) {
+            const int j = j0 + lane;
+            if (j > see_hi || j < see_lo) {
+#pragma unroll
+                for (int k = 0; k < SB / 4; ++k) {
+                    *reinterpret_cast<uint32_t*>(tile + KS_AT + lane * SB + 4 * k) = 0u;
+                    *reinterpret_cast<uint32_t*>(tile + VS_AT + lane * SB + 4 * k) = 0u;
+                }
+            }
+            __syncwarp();
+        };
+        auto scores = [&](const uint8_t* tile) {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+                uint32_t w0[S::K_BYTES / 4], w1[S::K_BYTES / 4];
+                const uint8_t* r0 = tile + (mt * 16 + key_of_row(g4)) * RB + t4 * S::K_BYTES;
+                take<S::K_BYTES>(w0, r0);
+                take<S::K_BYTES>(w1, r0 + 8 * RB);
+                uint32_t a0[SB / 4], a1[SB / 4];
+                take<SB>(a0, tile + KS_AT + (mt * 16 + key_of_row(g4)) * SB);
+                take<SB>(a1, tile + KS_AT + (mt * 16 + key_of_row(g4) + 8) * SB);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.f;
+#pragma unroll
+                for (int gi = 0; gi < G; ++gi) {
+                    uint32_t x0[4], x1[4];
+                    if constexpr (BITS == 4) {
+                        spread<4>(x0, w0[gi >> 1], w0[(gi + G) >> 1], gi & 1);
+                        spread<4>(x1, w1[gi >> 1], w1[(gi + G) >> 1], gi & 1);
+                    } else {
+                        spread<8>(x0, w0[gi], w0[gi + G], 0);
+                        spread<8>(x1, w1[gi], w1[gi + G], 0);
+                    }
+                    const float f0 = gi & 1 ? high_f32(a0[gi >> 1]) : low_f32(a0[gi >> 1]);
+                    const float f1 = gi & 1 ? high_f32(a1[gi >> 1]) : low_f32(a1[gi >> 1]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float c[4];
+                        mma(c, x0[0], x1[0], x0[1], x1[1], qf[nt][gi][0], qf[nt][gi][1], offset[nt][gi][0], offset[nt][gi][1],
+                            offset[nt][gi][0], offset[nt][gi][1]);
+                        mma(c, x0[2], x1[2], x0[3], x1[3], qf[nt][gi][2], qf[nt][gi][3]);
+                        s[nt][mt][0] = fmaf(f0, c[0], s[nt][mt][0]);
+                        s[nt][mt][1] = fmaf(f0, c[1], s[nt][mt][1]);
+                        s[nt][mt][2] = fmaf(f1, c[2], s[nt][mt][2]);
+                        s[nt][mt][3] = fmaf(f1, c[3], s[nt][mt][3]);
+                    }
+                }
+            }
+        };
+        auto weights = [&](int j0, bool cut) {
+            bool raise = false;
+            float top[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                if (cut) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int pos = en.context + min(column0 + nt * 8 + 2 * t4 + c, columns - 1) / group;
+                        const int hi = min(pos, see_hi), lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+#pragma unroll
+                        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const int j = j0 + mt * 16 + key_of_row(g4) + h * 8;
+                                if (j > hi || j < lo) s[nt][mt][2 * h + c] = -INFINITY;
+                            }
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    top[nt][c] = fmaxf(fmaxf(s[nt][0][c], s[nt][0][2 + c]), fmaxf(s[nt][1][c], s[nt][1][2 + c])) * p.score_scale;
+                    raise |= top[nt][c] > m[nt][c] + 8.f;
+                }
+            }
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float f[2];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float mx = fmaxf(m[nt][c], top[nt][c]);
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        f[c] = m[nt][c] == -INFINITY ? 0.f : exp2_fast(m[nt][c] - mx);
+                        m[nt][c] = mx;
+                        l[nt][c] *= f[c];
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        ones[nt][k] *= f[k & 1];
+#pragma unroll
+                        for (int d = 0; d < 2 * G; ++d) o[nt][d][k] *= f[k & 1];
+                    }
+                }
+            }
+            // (times 2^60)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float back[2] = {(m[nt][0] == -INFINITY ? 0.f : m[nt][0]) - 60.f, (m[nt][1] == -INFINITY ? 0.f : m[nt][1]) - 60.f};
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt) {
+                    float e[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        e[k] = exp2_fast(fmaf(s[nt][mt][k], p.score_scale, -back[k & 1]));
+                        l[nt][k & 1] += e[k];
+                    }
+                    w[nt][mt][0] = transposed(pack2(e[0], e[1]));
+                    w[nt][mt][1] = transposed(pack2(e[2], e[3]));
+                }
+            }
+        };
+        auto add_values = [&](const uint8_t* tile) {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+                uint32_t v[4][S::V_BYTES / 4], f[4][SB / 4];           // keys t, 4 + t, 8 + t, 12 + t
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    take<S::V_BYTES>(v[k], tile + V_AT + (mt * 16 + 4 * k + t4) * RB + g4 * S::V_BYTES);
+                    take<SB>(f[k], tile + VS_AT + (mt * 16 + 4 * k + t4) * SB);
+                }
+#pragma unroll
+                for (int gi = 0; gi < G; ++gi) {
+                    uint32_t x0[4], x1[4];                             // keys of the first and the second half of the rows
+                    constexpr int W = BITS == 4 ? 1 : 0;
+                    spread<BITS>(x0, v[0][gi >> W], v[1][gi >> W], gi & 1);
+                    spread<BITS>(x1, v[2][gi >> W], v[3][gi >> W], gi & 1);
+                    const uint32_t f0 = __byte_perm(f[0][gi >> 1], f[1][gi >> 1], gi & 1 ? 0x7632 : 0x5410);
+                    const uint32_t f1 = __byte_perm(f[2][gi >> 1], f[3][gi >> 1], gi & 1 ? 0x7632 : 0x5410);
+                    const uint32_t one = g4 == gi ? 0x3f803f80u : 0u;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint32_t b0 = times2(w[nt][mt][0], f0), b1 = times2(w[nt][mt][1], f1);
+                        mma(o[nt][2 * gi], x0[0], x0[1], x1[0], x1[1], b0, b1);
+                        mma(o[nt][2 * gi + 1], x0[2], x0[3], x1[2], x1[3], b0, b1);
+                        mma(ones[nt], one, 0u, one, 0u, b0, b1);
+                    }
+                }
+            }
+        };
         for (int i = 0; i < n; ++i) {
             if (i + STAGES - 1 < n) fetch(i + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
             cp_async_commit();
@@ -405,149 +551,10 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             // (the warps of a step may all be outside what is seen, but for one)
             if (j0 <= see_hi && j0 + WARP_KEYS > see_lo) {
                 const bool cut = j0 + WARP_KEYS - 1 > all_hi || j0 < all_lo;
-                if (cut) {
-                    // rows that no column sees may hold anything: their scales become 0 (their codes are numbers anyhow)
-                    const int j = j0 + lane;
-                    if (j > see_hi || j < see_lo) {
-#pragma unroll
-                        for (int k = 0; k < SB / 4; ++k) {
-                            *reinterpret_cast<uint32_t*>(tile + KS_AT + lane * SB + 4 * k) = 0u;
-                            *reinterpret_cast<uint32_t*>(tile + VS_AT + lane * SB + 4 * k) = 0u;
-                        }
-                    }
-                    __syncwarp();
-                }
-                // -- scores, to be multiplied by score_scale for units of log2
-                float s[NT][2][4];
-#pragma unroll
-                for (int mt = 0; mt < 2; ++mt) {
-                    uint32_t w0[S::K_BYTES / 4], w1[S::K_BYTES / 4];
-                    const uint8_t* r0 = tile + (mt * 16 + key_of_row(g4)) * RB + t4 * S::K_BYTES;
-                    take<S::K_BYTES>(w0, r0);
-                    take<S::K_BYTES>(w1, r0 + 8 * RB);
-                    uint32_t a0[SB / 4], a1[SB / 4];
-                    take<SB>(a0, tile + KS_AT + (mt * 16 + key_of_row(g4)) * SB);
-                    take<SB>(a1, tile + KS_AT + (mt * 16 + key_of_row(g4) + 8) * SB);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.f;
-#pragma unroll
-                    for (int gi = 0; gi < G; ++gi) {
-                        uint32_t x0[4], x1[4];
-                        if constexpr (BITS == 4) {
-                            spread<4>(x0, w0[gi >> 1], w0[(gi + G) >> 1], gi & 1);
-                            spread<4>(x1, w1[gi >> 1], w1[(gi + G) >> 1], gi & 1);
-                        } else {
-                            spread<8>(x0, w0[gi], w0[gi + G], 0);
-                            spread<8>(x1, w1[gi], w1[gi + G], 0);
-                        }
-                        const float f0 = gi & 1 ? high_f32(a0[gi >> 1]) : low_f32(a0[gi >> 1]);
-                        const float f1 = gi & 1 ? high_f32(a1[gi >> 1]) : low_f32(a1[gi >> 1]);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            float c[4];
-                            mma(c, x0[0], x1[0], x0[1], x1[1], qf[nt][gi][0], qf[nt][gi][1], offset[nt][gi][0], offset[nt][gi][1],
-                                offset[nt][gi][0], offset[nt][gi][1]);
-                            mma(c, x0[2], x1[2], x0[3], x1[3], qf[nt][gi][2], qf[nt][gi][3]);
-                            s[nt][mt][0] = fmaf(f0, c[0], s[nt][mt][0]);
-                            s[nt][mt][1] = fmaf(f0, c[1], s[nt][mt][1]);
-                            s[nt][mt][2] = fmaf(f1, c[2], s[nt][mt][2]);
-                            s[nt][mt][3] = fmaf(f1, c[3], s[nt][mt][3]);
-                        }
-                    }
-                }
-                bool raise = false;
-                float top[NT][2];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    if (cut) {
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const int pos = en.context + min(column0 + nt * 8 + 2 * t4 + c, columns - 1) / group;
-                            const int hi = min(pos, see_hi), lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-#pragma unroll
-                            for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                                for (int h = 0; h < 2; ++h) {
-                                    const int j = j0 + mt * 16 + key_of_row(g4) + h * 8;
-                                    if (j > hi || j < lo) s[nt][mt][2 * h + c] = -INFINITY;
-                                }
-                        }
-                    }
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        top[nt][c] = fmaxf(fmaxf(s[nt][0][c], s[nt][0][2 + c]), fmaxf(s[nt][1][c], s[nt][1][2 + c])) * p.score_scale;
-                        raise |= top[nt][c] > m[nt][c] + 8.f;
-                    }
-                }
-                if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float f[2];
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            float mx = fmaxf(m[nt][c], top[nt][c]);
-                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                            f[c] = m[nt][c] == -INFINITY ? 0.f : exp2_fast(m[nt][c] - mx);
-                            m[nt][c] = mx;
-                            l[nt][c] *= f[c];
-                        }
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            ones[nt][k] *= f[k & 1];
-#pragma unroll
-                            for (int d = 0; d < 2 * G; ++d) o[nt][d][k] *= f[k & 1];
-                        }
-                    }
-                }
-                // -- weights (times 2^60), and the weighted sums
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const float back = (m[nt][c] == -INFINITY ? 0.f : m[nt][c]) - 60.f;
-#pragma unroll
-                        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const float w = exp2_fast(fmaf(s[nt][mt][2 * h + c], p.score_scale, -back));
-                                s[nt][mt][2 * h + c] = w;
-                                l[nt][c] += w;
-                            }
-                    }
-#pragma unroll
-                for (int mt = 0; mt < 2; ++mt) {
-                    uint32_t v[4][S::V_BYTES / 4], f[4][SB / 4];       // keys t, 4 + t, 8 + t, 12 + t
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        take<S::V_BYTES>(v[k], tile + V_AT + (mt * 16 + 4 * k + t4) * RB + g4 * S::V_BYTES);
-                        take<SB>(f[k], tile + VS_AT + (mt * 16 + 4 * k + t4) * SB);
-                    }
-                    uint32_t w[NT][2];
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        w[nt][0] = transposed(pack2(s[nt][mt][0], s[nt][mt][1]));
-                        w[nt][1] = transposed(pack2(s[nt][mt][2], s[nt][mt][3]));
-                    }
-#pragma unroll
-                    for (int gi = 0; gi < G; ++gi) {
-                        uint32_t x0[4], x1[4];                         // keys of the first and the second half of the rows
-                        constexpr int W = BITS == 4 ? 1 : 0;
-                        spread<BITS>(x0, v[0][gi >> W], v[1][gi >> W], gi & 1);
-                        spread<BITS>(x1, v[2][gi >> W], v[3][gi >> W], gi & 1);
-                        const uint32_t f0 = __byte_perm(f[0][gi >> 1], f[1][gi >> 1], gi & 1 ? 0x7632 : 0x5410);
-                        const uint32_t f1 = __byte_perm(f[2][gi >> 1], f[3][gi >> 1], gi & 1 ? 0x7632 : 0x5410);
-                        const uint32_t one = g4 == gi ? 0x3f803f80u : 0u;
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            const uint32_t b0 = times2(w[nt][0], f0), b1 = times2(w[nt][1], f1);
-                            mma(o[nt][2 * gi], x0[0], x0[1], x1[0], x1[1], b0, b1);
-                            mma(o[nt][2 * gi + 1], x0[2], x0[3], x1[2], x1[3], b0, b1);
-                            mma(ones[nt], one, 0u, one, 0u, b0, b1);
-                        }
-                    }
-                }
+                if (cut) arrived(j0, tile);
+                scores(tile);
+                weights(j0, cut);
+                add_values(tile);
             }
             __syncwarp();
             stage = stage + 1 == STAGES ? 0 : stage + 1;
