@@ -772,40 +772,52 @@ extern "C" long long kipp_attn_quant_scratch_bytes(int head_dim) {
     return 2LL * MOST_CTAS * MOST_COLUMNS * (head_dim + 2) * 4;
 }
 
-// out, q: bf16 [tokens][n_q][head_dim].  The entries that bring 1 to `most` tokens; the others are left alone.
-extern "C" int kipp_attn_quant(void* out, const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
-                               const void* v_scales, int bits, int n_pages, int page_size, const int* q_start, const int* context_len,
-                               const int* block_table, int table_width, int entries, int most, int n_q, int n_kv, int head_dim,
-                               float scale, int window, void* scratch, long long scratch_bytes, int* status, void* stream) {
+struct KippAttnQuant {
+    void* out; const void* q;                           // bf16 [tokens][n_q][head_dim]
+    const void *k_codes, *k_scales, *v_codes, *v_scales;
+    const int *q_start, *context_len, *block_table;
+    void* scratch;
+    int* status;
+    void* stream;
+    long long scratch_bytes;
+    int bits, n_pages, page_size, table_width, entries, most, n_q, n_kv, head_dim, window;
+    float scale;
+};
+
+// The entries that bring 1 to `most` tokens; the others are left alone.
+extern "C" int kipp_attn_quant(const KippAttnQuant* a) {
+    const int bits = a->bits, head_dim = a->head_dim, n_q = a->n_q, n_kv = a->n_kv, entries = a->entries, most = a->most, page_size = a->page_size;
     if (entries <= 0 || most <= 0) return 0;
-    if (!kipp_attn_quant_supported(bits, head_dim, n_q, n_kv) || page_size <= 0 || n_pages <= 0 || table_width <= 0 || window < 0 ||
-        status == nullptr || scratch == nullptr)
+    if (!kipp_attn_quant_supported(bits, head_dim, n_q, n_kv) || page_size <= 0 || a->n_pages <= 0 || a->table_width <= 0 || a->window < 0 ||
+        a->status == nullptr || a->scratch == nullptr)
         return KIPP_ERR_ARG;
-    if (scratch_bytes < kipp_attn_quant_scratch_bytes(head_dim)) return -4;
-    if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scales | (uintptr_t)v_scales | (uintptr_t)scratch) & 15) != 0) return -3;
+    if (a->scratch_bytes < kipp_attn_quant_scratch_bytes(head_dim)) return -4;
+    if ((((uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->k_codes | (uintptr_t)a->v_codes | (uintptr_t)a->k_scales | (uintptr_t)a->v_scales |
+          (uintptr_t)a->scratch) & 15) != 0)
+        return -3;
     // (row numbers of pages and steps of all rows are 32-bit)
     const long long cols = columns_of(head_dim, (long long)most * (n_q / n_kv));
-    const long long room = (long long)table_width * page_size, steps = (room + STEP - 1) / STEP;
+    const long long room = (long long)a->table_width * page_size, steps = (room + STEP - 1) / STEP;
     const long long blocks = n_kv * (((long long)most * (n_q / n_kv) + cols - 1) / cols);
-    if ((long long)n_pages * n_kv * page_size > 0x7fffffffLL || room > 0x7fffffffLL || blocks > 0x3fffffffLL / entries / (steps + ROW_COST) ||
-        (long long)most * n_q > 0x3fffffffLL)
+    if ((long long)a->n_pages * n_kv * page_size > 0x7fffffffLL || room > 0x7fffffffLL ||
+        blocks > 0x3fffffffLL / entries / (steps + ROW_COST) || (long long)most * n_q > 0x3fffffffLL)
         return KIPP_ERR_ARG;
     Params p = {};
-    p.out = (bf16*)out; p.q = (const bf16*)q;
-    p.k_codes = (const uint8_t*)k_codes; p.k_scales = (const uint8_t*)k_scales;
-    p.v_codes = (const uint8_t*)v_codes; p.v_scales = (const uint8_t*)v_scales;
-    p.q_start = q_start; p.context_len = context_len; p.block_table = block_table;
-    p.entries = entries; p.table_width = table_width; p.page_size = page_size; p.n_pages = n_pages; p.most = most;
+    p.out = (bf16*)a->out; p.q = (const bf16*)a->q;
+    p.k_codes = (const uint8_t*)a->k_codes; p.k_scales = (const uint8_t*)a->k_scales;
+    p.v_codes = (const uint8_t*)a->v_codes; p.v_scales = (const uint8_t*)a->v_scales;
+    p.q_start = a->q_start; p.context_len = a->context_len; p.block_table = a->block_table;
+    p.entries = entries; p.table_width = a->table_width; p.page_size = page_size; p.n_pages = a->n_pages; p.most = most;
     p.page_shift = -1;
     for (int i = 0; i < 31; ++i) if (page_size == 1 << i) p.page_shift = i;
-    p.n_q = n_q; p.n_kv = n_kv; p.group = n_q / n_kv; p.window = window;
-    p.score_scale = fabsf(scale) * 1.4426950408889634f * 0x1p73f;
-    p.query_scale = scale < 0.f ? -0x1p60f : 0x1p60f;
-    p.part_o = (float*)scratch;
+    p.n_q = n_q; p.n_kv = n_kv; p.group = n_q / n_kv; p.window = a->window;
+    p.score_scale = fabsf(a->scale) * 1.4426950408889634f * 0x1p73f;
+    p.query_scale = a->scale < 0.f ? -0x1p60f : 0x1p60f;
+    p.part_o = (float*)a->scratch;
     p.part_ml = p.part_o + 2LL * MOST_CTAS * MOST_COLUMNS * head_dim;
     p.most_blocks = (int)blocks;
-    p.status = status;
-    cudaStream_t s = (cudaStream_t)stream;
+    p.status = a->status;
+    cudaStream_t s = (cudaStream_t)a->stream;
 #define KIPP_CASE(d, b)                                                                                            \
     if (head_dim == d && bits == b) {                                                                              \
         if (cols == 8) return page_size % 16 == 0 ? launch<d, b, 1, true>(p, steps, s) : launch<d, b, 1, false>(p, steps, s);        \

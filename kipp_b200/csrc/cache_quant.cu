@@ -330,24 +330,53 @@ bool pages_ok(const QuantPages& g, int bits, int head_dim) {
 }
 }  // namespace
 
-// Norm, rotation and the write of a step's keys and values as codes; queries to q_out
-// [tokens][n_q][head_dim] in the projection's type.  write_cache 0: queries only.
-extern "C" int kipp_quant_cache_write(const void* qkv, long long ld_qkv, void* q_out, void* k_codes, void* k_scales, void* v_codes,
-                                      void* v_scales, int bits, int n_pages, int page_size, int dtype, const void* q_norm_w,
-                                      const void* k_norm_w, int norm_dtype, float eps, const void* cos_sin, int rotary_dim,
-                                      const int* positions, const int* entry_of_token, const int* block_table, int table_width,
-                                      int tokens, int n_q, int n_kv, int head_dim, int write_cache, int* status, void* stream) {
-    if (tokens <= 0) return 0;
-    const QuantPages pages = {(uint8_t*)k_codes, (bf16*)k_scales, (uint8_t*)v_codes, (bf16*)v_scales, n_pages, page_size, n_kv};
-    if (!pages_ok(pages, bits, head_dim) || n_q <= 0 || (q_norm_w == nullptr) != (k_norm_w == nullptr) || rotary_dim < 0 ||
-        rotary_dim > head_dim || (rotary_dim & 1) || table_width <= 0 || status == nullptr || ld_qkv < (long long)(n_q + 2 * n_kv) * head_dim)
+// The arguments of the entry points, as one structure each (a caller that packs them spends a quarter of what passing them
+// one by one costs it from Python).
+struct KippQuantWrite {
+    const void* qkv; void* q_out;                       // [tokens][ld_qkv], [tokens][n_q][head_dim], of one type
+    void *k_codes, *k_scales, *v_codes, *v_scales;
+    const void *q_norm_w, *k_norm_w, *cos_sin;          // or null
+    const int *positions, *entry_of_token, *block_table;
+    int* status;
+    void* stream;
+    long long ld_qkv;
+    int bits, n_pages, page_size, dtype, norm_dtype, rotary_dim, table_width, tokens, n_q, n_kv, head_dim, write_cache;
+    float eps;
+};
+struct KippQuantRead {
+    void *k_out, *v_out;
+    const void *k_codes, *k_scales, *v_codes, *v_scales;
+    const int* list;                                    // pages
+    int* status;
+    void* stream;
+    int out_dtype, bits, n_pages, page_size, n, n_kv, head_dim;
+};
+struct KippQuantReadEntries {
+    void *k_out, *v_out;
+    int* table_out;
+    const void *k_codes, *k_scales, *v_codes, *v_scales;
+    const int *q_start, *context_len, *block_table;
+    int* status;
+    void* stream;
+    int out_dtype, bits, n_pages, page_size, table_width, first_entry, entries, window, n_kv, head_dim;
+};
+
+// Norm, rotation and the write of a step's keys and values as codes; queries to q_out in the projection's type.
+// write_cache 0: queries only.
+extern "C" int kipp_quant_cache_write(const KippQuantWrite* a) {
+    if (a->tokens <= 0) return 0;
+    const QuantPages pages = {(uint8_t*)a->k_codes, (bf16*)a->k_scales, (uint8_t*)a->v_codes, (bf16*)a->v_scales, a->n_pages, a->page_size, a->n_kv};
+    if (!pages_ok(pages, a->bits, a->head_dim) || a->n_q <= 0 || (a->q_norm_w == nullptr) != (a->k_norm_w == nullptr) || a->rotary_dim < 0 ||
+        a->rotary_dim > a->head_dim || (a->rotary_dim & 1) || a->table_width <= 0 || a->status == nullptr ||
+        a->ld_qkv < (long long)(a->n_q + 2 * a->n_kv) * a->head_dim)
         return KIPP_ERR_ARG;
-    if ((dtype != KIPP_DT_F32 && dtype != KIPP_DT_BF16) || (norm_dtype != KIPP_DT_F32 && norm_dtype != KIPP_DT_BF16)) return KIPP_ERR_DTYPE;
-    const WriteParams p = {qkv, ld_qkv, q_out, pages, q_norm_w, k_norm_w, norm_dtype, eps, rotary_dim > 0 ? (const float2*)cos_sin : nullptr,
-                           rotary_dim, positions, entry_of_token, block_table, table_width, tokens, n_q, head_dim, write_cache & 1, status};
-    cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == KIPP_DT_F32) return bits == 4 ? launch_write<float, 4>(p, s) : launch_write<float, 8>(p, s);
-    return bits == 4 ? launch_write<bf16, 4>(p, s) : launch_write<bf16, 8>(p, s);
+    if ((a->dtype != KIPP_DT_F32 && a->dtype != KIPP_DT_BF16) || (a->norm_dtype != KIPP_DT_F32 && a->norm_dtype != KIPP_DT_BF16)) return KIPP_ERR_DTYPE;
+    const WriteParams p = {a->qkv, a->ld_qkv, a->q_out, pages, a->q_norm_w, a->k_norm_w, a->norm_dtype, a->eps,
+                           a->rotary_dim > 0 ? (const float2*)a->cos_sin : nullptr, a->rotary_dim, a->positions, a->entry_of_token,
+                           a->block_table, a->table_width, a->tokens, a->n_q, a->head_dim, a->write_cache & 1, a->status};
+    cudaStream_t s = (cudaStream_t)a->stream;
+    if (a->dtype == KIPP_DT_F32) return a->bits == 4 ? launch_write<float, 4>(p, s) : launch_write<float, 8>(p, s);
+    return a->bits == 4 ? launch_write<bf16, 4>(p, s) : launch_write<bf16, 8>(p, s);
 }
 
 static bool read_aligned(const QuantPages& g, const void* k_out, const void* v_out) {
@@ -356,35 +385,30 @@ static bool read_aligned(const QuantPages& g, const void* k_out, const void* v_o
 
 // k_out and v_out [n][n_kv][page_size][head_dim] of out_dtype: what pages list[0 .. n) stand for.  A
 // negative number gives zeros.
-extern "C" int kipp_quant_cache_read(void* k_out, void* v_out, int out_dtype, const void* k_codes, const void* k_scales,
-                                     const void* v_codes, const void* v_scales, int bits, int n_pages, int page_size, const int* list,
-                                     int n, int n_kv, int head_dim, int* status, void* stream) {
-    if (n <= 0) return 0;
-    const QuantPages pages = {(uint8_t*)k_codes, (bf16*)k_scales, (uint8_t*)v_codes, (bf16*)v_scales, n_pages, page_size, n_kv};
-    if (!pages_ok(pages, bits, head_dim) || k_out == nullptr || v_out == nullptr || list == nullptr || status == nullptr) return KIPP_ERR_ARG;
-    if (out_dtype != KIPP_DT_F32 && out_dtype != KIPP_DT_BF16) return KIPP_ERR_DTYPE;
-    if (!read_aligned(pages, k_out, v_out)) return -3;
-    ReadParams p = {k_out, v_out, pages, list, n, head_dim, status, nullptr, nullptr, nullptr, 0, 0, 0};
-    return launch_read<false>(p, bits, out_dtype, (cudaStream_t)stream);
+extern "C" int kipp_quant_cache_read(const KippQuantRead* a) {
+    if (a->n <= 0) return 0;
+    const QuantPages pages = {(uint8_t*)a->k_codes, (bf16*)a->k_scales, (uint8_t*)a->v_codes, (bf16*)a->v_scales, a->n_pages, a->page_size, a->n_kv};
+    if (!pages_ok(pages, a->bits, a->head_dim) || a->k_out == nullptr || a->v_out == nullptr || a->list == nullptr || a->status == nullptr)
+        return KIPP_ERR_ARG;
+    if (a->out_dtype != KIPP_DT_F32 && a->out_dtype != KIPP_DT_BF16) return KIPP_ERR_DTYPE;
+    if (!read_aligned(pages, a->k_out, a->v_out)) return -3;
+    ReadParams p = {a->k_out, a->v_out, pages, a->list, a->n, a->head_dim, a->status, nullptr, nullptr, nullptr, 0, 0, 0};
+    return launch_read<false>(p, a->bits, a->out_dtype, (cudaStream_t)a->stream);
 }
 
 // The pages that the tokens of entries first_entry .. first_entry + entries - 1 see, read back into pages of
 // their own (entry by entry, table_width pages each), and the block table of those: table_out has the
 // step's shape and only those entries' rows are written.  The pages no token sees are neither read nor
 // written; their table entries are -1.
-extern "C" int kipp_quant_cache_read_entries(void* k_out, void* v_out, int* table_out, int out_dtype, const void* k_codes,
-                                             const void* k_scales, const void* v_codes, const void* v_scales, int bits, int n_pages,
-                                             int page_size, const int* q_start, const int* context_len, const int* block_table,
-                                             int table_width, int first_entry, int entries, int window, int n_kv, int head_dim,
-                                             int* status, void* stream) {
-    if (entries <= 0) return 0;
-    const QuantPages pages = {(uint8_t*)k_codes, (bf16*)k_scales, (uint8_t*)v_codes, (bf16*)v_scales, n_pages, page_size, n_kv};
-    if (!pages_ok(pages, bits, head_dim) || k_out == nullptr || v_out == nullptr || table_out == nullptr || status == nullptr ||
-        table_width <= 0 || first_entry < 0 || window < 0 || (long long)entries * table_width > 65535)
+extern "C" int kipp_quant_cache_read_entries(const KippQuantReadEntries* a) {
+    if (a->entries <= 0) return 0;
+    const QuantPages pages = {(uint8_t*)a->k_codes, (bf16*)a->k_scales, (uint8_t*)a->v_codes, (bf16*)a->v_scales, a->n_pages, a->page_size, a->n_kv};
+    if (!pages_ok(pages, a->bits, a->head_dim) || a->k_out == nullptr || a->v_out == nullptr || a->table_out == nullptr || a->status == nullptr ||
+        a->table_width <= 0 || a->first_entry < 0 || a->window < 0 || (long long)a->entries * a->table_width > 65535)
         return KIPP_ERR_ARG;
-    if (out_dtype != KIPP_DT_F32 && out_dtype != KIPP_DT_BF16) return KIPP_ERR_DTYPE;
-    if (!read_aligned(pages, k_out, v_out)) return -3;
-    ReadParams p = {k_out, v_out, pages, block_table, entries * table_width, head_dim, status, table_out, q_start, context_len, table_width,
-                    first_entry, window};
-    return launch_read<true>(p, bits, out_dtype, (cudaStream_t)stream);
+    if (a->out_dtype != KIPP_DT_F32 && a->out_dtype != KIPP_DT_BF16) return KIPP_ERR_DTYPE;
+    if (!read_aligned(pages, a->k_out, a->v_out)) return -3;
+    ReadParams p = {a->k_out, a->v_out, pages, a->block_table, a->entries * a->table_width, a->head_dim, a->status, a->table_out, a->q_start,
+                    a->context_len, a->table_width, a->first_entry, a->window};
+    return launch_read<true>(p, a->bits, a->out_dtype, (cudaStream_t)a->stream);
 }

@@ -5,13 +5,14 @@ pages of it back, ``attention_quantized`` is ``attention`` over it."""
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
 
 from .ops import KernelError, _check, _fn, _ptr, c_float, c_int, c_void_p, dtype_code, rope_table
 
-c_ll = ctypes.c_longlong
+c_ll, c_char_p = ctypes.c_longlong, ctypes.c_char_p
 READ_BYTES = 1 << 30          # most bytes of keys and values that attention reads back at a time
 
 
@@ -20,29 +21,32 @@ class QuantizedPages:
     ``[pages, n_kv, page_size, D / 32]`` of keys and of values.  D is a multiple of 32, at most 512."""
 
     def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor, bits: int):
-        if bits not in (4, 8):
+        if bits != 4 and bits != 8:
             raise KernelError(f"a quantised cache holds 8 or 4 bits, not {bits}")
-        if k_codes.dtype != torch.uint8 or v_codes.dtype != torch.uint8 or k_scales.dtype != torch.bfloat16 or v_scales.dtype != torch.bfloat16:
+        u8, bf16 = torch.uint8, torch.bfloat16
+        if k_codes.dtype != u8 or v_codes.dtype != u8 or k_scales.dtype != bf16 or v_scales.dtype != bf16:
             raise KernelError("QuantizedPages: codes are uint8 and scales bfloat16")
-        shape, s_shape, device = k_codes.shape, k_scales.shape, k_codes.get_device()
-        if len(shape) != 4 or len(s_shape) != 4 or shape[:3] != s_shape[:3] or v_codes.shape != shape or v_scales.shape != s_shape:
-            raise KernelError("QuantizedPages: codes and scales are [pages, n_kv, page_size, ..], keys and values alike")
+        shape, device = k_codes.shape, k_codes.get_device()
+        if len(shape) != 4:
+            raise KernelError("QuantizedPages: codes and scales are [pages, n_kv, page_size, ..]")
+        n_pages, n_kv, page_size, row = shape
+        D = row * 8 // bits
+        if D % 32 or D > 512 or n_pages <= 0 or n_kv <= 0 or page_size <= 0 or D <= 0:
+            raise KernelError(f"QuantizedPages: {n_pages} pages, {n_kv} heads, {page_size} tokens a page, {D} channels a head: heads are a "
+                              "multiple of 32 channels, at most 512")
+        s_shape = (n_pages, n_kv, page_size, D // 32)
+        if v_codes.shape != shape or k_scales.shape != s_shape or v_scales.shape != s_shape:
+            raise KernelError(f"QuantizedPages: keys and values must be alike, with scales {s_shape}")
         if not (k_codes.is_contiguous() and k_scales.is_contiguous() and v_codes.is_contiguous() and v_scales.is_contiguous()):
             raise KernelError("QuantizedPages: codes and scales must be contiguous")
         if k_scales.get_device() != device or v_codes.get_device() != device or v_scales.get_device() != device:
             raise KernelError("QuantizedPages: codes and scales must be on one device")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales, self.bits = k_codes, k_scales, v_codes, v_scales, bits
-        self.n_pages, self.n_kv, self.page_size, row = shape
-        self.head_dim = D = row * 8 // bits
-        if D % 32 or D > 512 or s_shape[3] * 32 != D:
-            raise KernelError(f"QuantizedPages: {D} channels and {s_shape[3]} scales a head; heads are a multiple of "
-                              "32 channels, at most 512, with a scale for every 32")
-        if min(shape) <= 0:
-            raise KernelError("QuantizedPages: no pages")
+        self.n_pages, self.n_kv, self.page_size, self.head_dim = n_pages, n_kv, page_size, D
         self.device_index = device
         # (what a launch is given: the tensors are held, so the addresses stay)
-        self.addresses = (k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr())
-        self.aligned = all(a % 16 == 0 for a in self.addresses)
+        self.addresses = a, b, c, d = k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr()
+        self.aligned = (a | b | c | d) % 16 == 0
 
     @classmethod
     def zeros(cls, n_pages: int, n_kv: int, page_size: int, head_dim: int, bits: int, device) -> "QuantizedPages":
@@ -76,14 +80,12 @@ def _lists(what: str, **tensors: torch.Tensor) -> None:
             raise KernelError(f"{what}: {name} must be a contiguous int32 tensor")
 
 
-_PAGES = [c_void_p] * 4 + [c_int] * 3                     # addresses, bits, pages, page size
-_WRITE = [c_void_p, c_ll, c_void_p, *_PAGES, c_int, c_void_p, c_void_p, c_int, c_float, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
-          c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]
-_READ = [c_void_p, c_void_p, c_int, *_PAGES, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]
-_READ_ENTRIES = [c_void_p, c_void_p, c_void_p, c_int, *_PAGES, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
-                 c_void_p, c_void_p]
-_ATTEND = [c_void_p, c_void_p, *_PAGES, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p,
-           c_ll, c_void_p, c_void_p]
+# the structures of the C entry points (csrc/cache_quant.cu, csrc/attention_quant.cu): addresses, then sizes
+_WRITE, _READ, _READ_ENTRIES, _ATTEND = (struct.Struct(f) for f in ("14Qq12if", "9Q7i", "12Q10i", "12Qq10if"))
+
+
+def _call(lib: str, name: str, packed: bytes, what: str) -> None:
+    _check(_fn(lib, name, [c_char_p])(packed), what)
 
 
 def qk_norm_rope_write_quantized(qkv: torch.Tensor, q_out: torch.Tensor, pages: QuantizedPages, q_norm_w: Optional[torch.Tensor],
@@ -95,7 +97,7 @@ def qk_norm_rope_write_quantized(qkv: torch.Tensor, q_out: torch.Tensor, pages: 
     ``block_table`` [entries, width].  ``cos_sin`` is the step's ``rope_table``; without it the table is made here.
     A position whose page is not mapped is not written: status word 0 becomes 2."""
     what, D, n_kv = "qk_norm_rope_write_quantized", pages.head_dim, pages.n_kv
-    shape, dtype, q_norm, k_norm, table, norm_dtype = qkv.shape, qkv.dtype, None, None, None, 0
+    shape, dtype, q_norm, k_norm, table, norm_dtype = qkv.shape, qkv.dtype, 0, 0, 0, 0
     if len(shape) != 2 or shape[1] != (n_q + 2 * n_kv) * D or shape[0] < tokens or qkv.stride(1) != 1:
         raise KernelError(f"{what}: qkv has the wrong shape")
     if q_out.dtype != dtype or not q_out.is_contiguous() or q_out.numel() < tokens * n_q * D:
@@ -126,10 +128,11 @@ def qk_norm_rope_write_quantized(qkv: torch.Tensor, q_out: torch.Tensor, pages: 
             raise KernelError(f"{what}: cos_sin must be contiguous float32 [tokens, rotary_dim / 2, 2] on the step's device")
         table = cos_sin.data_ptr()
     _status(status, what)
-    f = _fn("cache_quant", "kipp_quant_cache_write", _WRITE)
-    _check(f(qkv.data_ptr(), qkv.stride(0), q_out.data_ptr(), *pages.addresses, pages.bits, pages.n_pages, pages.page_size, dtype_code(dtype),
-             q_norm, k_norm, norm_dtype, eps, table, rotary_dim, positions.data_ptr(), entry_of_token.data_ptr(), block_table.data_ptr(),
-             block_table.shape[1], tokens, n_q, n_kv, D, 1 if write_cache else 0, status.data_ptr(), stream), what)
+    _call("cache_quant", "kipp_quant_cache_write",
+          _WRITE.pack(qkv.data_ptr(), q_out.data_ptr(), *pages.addresses, q_norm, k_norm, table, positions.data_ptr(),
+                      entry_of_token.data_ptr(), block_table.data_ptr(), status.data_ptr(), stream, qkv.stride(0), pages.bits, pages.n_pages,
+                      pages.page_size, dtype_code(dtype), norm_dtype, rotary_dim, block_table.shape[1], tokens, n_q, n_kv, D,
+                      1 if write_cache else 0, eps), what)
 
 
 def read_quantized_pages(k_out: torch.Tensor, v_out: torch.Tensor, pages: QuantizedPages, page_list: torch.Tensor,
@@ -144,9 +147,9 @@ def read_quantized_pages(k_out: torch.Tensor, v_out: torch.Tensor, pages: Quanti
         raise KernelError(f"{what}: k_out and v_out must be contiguous, of one dtype and {shape}")
     _status(status, what)
     stream = _launch_stream(what, pages.device_index, k_out, v_out, page_list, status)
-    f = _fn("cache_quant", "kipp_quant_cache_read", _READ)
-    _check(f(k_out.data_ptr(), v_out.data_ptr(), dtype_code(k_out.dtype), *pages.addresses, pages.bits, pages.n_pages, pages.page_size,
-             page_list.data_ptr(), n, pages.n_kv, pages.head_dim, status.data_ptr(), stream), what)
+    _call("cache_quant", "kipp_quant_cache_read",
+          _READ.pack(k_out.data_ptr(), v_out.data_ptr(), *pages.addresses, page_list.data_ptr(), status.data_ptr(), stream,
+                     dtype_code(k_out.dtype), pages.bits, pages.n_pages, pages.page_size, n, pages.n_kv, pages.head_dim), what)
 
 
 def _read_entries(pages: QuantizedPages, dtype: torch.dtype, meta, block_table: torch.Tensor, first: int, entries: int, window: int,
@@ -155,10 +158,10 @@ def _read_entries(pages: QuantizedPages, dtype: torch.dtype, meta, block_table: 
     width = block_table.shape[1]
     k = torch.empty((entries * width, pages.n_kv, pages.page_size, pages.head_dim), dtype=dtype, device=table.device)
     v = torch.empty_like(k)
-    f = _fn("cache_quant", "kipp_quant_cache_read_entries", _READ_ENTRIES)
-    _check(f(k.data_ptr(), v.data_ptr(), table.data_ptr(), dtype_code(dtype), *pages.addresses, pages.bits, pages.n_pages, pages.page_size,
-             meta.q_start.data_ptr(), meta.context_len.data_ptr(), block_table.data_ptr(), width, first, entries, window, pages.n_kv,
-             pages.head_dim, status.data_ptr(), stream), "read_entries")
+    _call("cache_quant", "kipp_quant_cache_read_entries",
+          _READ_ENTRIES.pack(k.data_ptr(), v.data_ptr(), table.data_ptr(), *pages.addresses, meta.q_start.data_ptr(),
+                             meta.context_len.data_ptr(), block_table.data_ptr(), status.data_ptr(), stream, dtype_code(dtype), pages.bits,
+                             pages.n_pages, pages.page_size, width, first, entries, window, pages.n_kv, pages.head_dim), "read_entries")
     return k, v
 
 
@@ -253,10 +256,10 @@ def _direct(out, q, pages, meta, block_table, n_q, scale, window, status, most: 
     if need is None:
         need = _scratch_bytes[D] = _fn("attention_quant", "kipp_attn_quant_scratch_bytes", [c_int], restype=c_ll)(D)
     scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
-    f = _fn("attention_quant", "kipp_attn_quant", _ATTEND)
-    _check(f(out.data_ptr(), q.data_ptr(), *pages.addresses, pages.bits, pages.n_pages, pages.page_size, meta.q_start.data_ptr(),
-             meta.context_len.data_ptr(), block_table.data_ptr(), block_table.shape[1], len(meta.q_lens), most, n_q, pages.n_kv, D, scale,
-             window, scratch.data_ptr(), need, status.data_ptr(), stream), "attn_quant")
+    _call("attention_quant", "kipp_attn_quant",
+          _ATTEND.pack(out.data_ptr(), q.data_ptr(), *pages.addresses, meta.q_start.data_ptr(), meta.context_len.data_ptr(),
+                       block_table.data_ptr(), scratch.data_ptr(), status.data_ptr(), stream, need, pages.bits, pages.n_pages,
+                       pages.page_size, block_table.shape[1], len(meta.q_lens), most, n_q, pages.n_kv, D, window, scale), "attn_quant")
 
 
 def _portions(out, q, pages, meta, block_table, n_q, scale, window, status, span, stream: int) -> None:
