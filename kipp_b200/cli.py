@@ -8,8 +8,8 @@ src/kipp_cli.c:571-610): --model, --decode, --temperature, --top-p, --top-k,
 --min-p, --seed, --top, --ctx.  The prompt is token ids (there is no
 tokenizer here): --prompt-ids (repeat it for several prompts), --prompt-file or
 --random-prompt.  --backend
-and --kv-quant have one value each here (cuda, the compute dtype's cache), so
---dtype stands in their place.  Output: ``generated\\t<ids>`` on stdout, the
+has one value here (cuda), so --dtype stands in its place; --kv-quant takes none (the compute
+dtype's cache), int8 and int4.  Output: ``generated\\t<ids>`` on stdout, the
 final top-N logits as ``rank\\tid\\tlogit``, and on stderr the line
 ``KIPP_METRIC backend=... prefill_tokens=... prefill_seconds=...
 decode_tokens=... decode_seconds=...`` (src/kipp_cli.c:1213-1217).
@@ -36,6 +36,8 @@ def build_parser() -> argparse.ArgumentParser:
     prompt.add_argument("--random-prompt", type=int, metavar="LEN", help="LEN seeded random token ids")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"],
                     help="compute precision (default bfloat16; float32 = true 32-bit path)")
+    ap.add_argument("--kv-quant", default="none", choices=["none", "int8", "int4"],
+                    help="bits of the cached keys and values, in groups of 32 channels (default none: the compute dtype)")
     ap.add_argument("--decode", type=int, default=0, help="greedy/sampled tokens to generate")
     ap.add_argument("--temperature", type=float, default=0.0, help="0 = greedy argmax (default)")
     ap.add_argument("--top-p", type=float, default=1.0, help="nucleus mass, 0 < F <= 1 (default 1)")
@@ -142,7 +144,7 @@ def main(argv=None) -> int:
         return 2
     llm = LLM(args.model if args.model is not None else config, dtype=args.dtype, device=args.device,
               kv_block_size=page, kv_tokens=cache_tokens, ctx=capacity, max_requests=max(len(prompts), 1),
-              max_batch_tokens=max(args.max_batch_tokens or args.chunk, 1), chunk=args.chunk, policy=args.policy,
+              max_batch_tokens=max(args.max_batch_tokens or args.chunk, 1), chunk=args.chunk, policy=args.policy, kv_quant=args.kv_quant,
               seed=args.weights_seed or 0, stop_token_ids=tuple(args.stop_token or ()),
               **({"sigma": init.get("sigma"), "norm_jitter": init.get("norm_jitter", 0.1)}
                  if args.model is None else {}))

@@ -227,7 +227,9 @@ private:
         PagedKVSpec spec;
         std::vector<long long> cache_keys;    // (cache id, mixer slot) of the runs that share these pools, in storage order
         int n_pages = 0;
-        DeviceBuffer k, v;                    // [caches, pages, kv_heads, page_size, head_dim (values: value dim)]
+        DeviceBuffer k, v;                    // [caches, pages, kv_heads, page_size, head_dim (values: value dim)], or codes
+        DeviceBuffer k_scales, v_scales;      // of codes: [caches, pages, kv_heads, page_size, head_dim / 32] bfloat16
+        size_t scale_stride = 0;              // bytes between two caches of those
         size_t cache_stride = 0;              // bytes between two caches of the group's keys
         size_t value_stride = 0;              // ... and of its values
     };
@@ -260,6 +262,7 @@ private:
 
     void check_memory(const std::vector<TensorSpec>& specs);
     size_t workspace_estimate() const;
+    size_t cache_row_bytes(const PagedKVSpec& spec) const;
     void build_cache();
     void validate(const StepEntryView* entries, int n, StepShape& shape, std::vector<int>& rows);
     std::vector<int> table_widths(const std::vector<int64_t>& rids, int bucket) const;
@@ -330,7 +333,7 @@ inline void AttentionMixer::forward(StepContext& ctx, const LayerRun& run, int m
     NormFold fold_in;
     const PagedCacheView cache = ctx.cache_view(run, mixer_slot);       // pages of this run's cache id
     const int rot = position_->rotary_dim();
-    const bool to_heads = !mix_path_ && ctx.dtype == dtype_ && !ctx.kv_round_bf16 &&
+    const bool to_heads = !mix_path_ && ctx.dtype == dtype_ && !ctx.kv_round_bf16 && cache.bits == 0 &&
                           Ops::projection_to_heads_ok(dtype_, h, hidden_, w_qkv_, hidden_, T, head_dim_, rot);
     // the step's (cos, sin) table: the same for every layer that rotates alike; laid out by
     // pair for the projection that rotates its own heads
@@ -439,7 +442,13 @@ inline void AttentionMixer::forward(StepContext& ctx, const LayerRun& run, int m
         void* qkv = ctx.workspace->buffer("qkv", (size_t)T * qkv_cols * es);
         ops.gemm(qkv, ctx.dtype, qkv_cols, h, hidden_, w_qkv_, hidden_, dtype_, T, qkv_cols, hidden_, EPI_STORE,
                  fold_input(ctx, fold_in));
-        if (Ops::attention_decode_fused_ok(work, ctx.dtype, heads_, kv_heads_, head_dim_, rot)) {
+        if (cache.bits != 0) {
+            void* q = ctx.workspace->buffer("q", (size_t)T * q_dim_ * es);
+            ops.qk_norm_rope_write_quantized(qkv, qkv_cols, q, cache, ctx.dtype, qn, kn, norm_dtype_, eps_, cos_sin, rot, m.positions,
+                                             m.entry_of_token, T, heads_, kv_heads_, head_dim_, run.writes_cache);
+            ops.attention_quantized(attn, q, cache, ctx.dtype, work, m.shape.q_lens, m.positions, m.entry_of_token, m.q_start,
+                                    m.context_len, heads_, kv_heads_, head_dim_, scale_, window_);
+        } else if (Ops::attention_decode_fused_ok(work, ctx.dtype, heads_, kv_heads_, head_dim_, rot)) {
             // decoded tokens only: norm, rotation and the cache write happen inside the attention
             // kernel, straight from the projection's output
             ops.attention_decode_fused(attn, qkv, qkv_cols, cache, qn, kn, norm_dtype_, eps_, cos_sin,
@@ -532,6 +541,16 @@ inline Engine::Engine(std::unique_ptr<ModelPlan> plan, TensorSource& source, con
     if (opt_.max_requests <= 0) fail(KIPP_E_ARGUMENT, "max_requests must be positive");
     if (opt_.max_batch_tokens <= 0) fail(KIPP_E_ARGUMENT, "max_batch_tokens must be positive");
     if (opt_.cache_tokens < 0) fail(KIPP_E_ARGUMENT, "cache_tokens must not be negative");
+    if (opt_.kv_bits != 0) {
+        if (opt_.kv_bits != 4 && opt_.kv_bits != 8) fail(KIPP_E_ARGUMENT, format("keys and values are cached in 4 or 8 bits or in the compute type, not in %d bits", opt_.kv_bits));
+        if (opt_.kv_round_bf16 || opt_.own_length_splits)
+            fail(KIPP_E_ARGUMENT, "a cache of 4 or 8 bits goes neither with kv_round_bf16 nor with own_length_splits");
+        for (auto& run : plan_->order)
+            for (Mixer* mixer : plan_->layers[(size_t)run.layer].second->mixers())
+                if (mixer->cache_spec() && !mixer->takes_quantised_cache())
+                    fail(KIPP_E_CONFIG, format("layer %d: a cache of %d bits holds heads of a multiple of 32 channels of plain grouped-query "
+                                               "attention only", run.layer, opt_.kv_bits));
+    }
     int count = 0;
     if (cudaGetDeviceCount(&count) != cudaSuccess || count <= 0) {
         cudaGetLastError();
@@ -582,6 +601,12 @@ inline Engine::~Engine() {
     if (stream_) cudaStreamDestroy(stream_);
 }
 
+// Bytes that a token's keys and values take in one cache.
+inline size_t Engine::cache_row_bytes(const PagedKVSpec& s) const {
+    const size_t dims = (size_t)s.kv_heads * (s.head_dim + s.stored_v_dim());
+    return opt_.kv_bits ? dims * opt_.kv_bits / 8 + dims / 16 : dims * dtype_size(dtype_);
+}
+
 inline size_t Engine::workspace_estimate() const {
     // per token: the float32 residual, the normed copy, q/k/v, q, the attention output, the
     // feed-forward's activation (sizes are not known here per part: four hidden-wide rows of
@@ -608,7 +633,7 @@ inline void Engine::check_memory(const std::vector<TensorSpec>& specs) {
         auto mixers = plan_->layers[(size_t)run.layer].second->mixers();
         for (size_t s = 0; s < mixers.size(); ++s)
             if (auto cs = mixers[s]->cache_spec(); cs && seen.insert(cache_key(run.cache, (int)s)).second)
-                per_token += (size_t)cs->kv_heads * (cs->head_dim + cs->stored_v_dim()) * es;
+                per_token += cache_row_bytes(*cs);
     }
     size_t free_bytes = 0, total = 0;
     cuda_check(cudaMemGetInfo(&free_bytes, &total), "cudaMemGetInfo");
@@ -680,8 +705,17 @@ inline void Engine::build_cache() {
         g.spec = spec;
         g.cache_keys = by_spec[spec];
         g.n_pages = n_pages;
-        g.cache_stride = (size_t)n_pages * spec.kv_heads * opt_.page_size * spec.head_dim * es;
-        g.value_stride = (size_t)n_pages * spec.kv_heads * opt_.page_size * spec.stored_v_dim() * es;
+        const size_t rows = (size_t)n_pages * spec.kv_heads * opt_.page_size;
+        g.cache_stride = opt_.kv_bits ? rows * spec.head_dim * opt_.kv_bits / 8 : rows * spec.head_dim * es;
+        g.value_stride = opt_.kv_bits ? g.cache_stride : rows * spec.stored_v_dim() * es;
+        if (opt_.kv_bits) {
+            g.scale_stride = (rows * (spec.head_dim / 32) * 2 + 255) / 256 * 256;      // (kernels want 16-byte boundaries)
+            const size_t scale_bytes = g.scale_stride * g.cache_keys.size();
+            g.k_scales.reset(scale_bytes, "scales of the keys");
+            g.v_scales.reset(scale_bytes, "scales of the values");
+            cuda_check(cudaMemsetAsync(g.k_scales.get(), 0, scale_bytes, stream_), "clearing the scales");
+            cuda_check(cudaMemsetAsync(g.v_scales.get(), 0, scale_bytes, stream_), "clearing the scales");
+        }
         const size_t bytes = g.cache_stride * g.cache_keys.size(), value_bytes = g.value_stride * g.cache_keys.size();
         g.k.reset(bytes, "key pages");
         g.v.reset(value_bytes, "value pages");
@@ -720,6 +754,11 @@ inline PagedCacheView Engine::cache_view(const StepMeta& meta, const LayerRun& r
     v.block_table = meta.block_tables[(size_t)it->second.first];
     v.table_width = meta.table_widths[(size_t)it->second.first];
     v.page_size = opt_.page_size;
+    if (opt_.kv_bits) {
+        v.bits = opt_.kv_bits;
+        v.k_scales = static_cast<char*>(g.k_scales.get()) + g.scale_stride * (size_t)it->second.second;
+        v.v_scales = static_cast<char*>(g.v_scales.get()) + g.scale_stride * (size_t)it->second.second;
+    }
     return v;
 }
 
@@ -1487,7 +1526,7 @@ inline size_t Engine::weight_bytes() const {
 inline size_t Engine::cache_bytes_per_token() const {
     size_t n = 0;
     for (auto& g : groups_)
-        n += g.cache_keys.size() * g.spec.kv_heads * (g.spec.head_dim + g.spec.stored_v_dim()) * dtype_size(dtype_);
+        n += g.cache_keys.size() * cache_row_bytes(g.spec);
     return n;
 }
 
@@ -1517,6 +1556,7 @@ inline std::string Engine::info_json() {
     j.set("cuda_graphs", graphable());
     j.set("kv_round_bf16", opt_.kv_round_bf16 != 0);
     j.set("own_length_splits", opt_.own_length_splits != 0);
+    j.set("kv_bits", opt_.kv_bits);
     j.set("workspace_bytes", (long long)workspace_.bytes());
     Json groups = Json::array();
     for (size_t g = 0; g < groups_.size(); ++g) {

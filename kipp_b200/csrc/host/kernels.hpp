@@ -74,6 +74,45 @@ struct PagedCacheView {
     const int* block_table = nullptr;      // int32 [entries, table_width] of this step
     int table_width = 0;
     int page_size = 0;
+    // A quantised cache (bits 4 or 8; quant_format.cuh of the kernel libraries): the pages hold codes, [pages, kv_heads, page_size,
+    // head_dim * bits / 8] bytes, and these their scales, bfloat16 [pages, kv_heads, page_size, head_dim / 32].
+    int bits = 0;
+    void* k_scales = nullptr;
+    void* v_scales = nullptr;
+};
+
+// The arguments of the quantised cache's entry points (the layouts are the kernel libraries', cache_quant.cu and
+// attention_quant.cu).
+struct QuantWriteArgs {
+    const void* qkv; void* q_out;
+    void *k_codes, *k_scales, *v_codes, *v_scales;
+    const void *q_norm_w, *k_norm_w, *cos_sin;
+    const int *positions, *entry_of_token, *block_table;
+    int* status;
+    void* stream;
+    long long ld_qkv;
+    int bits, n_pages, page_size, dtype, norm_dtype, rotary_dim, table_width, tokens, n_q, n_kv, head_dim, write_cache;
+    float eps;
+};
+struct QuantReadEntriesArgs {
+    void *k_out, *v_out;
+    int* table_out;
+    const void *k_codes, *k_scales, *v_codes, *v_scales;
+    const int *q_start, *context_len, *block_table;
+    int* status;
+    void* stream;
+    int out_dtype, bits, n_pages, page_size, table_width, first_entry, entries, window, n_kv, head_dim;
+};
+struct QuantAttentionArgs {
+    void* out; const void* q;
+    const void *k_codes, *k_scales, *v_codes, *v_scales;
+    const int *q_start, *context_len, *block_table;
+    void* scratch;
+    int* status;
+    void* stream;
+    long long scratch_bytes;
+    int bits, n_pages, page_size, table_width, entries, most, n_q, n_kv, head_dim, window;
+    float scale;
 };
 
 // Options of the mixed-head attention kernel beside the mix (the layout is the kernel library's
@@ -1042,6 +1081,108 @@ public:
         run(f(out, q, cache.k_pages, cache.v_pages, dtype, positions, entry_of_token, cache.block_table,
               cache.table_width, cache.page_size, work.tokens, n_q, n_kv, head_dim, scale, window, status, stream),
             "attention_simt");
+    }
+
+    // -- the quantised cache ------------------------------------------------------------------
+    // qk_norm_rope_write with keys and values as codes.
+    void qk_norm_rope_write_quantized(const void* qkv, long long ld_qkv, void* q_out, const PagedCacheView& cache, int dtype,
+                                      const void* q_norm_w, const void* k_norm_w, int norm_dtype, float eps, const float* cos_sin,
+                                      int rotary_dim, const int* positions, const int* entry_of_token, int tokens, int n_q, int n_kv,
+                                      int head_dim, bool write_cache) {
+        using Fn = int (*)(const QuantWriteArgs*);
+        static Fn f = kernel_symbol<Fn>("cache_quant", "kipp_quant_cache_write");
+        const QuantWriteArgs a = {qkv, q_out, cache.k_pages, cache.k_scales, cache.v_pages, cache.v_scales, q_norm_w, k_norm_w, cos_sin,
+                                  positions, entry_of_token, cache.block_table, status, stream, ld_qkv, cache.bits, cache.n_pages,
+                                  cache.page_size, dtype, norm_dtype, cos_sin ? rotary_dim : 0, cache.table_width, tokens, n_q, n_kv,
+                                  head_dim, write_cache ? 1 : 0, eps};
+        run(f(&a), "quant_cache_write");
+    }
+    // What entries first .. first + entries - 1 see, read back into pages of their own: the view of those.
+    PagedCacheView quant_read_entries(const PagedCacheView& cache, int dtype, const int* q_start, const int* context_len, int first,
+                                      int entries, int all_entries, int n_kv, int head_dim, int window) {
+        using Fn = int (*)(const QuantReadEntriesArgs*);
+        static Fn f = kernel_symbol<Fn>("cache_quant", "kipp_quant_cache_read_entries");
+        PagedCacheView v = cache;
+        v.bits = 0;
+        v.k_scales = v.v_scales = nullptr;
+        v.n_pages = entries * cache.table_width;
+        const size_t bytes = (size_t)v.n_pages * n_kv * cache.page_size * head_dim * dtype_size(dtype);
+        v.k_pages = workspace->buffer("quant_keys", bytes);
+        v.v_pages = workspace->buffer("quant_values", bytes);
+        int* table = workspace->get<int>("quant_table", (size_t)all_entries * cache.table_width);
+        v.block_table = table;
+        const QuantReadEntriesArgs a = {v.k_pages, v.v_pages, table, cache.k_pages, cache.k_scales, cache.v_pages, cache.v_scales, q_start,
+                                        context_len, cache.block_table, status, stream, dtype, cache.bits, cache.n_pages, cache.page_size,
+                                        cache.table_width, first, entries, window, n_kv, head_dim};
+        run(f(&a), "quant_cache_read");
+        return v;
+    }
+    static bool attention_quant_supported(int bits, int head_dim, int n_q, int n_kv) {
+        using Fn = int (*)(int, int, int, int);
+        static Fn f = kernel_symbol<Fn>("attention_quant", "kipp_attn_quant_supported");
+        return f(bits, head_dim, n_q, n_kv) != 0;
+    }
+    // The entries of up to `most` tokens, over the codes.
+    void attention_quant_direct(void* out, const void* q, const PagedCacheView& cache, const int* q_start, const int* context_len,
+                                int entries, int most, int n_q, int n_kv, int head_dim, float scale, int window) {
+        using Fn = int (*)(const QuantAttentionArgs*);
+        using Fb = long long (*)(int);
+        static Fn f = kernel_symbol<Fn>("attention_quant", "kipp_attn_quant");
+        static Fb bytes = kernel_symbol<Fb>("attention_quant", "kipp_attn_quant_scratch_bytes");
+        const long long need = bytes(head_dim);
+        const QuantAttentionArgs a = {out, q, cache.k_pages, cache.k_scales, cache.v_pages, cache.v_scales, q_start, context_len,
+                                      cache.block_table, workspace->buffer("quant_attention_scratch", (size_t)need), status, stream, need,
+                                      cache.bits, cache.n_pages, cache.page_size, cache.table_width, entries, most, n_q, n_kv, head_dim,
+                                      window, scale};
+        run(f(&a), "attn_quant", 2);
+    }
+    // Causal grouped-query attention over a quantised cache.  bfloat16 heads of 64, 128 and 256 run on the codes; where portions of
+    // PREFILL_TC_MIN_TOKENS and more are among the entries, those of more than one token read their pages back for the tcgen05
+    // prompt kernel, as long as the pages have room in EXPAND_MAX_BYTES; other heads and 32-bit read back always, as many entries at
+    // a time as have room there.  Which it is depends on the step's shape only.
+    void attention_quantized(void* out, const void* q, const PagedCacheView& cache, int dtype, const AttentionWork& work,
+                             const std::vector<int>& q_lens, const int* positions, const int* entry_of_token, const int* q_start,
+                             const int* context_len, int n_q, int n_kv, int head_dim, float scale, int window) {
+        const int entries = (int)q_lens.size();
+        const long long page_bytes = 2LL * n_kv * cache.page_size * head_dim * (long long)dtype_size(dtype);
+        const long long at_once = std::max(1LL, std::min(EXPAND_MAX_BYTES / (page_bytes * cache.table_width), 65535LL / cache.table_width));
+        if (dtype == BF16 && attention_quant_supported(cache.bits, head_dim, n_q, n_kv)) {
+            int first = -1, last = -1, longest = 1;
+            bool single = false;
+            for (int e = 0; e < entries; ++e) {
+                longest = std::max(longest, q_lens[(size_t)e]);
+                if (q_lens[(size_t)e] == 1) single = true;
+                if (q_lens[(size_t)e] > 1) { if (first < 0) first = e; last = e; }
+            }
+            const bool portions = prefill_tensor_core && longest >= PREFILL_TC_MIN_TOKENS && work.n_prefill_items128 > 0 &&
+                                  last - first + 1 <= at_once && attention_tc_supported(head_dim, n_q, n_kv, cache.page_size);
+            if (!portions || single)
+                attention_quant_direct(out, q, cache, q_start, context_len, entries, portions ? 1 : longest, n_q, n_kv, head_dim, scale, window);
+            if (portions) {
+                AttentionWork only = work;
+                only.n_decode = 0;                     // (the prompt kernel alone)
+                attention_tensor_core(out, q, quant_read_entries(cache, dtype, q_start, context_len, first, last - first + 1, entries, n_kv,
+                                                                 head_dim, window),
+                                      only, q_start, context_len, n_q, n_kv, head_dim, scale, window);
+            }
+            return;
+        }
+        using Fn = int (*)(void*, const void*, const void*, const void*, int, const int*, const int*, const int*, int,
+                           int, int, int, int, int, float, int, int*, void*);
+        static Fn f = kernel_symbol<Fn>("attention_simt", "kipp_paged_attention_simt");
+        const size_t row = (size_t)n_q * head_dim * dtype_size(dtype);
+        size_t at = 0;
+        for (int e = 0; e < entries; e += (int)at_once) {
+            const int n = std::min((int)at_once, entries - e);
+            int tokens = 0;
+            for (int i = e; i < e + n; ++i) tokens += q_lens[(size_t)i];
+            if (tokens == 0) continue;
+            const PagedCacheView v = quant_read_entries(cache, dtype, q_start, context_len, e, n, entries, n_kv, head_dim, window);
+            run(f(static_cast<char*>(out) + at * row, static_cast<const char*>(q) + at * row, v.k_pages, v.v_pages, dtype, positions + at,
+                  entry_of_token + at, v.block_table, v.table_width, v.page_size, tokens, n_q, n_kv, head_dim, scale, window, status, stream),
+                "attention_simt");
+            at += (size_t)tokens;
+        }
     }
 
     // Whether a step can take attention_decode_fused: decoded tokens only, bfloat16, a head size

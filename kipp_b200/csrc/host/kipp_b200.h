@@ -70,6 +70,10 @@ typedef struct {
                                   reference's storage contract (src/kipp.c:2806-2811) */
     int own_length_splits;     /* decode attention splits from each token's own context only, so that a
                                   token's bfloat16 result does not depend on its neighbours in the batch */
+    int kv_bits;               /* 8 or 4: keys and values are cached in that many bits, in groups of 32 channels with a
+                                  bfloat16 scale each (the reference's --kv-quant, src/kipp.h:50-53); 0: in the compute
+                                  type.  For models all of whose caches are plain grouped-query attention's; excludes
+                                  kv_round_bf16 and own_length_splits. */
 } kipp_engine_options;
 
 void kipp_engine_default_options(kipp_engine_options* options);

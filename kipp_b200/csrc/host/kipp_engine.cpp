@@ -97,6 +97,7 @@ void kipp_engine_default_options(kipp_engine_options* o) {
     o->cuda_graphs = 1;
     o->kv_round_bf16 = 0;
     o->own_length_splits = 0;
+    o->kv_bits = 0;
 }
 
 void kipp_set_library_resolver(kipp_library_resolver resolver) { KernelLibraries::get().set_resolver(resolver); }

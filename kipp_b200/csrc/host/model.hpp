@@ -225,6 +225,7 @@ public:
 class Mixer : public Part {
 public:
     virtual std::optional<PagedKVSpec> cache_spec() const { return std::nullopt; }
+    virtual bool takes_quantised_cache() const { return false; }       // its cache may hold codes (PagedCacheView::bits)
     virtual std::optional<StateSpec> state_spec() const { return std::nullopt; }
     // the planner of the work lists this mixer's kernels read beside the common metadata, if any
     virtual std::shared_ptr<WorkPlanner> planner(const DeviceInfo& device, bool own_length_splits) { return nullptr; }

@@ -769,6 +769,8 @@ public:
         return PagedKVSpec{kv_heads_, maps_ * head_dim_, opt_.forget_blocks ? opt_.chunk : window_, v_dim_,
                            window_ > 0 ? opt_.keep_first : 0};
     }
+    // whole groups of 32 channels; none of the options that the mixed-head path stands for
+    bool takes_quantised_cache() const override { return !mix_path_ && head_dim_ % 32 == 0 && head_dim_ <= 512; }
     std::shared_ptr<WorkPlanner> planner(const DeviceInfo& dev, bool own_length) override {
         if (mix_path_) {                          // (entry, first token) per tile of its tensor-core prompt kernel
             mix_planner_ = std::make_shared<MixTilePlanner>(Ops::attention_mix_tile());

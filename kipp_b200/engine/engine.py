@@ -30,7 +30,7 @@ from ..parts.base import PagedKVSpec
 from ..weights.loader import Checkpoint, storage_dtype
 from ..weights.random_init import random_tensors
 from .batch import StepEntry
-from .runtime import parse_dtype
+from .runtime import parse_dtype, parse_kv_quant
 
 _TYPESTR = {torch.float32: "<f4", torch.int32: "<i4", torch.bfloat16: "<i2", torch.float16: "<f2",
             torch.int64: "<i8", torch.uint8: "|u1", torch.float64: "<f8"}
@@ -161,10 +161,11 @@ class Engine:
                  device: str | torch.device = "cuda:0", page_size: int = 16,
                  cache_tokens: Optional[int] = 8192, max_requests: int = 64, max_batch_tokens: int = 8192,
                  max_logit_rows: Optional[int] = None, cuda_graphs: bool = True, kv_round_bf16: bool = False,
-                 own_length_splits: bool = False):
+                 own_length_splits: bool = False, kv_quant: Optional[str] = None):
         """``tensors`` maps checkpoint names to torch tensors (CPU or CUDA); with
         ``folder`` the library reads the model folder itself.  ``cache_tokens``
-        None sizes the cache from the free device memory."""
+        None sizes the cache from the free device memory.  ``kv_quant`` "int8" or "int4" caches
+        keys and values in 8 or 4 bits (plain grouped-query attention only)."""
         self.spec = spec
         self.device = torch.device(device)
         if self.device.type != "cuda":
@@ -192,6 +193,7 @@ class Engine:
         opt.cuda_graphs = 1 if cuda_graphs else 0
         opt.kv_round_bf16 = 1 if kv_round_bf16 else 0
         opt.own_length_splits = 1 if own_length_splits else 0
+        opt.kv_bits = parse_kv_quant(kv_quant)
         plan, external = spec.to_plan()
         self._external = external
         handle = ctypes.c_void_p()

@@ -45,6 +45,7 @@ class LLM:
     ``max_batch_tokens`` token budget of one step
     ``chunk``            largest prompt portion of one request in one step
     ``policy``           "reserve" or "preempt": what happens when pages run out
+    ``kv_quant``         "int8" or "int4": keys and values cached in 8 or 4 bits (an engine option)
     """
 
     def __init__(self, model, *, dtype="bfloat16", device="cuda:0", kv_block_size: int = 16,

@@ -1,4 +1,4 @@
-"""Compute dtypes by name."""
+"""Compute dtypes and cache formats by name."""
 from __future__ import annotations
 
 import torch
@@ -15,3 +15,12 @@ def parse_dtype(name) -> torch.dtype:
         return table[str(name).lower()]
     except KeyError:
         raise ValueError(f"unknown dtype {name!r}; use bfloat16 or float32") from None
+
+
+def parse_kv_quant(name) -> int:
+    """Bits of a cached key or value element: 0 stands for the compute dtype."""
+    table = {None: 0, "none": 0, "int8": 8, "int4": 4}
+    try:
+        return table[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"unknown kv_quant {name!r}; use int8, int4 or none") from None

@@ -24,7 +24,7 @@ class KernelError(RuntimeError):
 class EngineOptions(Structure):
     _fields_ = [("dtype", c_int), ("device", c_int), ("page_size", c_int), ("cache_tokens", c_longlong),
                 ("max_requests", c_int), ("max_batch_tokens", c_int), ("max_logit_rows", c_int),
-                ("cuda_graphs", c_int), ("kv_round_bf16", c_int), ("own_length_splits", c_int)]
+                ("cuda_graphs", c_int), ("kv_round_bf16", c_int), ("own_length_splits", c_int), ("kv_bits", c_int)]
 
 
 class TensorInfo(Structure):
