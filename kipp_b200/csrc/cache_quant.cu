@@ -104,7 +104,8 @@ __global__ void __launch_bounds__(128) quant_write_any_kernel(const WriteParams 
         const float x = quant_input(row[c]);
         const float hi = warp_max(x), lo = -warp_max(-x);
         const uint16_t sb = quant_scale<BITS>(hi, lo);
-        const uint32_t code = quant_code<BITS>(x, quant_scale_value(sb));
+        const float scale = quant_scale_value(sb);
+        const uint32_t code = (uint32_t)quant_code<BITS>(x, scale, quant_inverse(scale));
         if (BITS == 8) {
             codes[c] = (uint8_t)code;
         } else {
@@ -125,39 +126,41 @@ __device__ __forceinline__ void put8(float* p, const float (&x)[8]) {
     reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
     reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
-template <int BITS> __device__ __forceinline__ void put_codes(uint8_t* p, const float (&x)[8], float s0, float s1) {
-    uint32_t c[8];
+template <int BITS> __device__ __forceinline__ void put_codes(uint8_t* p, const float (&x)[8], float s0, float i0, float s1, float i1) {
+    float c[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = quant_code<BITS>(x[i], i < 4 ? s0 : s1);
-    if (BITS == 4) {
-        uint32_t w = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w |= c[i] << (4 * i);
-        *reinterpret_cast<uint32_t*>(p) = w;
-    } else {
-        *reinterpret_cast<uint2*>(p) = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
-    }
+    for (int i = 0; i < 8; ++i) c[i] = i < 4 ? quant_code<BITS>(x[i], s0, i0) : quant_code<BITS>(x[i], s1, i1);
+    const uint32_t a = quant_pack4<BITS>(c[0], c[1], c[2], c[3]), b = quant_pack4<BITS>(c[4], c[5], c[6], c[7]);
+    if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(p) = a | b << 16;
+    else *reinterpret_cast<uint2*>(p) = make_uint2(a, b);
 }
 
-// Heads of 64, 128 or 256 channels, rotated whole or not at all, 16-byte aligned: HEAD_DIM / 16 lanes
-// share a (token, head), a lane holds 8 channels of the first half and their rotation partners, as
-// in rope_cache.cu.  Those are four runs of two groups; the four lanes whose numbers agree modulo
-// HEAD_DIM / 64 hold the same two groups, so a group's extremes are two exchanges away.
+// Heads of 64, 128 or 256 channels, rotated whole, by half or not at all, 16-byte aligned: HEAD_DIM / 16 lanes
+// share a (token, head), a lane holds 8 channels of the first half and the 8 half a head further, as
+// in rope_cache.cu.  A whole rotation's partners are those two; half a rotation's are the first ones of two lanes.  A lane has
+// four runs of two groups; the four lanes whose numbers agree modulo HEAD_DIM / 64 hold the same two groups, so a
+// group's extremes are two exchanges away.  The 64-bit sum of squares (16 conversions a lane on a pipe of 16 lanes) is
+// formed for keys only: queries get no codes, and four in five heads are theirs.
+// 2,048 tokens of 32 and 2 x 8 heads of 128, 8 bits: see the table of cases in the design document.
 constexpr int WRITE_THREADS = 128;
 template <typename T, int BITS, int HEAD_DIM>
 __global__ void __launch_bounds__(WRITE_THREADS) quant_write_kernel(const WriteParams p) {
     constexpr int LPH = HEAD_DIM / 16, HALF = HEAD_DIM / 2, G = HEAD_DIM / 32;
     pdl_launch_dependents();
-    pdl_wait();
     const int t = blockIdx.y, h = blockIdx.x * (WRITE_THREADS / LPH) + threadIdx.x / LPH, sub = threadIdx.x % LPH;
     const int n_kv = p.pages.n_kv;
     const bool is_q = h < p.n_q, is_k = !is_q && h < p.n_q + n_kv;
-    const bool active = h < p.n_q + 2 * n_kv && (is_q || p.write_cache);
+    const bool active = h < p.n_q + 2 * n_kv && (is_q || p.write_cache), normed = active && (is_q || is_k);
+    // (the step's lists and the weights, before the wait)
     long long at = -1;
-    if (active && !is_q) {
-        at = cache_row(p, t, is_k ? h - p.n_q : h - p.n_q - n_kv);
-        if (at < 0 && sub == 0) atomicExch(p.status, 2);
+    if (active && !is_q) at = cache_row(p, t, is_k ? h - p.n_q : h - p.n_q - n_kv);
+    float wa[8], wb[8];
+    if (p.q_norm_w != nullptr && normed) {        // both weights or neither (checked by the host)
+        const void* nw = is_q ? p.q_norm_w : p.k_norm_w;
+        load_w8(wa, nw, p.norm_dtype, sub * 8);
+        load_w8(wb, nw, p.norm_dtype, HALF + sub * 8);
     }
+    pdl_wait();
     // No lane leaves early: a warp holds several heads and all lanes take part in the exchanges.
     float a[8], b[8];
 #pragma unroll
@@ -167,29 +170,53 @@ __global__ void __launch_bounds__(WRITE_THREADS) quant_write_kernel(const WriteP
         take8(a, src);
         take8(b, src + HALF);
     }
-    if (p.q_norm_w != nullptr) {                  // both weights or neither (checked by the host)
-        double ss = 0.0;
+    const bool whole = p.rotary_dim == HEAD_DIM;
+    float4 cs[4];
+    if (p.cos_sin != nullptr && normed) {
+        const float4* row = reinterpret_cast<const float4*>(p.cos_sin + (size_t)t * (p.rotary_dim / 2) + (whole ? sub : sub % (LPH / 2)) * 8);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss += (double)a[i] * (double)a[i] + (double)b[i] * (double)b[i];
+        for (int i = 0; i < 4; ++i) cs[i] = row[i];
+    }
+    if (p.q_norm_w != nullptr) {
+        float mean;
+        if (__any_sync(0xffffffffu, is_k)) {
+            double ss = 0.0;
 #pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (active && (is_q || is_k)) {
-            const float r = norm_factor(mean_square(ss, HEAD_DIM), p.eps);
-            const void* nw = is_q ? p.q_norm_w : p.k_norm_w;
-            float w[8];
-            load_w8(w, nw, p.norm_dtype, sub * 8);
-            head_scale8(a, r, w);
-            load_w8(w, nw, p.norm_dtype, HALF + sub * 8);
-            head_scale8(b, r, w);
+            for (int i = 0; i < 8; ++i) ss += (double)a[i] * (double)a[i] + (double)b[i] * (double)b[i];
+#pragma unroll
+            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            mean = mean_square(ss, HEAD_DIM);
+        } else {
+            float ss = head_ssq8(a, b);
+#pragma unroll
+            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            mean = ss * (1.f / HEAD_DIM);
+        }
+        if (normed) {
+            const float r = norm_factor(mean, p.eps);
+            head_scale8(a, r, wa);
+            head_scale8(b, r, wb);
         }
     }
-    if (p.cos_sin != nullptr && active && (is_q || is_k)) {
-        const float4* cs = reinterpret_cast<const float4*>(p.cos_sin + (size_t)t * HALF + sub * 8);
+    if (p.cos_sin != nullptr) {
+        if (whole) {
+            if (normed) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 c = cs[i];
-            turn(a[2 * i], b[2 * i], make_float2(c.x, c.y));
-            turn(a[2 * i + 1], b[2 * i + 1], make_float2(c.z, c.w));
+                for (int i = 0; i < 4; ++i) {
+                    turn(a[2 * i], b[2 * i], make_float2(cs[i].x, cs[i].y));
+                    turn(a[2 * i + 1], b[2 * i + 1], make_float2(cs[i].z, cs[i].w));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float other = __shfl_xor_sync(0xffffffffu, a[i], LPH / 2);
+                if (normed) {
+                    const float2 c = i & 1 ? make_float2(cs[i / 2].z, cs[i / 2].w) : make_float2(cs[i / 2].x, cs[i / 2].y);
+                    if (sub < LPH / 2) turn(a[i], other, c);
+                    else { turn(other, a[i], c); }
+                }
+            }
         }
     }
     if (active && is_q) {
@@ -197,6 +224,7 @@ __global__ void __launch_bounds__(WRITE_THREADS) quant_write_kernel(const WriteP
         put8(dst, a);
         put8(dst + HALF, b);
     }
+    if (__all_sync(0xffffffffu, is_q)) return;
     float hi[2], lo[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -213,13 +241,17 @@ __global__ void __launch_bounds__(WRITE_THREADS) quant_write_kernel(const WriteP
             lo[r] = fminf(lo[r], __shfl_xor_sync(0xffffffffu, lo[r], o));
         }
     }
-    if (at < 0) return;
-    const uint16_t s0 = quant_scale<BITS>(hi[0], lo[0]), s1 = quant_scale<BITS>(hi[1], lo[1]);
+    if (at < 0) {                                 // unmapped page: refuse, never write
+        if (active && !is_q && sub == 0) atomicExch(p.status, 2);
+        return;
+    }
+    const uint16_t b0 = quant_scale<BITS>(hi[0], lo[0]), b1 = quant_scale<BITS>(hi[1], lo[1]);
+    const float s0 = quant_scale_value(b0), s1 = quant_scale_value(b1), i0 = quant_inverse(s0), i1 = quant_inverse(s1);
     uint8_t* codes = (is_k ? p.pages.k_codes : p.pages.v_codes) + (size_t)at * (HEAD_DIM * BITS / 8) + sub * BITS;
-    put_codes<BITS>(codes, a, quant_scale_value(s0), quant_scale_value(s1));
-    put_codes<BITS>(codes + HALF * BITS / 8, b, quant_scale_value(s0), quant_scale_value(s1));
+    put_codes<BITS>(codes, a, s0, i0, s1, i1);
+    put_codes<BITS>(codes + HALF * BITS / 8, b, s0, i0, s1, i1);
     if (sub < G / 2)
-        reinterpret_cast<uint32_t*>((is_k ? p.pages.k_scales : p.pages.v_scales) + (size_t)at * G)[sub] = (uint32_t)s0 | (uint32_t)s1 << 16;
+        reinterpret_cast<uint32_t*>((is_k ? p.pages.k_scales : p.pages.v_scales) + (size_t)at * G)[sub] = (uint32_t)b0 | (uint32_t)b1 << 16;
 }
 
 template <typename T, int BITS> int launch_write(const WriteParams& p, cudaStream_t s) {
@@ -227,7 +259,7 @@ template <typename T, int BITS> int launch_write(const WriteParams& p, cudaStrea
     const uintptr_t bits = (uintptr_t)p.qkv | (uintptr_t)p.q_out | (uintptr_t)p.q_norm_w | (uintptr_t)p.k_norm_w | (uintptr_t)p.cos_sin |
                            (uintptr_t)p.pages.k_codes | (uintptr_t)p.pages.v_codes | (uintptr_t)p.pages.k_scales | (uintptr_t)p.pages.v_scales;
     const bool aligned = (bits & 15) == 0 && p.ld * (long long)sizeof(T) % 16 == 0;
-    if (aligned && (p.cos_sin == nullptr || p.rotary_dim == D) && p.tokens <= 65535 && (D == 64 || D == 128 || D == 256)) {
+    if (aligned && (p.cos_sin == nullptr || p.rotary_dim == D || p.rotary_dim * 2 == D) && p.tokens <= 65535 && (D == 64 || D == 128 || D == 256)) {
         const int per = WRITE_THREADS / (D / 16);
         const dim3 grid((unsigned)((heads + per - 1) / per), (unsigned)p.tokens);
         auto kernel = D == 64 ? quant_write_kernel<T, BITS, 64> : D == 128 ? quant_write_kernel<T, BITS, 128> : quant_write_kernel<T, BITS, 256>;
@@ -250,33 +282,66 @@ struct ReadParams {
     int table_width, first_entry, window;
 };
 
-__device__ __forceinline__ void put_out(float* p, const float (&x)[8]) { put8(p, x); }
-__device__ __forceinline__ void put_out(bf16* p, const float (&x)[8]) { put8(p, x); }
-
-// eight channels from channel c on (a multiple of 8): two runs
-template <int BITS> __device__ __forceinline__ void values8(float (&x)[8], const uint8_t* codes, const uint16_t* scales, int c, int G) {
-    constexpr float L = BITS == 4 ? 8.f : 128.f;
-    const int g0 = (c >> 2) % G, g1 = g0 + 1 == G ? 0 : g0 + 1;
-    const float s0 = quant_scale_value(scales[g0]), s1 = quant_scale_value(scales[g1]);
-    if (BITS == 4) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + c / 2);
+// The eight channels that a word of 4-bit codes, or two of 8-bit, stand for, as bfloat16 pairs of (code - L) * 2^-13: a code in the
+// low bits of 16 is the number code * 2^-133 (attention_quant.cu), and one fused multiply-add makes it that, exactly.
+template <int BITS> __device__ __forceinline__ void whole_numbers(__nv_bfloat162 (&x)[4], const uint32_t* w) {
+    const __nv_bfloat162 up = __float2bfloat162_rn(0x1p120f), less = __float2bfloat162_rn(BITS == 4 ? -0x1p-10f : -0x1p-6f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = ((float)((w >> (4 * i)) & 15) - L) * (i < 4 ? s0 : s1);
-    } else {
-        const uint2 w = *reinterpret_cast<const uint2*>(codes + c);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = ((float)(((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 255) - L) * (i < 4 ? s0 : s1);
+    for (int i = 0; i < 4; ++i) {
+        uint32_t v;
+        if constexpr (BITS == 4) {
+            v = __byte_perm(w[0], w[0] >> 4, i | i << 4 | (4 + i) << 8 | (4 + i) << 12) & 0x000f000fu;       // byte i of both
+        } else {
+            v = __byte_perm(w[i >> 1], 0u, i & 1 ? 0x4342 : 0x4140);
+        }
+        x[i] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&v), up, less);
     }
 }
+template <int BITS> struct Unit { uint32_t w[BITS / 4]; uint16_t s[2]; };      // eight channels: codes, the scales of their two runs
+template <int BITS> __device__ __forceinline__ Unit<BITS> take_unit(const uint8_t* codes, const uint16_t* scales, int g0, int g1) {
+    Unit<BITS> u;
+    if constexpr (BITS == 4) u.w[0] = *reinterpret_cast<const uint32_t*>(codes);
+    else { const uint2 v = *reinterpret_cast<const uint2*>(codes); u.w[0] = v.x; u.w[1] = v.y; }
+    u.s[0] = scales[g0];
+    u.s[1] = scales[g1];
+    return u;
+}
+// (the scale times 2^13, exact, and one rounding)
+template <int BITS> __device__ __forceinline__ void put_unit(bf16* p, const Unit<BITS>& u) {
+    __nv_bfloat162 x[4];
+    whole_numbers<BITS>(x, u.w);
+    uint4 out;
+    uint32_t* o = reinterpret_cast<uint32_t*>(&out);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 s = __bfloat162bfloat162(__float2bfloat16_rn(quant_scale_value(u.s[i >> 1]) * 8192.f));
+        const __nv_bfloat162 r = __hmul2(x[i], s);
+        o[i] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+    *reinterpret_cast<uint4*>(p) = out;
+}
+template <int BITS> __device__ __forceinline__ void put_unit(float* p, const Unit<BITS>& u) {
+    __nv_bfloat162 x[4];
+    whole_numbers<BITS>(x, u.w);
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float s = quant_scale_value(u.s[i >> 1]) * 8192.f;
+        r[2 * i] = __low2float(x[i]) * s;
+        r[2 * i + 1] = __high2float(x[i]) * s;
+    }
+    put8(p, r);
+}
 
-// One block per (share of a page, page).  A page whose number is negative (unmapped) or past the pool
-// becomes zeros; past the pool is also reported.
+// One block per (share of a page, page); DIM is the head size, or 0 for any.  Every thread has UNROLL units of eight channels of keys
+// and of values on their way at once.  A page whose number is negative (unmapped) or past the pool becomes zeros; past the
+// pool is also reported.
 constexpr int READ_THREADS = 256;
-template <typename T, int BITS, bool ENTRIES>
+template <typename T, int BITS, bool ENTRIES, int DIM, int UNROLL>
 __global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const ReadParams p) {
     if constexpr (!ENTRIES) pdl_launch_dependents();      // (a step's table is read before a kernel's wait: this one lets none start early)
     pdl_wait();
-    const int i = blockIdx.y, D = p.head_dim, G = D / 32;
+    const int i = blockIdx.y, D = DIM > 0 ? DIM : p.head_dim, G = D / 32;
     const int page = p.list[ENTRIES ? (size_t)(p.first_entry + i / p.table_width) * p.table_width + i % p.table_width : (size_t)i];
     if constexpr (ENTRIES) {
         const int e = p.first_entry + i / p.table_width, slot = i % p.table_width;
@@ -289,27 +354,50 @@ __global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const ReadPara
     }
     const bool ok = page >= 0 && page < p.pages.n_pages;
     if (page >= p.pages.n_pages && threadIdx.x == 0) atomicExch(p.status, 3);
-    const int per_row = D / 8, rows = p.pages.n_kv * p.pages.page_size;
+    const int per_row = D / 8, rows = p.pages.n_kv * p.pages.page_size, units = rows * per_row;
     const size_t in = (size_t)(ok ? page : 0) * rows, out = (size_t)i * rows;
-    for (long long u = (long long)blockIdx.x * READ_THREADS + threadIdx.x; u < (long long)rows * per_row; u += (long long)gridDim.x * READ_THREADS) {
-        const int row = (int)(u / per_row), c = (int)(u - (long long)row * per_row) * 8;
-        float k[8], v[8];
+    const uint8_t *k_codes = p.pages.k_codes + in * (D * BITS / 8), *v_codes = p.pages.v_codes + in * (D * BITS / 8);
+    const uint16_t *k_scales = reinterpret_cast<const uint16_t*>(p.pages.k_scales) + in * G, *v_scales = reinterpret_cast<const uint16_t*>(p.pages.v_scales) + in * G;
+    T *k_out = static_cast<T*>(p.k_out) + out * D, *v_out = static_cast<T*>(p.v_out) + out * D;
+    for (int base = blockIdx.x * READ_THREADS * UNROLL; base < units; base += gridDim.x * READ_THREADS * UNROLL) {
+        Unit<BITS> k[UNROLL], v[UNROLL];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) k[j] = v[j] = 0.f;
-        if (ok) {
-            values8<BITS>(k, p.pages.k_codes + (in + row) * (D * BITS / 8), reinterpret_cast<const uint16_t*>(p.pages.k_scales) + (in + row) * G, c, G);
-            values8<BITS>(v, p.pages.v_codes + (in + row) * (D * BITS / 8), reinterpret_cast<const uint16_t*>(p.pages.v_scales) + (in + row) * G, c, G);
+        for (int j = 0; j < UNROLL; ++j) {
+            const int u = base + j * READ_THREADS + threadIdx.x;
+            k[j] = v[j] = Unit<BITS>{};
+            if (u < units && ok) {
+                const int row = u / per_row, c = u - row * per_row, g0 = 2 * c % G, g1 = g0 + 1 == G ? 0 : g0 + 1;
+                k[j] = take_unit<BITS>(k_codes + (size_t)u * BITS, k_scales + row * G, g0, g1);
+                v[j] = take_unit<BITS>(v_codes + (size_t)u * BITS, v_scales + row * G, g0, g1);
+            }
         }
-        put_out(static_cast<T*>(p.k_out) + (out + row) * D + c, k);
-        put_out(static_cast<T*>(p.v_out) + (out + row) * D + c, v);
+#pragma unroll
+        for (int j = 0; j < UNROLL; ++j) {
+            const int u = base + j * READ_THREADS + threadIdx.x;
+            if (u < units) {
+                put_unit<BITS>(k_out + (size_t)u * 8, k[j]);
+                put_unit<BITS>(v_out + (size_t)u * 8, v[j]);
+            }
+        }
     }
+}
+
+template <typename T, int BITS, bool ENTRIES> auto read_kernel(int head_dim, bool many) {
+    if (many) return head_dim == 64 ? quant_read_kernel<T, BITS, ENTRIES, 64, 4> : head_dim == 128 ? quant_read_kernel<T, BITS, ENTRIES, 128, 4>
+                   : head_dim == 256 ? quant_read_kernel<T, BITS, ENTRIES, 256, 4> : quant_read_kernel<T, BITS, ENTRIES, 0, 4>;
+    return head_dim == 64 ? quant_read_kernel<T, BITS, ENTRIES, 64, 1> : head_dim == 128 ? quant_read_kernel<T, BITS, ENTRIES, 128, 1>
+         : head_dim == 256 ? quant_read_kernel<T, BITS, ENTRIES, 256, 1> : quant_read_kernel<T, BITS, ENTRIES, 0, 1>;
 }
 
 template <bool ENTRIES> int launch_read(const ReadParams& p, int bits, int out_dtype, cudaStream_t s) {
     const long long units = (long long)p.pages.n_kv * p.pages.page_size * (p.head_dim / 8);
-    const unsigned x = (unsigned)((units + READ_THREADS * 4 - 1) / (READ_THREADS * 4));
-    auto kernel = out_dtype == KIPP_DT_F32 ? (bits == 4 ? quant_read_kernel<float, 4, ENTRIES> : quant_read_kernel<float, 8, ENTRIES>)
-                                           : (bits == 4 ? quant_read_kernel<bf16, 4, ENTRIES> : quant_read_kernel<bf16, 8, ENTRIES>);
+    if (units > 0x3fffffff) return KIPP_ERR_ARG;
+    // few pages, or small ones: a unit a thread, on more SMs
+    const bool many = units >= 4 * READ_THREADS && units * p.n > 4LL * READ_THREADS * kipp_sm_count();
+    const int per = READ_THREADS * (many ? 4 : 1);
+    const unsigned x = (unsigned)((units + per - 1) / per);
+    auto kernel = out_dtype == KIPP_DT_F32 ? (bits == 4 ? read_kernel<float, 4, ENTRIES>(p.head_dim, many) : read_kernel<float, 8, ENTRIES>(p.head_dim, many))
+                                           : (bits == 4 ? read_kernel<bf16, 4, ENTRIES>(p.head_dim, many) : read_kernel<bf16, 8, ENTRIES>(p.head_dim, many));
     // (a grid's second dimension ends at 65,535)
     for (int done = 0; done < p.n; done += 65535) {
         ReadParams q = p;

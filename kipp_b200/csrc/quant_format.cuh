@@ -37,9 +37,24 @@ template <int BITS> __device__ __forceinline__ uint16_t quant_scale(float hi, fl
 }
 __device__ __forceinline__ float quant_scale_value(uint16_t bits) { return __uint_as_float((uint32_t)bits << 16); }
 
-// The code of x; a scale of 0 (a group of zeros) has the code that stands for 0.
-template <int BITS> __device__ __forceinline__ uint32_t quant_code(float x, float scale) {
-    constexpr float L = BITS == 4 ? 8.f : 128.f;
-    const float q = scale == 0.f ? 0.f : rintf(__fdiv_rn(x, scale));
-    return (uint32_t)(int)(fminf(fmaxf(q, -L), L - 1.f) + L);
+// The code of x as a number, 0 to 2 L - 1; a scale of 0 (a group of zeros) has the code that stands for 0.  `inverse` is 1 / scale,
+// rounded: x * inverse is off from x / scale by 2^-22 of it, 2^-15 at most, so the rounding to a whole number is that of the
+// quotient unless it lies as near to the middle between two, and then the quotient is formed (one division a group instead of 32; the
+// whole number comes out of an addition of 1.5 * 2^23, ties to even, and no conversion).
+template <int BITS> __device__ __forceinline__ float quant_code(float x, float scale, float inverse) {
+    constexpr float L = BITS == 4 ? 8.f : 128.f, MAGIC = 12582912.f;
+    float q = fminf(fmaxf(__fmul_rn(x, inverse), -L), L - 1.f);
+    float r = __fsub_rn(__fadd_rn(q, MAGIC), MAGIC);
+    if (fabsf(q - r) > 0.5f - 0x1p-14f || inverse == 0.f)
+        r = scale == 0.f ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -L), L - 1.f);
+    return r + L;
+}
+// (0 where it may not be a number: a scale of 0, or a subnormal one)
+__device__ __forceinline__ float quant_inverse(float scale) { return fabsf(scale) < 0x1p-126f ? 0.f : __fdiv_rn(1.f, scale); }
+// four codes as whole numbers in one: their bits side by side in the low 4 BITS bits (exact: at most 2^24 of 4 bits' worth, or two
+// halves of 16)
+template <int BITS> __device__ __forceinline__ uint32_t quant_pack4(float c0, float c1, float c2, float c3) {
+    constexpr float MAGIC = 8388608.f;
+    if constexpr (BITS == 4) return __float_as_uint(fmaf(c3, 4096.f, fmaf(c2, 256.f, fmaf(c1, 16.f, c0))) + MAGIC) & 0xffffu;
+    return __byte_perm(__float_as_uint(fmaf(c1, 256.f, c0) + MAGIC), __float_as_uint(fmaf(c3, 256.f, c2) + MAGIC), 0x5410);
 }

@@ -48,7 +48,8 @@ def random_pages(n_pages, nkv, page, D, bits, seed=0):
 # ------------------------------------------------------------------ writing
 WRITES = [dict(D=128, nq=4, nkv=2, rot=128, page=16, norm=True), dict(D=64, nq=3, nkv=1, rot=64, page=8, norm=True, pad=8),
           dict(D=256, nq=2, nkv=2, rot=256, page=4, norm=True, w16=True), dict(D=128, nq=2, nkv=1, rot=0, page=5, norm=False),
-          dict(D=64, nq=2, nkv=2, rot=32, page=16, norm=True), dict(D=96, nq=3, nkv=1, rot=96, page=16, norm=True),
+          dict(D=64, nq=2, nkv=2, rot=32, page=16, norm=True), dict(D=256, nq=2, nkv=1, rot=128, page=16, norm=True), dict(D=128, nq=3, nkv=1, rot=64, page=8, norm=False),
+          dict(D=128, nq=2, nkv=1, rot=96, page=16, norm=True), dict(D=96, nq=3, nkv=1, rot=96, page=16, norm=True),
           dict(D=32, nq=1, nkv=1, rot=20, page=1, norm=False, pad=3), dict(D=512, nq=1, nkv=1, rot=512, page=2, norm=True),
           dict(D=128, nq=2, nkv=2, rot=128, page=16, norm=True, pad=1), dict(D=128, nq=4, nkv=2, rot=128, page=16, norm=False, long=70)]
 
@@ -78,7 +79,10 @@ def test_write(case, bits, dtype):
     assert st.tolist() == [0, 0, 0, 0]
     x = qkv.float().reshape(T, nq + 2 * nkv, D)
     want_q = Q.heads(x[:, :nq], qw, 1e-6, cos_sin, rot).to(dtype)
-    assert torch.equal(q_out.cpu(), want_q)
+    # (the queries' sum of squares may be formed in 32 bits: 2^-22 of the row beside the rounding to their type)
+    near_q = lambda got, want: ((got.cpu().double() - want.double()).abs() <= (2.0 ** -8 if dtype == BF16 else 2.0 ** -24) * want.double().abs()   # noqa: E731
+                                + 2.0 ** -21 * want.double().abs().amax(-1, keepdim=True)).all()
+    assert near_q(q_out, want_q)
     # (the plain form's own operations are those of the definition to rounding)
     if qw is not None and dtype == F32:
         exact = x[:, :nq].double() / ((x[:, :nq].double() ** 2).mean(-1, keepdim=True) + 1e-6).sqrt() * qw.double()
@@ -98,7 +102,7 @@ def test_write(case, bits, dtype):
     before = pages.k_codes.clone()
     K.qk_norm_rope_write_quantized(on(-wide)[:, :width], q_out, pages, on(qw), on(kw), 1e-6, None, rot, meta.positions,
                                    meta.entry_of_token, meta.block_tables[0], T, nq, False, st, cos_sin=on(cos_sin))
-    assert torch.equal(pages.k_codes, before) and torch.equal(q_out.cpu(), -want_q)
+    assert torch.equal(pages.k_codes, before) and near_q(q_out, -want_q)
 
 
 @pytest.mark.parametrize("D", [64, 96])
