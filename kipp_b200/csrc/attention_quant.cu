@@ -53,11 +53,15 @@ struct Params {
     int entries, table_width, page_size, page_shift, n_pages, most, n_q, n_kv, group, window;
     float score_scale, query_scale;  // |scale| * log2(e) * 2^73; 2^60 with the scale's sign
     float* part_o; float* part_ml;   // [2 ctas][columns][D], [2 ctas][columns][2]
+    // by CTA, the row that it begins and others go on with: (entry, kv head, 2 first column + the slot of its part, the row's last unit,
+    // or -1: there is no such row); behind them the cut
+    int4* shared;
     int ctas, most_blocks;           // most_blocks: rows of an entry of `most` tokens
     int* status;
 };
 
 constexpr int ROW_COST = 1;          // units of a row beside its steps
+constexpr int MANY_PARTS = 16;       // CTAs a row from which on 16 warps join its parts, not 4
 
 // One entry's share of the work.
 struct Entry {
@@ -239,6 +243,10 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
     __syncthreads();
     int entry = place.entry, at = place.at;
     pdl_wait();
+    if (threadIdx.x == 0 && p.shared != nullptr) {
+        p.shared[blockIdx.x] = make_int4(0, 0, 0, -1);
+        if (blockIdx.x == 0) p.shared[p.ctas] = make_int4(place.cuts.ctas, place.cuts.per, place.cuts.more, 0);
+    }
     if (entry < 0) return;
     const int run_first = place.cuts.start(blockIdx.x), run_end = place.cuts.start(blockIdx.x + 1);
 
@@ -618,6 +626,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                 *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * COLS + col) * 2) = make_float2(mx, sum);
             }
         }
+        if (threadIdx.x == THREADS - 1 && p.shared != nullptr && from == 0 && !whole)
+            p.shared[blockIdx.x] = make_int4(entry, g, 2 * column0 + (slot & 1), x - 1 + en.n_steps - n);
         __syncthreads();
         for (int i = threadIdx.x * 4; i < live * D; i += THREADS * 4) {
             const int col = i / D, d = i % D;
@@ -640,53 +650,25 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
     }
 }
 
-// Adds the parts of one head of one token of a row that CTAs shared, in an order that the cut alone sets.  Block x is
-// a row (BY_ROW) or the row that CTA x begins and the next one goes on with; y is the column.  A warp reads whole parts, D / 32
-// values a lane, every MERGE_WARPS-th of them.
-template <int D, int NT, int MERGE_WARPS, bool BY_ROW>
-__global__ void __launch_bounds__(MERGE_WARPS * 32) attn_quant_merge_kernel(const Params p) {
-    constexpr int COLS = 8 * NT, PER = D / 32, BATCH = 8;
-    __shared__ float sh_o[MERGE_WARPS][D], sh_l[MERGE_WARPS];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y;
-    // (every warp for itself, from the step's lists)
-    int row_start = 0;
-    const Place at = find_unit<COLS>(p, [&](int total, const Cut& c) {
-        return BY_ROW ? -1 : (int)blockIdx.x + 1 < c.ctas ? c.start(blockIdx.x + 1) - 1 : -1;
-    });
-    int e = at.entry, block;
-    Entry en;
-    if constexpr (BY_ROW) {
-        e = blockIdx.x / p.most_blocks;
-        block = blockIdx.x - e * p.most_blocks;
-        en = entry_of<COLS>(p, e);
-        int before = 0;
-        for (int i = lane; i < e; i += 32) before += entry_of<COLS>(p, i).units();
-        row_start = (int)__reduce_add_sync(0xffffffffu, (unsigned)before) + block * en.row_units();
-        if (block >= en.blocks) e = -1;
-    } else if (e >= 0) {
-        en = entry_of<COLS>(p, e);
-        block = at.at / en.row_units();
-        row_start = at.cuts.start(blockIdx.x + 1) - 1 - (at.at - block * en.row_units());
-    }
-    pdl_wait();
-    if (e < 0) return;
-    const int c0 = at.cuts.cta_of(row_start + ROW_COST), parts = at.cuts.cta_of(row_start + en.row_units() - 1) - c0 + 1;
-    const int g = block / en.column_blocks, c = (block - g * en.column_blocks) * COLS + col;
-    if (parts < 2 || (!BY_ROW && c0 != (int)blockIdx.x) || c >= en.q_len * p.group) return;
-    // (a CTA's first piece is in slot 0)
-    auto index = [&](int part) { return (size_t)(2 * (c0 + part) + (row_start > at.cuts.start(c0 + part) ? 1 : 0)) * COLS + col; };
+// One warp adds the parts first, first + step, .. of a column: D / 32 values a lane, `sum` of the weights.  `index` gives the place of a
+// part.  (What it needs of the first parts is asked for before the largest maximum is known.)
+template <int D, typename Index>
+__device__ __forceinline__ void add_parts(const Params& p, int first, int step, int parts, Index index, float (&acc)[D / 32], float& sum) {
+    constexpr int PER = D / 32, BATCH = D == 256 ? 4 : 8;
+    const int lane = threadIdx.x & 31;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
     float mx = -INFINITY;
     for (int i = lane; i < parts; i += 32) mx = fmaxf(mx, ml[index(i)].x);
-    float acc[PER], sum = 0.f;
+    bool known = false;
+    sum = 0.f;
 #pragma unroll
     for (int k = 0; k < PER; ++k) acc[k] = 0.f;
-    for (int first = warp; first < parts; first += MERGE_WARPS * BATCH) {
+    for (; first < parts; first += step * BATCH) {
         float r[BATCH][PER];
         float2 f[BATCH];
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
-            const int part = first + i * MERGE_WARPS;
+            const int part = first + i * step;
             f[i] = make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int k = 0; k < PER; ++k) r[i][k] = 0.f;
@@ -696,7 +678,8 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) attn_quant_merge_kernel(cons
                 for (int k = 0; k < PER; ++k) r[i][k] = p.part_o[index(part) * D + k * 32 + lane];
             }
         }
-        if (first == warp) mx = warp_max(mx);
+        if (!known) mx = warp_max(mx);
+        known = true;
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
             const float w = f[i].x == -INFINITY ? 0.f : exp2_fast(f[i].x - mx);
@@ -705,20 +688,77 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) attn_quant_merge_kernel(cons
             for (int k = 0; k < PER; ++k) acc[k] = fmaf(r[i][k], w, acc[k]);
         }
     }
+}
+template <int D> __device__ __forceinline__ bf16* result_of(const Params& p, int e, int g, int c) {
+    const int tok = c / p.group;
+    return p.out + ((size_t)(p.q_start[e] + tok) * p.n_q + g * p.group + (c - tok * p.group)) * D;
+}
+
+// Adds the parts of the row that CTA x of the first kernel began, in the order of the keys: a warp a column.
+constexpr int JOIN_WARPS = 4;
+template <int D, int NT>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) attn_quant_join_kernel(const Params p) {
+    constexpr int COLS = 8 * NT;
+    pdl_wait();
+    const int4 row = p.shared[blockIdx.x], cut = p.shared[p.ctas];
+    const int e = row.x, lane = threadIdx.x & 31;
+    if (row.w < 0) return;
+    Cut cuts;
+    cuts.ctas = cut.x;
+    cuts.per = cut.y;
+    cuts.more = cut.z;
+    const int parts = cuts.cta_of(row.w) - (int)blockIdx.x + 1;
+    const int columns = (p.q_start[e + 1] - p.q_start[e]) * p.group - (row.z >> 1);
+    for (int col = threadIdx.x >> 5; col < min(COLS, columns); col += JOIN_WARPS) {
+        auto index = [&](int part) { return (size_t)(2 * ((int)blockIdx.x + part) + (part == 0 ? row.z & 1 : 0)) * COLS + col; };
+        float acc[D / 32], sum;
+        add_parts<D>(p, 0, 1, parts, index, acc, sum);
+        bf16* out = result_of<D>(p, e, row.y, (row.z >> 1) + col);
 #pragma unroll
-    for (int k = 0; k < PER; ++k) sh_o[warp][k * 32 + lane] = acc[k];
+        for (int k = 0; k < D / 32; ++k) out[k * 32 + lane] = __float2bfloat16_rn(sum > 0.f ? acc[k] / sum : 0.f);
+    }
+}
+
+// The same where there are no more rows than CTAs: a block a row and column, MERGE_WARPS warps that share the parts.  What a block
+// is to do it finds from the step's lists before the wait.  (Eight tokens of 8,100 keys, 64 rows of some 7 parts: 25.5 us in all,
+// 26.5 with the kernel above; 64 of 2,048, 512 rows on 444 CTAs: 46.7 and 44.9.)
+template <int D, int NT, int MERGE_WARPS>
+__global__ void __launch_bounds__(MERGE_WARPS * 32) attn_quant_merge_kernel(const Params p) {
+    constexpr int COLS = 8 * NT;
+    __shared__ float sh_o[MERGE_WARPS][D], sh_l[MERGE_WARPS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y, e = blockIdx.x / p.most_blocks, block = blockIdx.x - e * p.most_blocks;
+    // (every warp for itself, from the step's lists)
+    const Entry en = entry_of<COLS>(p, e);
+    int total = 0, before = 0;
+    for (int i = lane; i < p.entries; i += 32) {
+        const int u = entry_of<COLS>(p, i).units();
+        total += u;
+        if (i < e) before += u;
+    }
+    const Cut cuts((int)__reduce_add_sync(0xffffffffu, (unsigned)total), p.ctas);
+    const int row_start = (int)__reduce_add_sync(0xffffffffu, (unsigned)before) + block * en.row_units();
+    pdl_wait();
+    if (block >= en.blocks) return;
+    const int c0 = cuts.cta_of(row_start + ROW_COST), parts = cuts.cta_of(row_start + en.row_units() - 1) - c0 + 1;
+    const int g = block / en.column_blocks, c = (block - g * en.column_blocks) * COLS + col;
+    if (parts < 2 || c >= en.q_len * p.group) return;
+    // (a CTA's first piece is in slot 0)
+    auto index = [&](int part) { return (size_t)(2 * (c0 + part) + (row_start > cuts.start(c0 + part) ? 1 : 0)) * COLS + col; };
+    float acc[D / 32], sum;
+    add_parts<D>(p, warp, MERGE_WARPS, parts, index, acc, sum);
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) sh_o[warp][k * 32 + lane] = acc[k];
     if (lane == 0) sh_l[warp] = sum;
     __syncthreads();
-    float total = 0.f;
+    sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < MERGE_WARPS; ++w) total += sh_l[w];
-    const int tok = c / p.group;
-    bf16* out = p.out + ((size_t)(p.q_start[e] + tok) * p.n_q + g * p.group + (c - tok * p.group)) * D;
+    for (int w = 0; w < MERGE_WARPS; ++w) sum += sh_l[w];
+    bf16* out = result_of<D>(p, e, g, c);
     for (int d = threadIdx.x; d < D; d += MERGE_WARPS * 32) {
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < MERGE_WARPS; ++w) v += sh_o[w][d];
-        out[d] = __float2bfloat16_rn(total > 0.f ? v / total : 0.f);
+        out[d] = __float2bfloat16_rn(sum > 0.f ? v / sum : 0.f);
     }
 }
 
@@ -749,14 +789,16 @@ template <int D, int BITS, int NT, bool TILES> int launch(Params p, long long st
     const int wave_ctas = wave<D, BITS, NT, TILES>();
     const long long rows = (long long)p.entries * p.most_blocks, units = rows * (steps_of_row + ROW_COST);
     p.ctas = (int)(units < wave_ctas ? units : wave_ctas);
+    const bool alone = steps_of_row <= 1, by_cta = !alone && rows > p.ctas;            // (alone: every row is one step, none is shared)
+    if (!by_cta) p.shared = nullptr;
     if (const int e = kipp_allow_smem(attn_quant_kernel<D, BITS, NT, TILES>, smem)) return e;
     if (const int e = kipp_launch(attn_quant_kernel<D, BITS, NT, TILES>, dim3((unsigned)p.ctas), dim3(THREADS), smem, s, 1, p)) return e;
-    if (steps_of_row <= 1) return 0;                   // every row is one step: none is shared
-    const int columns = p.most * p.group, y = columns < COLS ? columns : COLS;
-    // a block a row, or a CTA where those are fewer; rows of few are cut into many parts
-    if (rows > p.ctas) return kipp_launch(attn_quant_merge_kernel<D, NT, 2, false>, dim3((unsigned)p.ctas, (unsigned)y), dim3(64), 0, s, 1, p);
-    if (rows * 16 > p.ctas) return kipp_launch(attn_quant_merge_kernel<D, NT, 4, true>, dim3((unsigned)rows, (unsigned)y), dim3(128), 0, s, 1, p);
-    return kipp_launch(attn_quant_merge_kernel<D, NT, 16, true>, dim3((unsigned)rows, (unsigned)y), dim3(512), 0, s, 1, p);
+    if (alone) return 0;
+    if (by_cta) return kipp_launch(attn_quant_join_kernel<D, NT>, dim3((unsigned)p.ctas), dim3(JOIN_WARPS * 32), 0, s, 1, p);
+    const int columns = p.most * p.group;
+    const dim3 grid((unsigned)rows, (unsigned)(columns < COLS ? columns : COLS));
+    if (rows * MANY_PARTS > p.ctas) return kipp_launch(attn_quant_merge_kernel<D, NT, 4>, grid, dim3(128), 0, s, 1, p);
+    return kipp_launch(attn_quant_merge_kernel<D, NT, 16>, grid, dim3(512), 0, s, 1, p);
 }
 
 // 8 columns where they hold every query of a kv head, else 16 (heads of 256 have no room for their sums: always 8)
@@ -769,7 +811,7 @@ extern "C" int kipp_attn_quant_supported(int bits, int head_dim, int n_q, int n_
 }
 // Bytes of scratch of a launch (the parts of rows that several CTAs share), whatever the step.
 extern "C" long long kipp_attn_quant_scratch_bytes(int head_dim) {
-    return 2LL * MOST_CTAS * MOST_COLUMNS * (head_dim + 2) * 4;
+    return 2LL * MOST_CTAS * MOST_COLUMNS * (head_dim + 2) * 4 + (MOST_CTAS + 1) * 16LL;
 }
 
 struct KippAttnQuant {
@@ -815,6 +857,7 @@ extern "C" int kipp_attn_quant(const KippAttnQuant* a) {
     p.query_scale = a->scale < 0.f ? -0x1p60f : 0x1p60f;
     p.part_o = (float*)a->scratch;
     p.part_ml = p.part_o + 2LL * MOST_CTAS * MOST_COLUMNS * head_dim;
+    p.shared = (int4*)(p.part_ml + 2LL * MOST_CTAS * MOST_COLUMNS * 2);
     p.most_blocks = (int)blocks;
     p.status = a->status;
     cudaStream_t s = (cudaStream_t)a->stream;

@@ -116,11 +116,6 @@ __global__ void __launch_bounds__(128) quant_write_any_kernel(const WriteParams 
     }
 }
 
-__device__ __forceinline__ void take8(float (&x)[8], const bf16* p) { unpack8(x, *reinterpret_cast<const uint4*>(p)); }
-__device__ __forceinline__ void take8(float (&x)[8], const float* p) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
 __device__ __forceinline__ void put8(bf16* p, const float (&x)[8]) { *reinterpret_cast<uint4*>(p) = pack8(x); }
 __device__ __forceinline__ void put8(float* p, const float (&x)[8]) {
     reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -143,115 +138,139 @@ template <int BITS> __device__ __forceinline__ void put_codes(uint8_t* p, const 
 // formed for keys only: queries get no codes, and four in five heads are theirs.
 // 2,048 tokens of 32 and 2 x 8 heads of 128, 8 bits: see the table of cases in the design document.
 constexpr int WRITE_THREADS = 128;
+__device__ __forceinline__ void fetch8(uint4 (&raw)[1], const bf16* p) { raw[0] = *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ void fetch8(uint4 (&raw)[2], const float* p) {
+    raw[0] = reinterpret_cast<const uint4*>(p)[0];
+    raw[1] = reinterpret_cast<const uint4*>(p)[1];
+}
+__device__ __forceinline__ void spread8(float (&x)[8], const uint4 (&raw)[1]) { unpack8(x, raw[0]); }
+__device__ __forceinline__ void spread8(float (&x)[8], const uint4 (&raw)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        x[4 * i] = __uint_as_float(raw[i].x); x[4 * i + 1] = __uint_as_float(raw[i].y);
+        x[4 * i + 2] = __uint_as_float(raw[i].z); x[4 * i + 3] = __uint_as_float(raw[i].w);
+    }
+}
 template <typename T, int BITS, int HEAD_DIM>
 __global__ void __launch_bounds__(WRITE_THREADS) quant_write_kernel(const WriteParams p) {
-    constexpr int LPH = HEAD_DIM / 16, HALF = HEAD_DIM / 2, G = HEAD_DIM / 32;
+    constexpr int LPH = HEAD_DIM / 16, HALF = HEAD_DIM / 2, G = HEAD_DIM / 32, PER = WRITE_THREADS / LPH, RAW = sizeof(T) / 2;
     pdl_launch_dependents();
-    const int t = blockIdx.y, h = blockIdx.x * (WRITE_THREADS / LPH) + threadIdx.x / LPH, sub = threadIdx.x % LPH;
-    const int n_kv = p.pages.n_kv;
-    const bool is_q = h < p.n_q, is_k = !is_q && h < p.n_q + n_kv;
-    const bool active = h < p.n_q + 2 * n_kv && (is_q || p.write_cache), normed = active && (is_q || is_k);
-    // (the step's lists and the weights, before the wait)
-    long long at = -1;
-    if (active && !is_q) at = cache_row(p, t, is_k ? h - p.n_q : h - p.n_q - n_kv);
-    float wa[8], wb[8];
-    if (p.q_norm_w != nullptr && normed) {        // both weights or neither (checked by the host)
-        const void* nw = is_q ? p.q_norm_w : p.k_norm_w;
-        load_w8(wa, nw, p.norm_dtype, sub * 8);
-        load_w8(wb, nw, p.norm_dtype, HALF + sub * 8);
-    }
-    pdl_wait();
-    // No lane leaves early: a warp holds several heads and all lanes take part in the exchanges.
-    float a[8], b[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
-    if (active) {
-        const T* src = static_cast<const T*>(p.qkv) + (size_t)t * p.ld + (size_t)h * HEAD_DIM + sub * 8;
-        take8(a, src);
-        take8(b, src + HALF);
-    }
+    const int t = blockIdx.y, sub = threadIdx.x % LPH;
+    const int n_kv = p.pages.n_kv, heads = p.n_q + (p.write_cache ? 2 * n_kv : 0);
+    const T* const row = static_cast<const T*>(p.qkv) + (size_t)t * p.ld + sub * 8;
+    int h = blockIdx.x * PER + threadIdx.x / LPH;
+    // (the step's lists, before the wait)
+    const int pos = p.positions[t], slot = pos / p.pages.page_size;
+    int page = -1;
+    if (p.write_cache && pos >= 0 && slot < p.table_width) page = p.block_table[(size_t)p.entry_of_token[t] * p.table_width + slot];
+    if (page >= p.pages.n_pages) page = -1;
     const bool whole = p.rotary_dim == HEAD_DIM;
+    pdl_wait();
+    uint4 raw_a[RAW], raw_b[RAW];
+    if (h < heads) {
+        fetch8(raw_a, row + (size_t)h * HEAD_DIM);
+        fetch8(raw_b, row + (size_t)h * HEAD_DIM + HALF);
+    }
     float4 cs[4];
-    if (p.cos_sin != nullptr && normed) {
-        const float4* row = reinterpret_cast<const float4*>(p.cos_sin + (size_t)t * (p.rotary_dim / 2) + (whole ? sub : sub % (LPH / 2)) * 8);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) cs[i] = row[i];
-    }
-    if (p.q_norm_w != nullptr) {
-        float mean;
-        if (__any_sync(0xffffffffu, is_k)) {
-            double ss = 0.0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) ss += (double)a[i] * (double)a[i] + (double)b[i] * (double)b[i];
-#pragma unroll
-            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            mean = mean_square(ss, HEAD_DIM);
-        } else {
-            float ss = head_ssq8(a, b);
-#pragma unroll
-            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            mean = ss * (1.f / HEAD_DIM);
-        }
-        if (normed) {
-            const float r = norm_factor(mean, p.eps);
-            head_scale8(a, r, wa);
-            head_scale8(b, r, wb);
-        }
-    }
     if (p.cos_sin != nullptr) {
-        if (whole) {
+        const float4* c = reinterpret_cast<const float4*>(p.cos_sin + (size_t)t * (p.rotary_dim / 2) + (whole ? sub : sub % (LPH / 2)) * 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cs[i] = c[i];
+    }
+    float wa[8], wb[8];
+    const void* have = nullptr;                   // the norm whose weights these are
+    if (page < 0 && p.write_cache && blockIdx.x == 0 && threadIdx.x == 0) atomicExch(p.status, 2);      // unmapped page: refused, never written
+    // No lane leaves early: a warp holds several heads and all lanes take part in the exchanges.
+    for (int first = blockIdx.x * PER; first < heads; first += gridDim.x * PER, h += gridDim.x * PER) {
+        const bool active = h < heads, is_q = h < p.n_q, is_k = !is_q && h < p.n_q + n_kv, normed = active && (is_q || is_k);
+        float a[8], b[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+        if (active) { spread8(a, raw_a); spread8(b, raw_b); }
+        if (h + (int)gridDim.x * PER < heads) {
+            fetch8(raw_a, row + (size_t)(h + gridDim.x * PER) * HEAD_DIM);
+            fetch8(raw_b, row + (size_t)(h + gridDim.x * PER) * HEAD_DIM + HALF);
+        }
+        if (p.q_norm_w != nullptr) {              // both weights or neither (checked by the host)
+            const void* nw = is_q ? p.q_norm_w : p.k_norm_w;
+            if (normed && have != nw) {
+                load_w8(wa, nw, p.norm_dtype, sub * 8);
+                load_w8(wb, nw, p.norm_dtype, HALF + sub * 8);
+                have = nw;
+            }
+            float mean;
+            if (__any_sync(0xffffffffu, is_k)) {
+                double ss = 0.0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss += (double)a[i] * (double)a[i] + (double)b[i] * (double)b[i];
+#pragma unroll
+                for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                mean = mean_square(ss, HEAD_DIM);
+            } else {
+                float ss = head_ssq8(a, b);
+#pragma unroll
+                for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                mean = ss * (1.f / HEAD_DIM);
+            }
             if (normed) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    turn(a[2 * i], b[2 * i], make_float2(cs[i].x, cs[i].y));
-                    turn(a[2 * i + 1], b[2 * i + 1], make_float2(cs[i].z, cs[i].w));
-                }
+                const float r = norm_factor(mean, p.eps);
+                head_scale8(a, r, wa);
+                head_scale8(b, r, wb);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float other = __shfl_xor_sync(0xffffffffu, a[i], LPH / 2);
+        }
+        if (p.cos_sin != nullptr) {
+            if (whole) {
                 if (normed) {
-                    const float2 c = i & 1 ? make_float2(cs[i / 2].z, cs[i / 2].w) : make_float2(cs[i / 2].x, cs[i / 2].y);
-                    if (sub < LPH / 2) turn(a[i], other, c);
-                    else { turn(other, a[i], c); }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        turn(a[2 * i], b[2 * i], make_float2(cs[i].x, cs[i].y));
+                        turn(a[2 * i + 1], b[2 * i + 1], make_float2(cs[i].z, cs[i].w));
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float other = __shfl_xor_sync(0xffffffffu, a[i], LPH / 2);
+                    if (normed) {
+                        const float2 c = i & 1 ? make_float2(cs[i / 2].z, cs[i / 2].w) : make_float2(cs[i / 2].x, cs[i / 2].y);
+                        if (sub < LPH / 2) turn(a[i], other, c);
+                        else turn(other, a[i], c);
+                    }
                 }
             }
         }
-    }
-    if (active && is_q) {
-        T* dst = static_cast<T*>(p.q_out) + ((size_t)t * p.n_q + h) * HEAD_DIM + sub * 8;
-        put8(dst, a);
-        put8(dst + HALF, b);
-    }
-    if (__all_sync(0xffffffffu, is_q)) return;
-    float hi[2], lo[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        hi[r] = -INFINITY; lo[r] = INFINITY;
-#pragma unroll
-        for (int i = 4 * r; i < 4 * r + 4; ++i) {
-            a[i] = quant_input(a[i]); b[i] = quant_input(b[i]);
-            hi[r] = fmaxf(hi[r], fmaxf(a[i], b[i]));
-            lo[r] = fminf(lo[r], fminf(a[i], b[i]));
+        if (active && is_q) {
+            T* dst = static_cast<T*>(p.q_out) + ((size_t)t * p.n_q + h) * HEAD_DIM + sub * 8;
+            put8(dst, a);
+            put8(dst + HALF, b);
         }
+        if (__all_sync(0xffffffffu, is_q)) continue;
+        float hi[2], lo[2];
 #pragma unroll
-        for (int o = G / 2; o <= G; o <<= 1) {
-            hi[r] = fmaxf(hi[r], __shfl_xor_sync(0xffffffffu, hi[r], o));
-            lo[r] = fminf(lo[r], __shfl_xor_sync(0xffffffffu, lo[r], o));
+        for (int r = 0; r < 2; ++r) {
+            hi[r] = -INFINITY; lo[r] = INFINITY;
+#pragma unroll
+            for (int i = 4 * r; i < 4 * r + 4; ++i) {
+                a[i] = quant_input(a[i]); b[i] = quant_input(b[i]);
+                hi[r] = fmaxf(hi[r], fmaxf(a[i], b[i]));
+                lo[r] = fminf(lo[r], fminf(a[i], b[i]));
+            }
+#pragma unroll
+            for (int o = G / 2; o <= G; o <<= 1) {
+                hi[r] = fmaxf(hi[r], __shfl_xor_sync(0xffffffffu, hi[r], o));
+                lo[r] = fminf(lo[r], __shfl_xor_sync(0xffffffffu, lo[r], o));
+            }
         }
+        if (page < 0 || !active || is_q) continue;
+        const size_t at = ((size_t)page * n_kv + (is_k ? h - p.n_q : h - p.n_q - n_kv)) * p.pages.page_size + (pos - slot * p.pages.page_size);
+        const uint16_t b0 = quant_scale<BITS>(hi[0], lo[0]), b1 = quant_scale<BITS>(hi[1], lo[1]);
+        const float s0 = quant_scale_value(b0), s1 = quant_scale_value(b1), i0 = quant_inverse(s0), i1 = quant_inverse(s1);
+        uint8_t* codes = (is_k ? p.pages.k_codes : p.pages.v_codes) + at * (HEAD_DIM * BITS / 8) + sub * BITS;
+        put_codes<BITS>(codes, a, s0, i0, s1, i1);
+        put_codes<BITS>(codes + HALF * BITS / 8, b, s0, i0, s1, i1);
+        if (sub < G / 2)
+            reinterpret_cast<uint32_t*>((is_k ? p.pages.k_scales : p.pages.v_scales) + at * G)[sub] = (uint32_t)b0 | (uint32_t)b1 << 16;
     }
-    if (at < 0) {                                 // unmapped page: refuse, never write
-        if (active && !is_q && sub == 0) atomicExch(p.status, 2);
-        return;
-    }
-    const uint16_t b0 = quant_scale<BITS>(hi[0], lo[0]), b1 = quant_scale<BITS>(hi[1], lo[1]);
-    const float s0 = quant_scale_value(b0), s1 = quant_scale_value(b1), i0 = quant_inverse(s0), i1 = quant_inverse(s1);
-    uint8_t* codes = (is_k ? p.pages.k_codes : p.pages.v_codes) + (size_t)at * (HEAD_DIM * BITS / 8) + sub * BITS;
-    put_codes<BITS>(codes, a, s0, i0, s1, i1);
-    put_codes<BITS>(codes + HALF * BITS / 8, b, s0, i0, s1, i1);
-    if (sub < G / 2)
-        reinterpret_cast<uint32_t*>((is_k ? p.pages.k_scales : p.pages.v_scales) + (size_t)at * G)[sub] = (uint32_t)b0 | (uint32_t)b1 << 16;
 }
 
 template <typename T, int BITS> int launch_write(const WriteParams& p, cudaStream_t s) {
@@ -261,7 +280,10 @@ template <typename T, int BITS> int launch_write(const WriteParams& p, cudaStrea
     const bool aligned = (bits & 15) == 0 && p.ld * (long long)sizeof(T) % 16 == 0;
     if (aligned && (p.cos_sin == nullptr || p.rotary_dim == D || p.rotary_dim * 2 == D) && p.tokens <= 65535 && (D == 64 || D == 128 || D == 256)) {
         const int per = WRITE_THREADS / (D / 16);
-        const dim3 grid((unsigned)((heads + per - 1) / per), (unsigned)p.tokens);
+        // A block takes all heads of a token where there are tokens enough: the norms' weights and the angles are read once, and the
+        // next heads are on their way meanwhile.
+        const int shares = (heads + per - 1) / per;
+        const dim3 grid((unsigned)(p.tokens >= 4 * kipp_sm_count() ? 1 : shares), (unsigned)p.tokens);
         auto kernel = D == 64 ? quant_write_kernel<T, BITS, 64> : D == 128 ? quant_write_kernel<T, BITS, 128> : quant_write_kernel<T, BITS, 256>;
         return kipp_launch(kernel, grid, dim3(WRITE_THREADS), 0, s, 1, p);
     }
@@ -298,12 +320,18 @@ template <int BITS> __device__ __forceinline__ void whole_numbers(__nv_bfloat162
     }
 }
 template <int BITS> struct Unit { uint32_t w[BITS / 4]; uint16_t s[2]; };      // eight channels: codes, the scales of their two runs
-template <int BITS> __device__ __forceinline__ Unit<BITS> take_unit(const uint8_t* codes, const uint16_t* scales, int g0, int g1) {
+template <int BITS, bool EVEN> __device__ __forceinline__ Unit<BITS> take_unit(const uint8_t* codes, const uint16_t* scales, int g0, int g1) {
     Unit<BITS> u;
     if constexpr (BITS == 4) u.w[0] = *reinterpret_cast<const uint32_t*>(codes);
     else { const uint2 v = *reinterpret_cast<const uint2*>(codes); u.w[0] = v.x; u.w[1] = v.y; }
-    u.s[0] = scales[g0];
-    u.s[1] = scales[g1];
+    if constexpr (EVEN) {                                 // (an even number of groups: the two lie side by side)
+        const uint32_t both = *reinterpret_cast<const uint32_t*>(scales + g0);
+        u.s[0] = (uint16_t)both;
+        u.s[1] = (uint16_t)(both >> 16);
+    } else {
+        u.s[0] = scales[g0];
+        u.s[1] = scales[g1];
+    }
     return u;
 }
 // (the scale times 2^13, exact, and one rounding)
@@ -367,8 +395,8 @@ __global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const ReadPara
             k[j] = v[j] = Unit<BITS>{};
             if (u < units && ok) {
                 const int row = u / per_row, c = u - row * per_row, g0 = 2 * c % G, g1 = g0 + 1 == G ? 0 : g0 + 1;
-                k[j] = take_unit<BITS>(k_codes + (size_t)u * BITS, k_scales + row * G, g0, g1);
-                v[j] = take_unit<BITS>(v_codes + (size_t)u * BITS, v_scales + row * G, g0, g1);
+                k[j] = take_unit<BITS, (DIM > 0)>(k_codes + (size_t)u * BITS, k_scales + row * G, g0, g1);
+                v[j] = take_unit<BITS, (DIM > 0)>(v_codes + (size_t)u * BITS, v_scales + row * G, g0, g1);
             }
         }
 #pragma unroll
@@ -393,7 +421,7 @@ template <bool ENTRIES> int launch_read(const ReadParams& p, int bits, int out_d
     const long long units = (long long)p.pages.n_kv * p.pages.page_size * (p.head_dim / 8);
     if (units > 0x3fffffff) return KIPP_ERR_ARG;
     // few pages, or small ones: a unit a thread, on more SMs
-    const bool many = units >= 4 * READ_THREADS && units * p.n > 4LL * READ_THREADS * kipp_sm_count();
+    const bool many = units >= 4 * READ_THREADS && units * p.n > 32LL * READ_THREADS * kipp_sm_count();
     const int per = READ_THREADS * (many ? 4 : 1);
     const unsigned x = (unsigned)((units + per - 1) / per);
     auto kernel = out_dtype == KIPP_DT_F32 ? (bits == 4 ? read_kernel<float, 4, ENTRIES>(p.head_dim, many) : read_kernel<float, 8, ENTRIES>(p.head_dim, many))
