@@ -809,9 +809,10 @@ int columns_of(int head_dim, long long queries) { return head_dim == 256 || quer
 extern "C" int kipp_attn_quant_supported(int bits, int head_dim, int n_q, int n_kv) {
     return (bits == 4 || bits == 8) && (head_dim == 64 || head_dim == 128 || head_dim == 256) && n_kv > 0 && n_q > 0 && n_q % n_kv == 0;
 }
-// Bytes of scratch of a launch (the parts of rows that several CTAs share), whatever the step.
-extern "C" long long kipp_attn_quant_scratch_bytes(int head_dim) {
-    return 2LL * MOST_CTAS * MOST_COLUMNS * (head_dim + 2) * 4 + (MOST_CTAS + 1) * 16LL;
+// Bytes of scratch of a launch (the parts of rows that several CTAs share) whose block table has room for `room` keys an entry,
+// whatever the step: none where a row is one step.
+extern "C" long long kipp_attn_quant_scratch_bytes(int head_dim, long long room) {
+    return room <= STEP ? 0 : 2LL * MOST_CTAS * MOST_COLUMNS * (head_dim + 2) * 4 + (MOST_CTAS + 1) * 16LL;
 }
 
 struct KippAttnQuant {
@@ -831,9 +832,10 @@ extern "C" int kipp_attn_quant(const KippAttnQuant* a) {
     const int bits = a->bits, head_dim = a->head_dim, n_q = a->n_q, n_kv = a->n_kv, entries = a->entries, most = a->most, page_size = a->page_size;
     if (entries <= 0 || most <= 0) return 0;
     if (!kipp_attn_quant_supported(bits, head_dim, n_q, n_kv) || page_size <= 0 || a->n_pages <= 0 || a->table_width <= 0 || a->window < 0 ||
-        a->status == nullptr || a->scratch == nullptr)
+        a->status == nullptr)
         return KIPP_ERR_ARG;
-    if (a->scratch_bytes < kipp_attn_quant_scratch_bytes(head_dim)) return -4;
+    const long long need = kipp_attn_quant_scratch_bytes(head_dim, (long long)a->table_width * page_size);
+    if (a->scratch_bytes < need || (need > 0 && a->scratch == nullptr)) return -4;
     if ((((uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->k_codes | (uintptr_t)a->v_codes | (uintptr_t)a->k_scales | (uintptr_t)a->v_scales |
           (uintptr_t)a->scratch) & 15) != 0)
         return -3;

@@ -1126,15 +1126,15 @@ public:
     void attention_quant_direct(void* out, const void* q, const PagedCacheView& cache, const int* q_start, const int* context_len,
                                 int entries, int most, int n_q, int n_kv, int head_dim, float scale, int window) {
         using Fn = int (*)(const QuantAttentionArgs*);
-        using Fb = long long (*)(int);
+        using Fb = long long (*)(int, long long);
         static Fn f = kernel_symbol<Fn>("attention_quant", "kipp_attn_quant");
         static Fb bytes = kernel_symbol<Fb>("attention_quant", "kipp_attn_quant_scratch_bytes");
-        const long long need = bytes(head_dim);
+        const long long need = bytes(head_dim, (long long)cache.table_width * cache.page_size);
         const QuantAttentionArgs a = {out, q, cache.k_pages, cache.k_scales, cache.v_pages, cache.v_scales, q_start, context_len,
                                       cache.block_table, workspace->buffer("quant_attention_scratch", (size_t)need), status, stream, need,
                                       cache.bits, cache.n_pages, cache.page_size, cache.table_width, entries, most, n_q, n_kv, head_dim,
                                       window, scale};
-        run(f(&a), "attn_quant", 2);
+        run(f(&a), "attn_quant", need > 0 ? 2 : 1);
     }
     // Causal grouped-query attention over a quantised cache.  bfloat16 heads of 64, 128 and 256 run on the codes; where portions of
     // PREFILL_TC_MIN_TOKENS and more are among the entries, those of more than one token read their pages back for the tcgen05

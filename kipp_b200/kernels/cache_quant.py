@@ -74,10 +74,11 @@ def _status(status: torch.Tensor, what: str) -> None:
         raise KernelError(f"{what}: status must be a contiguous int32 tensor of 4 words")
 
 
-def _lists(what: str, **tensors: torch.Tensor) -> None:
-    for name, t in tensors.items():
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise KernelError(f"{what}: {name} must be a contiguous int32 tensor")
+def _lists(what: str, names: str, *tensors: torch.Tensor) -> None:
+    i32 = torch.int32
+    for t in tensors:
+        if t.dtype != i32 or not t.is_contiguous():
+            raise KernelError(f"{what}: {names} must be contiguous int32 tensors")
 
 
 # the structures of the C entry points (csrc/cache_quant.cu, csrc/attention_quant.cu): addresses, then sizes
@@ -102,7 +103,7 @@ def qk_norm_rope_write_quantized(qkv: torch.Tensor, q_out: torch.Tensor, pages: 
         raise KernelError(f"{what}: qkv has the wrong shape")
     if q_out.dtype != dtype or not q_out.is_contiguous() or q_out.numel() < tokens * n_q * D:
         raise KernelError(f"{what}: q_out must be contiguous, of qkv's dtype and hold every query")
-    _lists(what, positions=positions, entry_of_token=entry_of_token, block_table=block_table)
+    _lists(what, "positions, entry_of_token and block_table", positions, entry_of_token, block_table)
     if positions.numel() < tokens or entry_of_token.numel() < tokens or block_table.dim() != 2:
         raise KernelError(f"{what}: a position and an entry for every token, and a table [entries, width]")
     if (q_norm_w is None) != (k_norm_w is None):
@@ -141,7 +142,7 @@ def read_quantized_pages(k_out: torch.Tensor, v_out: torch.Tensor, pages: Quanti
     ``k_out``, ``v_out`` [len(page_list), n_kv, page_size, D].  A negative number gives zeros, one past the
     pool zeros and status word 0 = 3."""
     what, n = "read_quantized_pages", page_list.numel()
-    _lists(what, page_list=page_list)
+    _lists(what, "page_list", page_list)
     shape = (n, pages.n_kv, pages.page_size, pages.head_dim)
     if k_out.shape != shape or v_out.shape != shape or k_out.dtype != v_out.dtype or not (k_out.is_contiguous() and v_out.is_contiguous()):
         raise KernelError(f"{what}: k_out and v_out must be contiguous, of one dtype and {shape}")
@@ -223,7 +224,7 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
     t_shape = block_table.shape
     if len(t_shape) != 2 or t_shape[0] < entries or t_shape[1] == 0 or sum(q_lens) != tokens:
         raise KernelError(f"{what}: a row of block_table for every entry, and as many tokens as the entries bring")
-    _lists(what, block_table=block_table, q_start=meta.q_start, context_len=meta.context_len)
+    _lists(what, "block_table, q_start and context_len", block_table, meta.q_start, meta.context_len)
     if meta.q_start.numel() <= entries or meta.context_len.numel() < entries:
         raise KernelError(f"{what}: the step's lists are shorter than the step")
     _status(status, what)
@@ -251,15 +252,16 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
 
 def _direct(out, q, pages, meta, block_table, n_q, scale, window, status, most: int, stream: int) -> None:
     """The entries of up to ``most`` tokens, over the codes."""
-    D = pages.head_dim
-    need = _scratch_bytes.get(D)
+    D, width = pages.head_dim, block_table.shape[1]
+    key = (D, width * pages.page_size)
+    need = _scratch_bytes.get(key)
     if need is None:
-        need = _scratch_bytes[D] = _fn("attention_quant", "kipp_attn_quant_scratch_bytes", [c_int], restype=c_ll)(D)
-    scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+        need = _scratch_bytes[key] = _fn("attention_quant", "kipp_attn_quant_scratch_bytes", [c_int, c_ll], restype=c_ll)(*key)
+    scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     _call("attention_quant", "kipp_attn_quant",
           _ATTEND.pack(out.data_ptr(), q.data_ptr(), *pages.addresses, meta.q_start.data_ptr(), meta.context_len.data_ptr(),
-                       block_table.data_ptr(), scratch.data_ptr(), status.data_ptr(), stream, need, pages.bits, pages.n_pages,
-                       pages.page_size, block_table.shape[1], len(meta.q_lens), most, n_q, pages.n_kv, D, window, scale), "attn_quant")
+                       block_table.data_ptr(), scratch.data_ptr() if need else 0, status.data_ptr(), stream, need, pages.bits, pages.n_pages,
+                       pages.page_size, width, len(meta.q_lens), most, n_q, pages.n_kv, D, window, scale), "attn_quant")
 
 
 def _portions(out, q, pages, meta, block_table, n_q, scale, window, status, span, stream: int) -> None:
@@ -272,7 +274,7 @@ def _portions(out, q, pages, meta, block_table, n_q, scale, window, status, span
 
 def _by_reading(out, q, pages, meta, block_table, n_q, scale, window, status, stream: int) -> None:
     """Every entry's pages read back, as many entries at a time as READ_BYTES allow, and the attention over them."""
-    _lists("attention_quantized", positions=meta.positions, entry_of_token=meta.entry_of_token)
+    _lists("attention_quantized", "positions and entry_of_token", meta.positions, meta.entry_of_token)
     if min(meta.positions.numel(), meta.entry_of_token.numel()) < meta.tokens:
         raise KernelError("attention_quantized: the step's lists are shorter than the step")
     _launch_stream("attention_quantized", pages.device_index, meta.positions, meta.entry_of_token)
