@@ -104,8 +104,7 @@ __global__ void __launch_bounds__(128) quant_write_any_kernel(const WriteParams 
         const float x = quant_input(row[c]);
         const float hi = warp_max(x), lo = -warp_max(-x);
         const uint16_t sb = quant_scale<BITS>(hi, lo);
-        const float scale = quant_scale_value(sb);
-        const uint32_t code = (uint32_t)quant_code<BITS>(x, scale, quant_inverse(scale));
+        const uint32_t code = (uint32_t)(quant_code<BITS>(x, quant_scale_value(sb)) + (BITS == 4 ? 8.f : 128.f));
         if (BITS == 8) {
             codes[c] = (uint8_t)code;
         } else {
@@ -121,13 +120,9 @@ __device__ __forceinline__ void put8(float* p, const float (&x)[8]) {
     reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
     reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
-template <int BITS> __device__ __forceinline__ void put_codes(uint8_t* p, const float (&x)[8], float s0, float i0, float s1, float i1) {
-    float c[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = i < 4 ? quant_code<BITS>(x[i], s0, i0) : quant_code<BITS>(x[i], s1, i1);
-    const uint32_t a = quant_pack4<BITS>(c[0], c[1], c[2], c[3]), b = quant_pack4<BITS>(c[4], c[5], c[6], c[7]);
-    if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(p) = a | b << 16;
-    else *reinterpret_cast<uint2*>(p) = make_uint2(a, b);
+template <int BITS> __device__ __forceinline__ void put_codes(uint8_t* p, uint32_t first, uint32_t second) {
+    if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(p) = first | second << 16;
+    else *reinterpret_cast<uint2*>(p) = make_uint2(first, second);
 }
 
 // Heads of 64, 128 or 256 channels, rotated whole, by half or not at all, 16-byte aligned: HEAD_DIM / 16 lanes
@@ -136,7 +131,9 @@ template <int BITS> __device__ __forceinline__ void put_codes(uint8_t* p, const 
 // four runs of two groups; the four lanes whose numbers agree modulo HEAD_DIM / 64 hold the same two groups, so a
 // group's extremes are two exchanges away.  The 64-bit sum of squares (16 conversions a lane on a pipe of 16 lanes) is
 // formed for keys only: queries get no codes, and four in five heads are theirs.
-// 2,048 tokens of 32 and 2 x 8 heads of 128, 8 bits: see the table of cases in the design document.
+// Bound by arithmetic, not by memory: 2,048 tokens of 32 and 2 x 8 bfloat16 heads of 128 to 8 bits take 21.8 us (60 MB, 2.8 TB/s);
+// three prompts in float32 10.3 us (2.0 TB/s).  Eight tokens take 4.1 us, a launch and one chain of loads.  A block is no larger than
+// a token's heads need (15.8 -> 11.0 us for those prompts, of 12 and 2 x 2 heads of 64); 64, 192 and 384 threads were all slower than 128.
 constexpr int WRITE_THREADS = 128;
 __device__ __forceinline__ void fetch8(uint4 (&raw)[1], const bf16* p) { raw[0] = *reinterpret_cast<const uint4*>(p); }
 __device__ __forceinline__ void fetch8(uint4 (&raw)[2], const float* p) {
@@ -153,9 +150,9 @@ __device__ __forceinline__ void spread8(float (&x)[8], const uint4 (&raw)[2]) {
 }
 template <typename T, int BITS, int HEAD_DIM>
 __global__ void __launch_bounds__(WRITE_THREADS) quant_write_kernel(const WriteParams p) {
-    constexpr int LPH = HEAD_DIM / 16, HALF = HEAD_DIM / 2, G = HEAD_DIM / 32, PER = WRITE_THREADS / LPH, RAW = sizeof(T) / 2;
+    constexpr int LPH = HEAD_DIM / 16, HALF = HEAD_DIM / 2, G = HEAD_DIM / 32, RAW = sizeof(T) / 2;
     pdl_launch_dependents();
-    const int t = blockIdx.y, sub = threadIdx.x % LPH;
+    const int t = blockIdx.y, sub = threadIdx.x % LPH, PER = blockDim.x / LPH;
     const int n_kv = p.pages.n_kv, heads = p.n_q + (p.write_cache ? 2 * n_kv : 0);
     const T* const row = static_cast<const T*>(p.qkv) + (size_t)t * p.ld + sub * 8;
     int h = blockIdx.x * PER + threadIdx.x / LPH;
@@ -245,29 +242,49 @@ __global__ void __launch_bounds__(WRITE_THREADS) quant_write_kernel(const WriteP
             put8(dst + HALF, b);
         }
         if (__all_sync(0xffffffffu, is_q)) continue;
-        float hi[2], lo[2];
+        // (a number that quant_input changes is rare, and looked for all at once: what is not finite makes a sum of zeros a NaN)
+        float hi[2], lo[2], zero = 0.f;
+        auto extremes = [&] {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            hi[r] = -INFINITY; lo[r] = INFINITY;
+            for (int r = 0; r < 2; ++r) {
+                hi[r] = fmaxf(a[4 * r], b[4 * r]);
+                lo[r] = fminf(a[4 * r], b[4 * r]);
 #pragma unroll
-            for (int i = 4 * r; i < 4 * r + 4; ++i) {
-                a[i] = quant_input(a[i]); b[i] = quant_input(b[i]);
-                hi[r] = fmaxf(hi[r], fmaxf(a[i], b[i]));
-                lo[r] = fminf(lo[r], fminf(a[i], b[i]));
+                for (int i = 4 * r + 1; i < 4 * r + 4; ++i) {
+                    hi[r] = fmaxf(hi[r], fmaxf(a[i], b[i]));
+                    lo[r] = fminf(lo[r], fminf(a[i], b[i]));
+                }
             }
+        };
+        extremes();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) zero = fmaf(a[i], 0.f, fmaf(b[i], 0.f, zero));
+        if (__any_sync(0xffffffffu, zero != 0.f || fmaxf(hi[0], hi[1]) > QUANT_MOST || fminf(lo[0], lo[1]) < -QUANT_MOST)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { a[i] = quant_input(a[i]); b[i] = quant_input(b[i]); }
+            extremes();
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int o = G / 2; o <= G; o <<= 1) {
                 hi[r] = fmaxf(hi[r], __shfl_xor_sync(0xffffffffu, hi[r], o));
                 lo[r] = fminf(lo[r], __shfl_xor_sync(0xffffffffu, lo[r], o));
             }
-        }
         if (page < 0 || !active || is_q) continue;
         const size_t at = ((size_t)page * n_kv + (is_k ? h - p.n_q : h - p.n_q - n_kv)) * p.pages.page_size + (pos - slot * p.pages.page_size);
         const uint16_t b0 = quant_scale<BITS>(hi[0], lo[0]), b1 = quant_scale<BITS>(hi[1], lo[1]);
         const float s0 = quant_scale_value(b0), s1 = quant_scale_value(b1), i0 = quant_inverse(s0), i1 = quant_inverse(s1);
+        float doubt = 0.f;
+        uint32_t c[4] = {quant_codes4<BITS>(a, i0, doubt), quant_codes4<BITS>(a + 4, i1, doubt), quant_codes4<BITS>(b, i0, doubt),
+                         quant_codes4<BITS>(b + 4, i1, doubt)};
+        if (doubt > QUANT_DOUBT || i0 == 0.f || i1 == 0.f) {
+            c[0] = quant_codes4_defined<BITS>(a, s0); c[1] = quant_codes4_defined<BITS>(a + 4, s1);
+            c[2] = quant_codes4_defined<BITS>(b, s0); c[3] = quant_codes4_defined<BITS>(b + 4, s1);
+        }
         uint8_t* codes = (is_k ? p.pages.k_codes : p.pages.v_codes) + at * (HEAD_DIM * BITS / 8) + sub * BITS;
-        put_codes<BITS>(codes, a, s0, i0, s1, i1);
-        put_codes<BITS>(codes + HALF * BITS / 8, b, s0, i0, s1, i1);
+        put_codes<BITS>(codes, c[0], c[1]);
+        put_codes<BITS>(codes + HALF * BITS / 8, c[2], c[3]);
         if (sub < G / 2)
             reinterpret_cast<uint32_t*>((is_k ? p.pages.k_scales : p.pages.v_scales) + at * G)[sub] = (uint32_t)b0 | (uint32_t)b1 << 16;
     }
@@ -279,13 +296,13 @@ template <typename T, int BITS> int launch_write(const WriteParams& p, cudaStrea
                            (uintptr_t)p.pages.k_codes | (uintptr_t)p.pages.v_codes | (uintptr_t)p.pages.k_scales | (uintptr_t)p.pages.v_scales;
     const bool aligned = (bits & 15) == 0 && p.ld * (long long)sizeof(T) % 16 == 0;
     if (aligned && (p.cos_sin == nullptr || p.rotary_dim == D || p.rotary_dim * 2 == D) && p.tokens <= 65535 && (D == 64 || D == 128 || D == 256)) {
-        const int per = WRITE_THREADS / (D / 16);
+        const int lanes = heads * (D / 16), threads = lanes < WRITE_THREADS ? (lanes + 31) / 32 * 32 : WRITE_THREADS, per = threads / (D / 16);
         // A block takes all heads of a token where there are tokens enough: the norms' weights and the angles are read once, and the
         // next heads are on their way meanwhile.
         const int shares = (heads + per - 1) / per;
         const dim3 grid((unsigned)(p.tokens >= 4 * kipp_sm_count() ? 1 : shares), (unsigned)p.tokens);
         auto kernel = D == 64 ? quant_write_kernel<T, BITS, 64> : D == 128 ? quant_write_kernel<T, BITS, 128> : quant_write_kernel<T, BITS, 256>;
-        return kipp_launch(kernel, grid, dim3(WRITE_THREADS), 0, s, 1, p);
+        return kipp_launch(kernel, grid, dim3((unsigned)threads), 0, s, 1, p);
     }
     const long long blocks = ((long long)p.tokens * heads + 3) / 4;
     if (blocks > 0x7fffffffLL) return KIPP_ERR_ARG;

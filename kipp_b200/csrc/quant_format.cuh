@@ -37,24 +37,35 @@ template <int BITS> __device__ __forceinline__ uint16_t quant_scale(float hi, fl
 }
 __device__ __forceinline__ float quant_scale_value(uint16_t bits) { return __uint_as_float((uint32_t)bits << 16); }
 
-// The code of x as a number, 0 to 2 L - 1; a scale of 0 (a group of zeros) has the code that stands for 0.  `inverse` is 1 / scale,
-// rounded: x * inverse is off from x / scale by 2^-22 of it, 2^-15 at most, so the rounding to a whole number is that of the
-// quotient unless it lies as near to the middle between two, and then the quotient is formed (one division a group instead of 32; the
-// whole number comes out of an addition of 1.5 * 2^23, ties to even, and no conversion).
-template <int BITS> __device__ __forceinline__ float quant_code(float x, float scale, float inverse) {
-    constexpr float L = BITS == 4 ? 8.f : 128.f, MAGIC = 12582912.f;
-    float q = fminf(fmaxf(__fmul_rn(x, inverse), -L), L - 1.f);
-    float r = __fsub_rn(__fadd_rn(q, MAGIC), MAGIC);
-    if (fabsf(q - r) > 0.5f - 0x1p-14f || inverse == 0.f)
-        r = scale == 0.f ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -L), L - 1.f);
-    return r + L;
+// The code of x, formed as it is defined; a scale of 0 (a group of zeros) has the code that stands for 0.  Less L, as a number.
+template <int BITS> __device__ __forceinline__ float quant_code(float x, float scale) {
+    constexpr float L = BITS == 4 ? 8.f : 128.f;
+    return scale == 0.f ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -L), L - 1.f);
 }
-// (0 where it may not be a number: a scale of 0, or a subnormal one)
+// 1 / scale, or 0 where that may not be a number: a scale of 0, or a subnormal one.
 __device__ __forceinline__ float quant_inverse(float scale) { return fabsf(scale) < 0x1p-126f ? 0.f : __fdiv_rn(1.f, scale); }
-// four codes as whole numbers in one: their bits side by side in the low 4 BITS bits (exact: at most 2^24 of 4 bits' worth, or two
-// halves of 16)
-template <int BITS> __device__ __forceinline__ uint32_t quant_pack4(float c0, float c1, float c2, float c3) {
-    constexpr float MAGIC = 8388608.f;
-    if constexpr (BITS == 4) return __float_as_uint(fmaf(c3, 4096.f, fmaf(c2, 256.f, fmaf(c1, 16.f, c0))) + MAGIC) & 0xffffu;
-    return __byte_perm(__float_as_uint(fmaf(c1, 256.f, c0) + MAGIC), __float_as_uint(fmaf(c3, 256.f, c2) + MAGIC), 0x5410);
+// Four codes of one group, side by side in the low 4 BITS bits.  x * inverse is off from x / scale by 2^-22 of it, 2^-15 at most, so its
+// rounding to a whole number (an addition of 1.5 * 2^23 and a subtraction: ties to even, no conversion) is the quotient's unless it
+// lies as near to the middle between two; `doubt` then grows beyond QUANT_DOUBT and the codes have to be formed as they are defined.
+// They are put together as numbers too: whole ones below 2^24 add exactly.
+constexpr float QUANT_DOUBT = 0.5f - 0x1p-14f;
+template <int BITS> __device__ __forceinline__ uint32_t quant_pack4(float r0, float r1, float r2, float r3) {
+    if constexpr (BITS == 4)
+        return __float_as_uint(fmaf(r3, 4096.f, fmaf(r2, 256.f, fmaf(r1, 16.f, r0 + (8388608.f + 8.f * 4369.f))))) & 0xffffu;
+    return __byte_perm(__float_as_uint(fmaf(r1, 256.f, r0 + (8388608.f + 128.f * 257.f))),
+                       __float_as_uint(fmaf(r3, 256.f, r2 + (8388608.f + 128.f * 257.f))), 0x5410);
+}
+template <int BITS> __device__ __forceinline__ uint32_t quant_codes4(const float* x, float inverse, float& doubt) {
+    constexpr float L = BITS == 4 ? 8.f : 128.f, MAGIC = 12582912.f;
+    float r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float q = fminf(fmaxf(__fmul_rn(x[i], inverse), -L), L - 1.f);
+        r[i] = __fsub_rn(__fadd_rn(q, MAGIC), MAGIC);
+        doubt = fmaxf(doubt, fabsf(q - r[i]));
+    }
+    return quant_pack4<BITS>(r[0], r[1], r[2], r[3]);
+}
+template <int BITS> __device__ __forceinline__ uint32_t quant_codes4_defined(const float* x, float scale) {
+    return quant_pack4<BITS>(quant_code<BITS>(x[0], scale), quant_code<BITS>(x[1], scale), quant_code<BITS>(x[2], scale), quant_code<BITS>(x[3], scale));
 }
