@@ -13,8 +13,9 @@
 // is the number n * 2^-133 (subnormal up to 127; the exponent's first step goes on in the same line), and
 // mma.sync takes subnormals exactly.  Two codes then become an operand register by one mask.  Four-bit
 // codes in bits 4 to 7 count sixteenfold: their queries are divided by 16, the results at the end.  Queries
-// and weights carry a factor of 2^60 so that the sums stay clear of float32's lower end; all of these are
-// powers of two.
+// and weights carry a factor of 2^48, all of these being powers of two: sums of weighted codes then end below float32's upper end with
+// every value at the format's limit of 2^60 and every weight at 2^8 (2^48+8+57 a key), and a value of 2^-40 still leaves
+// them whole.  A query has to be below 2^80 (beyond it counts as infinite).
 //
 // Products are made the other way round from the kernels of attention_mma.cu, keys (then channels) as
 // rows, queries as columns, 8 at a time: mma.m16n8k16 with S^T = K Q^T, O^T = V^T P^T.  The codes are then the
@@ -51,7 +52,7 @@ struct Params {
     const uint8_t* k_codes; const uint8_t* k_scales; const uint8_t* v_codes; const uint8_t* v_scales;
     const int* q_start; const int* context_len; const int* block_table;
     int entries, table_width, page_size, page_shift, n_pages, most, n_q, n_kv, group, window;
-    float score_scale, query_scale;  // |scale| * log2(e) * 2^73; 2^60 with the scale's sign
+    float score_scale, query_scale;  // |scale| * log2(e) * 2^85; 2^48 with the scale's sign
     float* part_o; float* part_ml;   // [2 ctas][columns][D], [2 ctas][columns][2]
     // by CTA, the row that it begins and others go on with: (entry, kv head, 2 first column + the slot of its part, the row's last unit,
     // or -1: there is no such row); behind them the cut
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             return row;
         };
         // TILES: the rows of the tiles of 16 steps are looked up at once, a tile a lane, and a batch ahead; otherwise each lane's
-        // own key, a step ahead.  (What is not seen keeps whatever lies in the ring.)
+        // own key, a step ahead.  (A tile that is not there has scales of 0; its codes are whatever lies in the ring.)
         int rows = -1, rows_next;
         auto look_up = [&](int step) {
             if constexpr (TILES) rows_next = row_of(j_first + (step + (lane >> 1)) * STEP + (lane & 1) * 16);
@@ -308,7 +309,10 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
 #pragma unroll
                 for (int tile = 0; tile < 2; ++tile) {
                     const int row = __shfl_sync(0xffffffffu, rows, 2 * (step & 15) + tile);
-                    if (row < 0) continue;
+                    if (row < 0) {
+                        if (lane < 2 * SB) *reinterpret_cast<uint4*>(my + to_stage * S::WARP_STAGE + lane * 16 + s_to + tile * 16 * SB) = make_uint4(0u, 0u, 0u, 0u);
+                        continue;
+                    }
                     const uint8_t *k = k_lane + (size_t)row * RB, *v = v_lane + (size_t)row * RB;
 #pragma unroll
                     for (int i = 0; i < RB / 32; ++i) {
@@ -504,10 +508,10 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                     }
                 }
             }
-            // (times 2^60)
+            // (times 2^48)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const float back[2] = {(m[nt][0] == -INFINITY ? 0.f : m[nt][0]) - 60.f, (m[nt][1] == -INFINITY ? 0.f : m[nt][1]) - 60.f};
+                const float back[2] = {(m[nt][0] == -INFINITY ? 0.f : m[nt][0]) - 48.f, (m[nt][1] == -INFINITY ? 0.f : m[nt][1]) - 48.f};
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt) {
                     float e[4];
@@ -585,15 +589,15 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                 const int col = nt * 8 + 2 * t4 + c;
                 if (g4 == 0) {
                     w_m[warp * COLS + col] = m[nt][c];
-                    w_l[warp * COLS + col] = sum * 0x1p-60f;
+                    w_l[warp * COLS + col] = sum * 0x1p-48f;
                 }
             }
 #pragma unroll
             for (int gi = 0; gi < G; ++gi) {
                 // (row gi of the product with ones lies with lane 4 gi + t)
-                const float less[2] = {__shfl_sync(0xffffffffu, ones[nt][0], 4 * gi + t4) * (S::L * 0x1p-60f),
-                                       __shfl_sync(0xffffffffu, ones[nt][1], 4 * gi + t4) * (S::L * 0x1p-60f)};
-                constexpr float EVEN = 0x1p73f, ODD = BITS == 4 ? 0x1p69f : 0x1p73f;
+                const float less[2] = {__shfl_sync(0xffffffffu, ones[nt][0], 4 * gi + t4) * (S::L * 0x1p-48f),
+                                       __shfl_sync(0xffffffffu, ones[nt][1], 4 * gi + t4) * (S::L * 0x1p-48f)};
+                constexpr float EVEN = 0x1p85f, ODD = BITS == 4 ? 0x1p81f : 0x1p85f;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     float4 r;
@@ -855,8 +859,9 @@ extern "C" int kipp_attn_quant(const KippAttnQuant* a) {
     p.page_shift = -1;
     for (int i = 0; i < 31; ++i) if (page_size == 1 << i) p.page_shift = i;
     p.n_q = n_q; p.n_kv = n_kv; p.group = n_q / n_kv; p.window = a->window;
-    p.score_scale = fabsf(a->scale) * 1.4426950408889634f * 0x1p73f;
-    p.query_scale = a->scale < 0.f ? -0x1p60f : 0x1p60f;
+    // (a scale of 0 makes every score 0: by the queries, since a masked score times 0 would be no number)
+    p.score_scale = a->scale == 0.f ? 1.f : fabsf(a->scale) * 1.4426950408889634f * 0x1p85f;
+    p.query_scale = a->scale == 0.f ? 0.f : a->scale < 0.f ? -0x1p48f : 0x1p48f;
     p.part_o = (float*)a->scratch;
     p.part_ml = p.part_o + 2LL * MOST_CTAS * MOST_COLUMNS * head_dim;
     p.shared = (int4*)(p.part_ml + 2LL * MOST_CTAS * MOST_COLUMNS * 2);

@@ -316,9 +316,10 @@ struct ReadParams {
     const int* list;                // [n] pages, or the step's block table
     int n, head_dim;
     int* status;
-    // the entries' form: pages of entries that bring more than one token, and the table of those made
+    // the entries' form: the pages that entries from first_entry on see, and the table of those made
     int* table_out; const int* q_start; const int* context_len;
     int table_width, first_entry, window;
+    int at;                         // what the launch begins with, a page's place in the list or among the entries'
 };
 
 // The eight channels that a word of 4-bit codes, or two of 8-bit, stand for, as bfloat16 pairs of (code - L) * 2^-13: a code in the
@@ -386,8 +387,9 @@ template <typename T, int BITS, bool ENTRIES, int DIM, int UNROLL>
 __global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const ReadParams p) {
     if constexpr (!ENTRIES) pdl_launch_dependents();      // (a step's table is read before a kernel's wait: this one lets none start early)
     pdl_wait();
-    const int i = blockIdx.y, D = DIM > 0 ? DIM : p.head_dim, G = D / 32;
+    const int i = p.at + blockIdx.y, D = DIM > 0 ? DIM : p.head_dim, G = D / 32;
     const int page = p.list[ENTRIES ? (size_t)(p.first_entry + i / p.table_width) * p.table_width + i % p.table_width : (size_t)i];
+    int from = 0, to = 0;                         // the page's slots that a token sees
     if constexpr (ENTRIES) {
         const int e = p.first_entry + i / p.table_width, slot = i % p.table_width;
         const int tokens = p.q_start[e + 1] - p.q_start[e], first = p.context_len[e], len = first + tokens;
@@ -396,6 +398,8 @@ __global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const ReadPara
                           (long long)(slot + 1) * p.pages.page_size > seen;
         if (blockIdx.x == 0 && threadIdx.x == 0) p.table_out[(size_t)e * p.table_width + slot] = used ? i : -1;
         if (!used) return;
+        from = max(0, seen - slot * p.pages.page_size);
+        to = min(p.pages.page_size, len - slot * p.pages.page_size);
     }
     const bool ok = page >= 0 && page < p.pages.n_pages;
     if (page >= p.pages.n_pages && threadIdx.x == 0) atomicExch(p.status, 3);
@@ -410,8 +414,9 @@ __global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const ReadPara
         for (int j = 0; j < UNROLL; ++j) {
             const int u = base + j * READ_THREADS + threadIdx.x;
             k[j] = v[j] = Unit<BITS>{};
-            if (u < units && ok) {
-                const int row = u / per_row, c = u - row * per_row, g0 = 2 * c % G, g1 = g0 + 1 == G ? 0 : g0 + 1;
+            const int row = u / per_row, at = ENTRIES ? row % p.pages.page_size : 0;
+            if (u < units && ok && (!ENTRIES || (at >= from && at < to))) {
+                const int c = u - row * per_row, g0 = 2 * c % G, g1 = g0 + 1 == G ? 0 : g0 + 1;
                 k[j] = take_unit<BITS, (DIM > 0)>(k_codes + (size_t)u * BITS, k_scales + row * G, g0, g1);
                 v[j] = take_unit<BITS, (DIM > 0)>(v_codes + (size_t)u * BITS, v_scales + row * G, g0, g1);
             }
@@ -444,15 +449,10 @@ template <bool ENTRIES> int launch_read(const ReadParams& p, int bits, int out_d
     auto kernel = out_dtype == KIPP_DT_F32 ? (bits == 4 ? read_kernel<float, 4, ENTRIES>(p.head_dim, many) : read_kernel<float, 8, ENTRIES>(p.head_dim, many))
                                            : (bits == 4 ? read_kernel<bf16, 4, ENTRIES>(p.head_dim, many) : read_kernel<bf16, 8, ENTRIES>(p.head_dim, many));
     // (a grid's second dimension ends at 65,535)
-    for (int done = 0; done < p.n; done += 65535) {
-        ReadParams q = p;
-        if (ENTRIES && done > 0) return KIPP_ERR_ARG;
-        q.n = p.n - done < 65535 ? p.n - done : 65535;
-        q.list = p.list + (ENTRIES ? 0 : done);
-        const size_t skip = (size_t)done * p.pages.n_kv * p.pages.page_size * p.head_dim * (out_dtype == KIPP_DT_F32 ? 4 : 2);
-        q.k_out = static_cast<char*>(p.k_out) + skip;
-        q.v_out = static_cast<char*>(p.v_out) + skip;
-        if (const int e = kipp_launch(kernel, dim3(x, (unsigned)q.n), dim3(READ_THREADS), 0, s, 1, q)) return e;
+    for (ReadParams q = p; q.at < p.n; q.at += 65535) {
+        const unsigned y = (unsigned)(p.n - q.at < 65535 ? p.n - q.at : 65535);
+        if (const int e = kipp_launch(kernel, dim3(x, y), dim3(READ_THREADS), 0, s, 1, q)) return e;
+        if (p.n - q.at <= 65535) break;
     }
     return 0;
 }
@@ -525,23 +525,24 @@ extern "C" int kipp_quant_cache_read(const KippQuantRead* a) {
         return KIPP_ERR_ARG;
     if (a->out_dtype != KIPP_DT_F32 && a->out_dtype != KIPP_DT_BF16) return KIPP_ERR_DTYPE;
     if (!read_aligned(pages, a->k_out, a->v_out)) return -3;
-    ReadParams p = {a->k_out, a->v_out, pages, a->list, a->n, a->head_dim, a->status, nullptr, nullptr, nullptr, 0, 0, 0};
+    ReadParams p = {a->k_out, a->v_out, pages, a->list, a->n, a->head_dim, a->status, nullptr, nullptr, nullptr, 0, 0, 0, 0};
     return launch_read<false>(p, a->bits, a->out_dtype, (cudaStream_t)a->stream);
 }
 
 // The pages that the tokens of entries first_entry .. first_entry + entries - 1 see, read back into pages of
 // their own (entry by entry, table_width pages each), and the block table of those: table_out has the
 // step's shape and only those entries' rows are written.  The pages no token sees are neither read nor
-// written; their table entries are -1.
+// written; their table entries are -1.  The slots that no token sees, of pages that some are seen of, become zeros: they may hold
+// anything, and the attention over the pages multiplies them by weights of 0.
 extern "C" int kipp_quant_cache_read_entries(const KippQuantReadEntries* a) {
     if (a->entries <= 0) return 0;
     const QuantPages pages = {(uint8_t*)a->k_codes, (bf16*)a->k_scales, (uint8_t*)a->v_codes, (bf16*)a->v_scales, a->n_pages, a->page_size, a->n_kv};
     if (!pages_ok(pages, a->bits, a->head_dim) || a->k_out == nullptr || a->v_out == nullptr || a->table_out == nullptr || a->status == nullptr ||
-        a->table_width <= 0 || a->first_entry < 0 || a->window < 0 || (long long)a->entries * a->table_width > 65535)
+        a->table_width <= 0 || a->first_entry < 0 || a->window < 0 || (long long)a->entries * a->table_width > 0x7fffffffLL)
         return KIPP_ERR_ARG;
     if (a->out_dtype != KIPP_DT_F32 && a->out_dtype != KIPP_DT_BF16) return KIPP_ERR_DTYPE;
     if (!read_aligned(pages, a->k_out, a->v_out)) return -3;
     ReadParams p = {a->k_out, a->v_out, pages, a->block_table, a->entries * a->table_width, a->head_dim, a->status, a->table_out, a->q_start,
-                    a->context_len, a->table_width, a->first_entry, a->window};
+                    a->context_len, a->table_width, a->first_entry, a->window, 0};
     return launch_read<true>(p, a->bits, a->out_dtype, (cudaStream_t)a->stream);
 }

@@ -1145,7 +1145,7 @@ public:
                              const int* context_len, int n_q, int n_kv, int head_dim, float scale, int window) {
         const int entries = (int)q_lens.size();
         const long long page_bytes = 2LL * n_kv * cache.page_size * head_dim * (long long)dtype_size(dtype);
-        const long long at_once = std::max(1LL, std::min(EXPAND_MAX_BYTES / (page_bytes * cache.table_width), 65535LL / cache.table_width));
+        const long long at_once = std::max(1LL, EXPAND_MAX_BYTES / (page_bytes * cache.table_width));
         if (dtype == BF16 && attention_quant_supported(cache.bits, head_dim, n_q, n_kv)) {
             int first = -1, last = -1, longest = 1;
             bool single = false;

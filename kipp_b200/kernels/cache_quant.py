@@ -169,7 +169,7 @@ def _read_entries(pages: QuantizedPages, dtype: torch.dtype, meta, block_table: 
 def _entries_at_once(pages: QuantizedPages, dtype: torch.dtype, width: int) -> int:
     """How many entries' pages may be read back together."""
     per = 2 * pages.n_kv * pages.page_size * pages.head_dim * dtype.itemsize * width
-    return max(1, min(READ_BYTES // per, 65535 // width))
+    return max(1, READ_BYTES // per)
 
 
 PORTION_MIN = 64              # an entry of as many tokens is read back for the prompt kernel of 128-token tiles
@@ -209,7 +209,8 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
     ``meta`` is the step's metadata as for ``attention`` (``tokens``, ``q_lens``, ``positions``, ``entry_of_token``,
     ``q_start``, ``context_len``, and where entries bring 64 tokens or more the list of their 128-token tiles,
     ``prefill_work128`` and ``n_prefill_items128``).  bfloat16 with heads of 64, 128 or 256 runs on the codes themselves; longer
-    portions of prompts, other heads and float32 on pages that are read back.  ``impl`` forces a form for the whole step:
+    portions of prompts, other heads and float32 on pages that are read back.  A page that is not mapped, or past the pool, sets
+    status word 0 to 3.  ``impl`` forces a form for the whole step:
     "direct" or "read"."""
     what, D, n_kv, q_lens, tokens = "attention_quantized", pages.head_dim, pages.n_kv, meta.q_lens, meta.tokens
     window = int(window or 0)
@@ -219,8 +220,8 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
         raise KernelError(f"{what}: q must be contiguous [tokens, n_q, head_dim] with n_q a multiple of the cache's heads")
     if out.dtype != q.dtype or out.shape != shape or not out.is_contiguous():
         raise KernelError(f"{what}: out must be contiguous, of q's dtype and shape")
-    if window < 0:
-        raise KernelError(f"{what}: a window must not be negative")
+    if not 0 <= window < 1 << 31:
+        raise KernelError(f"{what}: a window of {window} tokens")
     t_shape = block_table.shape
     if len(t_shape) != 2 or t_shape[0] < entries or t_shape[1] == 0 or sum(q_lens) != tokens:
         raise KernelError(f"{what}: a row of block_table for every entry, and as many tokens as the entries bring")
