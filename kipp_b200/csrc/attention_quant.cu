@@ -209,16 +209,26 @@ template <int D, int BITS, int NT> constexpr int ctas_per_sm() {
 // r = 2 t + e + 8 h: a lane (g, t) then meets the values of keys t, 4 + t, 8 + t, 12 + t.
 __device__ __forceinline__ int key_of_row(int r) { return 4 * (r & 1) + ((r & 7) >> 1) + (r & 8); }
 
-// Two runs of four codes as four operand registers: x[i] holds code i of the first run in its low half and of
-// the second in its high half.  4 bits: `first` and `second` are words, HALF which half of them the run is;
-// codes 1 and 3 count sixteenfold.  8 bits: a run is a word.
-template <int BITS> __device__ __forceinline__ void spread(uint32_t (&x)[4], uint32_t first, uint32_t second, int half) {
+// Two runs of four codes of a key as four operand registers, two channels of one group in each.  4 bits: `first` and `second` are words,
+// `half` which half of them the run is; x[i] has code i of the first run in its low half and of the second in its high half, codes
+// 1 and 3 sixteenfold.  8 bits: a run is a word, and has codes 0 and 2, 1 and 3 in the halves of x[0], x[1] (x[2], x[3] the second).
+template <int BITS> __device__ __forceinline__ void spread_keys(uint32_t (&x)[4], uint32_t first, uint32_t second, int half) {
     if constexpr (BITS == 4) {
         const uint32_t w = __byte_perm(first, second, half ? 0x7632 : 0x5410), u = w >> 8;
         x[0] = w & 0x000f000fu; x[1] = w & 0x00f000f0u; x[2] = u & 0x000f000fu; x[3] = u & 0x00f000f0u;
     } else {
+        x[0] = first & 0x00ff00ffu; x[1] = __byte_perm(first, 0u, 0x4341); x[2] = second & 0x00ff00ffu; x[3] = __byte_perm(second, 0u, 0x4341);
+    }
+}
+// A run of two values, the first one's codes in the low halves.  (4 bits: x[0] and x[2] could keep both codes of a byte and the even
+// channels' sums be made as differences at the end, an instruction in six less and 2 % of the time; but they would then not
+// cancel exactly where every value is 0.)
+template <int BITS> __device__ __forceinline__ void spread_values(uint32_t (&x)[4], uint32_t first, uint32_t second, int half) {
+    if constexpr (BITS == 4) {
+        spread_keys<4>(x, first, second, half);
+    } else {
         const uint32_t w = __byte_perm(first, second, 0x5410), u = __byte_perm(first, second, 0x7632);
-        x[0] = w & 0x00ff00ffu; x[1] = (w >> 8) & 0x00ff00ffu; x[2] = u & 0x00ff00ffu; x[3] = (u >> 8) & 0x00ff00ffu;
+        x[0] = w & 0x00ff00ffu; x[1] = __byte_perm(w, 0u, 0x4341); x[2] = u & 0x00ff00ffu; x[3] = __byte_perm(u, 0u, 0x4341);
     }
 }
 
@@ -372,8 +382,9 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             sum *= -S::L * 0x1p-133f * p.query_scale;
             q_offsets[k * 32 + lane] = make_float2(__shfl_sync(0xffffffffu, sum, 8 * t4), __shfl_sync(0xffffffffu, sum, 8 * t4 + 4));
-            const uint32_t raw[4] = {__byte_perm(a.x, b.x, 0x5410), __byte_perm(a.x, b.x, 0x7632), __byte_perm(a.y, b.y, 0x5410),
-                                     __byte_perm(a.y, b.y, 0x7632)};
+            const uint32_t mid = BITS == 4 ? b.x : a.y, last = BITS == 4 ? a.y : b.x;              // (as spread_keys pairs the codes)
+            const uint32_t raw[4] = {__byte_perm(a.x, mid, 0x5410), __byte_perm(a.x, mid, 0x7632), __byte_perm(last, b.y, 0x5410),
+                                     __byte_perm(last, b.y, 0x7632)};
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -438,13 +449,9 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
 #pragma unroll
                 for (int gi = 0; gi < G; ++gi) {
                     uint32_t x0[4], x1[4];
-                    if constexpr (BITS == 4) {
-                        spread<4>(x0, w0[gi >> 1], w0[(gi + G) >> 1], gi & 1);
-                        spread<4>(x1, w1[gi >> 1], w1[(gi + G) >> 1], gi & 1);
-                    } else {
-                        spread<8>(x0, w0[gi], w0[gi + G], 0);
-                        spread<8>(x1, w1[gi], w1[gi + G], 0);
-                    }
+                    constexpr int W = BITS == 4 ? 1 : 0;
+                    spread_keys<BITS>(x0, w0[gi >> W], w0[(gi + G) >> W], gi & 1);
+                    spread_keys<BITS>(x1, w1[gi >> W], w1[(gi + G) >> W], gi & 1);
                     const float f0 = gi & 1 ? high_f32(a0[gi >> 1]) : low_f32(a0[gi >> 1]);
                     const float f1 = gi & 1 ? high_f32(a1[gi >> 1]) : low_f32(a1[gi >> 1]);
 #pragma unroll
@@ -538,8 +545,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                 for (int gi = 0; gi < G; ++gi) {
                     uint32_t x0[4], x1[4];                             // keys of the first and the second half of the rows
                     constexpr int W = BITS == 4 ? 1 : 0;
-                    spread<BITS>(x0, v[0][gi >> W], v[1][gi >> W], gi & 1);
-                    spread<BITS>(x1, v[2][gi >> W], v[3][gi >> W], gi & 1);
+                    spread_values<BITS>(x0, v[0][gi >> W], v[1][gi >> W], gi & 1);
+                    spread_values<BITS>(x1, v[2][gi >> W], v[3][gi >> W], gi & 1);
                     const uint32_t f0 = __byte_perm(f[0][gi >> 1], f[1][gi >> 1], gi & 1 ? 0x7632 : 0x5410);
                     const uint32_t f1 = __byte_perm(f[2][gi >> 1], f[3][gi >> 1], gi & 1 ? 0x7632 : 0x5410);
                     const uint32_t one = g4 == gi ? 0x3f803f80u : 0u;
