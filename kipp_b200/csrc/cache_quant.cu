@@ -131,9 +131,11 @@ template <int BITS> __device__ __forceinline__ void put_codes(uint8_t* p, uint32
 // four runs of two groups; the four lanes whose numbers agree modulo HEAD_DIM / 64 hold the same two groups, so a
 // group's extremes are two exchanges away.  The 64-bit sum of squares (16 conversions a lane on a pipe of 16 lanes) is
 // formed for keys only: queries get no codes, and four in five heads are theirs.
-// Bound by arithmetic, not by memory: 2,048 tokens of 32 and 2 x 8 bfloat16 heads of 128 to 8 bits take 21.8 us (60 MB, 2.8 TB/s);
-// three prompts in float32 10.3 us (2.0 TB/s).  Eight tokens take 4.1 us, a launch and one chain of loads.  A block is no larger than
-// a token's heads need (15.8 -> 11.0 us for those prompts, of 12 and 2 x 2 heads of 64); 64, 192 and 384 threads were all slower than 128.
+// Bound by its instructions (some 220 a warp and four query heads, three times as many where there are codes to make) and their
+// latencies, at 20 to 24 warps an SM, not by memory: 2,048 tokens of 32 and 2 x 8 bfloat16 heads of 128 to 8 bits take 17.4 us
+// (46 MB, 2.7 TB/s), 2,513 of 12 and 2 x 2 float32 heads of 64 to 4 bits 8.0 us (18 MB, 2.3 TB/s), eight tokens 2.6 us.  A block is no
+// larger than a token's heads need (those float32 heads: 15.8 us with 128 threads of which half are idle, 11.0 with 64); blocks of
+// 64, 192 and 384 threads were slower than 128, 8 blocks an SM of 64 registers a thread no faster than 6 of 80.
 constexpr int WRITE_THREADS = 128;
 __device__ __forceinline__ void fetch8(uint4 (&raw)[1], const bf16* p) { raw[0] = *reinterpret_cast<const uint4*>(p); }
 __device__ __forceinline__ void fetch8(uint4 (&raw)[2], const float* p) {
@@ -149,7 +151,7 @@ __device__ __forceinline__ void spread8(float (&x)[8], const uint4 (&raw)[2]) {
     }
 }
 template <typename T, int BITS, int HEAD_DIM>
-__global__ void __launch_bounds__(WRITE_THREADS) quant_write_kernel(const WriteParams p) {
+__global__ void __launch_bounds__(WRITE_THREADS, 6) quant_write_kernel(const WriteParams p) {
     constexpr int LPH = HEAD_DIM / 16, HALF = HEAD_DIM / 2, G = HEAD_DIM / 32, RAW = sizeof(T) / 2;
     pdl_launch_dependents();
     const int t = blockIdx.y, sub = threadIdx.x % LPH, PER = blockDim.x / LPH;
@@ -174,8 +176,6 @@ __global__ void __launch_bounds__(WRITE_THREADS) quant_write_kernel(const WriteP
 #pragma unroll
         for (int i = 0; i < 4; ++i) cs[i] = c[i];
     }
-    float wa[8], wb[8];
-    const void* have = nullptr;                   // the norm whose weights these are
     if (page < 0 && p.write_cache && blockIdx.x == 0 && threadIdx.x == 0) atomicExch(p.status, 2);      // unmapped page: refused, never written
     // No lane leaves early: a warp holds several heads and all lanes take part in the exchanges.
     for (int first = blockIdx.x * PER; first < heads; first += gridDim.x * PER, h += gridDim.x * PER) {
@@ -190,11 +190,6 @@ __global__ void __launch_bounds__(WRITE_THREADS) quant_write_kernel(const WriteP
         }
         if (p.q_norm_w != nullptr) {              // both weights or neither (checked by the host)
             const void* nw = is_q ? p.q_norm_w : p.k_norm_w;
-            if (normed && have != nw) {
-                load_w8(wa, nw, p.norm_dtype, sub * 8);
-                load_w8(wb, nw, p.norm_dtype, HALF + sub * 8);
-                have = nw;
-            }
             float mean;
             if (__any_sync(0xffffffffu, is_k)) {
                 double ss = 0.0;
@@ -211,8 +206,11 @@ __global__ void __launch_bounds__(WRITE_THREADS) quant_write_kernel(const WriteP
             }
             if (normed) {
                 const float r = norm_factor(mean, p.eps);
-                head_scale8(a, r, wa);
-                head_scale8(b, r, wb);
+                float w[8];
+                load_w8(w, nw, p.norm_dtype, sub * 8);
+                head_scale8(a, r, w);
+                load_w8(w, nw, p.norm_dtype, HALF + sub * 8);
+                head_scale8(b, r, w);
             }
         }
         if (p.cos_sin != nullptr) {
@@ -297,7 +295,7 @@ template <typename T, int BITS> int launch_write(const WriteParams& p, cudaStrea
     const bool aligned = (bits & 15) == 0 && p.ld * (long long)sizeof(T) % 16 == 0;
     if (aligned && (p.cos_sin == nullptr || p.rotary_dim == D || p.rotary_dim * 2 == D) && p.tokens <= 65535 && (D == 64 || D == 128 || D == 256)) {
         const int lanes = heads * (D / 16), threads = lanes < WRITE_THREADS ? (lanes + 31) / 32 * 32 : WRITE_THREADS, per = threads / (D / 16);
-        // A block takes all heads of a token where there are tokens enough: the norms' weights and the angles are read once, and the
+        // A block takes all heads of a token where there are tokens enough: the angles are read once, and the
         // next heads are on their way meanwhile.
         const int shares = (heads + per - 1) / per;
         const dim3 grid((unsigned)(p.tokens >= 4 * kipp_sm_count() ? 1 : shares), (unsigned)p.tokens);
