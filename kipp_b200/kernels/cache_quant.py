@@ -85,8 +85,14 @@ def _lists(what: str, names: str, *tensors: torch.Tensor) -> None:
 _WRITE, _READ, _READ_ENTRIES, _ATTEND = (struct.Struct(f) for f in ("14Qq12if", "9Q7i", "12Q10i", "12Qq10if"))
 
 
+_entries: dict = {}
+
+
 def _call(lib: str, name: str, packed: bytes, what: str) -> None:
-    _check(_fn(lib, name, [c_char_p])(packed), what)
+    f = _entries.get(name)
+    if f is None:
+        f = _entries[name] = _fn(lib, name, [c_char_p])
+    _check(f(packed), what)
 
 
 def qk_norm_rope_write_quantized(qkv: torch.Tensor, q_out: torch.Tensor, pages: QuantizedPages, q_norm_w: Optional[torch.Tensor],
@@ -99,8 +105,11 @@ def qk_norm_rope_write_quantized(qkv: torch.Tensor, q_out: torch.Tensor, pages: 
     A position whose page is not mapped is not written: status word 0 becomes 2."""
     what, D, n_kv = "qk_norm_rope_write_quantized", pages.head_dim, pages.n_kv
     shape, dtype, q_norm, k_norm, table, norm_dtype = qkv.shape, qkv.dtype, 0, 0, 0, 0
-    if len(shape) != 2 or shape[1] != (n_q + 2 * n_kv) * D or shape[0] < tokens or qkv.stride(1) != 1:
+    if len(shape) != 2 or shape[1] != (n_q + 2 * n_kv) * D or shape[0] < tokens:
         raise KernelError(f"{what}: qkv has the wrong shape")
+    ld, one = qkv.stride()
+    if one != 1:
+        raise KernelError(f"{what}: qkv's rows must be contiguous")
     if q_out.dtype != dtype or not q_out.is_contiguous() or q_out.numel() < tokens * n_q * D:
         raise KernelError(f"{what}: q_out must be contiguous, of qkv's dtype and hold every query")
     _lists(what, "positions, entry_of_token and block_table", positions, entry_of_token, block_table)
@@ -108,13 +117,15 @@ def qk_norm_rope_write_quantized(qkv: torch.Tensor, q_out: torch.Tensor, pages: 
         raise KernelError(f"{what}: a position and an entry for every token, and a table [entries, width]")
     if (q_norm_w is None) != (k_norm_w is None):
         raise KernelError(f"{what}: q and k norm weights must come together")
-    stream = _launch_stream(what, qkv.get_device(), q_out, pages.k_codes, positions, entry_of_token, block_table, status)
-    if q_norm_w is not None:
+    device = pages.device_index
+    if q_norm_w is None:
+        stream = _launch_stream(what, device, qkv, q_out, positions, entry_of_token, block_table, status)
+    else:
+        stream = _launch_stream(what, device, qkv, q_out, positions, entry_of_token, block_table, status, q_norm_w, k_norm_w)
         if q_norm_w.dtype != k_norm_w.dtype or q_norm_w.numel() != D or k_norm_w.numel() != D or \
                 not (q_norm_w.is_contiguous() and k_norm_w.is_contiguous()):
             raise KernelError(f"{what}: norm weights must be contiguous, alike and of the head's size")
-        norm_dtype, q_norm, k_norm = dtype_code(q_norm_w.dtype), _ptr(q_norm_w), _ptr(k_norm_w)
-        _launch_stream(what, pages.device_index, q_norm_w, k_norm_w)
+        norm_dtype, q_norm, k_norm = dtype_code(q_norm_w.dtype), q_norm_w.data_ptr(), k_norm_w.data_ptr()
     if rotary_dim < 0 or rotary_dim % 2 or rotary_dim > D:
         raise KernelError(f"{what}: rotary_dim must be even and at most the head's size")
     if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() * 2 != rotary_dim):
@@ -125,13 +136,13 @@ def qk_norm_rope_write_quantized(qkv: torch.Tensor, q_out: torch.Tensor, pages: 
                 raise KernelError(f"{what}: a rotation needs cos_sin or inv_freq")
             cos_sin = rope_table(positions, inv_freq, tokens)
         if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or cos_sin.numel() < tokens * rotary_dim or \
-                cos_sin.get_device() != pages.device_index:
+                cos_sin.get_device() != device:
             raise KernelError(f"{what}: cos_sin must be contiguous float32 [tokens, rotary_dim / 2, 2] on the step's device")
         table = cos_sin.data_ptr()
     _status(status, what)
     _call("cache_quant", "kipp_quant_cache_write",
           _WRITE.pack(qkv.data_ptr(), q_out.data_ptr(), *pages.addresses, q_norm, k_norm, table, positions.data_ptr(),
-                      entry_of_token.data_ptr(), block_table.data_ptr(), status.data_ptr(), stream, qkv.stride(0), pages.bits, pages.n_pages,
+                      entry_of_token.data_ptr(), block_table.data_ptr(), status.data_ptr(), stream, ld, pages.bits, pages.n_pages,
                       pages.page_size, dtype_code(dtype), norm_dtype, rotary_dim, block_table.shape[1], tokens, n_q, n_kv, D,
                       1 if write_cache else 0, eps), what)
 
