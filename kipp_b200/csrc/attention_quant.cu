@@ -15,7 +15,7 @@
 // codes in bits 4 to 7 count sixteenfold: their queries are divided by 16, the results at the end.  Queries
 // and weights carry a factor of 2^48, all of these being powers of two: sums of weighted codes then end below float32's upper end with
 // every value at the format's limit of 2^60 and every weight at 2^8 (2^48+8+57 a key), and a value of 2^-40 still leaves
-// them whole.  A query has to be below 2^80 (beyond it counts as infinite).
+// them whole; below, a key loses up to 2^-64 of a result.  A query has to be below 2^80 (beyond it counts as infinite).
 //
 // Products are made the other way round from the kernels of attention_mma.cu, keys (then channels) as
 // rows, queries as columns, 8 at a time: mma.m16n8k16 with S^T = K Q^T, O^T = V^T P^T.  The codes are then the

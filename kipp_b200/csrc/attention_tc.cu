@@ -58,10 +58,18 @@
 // the head).  The cap is c tanh(x / c) = c - 2 c / (1 + e^(2x / c)), an exponential and a reciprocal per
 // score in float32.  The weights keep float32 precision through the 16-bit product: p = hi + lo with
 // hi = bf16(p), lo = bf16(p - hi), both in the tile's own score buffer, two products per tile.
+//
+// A third form (H, kipp_attn_prefill_tc_half) takes keys and values as float16, multiplied by a power of two per entry and kv
+// head that brings the largest to 2^15: what a quantised cache (quant_format.cuh) holds is such numbers with 4 to 8 and 8 bits of
+// mantissa, and bfloat16 would round keys by 2^-9, which scores of loud queries carry into the weights (8 bits, queries of 3 times
+// a key's size: results off by 0.7 % of their norm, 0.17 % in this form, which is the rounding of the result).  A query
+// row becomes float16 in shared memory, by a power of two of its own; weights carry 2^7.  float16 keeps its 11 bits down to 2^-29 of the
+// largest number that way.
 #include "common.cuh"
 #include "attention_extras.cuh"
 #include "mbarrier.cuh"
 #include <cuda.h>
+#include <cuda_fp16.h>
 #include <math.h>
 #include <mutex>
 #include <unordered_map>
@@ -82,6 +90,11 @@ template <int N> __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint4& v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -254,9 +267,9 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo, uint
     d |= (uint64_t)2 << 61;                            // SWIZZLE_128B
     return d;
 }
-// bf16 x bf16 -> f32, A K-major, B K-major (b_mn = 0) or MN-major (b_mn = 1).
-__host__ __device__ constexpr uint32_t idesc(int m, int n, int b_mn) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
+// bf16 x bf16 (or f16 x f16) -> f32, A K-major, B K-major (b_mn = 0) or MN-major (b_mn = 1).
+__host__ __device__ constexpr uint32_t idesc(int m, int n, int b_mn, bool half = false) {
+    return (1u << 4) | (half ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(m >> 4) << 24);
 }
 
@@ -285,6 +298,7 @@ struct Params {
     const float* sink;          // [n_q] or null
     const bf16* gate; long long ld_gate; int gate_dims;
     float out_scale;
+    const float2* factors;      // the H form: [entries][n_kv], what keys and values are multiplied by
 };
 
 // D, DV: columns of the query / key tiles (64, 128, and in the X form 192) and of the value tile (64, 128, and in the X
@@ -299,11 +313,13 @@ template <int D, int DV> struct Cfg {
     // which would only stand waiting for tensor memory
     static constexpr int CTAS = DV > 128 || D > 128 ? 1 : 2;
     // 100,480 bytes at head_dim 128: two CTAs (plus the 1 KB the system keeps per CTA) fit in 227 KB
-    static constexpr size_t NEED = Q_BYTES + 2 * K_BYTES + 2 * V_BYTES + XCHG_BYTES + 144;   // 16 barriers, 2 words
+    static constexpr size_t NEED = Q_BYTES + 2 * K_BYTES + 2 * V_BYTES + XCHG_BYTES + 144;   // 17 barriers, 2 words
     static constexpr size_t SMEM = CTAS == 1 && NEED < 116 * 1024 ? 116 * 1024 : NEED;
 };
 
-template <int D, int DV, bool X>
+constexpr float HALF_WEIGHTS_LOG2 = 7.f;     // weights of up to 2^RESCALE_SLACK end at 2^15
+
+template <int D, int DV, bool X, bool H = false>
 __global__ void __launch_bounds__(THREADS, Cfg<D, DV>::CTAS)
 attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ CUtensorMap map_k4, const __grid_constant__ CUtensorMap map_v4,
@@ -327,6 +343,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     uint64_t* o_final = bars + 15;      // the last O += P V is complete                  (1, by commit)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    uint64_t* q_ready = bars + 17;      // H: the query tile is float16                  (8)
 
     // A kernel that follows may take tensor memory while it waits for this grid, so where a CTA needs all of its
     // SM's it lets the next kernel's blocks start only once it has it (below).
@@ -358,6 +375,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
         mbar_init(&s_full[0], 1); mbar_init(&s_full[1], 1);
         mbar_init(o_final, 1);
+        if constexpr (H) mbar_init(q_ready, SOFTMAX_THREADS / 32);
         *abort_flag = (q_tile & 1023u) ? 1 : 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -464,8 +482,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         // The whole warp walks the loop and waits; one elected lane issues.  (With one lane
         // alone in a branch of its own the operands of every product came out of that
         // lane's registers, and a product took 60 to 80 cycles to issue.)
-        constexpr uint32_t IDESC_S = idesc(BM, BN, 0);
-        bool ok = mbar_wait(q_full, 0, abort_flag);
+        constexpr uint32_t IDESC_S = idesc(BM, BN, 0, H);
+        bool ok = mbar_wait(H ? q_ready : q_full, 0, abort_flag);
         // S(tile i) = Q K^T into score buffer i & 1 from key stage i & 1, as soon as the
         // output product of tile i - 2 has read the weights that lie in that buffer:
         // up to two tiles ahead of the softmax warps, never waiting for them
@@ -495,7 +513,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
     } else if (warp == 10) {
         // ------------------------------------------------------------ MMA issuer: outputs
-        constexpr uint32_t IDESC_O = idesc(BM, DV, 1);
+        constexpr uint32_t IDESC_O = idesc(BM, DV, 1, H);
         bool ok = true;
         for (int i = 0; i < n_tiles; ++i) {
             const int b = i & 1, use = i >> 1;
@@ -536,6 +554,45 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16;   // this warp's tensor-memory lanes
         float m_run = -INFINITY, l_run = 0.f;
         bool ok = true;
+        float scale_log2 = p.scale_log2, v_back = 1.f;               // (H: what the factors come to taken back)
+        if constexpr (H) {
+            // this thread's half of its row of queries as float16, the row's largest below 2^15
+            if (!mbar_wait(q_full, 0, abort_flag)) { if (ok) atomicMax(&p.status[2], 1); ok = false; }
+            constexpr int CHUNKS = D / 16;
+            const uint32_t at = q_tile + (D == 128 ? ch * (BM * 128) : ch * 64) + row * 128;
+            uint4 w[CHUNKS];
+            uint32_t most = 0;
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) {
+                w[c] = ld_shared_v4(at + ((c + row) % CHUNKS) * 16);       // (every lane of eight another bank)
+                most = __vmaxu2(most, __vmaxu2(__vmaxu2(w[c].x & 0x7fff7fffu, w[c].y & 0x7fff7fffu),
+                                               __vmaxu2(w[c].z & 0x7fff7fffu, w[c].w & 0x7fff7fffu)));
+            }
+            float largest = fmaxf(__uint_as_float(most << 16), __uint_as_float(most & 0xffff0000u));
+            float* xb = xchg + 2 * BM;                     // (the second tile's)
+            xb[ch * BM + row] = largest;
+            named_barrier(1 + (warp & 3), 64);
+            largest = fmaxf(largest, xb[(ch ^ 1) * BM + row]);
+            const int e = max((int)(__float_as_uint(largest) >> 23) - 127, -100);
+            const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) {
+                uint32_t* v = reinterpret_cast<uint32_t*>(&w[c]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const __half2 q2 = __floats2half2_rn(__uint_as_float(v[k] << 16) * up, __uint_as_float(v[k] & 0xffff0000u) * up);
+                    v[k] = *reinterpret_cast<const uint32_t*>(&q2);
+                }
+                st_shared_v4(at + ((c + row) % CHUNKS) * 16, w[c]);
+            }
+            fence_async_proxy();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_ready);
+            const float2 f = p.factors[(size_t)entry * p.n_kv + g];
+            // (never 0: a masked score times 0 would be no number)
+            scale_log2 = fmaxf(scale_log2 * (1.f / up) * (1.f / f.x), 0x1p-126f);
+            v_back = 1.f / f.y;
+        }
         // (A failed wait does not leave the loop: every thread must meet every barrier;
         // once the abort flag is up the remaining waits return at once.)
         for (int i = 0; i < n_tiles; ++i) {
@@ -585,18 +642,23 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             // tile's maximum exceeds it by more than RESCALE_SLACK (weights up to
             // 2^RESCALE_SLACK, far inside bfloat16 and the fp32 sums); numerator and
             // denominator carry the same reference, so the quotient is unchanged.
-            const float cand = X ? raw : raw * p.scale_log2;        // scale > 0: the maximum commutes
+            const float cand = X ? raw : raw * scale_log2;          // scale > 0: the maximum commutes
             const float mx = (cand > m_run + RESCALE_SLACK || m_run == -INFINITY) ? fmaxf(m_run, cand) : m_run;
             const float corr = (m_run == -INFINITY) ? 0.f : (mx == m_run ? 1.f : fast_exp2(m_run - mx));
-            const float neg_base = (mx == -INFINITY) ? 0.f : -mx;
+            const float neg_base = (mx == -INFINITY) ? 0.f : H ? HALF_WEIGHTS_LOG2 - mx : -mx;
             float2 sum2 = make_float2(0.f, 0.f);
-            const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), base2 = make_float2(neg_base, neg_base);
+            const float2 scale2 = make_float2(scale_log2, scale_log2), base2 = make_float2(neg_base, neg_base);
             uint32_t packed[HB / 2], rest[X ? HB / 2 : 1];
 #pragma unroll
             for (int j = 0; j < HB; j += 2) {
                 const float2 x = X ? add2(make_float2(s[j], s[j + 1]), base2) : fma2(make_float2(s[j], s[j + 1]), scale2, base2);
                 const float2 pw = make_float2(fast_exp2(x.x), fast_exp2(x.y));
                 sum2 = add2(sum2, pw);
+                if constexpr (H) {
+                    const __half2 pk = __floats2half2_rn(pw.x, pw.y);
+                    packed[j / 2] = *reinterpret_cast<const uint32_t*>(&pk);
+                    continue;
+                }
                 __nv_bfloat162 pk = __floats2bfloat162_rn(pw.x, pw.y);
                 packed[j / 2] = *reinterpret_cast<uint32_t*>(&pk);
                 if constexpr (X) {
@@ -643,6 +705,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         named_barrier(1 + (warp & 3), 64);
         const float l_row = l_run + xl[(ch ^ 1) * BM + row];
         float inv = l_row > 0.f ? 1.f / l_row : 0.f;
+        if constexpr (H) inv *= v_back;
         const int v_dim = X ? p.v_dim : DV;
         const size_t token = (size_t)(qs + (live ? tok : 0));
         bf16* dst = p.out + (token * p.n_q + h) * v_dim;
@@ -985,11 +1048,11 @@ int query_map(CUtensorMap* out, const void* ptr, int tokens, int n_q, int head_d
     return r != CUDA_SUCCESS ? 1000 + (int)r : 0;
 }
 
-template <int D, int DV, bool X> int launch(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mk4, const CUtensorMap& mv4,
+template <int D, int DV, bool X, bool H = false> int launch(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mk4, const CUtensorMap& mv4,
                             const CUtensorMap& mq, const CUtensorMap& mo, const Params& p, int items, cudaStream_t s) {
     using C = Cfg<D, DV>;
-    if (const int e = kipp_allow_smem(attn_prefill_tc_kernel<D, DV, X>, C::SMEM)) return e;
-    return kipp_launch(attn_prefill_tc_kernel<D, DV, X>, dim3(p.n_q, items), dim3(THREADS), C::SMEM, s, 1, mk, mv, mk4, mv4, mq, mo, p);
+    if (const int e = kipp_allow_smem(attn_prefill_tc_kernel<D, DV, X, H>, C::SMEM)) return e;
+    return kipp_launch(attn_prefill_tc_kernel<D, DV, X, H>, dim3(p.n_q, items), dim3(THREADS), C::SMEM, s, 1, mk, mv, mk4, mv4, mq, mo, p);
 }
 }  // namespace
 
@@ -1017,7 +1080,7 @@ extern "C" int kipp_attn_prefill_tc_ex_supported(int head_dim, int v_dim, int n_
 static int prefill_tc(void* out, const void* q, int tokens, const void* k_pages, const void* v_pages, int n_pages,
                       const int* q_start, const int* context_len, const int* block_table, int table_width, int page_size,
                       const int* work, int items, int n_q, int n_kv, int head_dim, int v_dim, float scale, int window,
-                      float out_scale, const MixExtras* ex, int* status, void* stream) {
+                      float out_scale, const MixExtras* ex, const float2* factors, int* status, void* stream) {
     if (items <= 0) return 0;
     if (items > 65535) return KIPP_ERR_ARG;
     if (!kipp_attn_prefill_tc_page_ok(page_size) || n_pages <= 0 || window < 0 || status == nullptr || tokens <= 0)
@@ -1060,6 +1123,10 @@ static int prefill_tc(void* out, const void* q, int tokens, const void* k_pages,
     rc = pool_map(&mo, out, tokens, n_q * v_dim, 32);
     if (rc) return rc;
     cudaStream_t s = (cudaStream_t)stream;
+    p.factors = factors;
+    if (factors != nullptr)
+        return head_dim == 64 ? launch<64, 64, false, true>(mk, mv, mk4, mv4, mq, mo, p, items, s)
+                              : launch<128, 128, false, true>(mk, mv, mk4, mv4, mq, mo, p, items, s);
     if (ex == nullptr)
         return head_dim == 64 ? launch<64, 64, false>(mk, mv, mk4, mv4, mq, mo, p, items, s)
                               : launch<128, 128, false>(mk, mv, mk4, mv4, mq, mo, p, items, s);
@@ -1094,7 +1161,21 @@ extern "C" int kipp_attn_prefill_tc(void* out, const void* q, int tokens, const 
                                     int* status, void* stream) {
     if (items > 0 && !kipp_attn_prefill_tc_supported(head_dim, n_q, n_kv)) return KIPP_ERR_ARG;
     return prefill_tc(out, q, tokens, k_pages, v_pages, n_pages, q_start, context_len, block_table, table_width, page_size, work,
-                      items, n_q, n_kv, head_dim, head_dim, scale, window, 1.f, nullptr, status, stream);
+                      items, n_q, n_kv, head_dim, head_dim, scale, window, 1.f, nullptr, nullptr, status, stream);
+}
+
+// The H form: k_pages and v_pages float16, entry e's keys and values of kv head g multiplied by factors[e * n_kv + g] (two
+// numbers, powers of two).  q and out are bfloat16; scale > 0.
+extern "C" int kipp_attn_prefill_tc_half(void* out, const void* q, int tokens, const void* k_pages, const void* v_pages,
+                                         int n_pages, const int* q_start, const int* context_len,
+                                         const int* block_table, int table_width, int page_size, const int* work,
+                                         int items, int n_q, int n_kv, int head_dim, float scale, int window,
+                                         const void* factors, int* status, void* stream) {
+    if (items <= 0) return 0;
+    if (!kipp_attn_prefill_tc_supported(head_dim, n_q, n_kv) || factors == nullptr || !(scale > 0.f)) return KIPP_ERR_ARG;
+    if ((uintptr_t)factors & 7) return -3;
+    return prefill_tc(out, q, tokens, k_pages, v_pages, n_pages, q_start, context_len, block_table, table_width, page_size, work,
+                      items, n_q, n_kv, head_dim, head_dim, scale, window, 1.f, nullptr, static_cast<const float2*>(factors), status, stream);
 }
 
 extern "C" int kipp_attn_prefill_tc_ex(void* out, const void* q, int tokens, const void* k_pages, const void* v_pages,
@@ -1110,7 +1191,7 @@ extern "C" int kipp_attn_prefill_tc_ex(void* out, const void* q, int tokens, con
     // a gate per element is read 16 bytes at a time
     if (ex->gate != nullptr && ex->gate_dims && ((((uintptr_t)ex->gate + 2 * (size_t)ex->gate_off) & 15) || (ex->ld_gate & 7))) return -3;
     return prefill_tc(out, q, tokens, k_pages, v_pages, n_pages, q_start, context_len, block_table, table_width, page_size, work,
-                      items, n_q, n_kv, head_dim, v_dim, scale, window, out_scale, ex, status, stream);
+                      items, n_q, n_kv, head_dim, v_dim, scale, window, out_scale, ex, nullptr, status, stream);
 }
 
 // Whether kipp_latent_expand_tc takes the pages and is the faster form for `keys` cached tokens, new ones among them.  Its

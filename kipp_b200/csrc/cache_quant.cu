@@ -12,9 +12,11 @@
 // from a bfloat16 copy.
 //
 // Reading back: codes -> bfloat16 or float32 rows in pages of the same shape, for a list of pages, or
-// for the entries of a step with the block table of the pages made (prompt attention reads those).
+// for the entries of a step with the block table of the pages made (attention over more than a few tokens reads those); for
+// the prompt kernel as float16, by powers of two that bring the largest number of an entry's kv head to 2^15.
 #include "quant_format.cuh"
 #include "head_math.cuh"
+#include <cuda_fp16.h>
 
 namespace {
 
@@ -318,7 +320,72 @@ struct ReadParams {
     int* table_out; const int* q_start; const int* context_len;
     int table_width, first_entry, window;
     int at;                         // what the launch begins with, a page's place in the list or among the entries'
+    float2* factors;                // float16: [entries][n_kv], what keys and values are multiplied by
 };
+
+// The keys of entry e that its tokens see, [first, end): none where it brings no token.
+__device__ __forceinline__ int2 seen_keys(const ReadParams& p, int e) {
+    const int tokens = p.q_start[e + 1] - p.q_start[e], first = p.context_len[e];
+    if (tokens <= 0) return make_int2(0, 0);
+    return make_int2(p.window > 0 ? max(0, first - p.window + 1) : 0, first + tokens);
+}
+
+// The power of two that brings L times the largest scale below 2^15: of the scales of the keys and of the values that an entry's
+// tokens see, a block per kv head and entry.  (16 bytes of scales of 144 to 272 a token and head: the lists and two loads in a row
+// bound it, 3 us for 6,144 tokens.)
+constexpr int FACTOR_THREADS = 1024;
+template <int BITS, int G>
+__global__ void __launch_bounds__(FACTOR_THREADS) quant_factor_kernel(const ReadParams p) {
+    static_assert(G == 2 || G == 4, "the prompt kernel's heads");
+    __shared__ uint32_t sh[2][32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int g = blockIdx.x, e = p.first_entry + blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int2 seen = seen_keys(p, e);
+    const int* table = p.list + (size_t)e * p.table_width;
+    const int end = min((long long)seen.y, (long long)p.table_width * p.pages.page_size);
+    uint32_t most[2] = {0u, 0u};                  // pairs of bfloat16 without signs
+    for (int base = seen.x + threadIdx.x; base < end; base += 4 * FACTOR_THREADS) {
+        uint32_t k[4][G / 2], v[4][G / 2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = base + i * FACTOR_THREADS, slot = j / p.pages.page_size;
+            const int page = j < end ? table[slot] : -1;
+#pragma unroll
+            for (int w = 0; w < G / 2; ++w) k[i][w] = v[i][w] = 0u;
+            if (page >= 0 && page < p.pages.n_pages) {
+                const size_t row = ((size_t)page * p.pages.n_kv + g) * p.pages.page_size + (j - slot * p.pages.page_size);
+                const uint32_t* ks = reinterpret_cast<const uint32_t*>(p.pages.k_scales) + row * (G / 2);
+                const uint32_t* vs = reinterpret_cast<const uint32_t*>(p.pages.v_scales) + row * (G / 2);
+#pragma unroll
+                for (int w = 0; w < G / 2; ++w) { k[i][w] = ks[w]; v[i][w] = vs[w]; }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int w = 0; w < G / 2; ++w) {
+                most[0] = __vmaxu2(most[0], k[i][w] & 0x7fff7fffu);
+                most[1] = __vmaxu2(most[1], v[i][w] & 0x7fff7fffu);
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t one = __reduce_max_sync(0xffffffffu, max(most[i] & 0xffffu, most[i] >> 16));
+        if (lane == 0) sh[i][warp] = one;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        float f[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t bits = __reduce_max_sync(0xffffffffu, sh[i][lane]);
+            const int exponent = max((int)(bits >> 7) - 127, -100);
+            f[i] = __uint_as_float((uint32_t)(127 + 14 - exponent - (BITS == 4 ? 3 : 7)) << 23);
+        }
+        if (lane == 0) p.factors[(size_t)e * p.pages.n_kv + g] = make_float2(f[0], f[1]);
+    }
+}
 
 // The eight channels that a word of 4-bit codes, or two of 8-bit, stand for, as bfloat16 pairs of (code - L) * 2^-13: a code in the
 // low bits of 16 is the number code * 2^-133 (attention_quant.cu), and one fused multiply-add makes it that, exactly.
@@ -350,8 +417,21 @@ template <int BITS, bool EVEN> __device__ __forceinline__ Unit<BITS> take_unit(c
     }
     return u;
 }
-// (the scale times 2^13, exact, and one rounding)
-template <int BITS> __device__ __forceinline__ void put_unit(bf16* p, const Unit<BITS>& u) {
+// (the scale times 2^13, exact, and one rounding; `factor` is float16's)
+template <int BITS> __device__ __forceinline__ void put_unit(__half* p, const Unit<BITS>& u, float factor) {
+    __nv_bfloat162 x[4];
+    whole_numbers<BITS>(x, u.w);
+    uint4 out;
+    uint32_t* o = reinterpret_cast<uint32_t*>(&out);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float s = quant_scale_value(u.s[i >> 1]) * 8192.f * factor;
+        const __half2 r = __floats2half2_rn(__low2float(x[i]) * s, __high2float(x[i]) * s);
+        o[i] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+    *reinterpret_cast<uint4*>(p) = out;
+}
+template <int BITS> __device__ __forceinline__ void put_unit(bf16* p, const Unit<BITS>& u, float) {
     __nv_bfloat162 x[4];
     whole_numbers<BITS>(x, u.w);
     uint4 out;
@@ -364,7 +444,7 @@ template <int BITS> __device__ __forceinline__ void put_unit(bf16* p, const Unit
     }
     *reinterpret_cast<uint4*>(p) = out;
 }
-template <int BITS> __device__ __forceinline__ void put_unit(float* p, const Unit<BITS>& u) {
+template <int BITS> __device__ __forceinline__ void put_unit(float* p, const Unit<BITS>& u, float) {
     __nv_bfloat162 x[4];
     whole_numbers<BITS>(x, u.w);
     float r[8];
@@ -381,6 +461,8 @@ template <int BITS> __device__ __forceinline__ void put_unit(float* p, const Uni
 // and of values on their way at once.  A page whose number is negative (unmapped) or past the pool becomes zeros; past the
 // pool is also reported.
 constexpr int READ_THREADS = 256;
+template <typename T> struct IsHalf { static constexpr bool value = false; };
+template <> struct IsHalf<__half> { static constexpr bool value = true; };
 template <typename T, int BITS, bool ENTRIES, int DIM, int UNROLL>
 __global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const ReadParams p) {
     if constexpr (!ENTRIES) pdl_launch_dependents();      // (a step's table is read before a kernel's wait: this one lets none start early)
@@ -388,16 +470,16 @@ __global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const ReadPara
     const int i = p.at + blockIdx.y, D = DIM > 0 ? DIM : p.head_dim, G = D / 32;
     const int page = p.list[ENTRIES ? (size_t)(p.first_entry + i / p.table_width) * p.table_width + i % p.table_width : (size_t)i];
     int from = 0, to = 0;                         // the page's slots that a token sees
+    const float2* factors = nullptr;
     if constexpr (ENTRIES) {
         const int e = p.first_entry + i / p.table_width, slot = i % p.table_width;
-        const int tokens = p.q_start[e + 1] - p.q_start[e], first = p.context_len[e], len = first + tokens;
-        const int seen = p.window > 0 ? max(0, first - p.window + 1) : 0;
-        const bool used = tokens > 0 && page >= 0 && (long long)slot * p.pages.page_size < len &&
-                          (long long)(slot + 1) * p.pages.page_size > seen;
+        const int2 seen = seen_keys(p, e);
+        const bool used = page >= 0 && (long long)slot * p.pages.page_size < seen.y && (long long)(slot + 1) * p.pages.page_size > seen.x;
         if (blockIdx.x == 0 && threadIdx.x == 0) p.table_out[(size_t)e * p.table_width + slot] = used ? i : -1;
         if (!used) return;
-        from = max(0, seen - slot * p.pages.page_size);
-        to = min(p.pages.page_size, len - slot * p.pages.page_size);
+        from = max(0, seen.x - slot * p.pages.page_size);
+        to = min(p.pages.page_size, seen.y - slot * p.pages.page_size);
+        factors = p.factors + (size_t)e * p.pages.n_kv;
     }
     const bool ok = page >= 0 && page < p.pages.n_pages;
     if (page >= p.pages.n_pages && threadIdx.x == 0) atomicExch(p.status, 3);
@@ -423,8 +505,10 @@ __global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const ReadPara
         for (int j = 0; j < UNROLL; ++j) {
             const int u = base + j * READ_THREADS + threadIdx.x;
             if (u < units) {
-                put_unit<BITS>(k_out + (size_t)u * 8, k[j]);
-                put_unit<BITS>(v_out + (size_t)u * 8, v[j]);
+                float2 f = make_float2(1.f, 1.f);
+                if constexpr (IsHalf<T>::value) f = factors[u / (per_row * p.pages.page_size)];
+                put_unit<BITS>(k_out + (size_t)u * 8, k[j], f.x);
+                put_unit<BITS>(v_out + (size_t)u * 8, v[j], f.y);
             }
         }
     }
@@ -446,6 +530,19 @@ template <bool ENTRIES> int launch_read(const ReadParams& p, int bits, int out_d
     const unsigned x = (unsigned)((units + per - 1) / per);
     auto kernel = out_dtype == KIPP_DT_F32 ? (bits == 4 ? read_kernel<float, 4, ENTRIES>(p.head_dim, many) : read_kernel<float, 8, ENTRIES>(p.head_dim, many))
                                            : (bits == 4 ? read_kernel<bf16, 4, ENTRIES>(p.head_dim, many) : read_kernel<bf16, 8, ENTRIES>(p.head_dim, many));
+    if constexpr (ENTRIES) {
+        if (p.factors != nullptr) {
+            const bool wide = p.head_dim == 128;
+            auto factor = wide ? (bits == 4 ? quant_factor_kernel<4, 4> : quant_factor_kernel<8, 4>) : (bits == 4 ? quant_factor_kernel<4, 2> : quant_factor_kernel<8, 2>);
+            const dim3 grid((unsigned)p.pages.n_kv, (unsigned)(p.n / p.table_width));
+            if (grid.y > 65535) return KIPP_ERR_ARG;
+            if (const int e = kipp_launch(factor, grid, dim3(FACTOR_THREADS), 0, s, 1, p)) return e;
+            kernel = bits == 4 ? (wide ? (many ? quant_read_kernel<__half, 4, true, 128, 4> : quant_read_kernel<__half, 4, true, 128, 1>)
+                                       : (many ? quant_read_kernel<__half, 4, true, 64, 4> : quant_read_kernel<__half, 4, true, 64, 1>))
+                               : (wide ? (many ? quant_read_kernel<__half, 8, true, 128, 4> : quant_read_kernel<__half, 8, true, 128, 1>)
+                                       : (many ? quant_read_kernel<__half, 8, true, 64, 4> : quant_read_kernel<__half, 8, true, 64, 1>));
+        }
+    }
     // (a grid's second dimension ends at 65,535)
     for (ReadParams q = p; q.at < p.n; q.at += 65535) {
         const unsigned y = (unsigned)(p.n - q.at < 65535 ? p.n - q.at : 65535);
@@ -488,6 +585,7 @@ struct KippQuantReadEntries {
     const void *k_codes, *k_scales, *v_codes, *v_scales;
     const int *q_start, *context_len, *block_table;
     int* status;
+    void* factors;                                      // or null: float2 [entries of the step][n_kv]
     void* stream;
     int out_dtype, bits, n_pages, page_size, table_width, first_entry, entries, window, n_kv, head_dim;
 };
@@ -523,7 +621,7 @@ extern "C" int kipp_quant_cache_read(const KippQuantRead* a) {
         return KIPP_ERR_ARG;
     if (a->out_dtype != KIPP_DT_F32 && a->out_dtype != KIPP_DT_BF16) return KIPP_ERR_DTYPE;
     if (!read_aligned(pages, a->k_out, a->v_out)) return -3;
-    ReadParams p = {a->k_out, a->v_out, pages, a->list, a->n, a->head_dim, a->status, nullptr, nullptr, nullptr, 0, 0, 0, 0};
+    ReadParams p = {a->k_out, a->v_out, pages, a->list, a->n, a->head_dim, a->status, nullptr, nullptr, nullptr, 0, 0, 0, 0, nullptr};
     return launch_read<false>(p, a->bits, a->out_dtype, (cudaStream_t)a->stream);
 }
 
@@ -532,6 +630,7 @@ extern "C" int kipp_quant_cache_read(const KippQuantRead* a) {
 // step's shape and only those entries' rows are written.  The pages no token sees are neither read nor
 // written; their table entries are -1.  The slots that no token sees, of pages that some are seen of, become zeros: they may hold
 // anything, and the attention over the pages multiplies them by weights of 0.
+// With `factors` (heads of 64 and 128) the pages are float16, multiplied by the powers of two that it makes there.
 extern "C" int kipp_quant_cache_read_entries(const KippQuantReadEntries* a) {
     if (a->entries <= 0) return 0;
     const QuantPages pages = {(uint8_t*)a->k_codes, (bf16*)a->k_scales, (uint8_t*)a->v_codes, (bf16*)a->v_scales, a->n_pages, a->page_size, a->n_kv};
@@ -539,8 +638,11 @@ extern "C" int kipp_quant_cache_read_entries(const KippQuantReadEntries* a) {
         a->table_width <= 0 || a->first_entry < 0 || a->window < 0 || (long long)a->entries * a->table_width > 0x7fffffffLL)
         return KIPP_ERR_ARG;
     if (a->out_dtype != KIPP_DT_F32 && a->out_dtype != KIPP_DT_BF16) return KIPP_ERR_DTYPE;
-    if (!read_aligned(pages, a->k_out, a->v_out)) return -3;
+    if (a->factors != nullptr && (a->out_dtype != KIPP_DT_BF16 || (a->head_dim != 64 && a->head_dim != 128))) return KIPP_ERR_ARG;
+    if (!read_aligned(pages, a->k_out, a->v_out) || ((uintptr_t)a->factors & 7) != 0 ||
+        (a->factors != nullptr && (((uintptr_t)a->k_scales | (uintptr_t)a->v_scales) & 3) != 0))
+        return -3;
     ReadParams p = {a->k_out, a->v_out, pages, a->block_table, a->entries * a->table_width, a->head_dim, a->status, a->table_out, a->q_start,
-                    a->context_len, a->table_width, a->first_entry, a->window, 0};
+                    a->context_len, a->table_width, a->first_entry, a->window, 0, (float2*)a->factors};
     return launch_read<true>(p, a->bits, a->out_dtype, (cudaStream_t)a->stream);
 }

@@ -100,6 +100,7 @@ struct QuantReadEntriesArgs {
     const void *k_codes, *k_scales, *v_codes, *v_scales;
     const int *q_start, *context_len, *block_table;
     int* status;
+    void* factors;
     void* stream;
     int out_dtype, bits, n_pages, page_size, table_width, first_entry, entries, window, n_kv, head_dim;
 };
@@ -1097,9 +1098,10 @@ public:
                                   head_dim, write_cache ? 1 : 0, eps};
         run(f(&a), "quant_cache_write");
     }
-    // What entries first .. first + entries - 1 see, read back into pages of their own: the view of those.
+    // What entries first .. first + entries - 1 see, read back into pages of their own: the view of those.  With `factors` (two numbers
+    // an entry of the step and kv head, made here) the pages are float16, multiplied by those.
     PagedCacheView quant_read_entries(const PagedCacheView& cache, int dtype, const int* q_start, const int* context_len, int first,
-                                      int entries, int all_entries, int n_kv, int head_dim, int window) {
+                                      int entries, int all_entries, int n_kv, int head_dim, int window, float* factors = nullptr) {
         using Fn = int (*)(const QuantReadEntriesArgs*);
         static Fn f = kernel_symbol<Fn>("cache_quant", "kipp_quant_cache_read_entries");
         PagedCacheView v = cache;
@@ -1112,9 +1114,9 @@ public:
         int* table = workspace->get<int>("quant_table", (size_t)all_entries * cache.table_width);
         v.block_table = table;
         const QuantReadEntriesArgs a = {v.k_pages, v.v_pages, table, cache.k_pages, cache.k_scales, cache.v_pages, cache.v_scales, q_start,
-                                        context_len, cache.block_table, status, stream, dtype, cache.bits, cache.n_pages, cache.page_size,
+                                        context_len, cache.block_table, status, factors, stream, dtype, cache.bits, cache.n_pages, cache.page_size,
                                         cache.table_width, first, entries, window, n_kv, head_dim};
-        run(f(&a), "quant_cache_read");
+        run(f(&a), "quant_cache_read", factors != nullptr ? 2 : 1);
         return v;
     }
     static bool attention_quant_supported(int bits, int head_dim, int n_q, int n_kv) {
@@ -1154,16 +1156,21 @@ public:
                 if (q_lens[(size_t)e] == 1) single = true;
                 if (q_lens[(size_t)e] > 1) { if (first < 0) first = e; last = e; }
             }
-            const bool portions = prefill_tensor_core && longest >= PREFILL_TC_MIN_TOKENS && work.n_prefill_items128 > 0 &&
+            const bool portions = prefill_tensor_core && scale > 0.f && longest >= PREFILL_TC_MIN_TOKENS && work.n_prefill_items128 > 0 &&
                                   last - first + 1 <= at_once && attention_tc_supported(head_dim, n_q, n_kv, cache.page_size);
             if (!portions || single)
                 attention_quant_direct(out, q, cache, q_start, context_len, entries, portions ? 1 : longest, n_q, n_kv, head_dim, scale, window);
             if (portions) {
-                AttentionWork only = work;
-                only.n_decode = 0;                     // (the prompt kernel alone)
-                attention_tensor_core(out, q, quant_read_entries(cache, dtype, q_start, context_len, first, last - first + 1, entries, n_kv,
-                                                                 head_dim, window),
-                                      only, q_start, context_len, n_q, n_kv, head_dim, scale, window);
+                float* factors = workspace->get<float>("quant_factors", 2 * (size_t)entries * n_kv);
+                const PagedCacheView v = quant_read_entries(cache, dtype, q_start, context_len, first, last - first + 1, entries, n_kv, head_dim,
+                                                            window, factors);
+                using Fn = int (*)(void*, const void*, int, const void*, const void*, int, const int*, const int*, const int*, int, int,
+                                   const int*, int, int, int, int, float, int, const void*, int*, void*);
+                static Fn f = kernel_symbol<Fn>("attention_tc", "kipp_attn_prefill_tc_half");
+                run(f(out, q, work.tokens, v.k_pages, v.v_pages, v.n_pages, q_start, context_len, v.block_table, v.table_width, v.page_size,
+                      work.prefill_work128, work.n_prefill_items128, n_q, n_kv, head_dim, scale, window, factors, status, stream),
+                    "attn_prefill_tc");
+                ++tc_prefill_launches;
             }
             return;
         }

@@ -82,7 +82,7 @@ def _lists(what: str, names: str, *tensors: torch.Tensor) -> None:
 
 
 # the structures of the C entry points (csrc/cache_quant.cu, csrc/attention_quant.cu): addresses, then sizes
-_WRITE, _READ, _READ_ENTRIES, _ATTEND = (struct.Struct(f) for f in ("14Qq12if", "9Q7i", "12Q10i", "12Qq10if"))
+_WRITE, _READ, _READ_ENTRIES, _ATTEND = (struct.Struct(f) for f in ("14Qq12if", "9Q7i", "13Q10i", "12Qq10if"))
 
 
 _entries: dict = {}
@@ -165,15 +165,16 @@ def read_quantized_pages(k_out: torch.Tensor, v_out: torch.Tensor, pages: Quanti
 
 
 def _read_entries(pages: QuantizedPages, dtype: torch.dtype, meta, block_table: torch.Tensor, first: int, entries: int, window: int,
-                  status: torch.Tensor, table: torch.Tensor, stream: int):
-    """Pages of what ``entries`` entries from ``first`` on see, in ``dtype``, and their rows of ``table``."""
+                  status: torch.Tensor, table: torch.Tensor, stream: int, factors: Optional[torch.Tensor] = None):
+    """Pages of what ``entries`` entries from ``first`` on see, in ``dtype``, and their rows of ``table``.  With ``factors`` (float32
+    [entries of the step, n_kv, 2], made here) the pages' 16 bits are float16, multiplied by those."""
     width = block_table.shape[1]
     k = torch.empty((entries * width, pages.n_kv, pages.page_size, pages.head_dim), dtype=dtype, device=table.device)
     v = torch.empty_like(k)
     _call("cache_quant", "kipp_quant_cache_read_entries",
           _READ_ENTRIES.pack(k.data_ptr(), v.data_ptr(), table.data_ptr(), *pages.addresses, meta.q_start.data_ptr(),
-                             meta.context_len.data_ptr(), block_table.data_ptr(), status.data_ptr(), stream, dtype_code(dtype), pages.bits,
-                             pages.n_pages, pages.page_size, width, first, entries, window, pages.n_kv, pages.head_dim), "read_entries")
+                             meta.context_len.data_ptr(), block_table.data_ptr(), status.data_ptr(), 0 if factors is None else factors.data_ptr(), stream,
+                             dtype_code(dtype), pages.bits, pages.n_pages, pages.page_size, width, first, entries, window, pages.n_kv, pages.head_dim), "read_entries")
     return k, v
 
 
@@ -197,13 +198,13 @@ def _direct_ok(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPages, n_q: i
     return q.dtype == torch.bfloat16 and _supported[key] and pages.aligned and (q.data_ptr() | out.data_ptr()) % 16 == 0
 
 
-def _plan(out, q, pages, meta, block_table, n_q):
+def _plan(out, q, pages, meta, block_table, n_q, scale=1.0):
     """(form of the entries of one token, form of the others, the entries of more than one token from the first to the last):
-    forms "direct" (the kernel over codes), "portion" (read back, tcgen05 prompt kernel) and "read" (read back, CUDA cores).
+    forms "direct" (the kernel over codes), "portion" (read back, tcgen05 prompt kernel, for positive scales) and "read" (read back, CUDA cores).
     The prompt kernel reads a key and a value once for 128 tokens, the kernel over codes once for 8 or 16 columns."""
     if not _direct_ok(out, q, pages, n_q):
         return "read", "read", None
-    if max(meta.q_lens) >= PORTION_MIN and getattr(meta, "prefill_work128", None) is not None:
+    if scale > 0 and max(meta.q_lens) >= PORTION_MIN and getattr(meta, "prefill_work128", None) is not None:
         from . import attention_bf16
         several = [e for e, n in enumerate(meta.q_lens) if n > 1]
         span = (several[0], several[-1] + 1)
@@ -221,7 +222,8 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
     ``q_start``, ``context_len``, and where entries bring 64 tokens or more the list of their 128-token tiles,
     ``prefill_work128`` and ``n_prefill_items128``).  bfloat16 with heads of 64, 128 or 256 runs on the codes themselves; longer
     portions of prompts, other heads and float32 on pages that are read back.  A page that is not mapped, or past the pool, sets
-    status word 0 to 3.  ``impl`` forces a form for the whole step:
+    status word 0 to 3.  On the codes a result is off by up to 2^-64 a key beside its roundings (values of 2^-40 and less feel it), and
+    queries of 2^80 and more count as infinite.  ``impl`` forces a form for the whole step:
     "direct" or "read"."""
     what, D, n_kv, q_lens, tokens = "attention_quantized", pages.head_dim, pages.n_kv, meta.q_lens, meta.tokens
     window = int(window or 0)
@@ -244,7 +246,7 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
     if tokens == 0:
         return
     if impl is None:
-        single, several, span = _plan(out, q, pages, meta, block_table, n_q)
+        single, several, span = _plan(out, q, pages, meta, block_table, n_q, scale)
     elif impl in ("direct", "read"):
         single, several, span = impl, impl, None
         if impl == "direct" and not _direct_ok(out, q, pages, n_q):
@@ -277,11 +279,17 @@ def _direct(out, q, pages, meta, block_table, n_q, scale, window, status, most: 
 
 
 def _portions(out, q, pages, meta, block_table, n_q, scale, window, status, span, stream: int) -> None:
-    """The entries of more than one token: their pages read back, and the prompt kernel over those."""
+    """The entries of more than one token: their pages read back as float16, and the prompt kernel over those."""
     table = torch.empty_like(block_table)
-    k, v = _read_entries(pages, q.dtype, meta, block_table, span[0], span[1] - span[0], window, status, table, stream)
-    from . import attention_bf16
-    attention_bf16.prefill_tc(out, q, k, v, meta, table, pages.page_size, n_q, pages.n_kv, pages.head_dim, scale, window, status)
+    factors = torch.empty((len(meta.q_lens), pages.n_kv, 2), dtype=torch.float32, device=q.device)
+    k, v = _read_entries(pages, q.dtype, meta, block_table, span[0], span[1] - span[0], window, status, table, stream, factors)
+    f = _fn("attention_tc", "kipp_attn_prefill_tc_half",
+            [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
+             c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_void_p])
+    _check(f(out.data_ptr(), q.data_ptr(), q.shape[0], k.data_ptr(), v.data_ptr(), k.shape[0], meta.q_start.data_ptr(),
+             meta.context_len.data_ptr(), table.data_ptr(), table.shape[1], pages.page_size, _ptr(meta.prefill_work128),
+             meta.n_prefill_items128, n_q, pages.n_kv, pages.head_dim, scale, window, factors.data_ptr(), status.data_ptr(), stream),
+           "attn_prefill_tc")
 
 
 def _by_reading(out, q, pages, meta, block_table, n_q, scale, window, status, stream: int) -> None:
