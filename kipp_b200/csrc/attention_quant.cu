@@ -22,9 +22,11 @@
 // register operand, and a warp that serves the few queries of a kv head (the heads of its group times
 // the tokens) wastes fewer columns.  P^T turns from result to operand by movmatrix.
 //
-// What bounds it: at 4 bits a 16-byte load holds 32 keys' channels, so the instructions that take codes apart
-// (about 1.4 a code pair, keys and values together) and the softmax stand against HBM's rate; each warp works on
-// its own 32 keys of a step of 128 with its own maximum, fetches its own rows, and meets the other three
+// What bounds it: at 4 bits a warp executes some 550 instructions for 32 keys of 128 channels, 270 of them on the integer
+// pipe (which takes a warp's in two cycles), and a lone warp needs 2,500 cycles for them; with three warps a scheduler issue is
+// half busy and the integer pipe too, and keys and values come at 4.7 to 5.1 TB/s (8 tokens behind 8,100 keys, 32 query and 8 key
+// heads: 24.9 us with the joining of the parts, 75 MB).  At 8 bits it is the memory, 6.0 TB/s (64 tokens behind 2,048: 57.4 us, 287 MB).
+// Each warp works on its own 32 keys of a step of 128 with its own maximum, fetches its own rows, and meets the other three
 // warps only at the end of a piece.  A maximum is raised only when a score passes it by 2^8.
 //
 // Rows come by cp.async into a ring per warp.  Where the page size is a multiple of 16, 16 keys of one kv head
