@@ -613,7 +613,9 @@ inline size_t Engine::workspace_estimate() const {
     // slack stand for them), and the logits rows
     const size_t es = dtype_size(dtype_);
     const size_t per_token = (size_t)plan_->hidden_size * (4 * (size_t)(plan_->streams + (plan_->streams > 1 ? 2 : 0)) + es * 12);
-    return per_token * (size_t)opt_.max_batch_tokens + (size_t)opt_.max_logit_rows * plan_->vocab_size * 4 + (64u << 20);
+    // a quantised cache: the pages that a step reads back, and the parts of rows of its attention
+    const size_t read_back = opt_.kv_bits ? (size_t)Ops::EXPAND_MAX_BYTES + (40u << 20) : 0;
+    return per_token * (size_t)opt_.max_batch_tokens + (size_t)opt_.max_logit_rows * plan_->vocab_size * 4 + (64u << 20) + read_back;
 }
 
 // Refuse before anything is uploaded when weights, cache and workspace cannot fit (the
