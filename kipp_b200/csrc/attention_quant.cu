@@ -64,7 +64,6 @@ struct Params {
 };
 
 constexpr int ROW_COST = 1;          // units of a row beside its steps
-constexpr int MANY_PARTS = 16;       // CTAs a row from which on 16 warps join its parts, not 4
 
 // One entry's share of the work.
 struct Entry {
@@ -808,13 +807,16 @@ template <int D, int BITS, int NT, bool TILES> int launch(Params p, long long st
     if (const int e = kipp_launch(attn_quant_kernel<D, BITS, NT, TILES>, dim3((unsigned)p.ctas), dim3(THREADS), smem, s, 1, p)) return e;
     if (alone) return 0;
     if (by_cta) return kipp_launch(attn_quant_join_kernel<D, NT>, dim3((unsigned)p.ctas), dim3(JOIN_WARPS * 32), 0, s, 1, p);
-    const int columns = p.most * p.group;
-    const dim3 grid((unsigned)rows, (unsigned)(columns < COLS ? columns : COLS));
-    if (rows * MANY_PARTS > p.ctas) return kipp_launch(attn_quant_merge_kernel<D, NT, 4>, grid, dim3(128), 0, s, 1, p);
-    return kipp_launch(attn_quant_merge_kernel<D, NT, 16>, grid, dim3(512), 0, s, 1, p);
+    // 16 warps a row and column where there are parts for all of them and an SM for every block (one token behind 8,000 keys, 8 rows: 10.6
+    // us in all, 11.9 with 4; 13 entries of two tokens, 26 rows of 12 columns: 17.1 and 12.5)
+    const int columns = p.most * p.group, live = columns < COLS ? columns : COLS;
+    const dim3 grid((unsigned)rows, (unsigned)live);
+    if (rows * 16 <= p.ctas && rows * live <= kipp_sm_count()) return kipp_launch(attn_quant_merge_kernel<D, NT, 16>, grid, dim3(512), 0, s, 1, p);
+    return kipp_launch(attn_quant_merge_kernel<D, NT, 4>, grid, dim3(128), 0, s, 1, p);
 }
 
-// 8 columns where they hold every query of a kv head, else 16 (heads of 256 have no room for their sums: always 8)
+// 8 columns where they hold every query of a kv head (8 tokens behind 8,100 keys, 4 queries each: 25.2 us, 31.7 with 16), else 16 (12
+// queries: 35.5 us, 42.3 with 8); heads of 256 have no room for their sums: always 8
 int columns_of(int head_dim, long long queries) { return head_dim == 256 || queries <= 8 ? 8 : 16; }
 }  // namespace
 

@@ -1139,8 +1139,8 @@ public:
         run(f(&a), "attn_quant", need > 0 ? 2 : 1);
     }
     // Causal grouped-query attention over a quantised cache.  bfloat16 heads of 64, 128 and 256 run on the codes; where portions of
-    // PREFILL_TC_MIN_TOKENS and more are among the entries, those of more than one token read their pages back for the tcgen05
-    // prompt kernel, as long as the pages have room in EXPAND_MAX_BYTES; other heads and 32-bit read back always, as many entries at
+    // PREFILL_TC_MIN_TOKENS and more are among the entries and it pays, those of more than one token read their pages back for the
+    // tcgen05 prompt kernel, as long as the pages have room in EXPAND_MAX_BYTES; other heads and 32-bit read back always, as many entries at
     // a time as have room there.  Which it is depends on the step's shape only.
     void attention_quantized(void* out, const void* q, const PagedCacheView& cache, int dtype, const AttentionWork& work,
                              const std::vector<int>& q_lens, const int* positions, const int* entry_of_token, const int* q_start,
@@ -1150,13 +1150,25 @@ public:
         const long long at_once = std::max(1LL, EXPAND_MAX_BYTES / (page_bytes * cache.table_width));
         if (dtype == BF16 && attention_quant_supported(cache.bits, head_dim, n_q, n_kv)) {
             int first = -1, last = -1, longest = 1;
+            long long several = 0, tokens = 0, tiles = 0;
             bool single = false;
             for (int e = 0; e < entries; ++e) {
-                longest = std::max(longest, q_lens[(size_t)e]);
-                if (q_lens[(size_t)e] == 1) single = true;
-                if (q_lens[(size_t)e] > 1) { if (first < 0) first = e; last = e; }
+                const int n = q_lens[(size_t)e];
+                longest = std::max(longest, n);
+                if (n == 1) single = true;
+                if (n <= 1) continue;
+                if (first < 0) first = e;
+                last = e;
+                ++several;
+                tokens += n;
+                tiles += (n + 127) / 128;
             }
-            const bool portions = prefill_tensor_core && scale > 0.f && longest >= PREFILL_TC_MIN_TOKENS && work.n_prefill_items128 > 0 &&
+            // Whether reading back pays.  Per cached key the codes cost 4 ps a query; a wave of 296 tiles of the prompt kernel costs as much
+            // as 4,096 of them, however full it is, and reading back a key of a kv head as 64.  (32 query and 8 key heads of 128: 64
+            // and 128 tokens behind 4,096 keys 38 and 67 us on the codes, 91 and 67 read back; four entries of 32 and 64 behind 2,048 in 8
+            // bits 50 and 75, 62 and 62.)
+            const bool pays = n_q * tokens > 4096 * ((n_q * tiles + 295) / 296) + 64 * n_kv * several;
+            const bool portions = prefill_tensor_core && pays && scale > 0.f && longest >= PREFILL_TC_MIN_TOKENS && work.n_prefill_items128 > 0 &&
                                   last - first + 1 <= at_once && attention_tc_supported(head_dim, n_q, n_kv, cache.page_size);
             if (!portions || single)
                 attention_quant_direct(out, q, cache, q_start, context_len, entries, portions ? 1 : longest, n_q, n_kv, head_dim, scale, window);

@@ -184,7 +184,17 @@ def _entries_at_once(pages: QuantizedPages, dtype: torch.dtype, width: int) -> i
     return max(1, READ_BYTES // per)
 
 
-PORTION_MIN = 64              # an entry of as many tokens is read back for the prompt kernel of 128-token tiles
+PORTION_MIN = 64              # the longest entry's tokens from which on reading back for the prompt kernel may pay
+
+
+def _portions_pay(q_lens, n_q: int, n_kv: int) -> bool:
+    """Whether the entries of more than one token are read back for the prompt kernel of 128-token tiles, or run on the codes.  Per
+    cached key the codes cost 4 ps a query; a wave of 296 tiles costs as much as 4,096 of them, however full it is, and reading back
+    a key of a kv head as 64.  32 query and 8 key heads of 128: 64 and 128 tokens behind 4,096 keys 38 and 67 us on the codes, 91 and
+    67 read back; four entries of 32 and 64 behind 2,048 (8 bits) 50 and 75, 62 and 62; 12 heads of 64, 64 tokens 10 and 27."""
+    several = [n for n in q_lens if n > 1]
+    tiles = sum((n + 127) // 128 for n in several)
+    return n_q * sum(several) > 4096 * -(-n_q * tiles // 296) + 64 * n_kv * len(several)
 
 
 _supported: dict = {}
@@ -198,18 +208,28 @@ def _direct_ok(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPages, n_q: i
     return q.dtype == torch.bfloat16 and _supported[key] and pages.aligned and (q.data_ptr() | out.data_ptr()) % 16 == 0
 
 
+def _portion_span(q, pages, meta, block_table, n_q, scale):
+    """The entries of more than one token from the first to the last, where the prompt kernel takes them, or None."""
+    if not scale > 0 or getattr(meta, "prefill_work128", None) is None:
+        return None
+    several = [e for e, n in enumerate(meta.q_lens) if n > 1]
+    if not several:
+        return None
+    from . import attention_bf16
+    if not attention_bf16.prefill_tc_supported(pages.head_dim, n_q, pages.n_kv, pages.page_size):
+        return None
+    return several[0], several[-1] + 1
+
+
 def _plan(out, q, pages, meta, block_table, n_q, scale=1.0):
     """(form of the entries of one token, form of the others, the entries of more than one token from the first to the last):
     forms "direct" (the kernel over codes), "portion" (read back, tcgen05 prompt kernel, for positive scales) and "read" (read back, CUDA cores).
     The prompt kernel reads a key and a value once for 128 tokens, the kernel over codes once for 8 or 16 columns."""
     if not _direct_ok(out, q, pages, n_q):
         return "read", "read", None
-    if scale > 0 and max(meta.q_lens) >= PORTION_MIN and getattr(meta, "prefill_work128", None) is not None:
-        from . import attention_bf16
-        several = [e for e, n in enumerate(meta.q_lens) if n > 1]
-        span = (several[0], several[-1] + 1)
-        if attention_bf16.prefill_tc_supported(pages.head_dim, n_q, pages.n_kv, pages.page_size) and \
-                span[1] - span[0] <= _entries_at_once(pages, q.dtype, block_table.shape[1]):
+    if max(meta.q_lens) >= PORTION_MIN and _portions_pay(meta.q_lens, n_q, pages.n_kv):
+        span = _portion_span(q, pages, meta, block_table, n_q, scale)
+        if span is not None and span[1] - span[0] <= _entries_at_once(pages, q.dtype, block_table.shape[1]):
             return "direct", "portion", span
     return "direct", "direct", None
 
@@ -220,11 +240,11 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
 
     ``meta`` is the step's metadata as for ``attention`` (``tokens``, ``q_lens``, ``positions``, ``entry_of_token``,
     ``q_start``, ``context_len``, and where entries bring 64 tokens or more the list of their 128-token tiles,
-    ``prefill_work128`` and ``n_prefill_items128``).  bfloat16 with heads of 64, 128 or 256 runs on the codes themselves; longer
+    ``prefill_work128`` and ``n_prefill_items128``).  bfloat16 with heads of 64, 128 or 256 runs on the codes themselves; long
     portions of prompts, other heads and float32 on pages that are read back.  A page that is not mapped, or past the pool, sets
     status word 0 to 3.  On the codes a result is off by up to 2^-64 a key beside its roundings (values of 2^-40 and less feel it), and
-    queries of 2^80 and more count as infinite.  ``impl`` forces a form for the whole step:
-    "direct" or "read"."""
+    queries of 2^80 and more count as infinite.  ``impl`` forces a form:
+    "direct" or "read" for the whole step, "portion" (long portions') for every entry of more than one token."""
     what, D, n_kv, q_lens, tokens = "attention_quantized", pages.head_dim, pages.n_kv, meta.q_lens, meta.tokens
     window = int(window or 0)
     dtype_code(q.dtype)
@@ -247,6 +267,11 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
         return
     if impl is None:
         single, several, span = _plan(out, q, pages, meta, block_table, n_q, scale)
+    elif impl == "portion":
+        single, several, span = "direct", "portion", _portion_span(q, pages, meta, block_table, n_q, scale)
+        if span is None or not _direct_ok(out, q, pages, n_q):
+            raise KernelError(f"{what}: portions are read back for bfloat16 heads of 64 or 128, 16-byte aligned, a positive scale and a "
+                              "list of their 128-token tiles")
     elif impl in ("direct", "read"):
         single, several, span = impl, impl, None
         if impl == "direct" and not _direct_ok(out, q, pages, n_q):

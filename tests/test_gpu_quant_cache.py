@@ -219,11 +219,12 @@ def test_attention(shape, bits, window, dtype):
         meta, table, n_pages = step(layout, page, li, width=None if li % 2 else 200 if page > 8 else None)
         pages, k, v = random_pages(n_pages, nkv, page, D, bits, li)
         q = (2 * torch.randn(meta.tokens, nq, D, generator=torch.Generator().manual_seed(li))).to(dtype).to(DEV)
-        for impl in (None, "direct", "read") if dtype == BF16 and D != 96 else (None,):
+        long = dtype == BF16 and D in (64, 128) and page in (8, 16, 32, 64) and max(n for _, n in layout) >= 64
+        for impl in (None, "direct", "read") + ("portion",) * long if dtype == BF16 and D != 96 else (None,):
             out, st = attend(pages, meta, q, nq, D ** -0.5, window, impl=impl)
             assert st.tolist() == [0, 0, 0, 0]
-            one, several, _ = cache_quant._plan(out, q, pages, meta, meta.block_tables[0], nq) if impl is None else (impl, impl, None)
-            assert (one == "read") == (dtype == F32 or D == 96 or impl == "read")
-            check(out, q, meta, table, k, v, layout, nkv, page, window, D ** -0.5, lambda e: (one if layout[e][1] == 1 else several) == "read")
+            form = impl or cache_quant._plan(out, q, pages, meta, meta.block_tables[0], nq)[0]
+            assert (form == "read") == (dtype == F32 or D == 96 or impl == "read")
+            check(out, q, meta, table, k, v, layout, nkv, page, window, D ** -0.5, lambda e: form == "read")
             again, _ = attend(pages, meta, q, nq, D ** -0.5, window, impl=impl)
             assert torch.equal(out, again)                 # no sum depends on which block ends first

@@ -49,7 +49,7 @@ def test_prompts_of_large_and_small_numbers(bits, D, k_power, v_power, q_power):
     v[:, 1] *= 2.0 ** -9
     q = queries(meta, nq, D, 1)
     scale = D ** -0.5 * 2.0 ** (-k_power - q_power)
-    out, st = attend(pages, meta, q * 2.0 ** q_power, nq, scale)
+    out, st = attend(pages, meta, q * 2.0 ** q_power, nq, scale, impl="portion")
     assert st.tolist() == [0] * 4
     # (single tokens: the kernel over codes, see check)
     check(out.float() * 2.0 ** -v_power, q, meta, table, k, v, layout, nkv, page, None, D ** -0.5, lambda e: False,
@@ -63,7 +63,7 @@ def test_loud_queries_see_the_keys_as_they_are(bits):
     meta, table, n_pages = step(layout, page, 1)
     pages, k, v = random_pages(n_pages, nkv, page, D, bits, 1)
     q = 4 * queries(meta, nq, D, 1)
-    for impl in (None, "direct"):
+    for impl in ("portion", "direct"):
         out, st = attend(pages, meta, q, nq, D ** -0.5, impl=impl)
         check(out, q, meta, table, k, v, layout, nkv, page, None, D ** -0.5, lambda e: False)
 
@@ -77,6 +77,8 @@ def test_attention_of_other_scales(scale, impl):
     q = queries(meta, nq, D, 1)
     out, st = attend(pages, meta, q, nq, scale, 50, impl=impl)
     check(out, q, meta, table, k, v, layout, nkv, page, 50, scale, lambda e: impl == "read")
+    with pytest.raises(KernelError):                        # (its maximum is that of the scores before the scale)
+        attend(pages, meta, q, nq, scale, impl="portion")
 
 
 # ------------------------------------------------------------------ how rows are shared
@@ -97,9 +99,8 @@ def test_rows_that_blocks_share(D, nq, nkv, bits, entries, longest, window):
 
 
 # ------------------------------------------------------------------ what no token sees
-@pytest.mark.parametrize("page", [16, 5])
 @pytest.mark.parametrize("bits", [4, 8])
-@pytest.mark.parametrize("impl", ["direct", "read", None])
+@pytest.mark.parametrize("impl,page", [("direct", 16), ("direct", 5), ("read", 16), ("read", 5), ("portion", 16)])
 def test_rows_that_no_token_sees_may_hold_anything(impl, bits, page):
     """Slots behind the last token, pages of nobody and pages before the window (which need not be mapped); rows of the result behind
     the last token stay."""
@@ -238,15 +239,28 @@ def test_a_captured_prompt():
     meta, table, n_pages = step(layout, page, 3)
     pages, k, v = random_pages(n_pages, nkv, page, D, 4, 3)
     q = queries(meta, nq, D, 3)
-    want, st = attend(pages, meta, q, nq, D ** -0.5)
+    want, st = attend(pages, meta, q, nq, D ** -0.5, impl="portion")
     out, st = torch.zeros_like(want), status()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        K.attention_quantized(out, q, pages, meta, meta.block_tables[0], nq, D ** -0.5, None, st)
+        K.attention_quantized(out, q, pages, meta, meta.block_tables[0], nq, D ** -0.5, None, st, impl="portion")
     for _ in range(2):
         out.zero_()
         graph.replay()
         assert torch.equal(out, want) and st.tolist() == [0] * 4
+
+
+def test_long_portions_choose_the_prompt_kernel():
+    """Where reading back pays, portions go that way by themselves; a few tokens and small steps stay on the codes."""
+    from kipp_b200.kernels.cache_quant import _plan
+    for layout, form in (([(100, 128), (0, 70), (50, 1)], "portion"), ([(100, 64)], "direct"), ([(9, 4)] * 30, "direct")):
+        nq, nkv, D, page = 32, 2, 64, 16
+        meta, table, n_pages = step(layout, page, 3)
+        pages, k, v = random_pages(n_pages, nkv, page, D, 8, 3)
+        q = queries(meta, nq, D, 3)
+        assert _plan(q, q, pages, meta, meta.block_tables[0], nq, 1.0)[1] == form
+        out, st = attend(pages, meta, q, nq, D ** -0.5)
+        check(out, q, meta, table, k, v, layout, nkv, page, None, D ** -0.5, lambda e: False)
 
 
 # ------------------------------------------------------------------ sizes

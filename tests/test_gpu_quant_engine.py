@@ -96,6 +96,23 @@ def test_batches_bursts_and_graphs(name, kv_quant):
     eng.cache.check()
 
 
+@pytest.mark.parametrize("kv_quant", ["int8", "int4"])
+def test_long_portions(kv_quant):
+    """Two prompts long enough for the prompt kernel over pages that are read back, beside a decoded token; then a long portion behind
+    what is cached.  (The bound of test_engine_in_bfloat16.)"""
+    eng = engine("E", kv_quant, "bfloat16", max_batch_tokens=1024)
+    texts = {r: random_tokens("E", n, seed=30 + i) for i, (r, n) in enumerate((("a", 900), ("b", 330), ("c", 9)))}
+    eng.step([StepEntry("c", texts["c"][:8], [])], check=True)
+    eng.profile_start()
+    out = eng.step([StepEntry("c", texts["c"][8:], [0]), StepEntry("a", texts["a"][:300], list(range(300))),
+                    StepEntry("b", texts["b"], list(range(330)))], check=True).double().cpu()
+    late = eng.step([StepEntry("a", texts["a"][300:], list(range(600)))], check=True).double().cpu()
+    assert "attn_prefill_tc" in eng.profile_stop()
+    for got, r, cut in ((out[:1], "c", slice(8, 9)), (out[1:301], "a", slice(0, 300)), (out[301:], "b", slice(0, 330)), (late, "a", slice(300, 900))):
+        want, unrounded = (x[cut] for x in (plain("E", "bfloat16", texts[r], BITS[kv_quant]), plain_logits("E", "bfloat16", texts[r]).double()))
+        assert nmse(got, want) <= 1e-4 + 0.5 * nmse(unrounded, want), r
+
+
 def test_pages_are_reused():
     """A request on pages that others left gives what it gives on fresh ones, bit for bit, a truncated one goes on from where it was cut."""
     eng = engine("E", "int4", "bfloat16", cache_tokens=160)
