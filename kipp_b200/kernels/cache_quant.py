@@ -57,6 +57,9 @@ class QuantizedPages:
         return cls(codes(), scales(), codes(), scales(), bits)
 
 
+_current_device, _current_stream, _I32 = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.int32
+
+
 def _launch_stream(what: str, device: int, *tensors: torch.Tensor) -> int:
     """The current stream; every tensor must lie on the current device, where a launch goes whatever the tensors' own."""
     if device < 0:
@@ -64,20 +67,19 @@ def _launch_stream(what: str, device: int, *tensors: torch.Tensor) -> int:
     for t in tensors:
         if t.get_device() != device:
             raise KernelError(f"{what}: the tensors are on several devices")
-    if device != torch._C._cuda_getDevice():
-        raise KernelError(f"{what}: the tensors are on cuda:{device} and the current device is cuda:{torch._C._cuda_getDevice()}")
-    return torch._C._cuda_getCurrentRawStream(device)
+    if device != _current_device():
+        raise KernelError(f"{what}: the tensors are on cuda:{device} and the current device is cuda:{_current_device()}")
+    return _current_stream(device)
 
 
 def _status(status: torch.Tensor, what: str) -> None:
-    if status.dtype != torch.int32 or status.numel() < 4 or not status.is_contiguous():
+    if status.dtype is not _I32 or status.numel() < 4 or not status.is_contiguous():
         raise KernelError(f"{what}: status must be a contiguous int32 tensor of 4 words")
 
 
 def _lists(what: str, names: str, *tensors: torch.Tensor) -> None:
-    i32 = torch.int32
     for t in tensors:
-        if t.dtype != i32 or not t.is_contiguous():
+        if t.dtype is not _I32 or not t.is_contiguous():
             raise KernelError(f"{what}: {names} must be contiguous int32 tensors")
 
 
@@ -247,22 +249,25 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
     "direct" or "read" for the whole step, "portion" (long portions') for every entry of more than one token."""
     what, D, n_kv, q_lens, tokens = "attention_quantized", pages.head_dim, pages.n_kv, meta.q_lens, meta.tokens
     window = int(window or 0)
-    dtype_code(q.dtype)
-    shape, entries = q.shape, len(q_lens)
-    if len(shape) != 3 or shape[1] != n_q or shape[2] != D or shape[0] < tokens or n_q % n_kv or not q.is_contiguous():
+    shape, entries, dtype = q.shape, len(q_lens), q.dtype
+    dtype_code(dtype)
+    if len(shape) != 3:
+        raise KernelError(f"{what}: q must be [tokens, n_q, head_dim]")
+    rows, heads, dims = shape
+    if heads != n_q or dims != D or rows < tokens or n_q % n_kv or not q.is_contiguous():
         raise KernelError(f"{what}: q must be contiguous [tokens, n_q, head_dim] with n_q a multiple of the cache's heads")
-    if out.dtype != q.dtype or out.shape != shape or not out.is_contiguous():
+    if out.dtype is not dtype or out.shape != shape or not out.is_contiguous():
         raise KernelError(f"{what}: out must be contiguous, of q's dtype and shape")
     if not 0 <= window < 1 << 31:
         raise KernelError(f"{what}: a window of {window} tokens")
-    t_shape = block_table.shape
+    t_shape, q_start, context_len = block_table.shape, meta.q_start, meta.context_len
     if len(t_shape) != 2 or t_shape[0] < entries or t_shape[1] == 0 or sum(q_lens) != tokens:
         raise KernelError(f"{what}: a row of block_table for every entry, and as many tokens as the entries bring")
-    _lists(what, "block_table, q_start and context_len", block_table, meta.q_start, meta.context_len)
-    if meta.q_start.numel() <= entries or meta.context_len.numel() < entries:
+    _lists(what, "block_table, q_start and context_len", block_table, q_start, context_len)
+    if q_start.numel() <= entries or context_len.numel() < entries:
         raise KernelError(f"{what}: the step's lists are shorter than the step")
     _status(status, what)
-    stream = _launch_stream(what, pages.device_index, q, out, block_table, meta.q_start, meta.context_len, status)
+    stream = _launch_stream(what, pages.device_index, q, out, block_table, q_start, context_len, status)
     if tokens == 0:
         return
     if impl is None:
@@ -296,7 +301,8 @@ def _direct(out, q, pages, meta, block_table, n_q, scale, window, status, most: 
     need = _scratch_bytes.get(key)
     if need is None:
         need = _scratch_bytes[key] = _fn("attention_quant", "kipp_attn_quant_scratch_bytes", [c_int, c_ll], restype=c_ll)(*key)
-    scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    # (a block of the caching allocator's, of q's type: new_empty is its cheapest way there)
+    scratch = q.new_empty((need + 1) // 2) if need else None
     _call("attention_quant", "kipp_attn_quant",
           _ATTEND.pack(out.data_ptr(), q.data_ptr(), *pages.addresses, meta.q_start.data_ptr(), meta.context_len.data_ptr(),
                        block_table.data_ptr(), scratch.data_ptr() if need else 0, status.data_ptr(), stream, need, pages.bits, pages.n_pages,
