@@ -22,10 +22,16 @@
 // register operand, and a warp that serves the few queries of a kv head (the heads of its group times
 // the tokens) wastes fewer columns.  P^T turns from result to operand by movmatrix.
 //
-// What bounds it: at 4 bits a warp executes some 550 instructions for 32 keys of 128 channels, 270 of them on the integer
-// pipe (which takes a warp's in two cycles), and a lone warp needs 2,500 cycles for them; with three warps a scheduler issue is
-// half busy and the integer pipe too, and keys and values come at 4.7 to 5.1 TB/s (8 tokens behind 8,100 keys, 32 query and 8 key
-// heads: 24.9 us with the joining of the parts, 75 MB).  At 8 bits it is the memory, 6.0 TB/s (64 tokens behind 2,048: 57.4 us, 287 MB).
+// Up to four columns in 4 bits (the tokens of a decode step): a word of codes has a run of one group in its low half and of the next in its
+// high half, and the two would have to be brought together with another word's before they can share a product.  Instead the
+// four columns stand twice among the eight, with the first group's queries (weights) in one half of the inner dimension and the
+// second's in the other, zeros elsewhere: a word is used as it is, both groups' sums come out of one product, and the accumulators
+// are half as many.
+//
+// What bounds it: at 4 bits a warp executes some 500 instructions for 32 keys of 128 channels, 230 of them on the integer
+// pipe (which takes a warp's in two cycles), and a lone warp needs over 2,000 cycles for them; with three warps a scheduler issue is
+// half busy and the integer pipe too, and keys and values come at some 5 TB/s (8 tokens behind 8,100 keys, 32 query and 8 key
+// heads: 23.2 us with the joining of the parts, 75 MB).  At 8 bits it is the memory, 6.0 TB/s (64 tokens behind 2,048: 57.4 us, 287 MB).
 // Each warp works on its own 32 keys of a step of 128 with its own maximum, fetches its own rows, and meets the other three
 // warps only at the end of a piece.  A maximum is raised only when a score passes it by 2^8.
 //
@@ -195,12 +201,14 @@ template <int D, int BITS> struct Shape {
     static constexpr int K_BYTES = RB / 4, V_BYTES = RB / 8; // a lane's stretch of a key's row and of a value's
     static constexpr int WARP_STAGE = WARP_KEYS * 2 * (RB + SB);
     // Steps in the ring, and CTAs an SM (ctas_per_sm).  Heads of 128: three CTAs of 168 registers a thread and four steps (4 bits,
-    // 8 tokens of 8,100 keys 26.1 us; four CTAs of 128 registers and three steps 28.5).  A step's scores made beside the one before's
+    // 8 tokens of 8,100 keys in 8 columns 26.1 us, in 4 23.2; four CTAs of 128 registers and three steps 28.5 and 23.5).  A step's scores made beside the one before's
     // values, two streams of instructions, gave nothing (26.1).
     static constexpr int STAGES = RB == 128 && D == 128 ? 2 : D == 256 ? 3 : 4;
     static constexpr float L = BITS == 4 ? 8.f : 128.f;
 };
-template <int D, int NT> constexpr int q_bytes() { return NT * (D / 32) * 32 * 24; }          // the queries of a piece as operands
+// NT: tiles of 8 columns, or 0: four columns (4 bits only), each of them twice, for the two groups whose runs share a word.
+constexpr int columns_of_tiles(int nt) { return nt == 0 ? 4 : 8 * nt; }
+template <int D, int NT> constexpr int q_bytes() { return NT == 0 ? (D / 64) * 32 * 40 : NT * (D / 32) * 32 * 24; }  // a piece's queries as operands
 template <int D, int BITS, int NT> constexpr bool q_in_ring() { return q_bytes<D, NT>() <= Shape<D, BITS>::WARP_STAGE; }
 template <int D, int BITS, int NT> constexpr int ctas_per_sm() {
     return D == 256 ? (BITS == 4 ? 2 : 1) : NT == 2 ? (D == 64 ? 3 : 2) : D == 128 ? 3 : 4;
@@ -221,6 +229,11 @@ template <int BITS> __device__ __forceinline__ void spread_keys(uint32_t (&x)[4]
         x[0] = first & 0x00ff00ffu; x[1] = __byte_perm(first, 0u, 0x4341); x[2] = second & 0x00ff00ffu; x[3] = __byte_perm(second, 0u, 0x4341);
     }
 }
+// A word of 4-bit codes, a run of two groups: code i of the first group's in the low half of x[i], of the second's in the high half.
+__device__ __forceinline__ void spread_word(uint32_t (&x)[4], uint32_t w) {
+    const uint32_t u = w >> 8;
+    x[0] = w & 0x000f000fu; x[1] = w & 0x00f000f0u; x[2] = u & 0x000f000fu; x[3] = u & 0x00f000f0u;
+}
 // A run of two values, the first one's codes in the low halves.  (4 bits: x[0] and x[2] could keep both codes of a byte and the even
 // channels' sums be made as differences at the end, an instruction in six less and 2 % of the time; but they would then not
 // cancel exactly where every value is 0.)
@@ -237,7 +250,10 @@ template <int BITS> __device__ __forceinline__ void spread_values(uint32_t (&x)[
 template <int D, int BITS, int NT, bool TILES>
 __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quant_kernel(const Params p) {
     using S = Shape<D, BITS>;
-    constexpr int G = S::G, RB = S::RB, SB = S::SB, COLS = 8 * NT, WO = D + 4, STAGES = S::STAGES;
+    constexpr int G = S::G, RB = S::RB, SB = S::SB, COLS = columns_of_tiles(NT), WO = D + 4, STAGES = S::STAGES;
+    constexpr bool FOUR = NT == 0;
+    constexpr int T = FOUR ? 1 : NT, PAIRS = G / 2, SETS = FOUR ? PAIRS : G;       // operand sets: a pair of groups, or a group
+    static_assert(!FOUR || BITS == 4, "two groups share a word in 4 bits only");
     constexpr int RING = WARPS * STAGES * S::WARP_STAGE;
     constexpr bool Q_IN_RING = q_in_ring<D, BITS, NT>();
     extern __shared__ __align__(128) uint8_t smem[];
@@ -351,15 +367,15 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
         };
         look_up(0);
         // -- the queries are asked for first: a warp makes operands of every fourth group's
-        constexpr int MINE = (NT * G + WARPS - 1) / WARPS;
+        constexpr int MINE = (T * SETS + WARPS - 1) / WARPS;
         uint2 q_raw[MINE][2];
 #pragma unroll
         for (int i = 0; i < MINE; ++i) {
-            const int k = warp + i * WARPS, c = column0 + k / G * 8 + g4;
+            const int k = warp + i * WARPS, c = column0 + (FOUR ? g4 & 3 : k / G * 8 + g4);
             q_raw[i][0] = q_raw[i][1] = make_uint2(0u, 0u);
-            if (k < NT * G && c < columns) {
-                const int tok = c / group;
-                const bf16* src = p.q + ((size_t)(qs + tok) * p.n_q + g * group + (c - tok * group)) * D + t4 * (D / 4) + 4 * (k % G);
+            if (k < T * SETS && c < columns) {
+                const int tok = c / group, run = FOUR ? 2 * k + (g4 >> 2) : k % G;
+                const bf16* src = p.q + ((size_t)(qs + tok) * p.n_q + g * group + (c - tok * group)) * D + t4 * (D / 4) + 4 * run;
                 q_raw[i][0] = *reinterpret_cast<const uint2*>(src);
                 q_raw[i][1] = *reinterpret_cast<const uint2*>(src + 4 * G);
             }
@@ -372,17 +388,33 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
 
         // -- as operands, with what the offset of their codes comes to (through the first warp's free stage, where they have room)
         uint4* const q_operands = reinterpret_cast<uint4*>(Q_IN_RING ? smem + (stage + STAGES - 1) % STAGES * S::WARP_STAGE : smem + RING);
-        float2* const q_offsets = reinterpret_cast<float2*>(q_operands + NT * G * 32);
+        float2* const q_offsets = reinterpret_cast<float2*>(q_operands + (FOUR ? 2 * PAIRS : NT * G) * 32);
 #pragma unroll
         for (int i = 0; i < MINE; ++i) {
             const int k = warp + i * WARPS;
-            if (k >= NT * G) break;
+            if (k >= T * SETS) break;
             const uint2 a = q_raw[i][0], b = q_raw[i][1];
             float sum = (low_f32(a.x) + high_f32(a.x)) + (low_f32(a.y) + high_f32(a.y)) + (low_f32(b.x) + high_f32(b.x)) + (low_f32(b.y) + high_f32(b.y));
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             sum *= -S::L * 0x1p-133f * p.query_scale;
             q_offsets[k * 32 + lane] = make_float2(__shfl_sync(0xffffffffu, sum, 8 * t4), __shfl_sync(0xffffffffu, sum, 8 * t4 + 4));
+            if constexpr (FOUR) {
+                // code 0 .. 3 of the lane's run, in the half of the register that the run's codes come in
+                const uint2 run[2] = {a, b};
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint32_t pair = c < 2 ? run[n].x : run[n].y;
+                        const float f = (c & 1 ? high_f32(pair) * 0.0625f : low_f32(pair)) * p.query_scale;
+                        w[c] = g4 < 4 ? pack2(f, 0.f) : pack2(0.f, f);
+                    }
+                    q_operands[(2 * k + n) * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                continue;
+            }
             const uint32_t mid = BITS == 4 ? b.x : a.y, last = BITS == 4 ? a.y : b.x;              // (as spread_keys pairs the codes)
             const uint32_t raw[4] = {__byte_perm(a.x, mid, 0x5410), __byte_perm(a.x, mid, 0x7632), __byte_perm(last, b.y, 0x5410),
                                      __byte_perm(last, b.y, 0x7632)};
@@ -395,24 +427,28 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             q_operands[k * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
         }
         __syncthreads();
-        uint32_t qf[NT][G][4];
-        float offset[NT][G][2];
+        uint32_t qf[T][G][4];
+        float offset[T][SETS][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < T; ++nt) {
 #pragma unroll
             for (int gi = 0; gi < G; ++gi) {
                 const uint4 w = q_operands[(nt * G + gi) * 32 + lane];
-                const float2 f = q_offsets[(nt * G + gi) * 32 + lane];
                 qf[nt][gi][0] = w.x; qf[nt][gi][1] = w.y; qf[nt][gi][2] = w.z; qf[nt][gi][3] = w.w;
-                offset[nt][gi][0] = f.x; offset[nt][gi][1] = f.y;
             }
+#pragma unroll
+            for (int k = 0; k < SETS; ++k) {
+                const float2 f = q_offsets[(nt * SETS + k) * 32 + lane];
+                offset[nt][k][0] = f.x; offset[nt][k][1] = f.y;
+            }
+        }
         if constexpr (Q_IN_RING) __syncthreads();
 
-        float o[NT][2 * G][4], ones[NT][4], m[NT][2], l[NT][2];
+        float o[T][2 * SETS][4], ones[T][4], m[T][2], l[T][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int nt = 0; nt < T; ++nt) {
 #pragma unroll
-            for (int i = 0; i < 2 * G; ++i)
+            for (int i = 0; i < 2 * SETS; ++i)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) o[nt][i][k] = 0.f;
 #pragma unroll
@@ -421,8 +457,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             l[nt][0] = l[nt][1] = 0.f;
         }
 
-        float s[NT][2][4];                                     // scores of a step, to be multiplied by score_scale for units of log2
-        uint32_t w[NT][2][2];                                  // its weights as operands
+        float s[T][2][4];                                     // scores of a step, to be multiplied by score_scale for units of log2
+        uint32_t w[T][2][2];                                  // its weights as operands
         // The rows of a step that no column sees may hold anything: their scales become 0 (their codes are numbers anyhow).
         auto arrived = [&](int j0, uint8_t* tile) {
             const int j = j0 + lane;
@@ -446,7 +482,33 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                 take<SB>(a0, tile + KS_AT + (mt * 16 + key_of_row(g4)) * SB);
                 take<SB>(a1, tile + KS_AT + (mt * 16 + key_of_row(g4) + 8) * SB);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.f;
+                for (int nt = 0; nt < T; ++nt) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.f;
+                if constexpr (FOUR) {
+                    const uint32_t half = t4 < 2 ? 0x1044 : 0x3244;        // this lane's columns are of the first or the second group
+#pragma unroll
+                    for (int k = 0; k < PAIRS; ++k) {
+                        float c[4];
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            const int at = k + n * PAIRS;
+                            uint32_t x0[4], x1[4];
+                            spread_word(x0, w0[at]);
+                            spread_word(x1, w1[at]);
+                            if (n == 0) mma(c, x0[0], x1[0], x0[1], x1[1], qf[0][2 * k][0], qf[0][2 * k][1], offset[0][k][0], offset[0][k][1],
+                                            offset[0][k][0], offset[0][k][1]);
+                            else mma(c, x0[0], x1[0], x0[1], x1[1], qf[0][2 * k + 1][0], qf[0][2 * k + 1][1]);
+                            mma(c, x0[2], x1[2], x0[3], x1[3], qf[0][2 * k + n][2], qf[0][2 * k + n][3]);
+                        }
+                        const float f0 = __uint_as_float(__byte_perm(a0[k], 0u, half)), f1 = __uint_as_float(__byte_perm(a1[k], 0u, half));
+                        s[0][mt][0] = fmaf(f0, c[0], s[0][mt][0]);
+                        s[0][mt][1] = fmaf(f0, c[1], s[0][mt][1]);
+                        s[0][mt][2] = fmaf(f1, c[2], s[0][mt][2]);
+                        s[0][mt][3] = fmaf(f1, c[3], s[0][mt][3]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[0][mt][k] += __shfl_xor_sync(0xffffffffu, s[0][mt][k], 2);
+                    continue;
+                }
 #pragma unroll
                 for (int gi = 0; gi < G; ++gi) {
                     uint32_t x0[4], x1[4];
@@ -456,7 +518,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                     const float f0 = gi & 1 ? high_f32(a0[gi >> 1]) : low_f32(a0[gi >> 1]);
                     const float f1 = gi & 1 ? high_f32(a1[gi >> 1]) : low_f32(a1[gi >> 1]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
+                    for (int nt = 0; nt < T; ++nt) {
                         float c[4];
                         mma(c, x0[0], x1[0], x0[1], x1[1], qf[nt][gi][0], qf[nt][gi][1], offset[nt][gi][0], offset[nt][gi][1],
                             offset[nt][gi][0], offset[nt][gi][1]);
@@ -471,13 +533,13 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
         };
         auto weights = [&](int j0, bool cut) {
             bool raise = false;
-            float top[NT][2];
+            float top[T][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+            for (int nt = 0; nt < T; ++nt) {
                 if (cut) {
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        const int pos = en.context + min(column0 + nt * 8 + 2 * t4 + c, columns - 1) / group;
+                        const int pos = en.context + min(column0 + (FOUR ? (2 * t4 + c) & 3 : nt * 8 + 2 * t4 + c), columns - 1) / group;
                         const int hi = min(pos, see_hi), lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
 #pragma unroll
                         for (int mt = 0; mt < 2; ++mt)
@@ -496,7 +558,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             }
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
+                for (int nt = 0; nt < T; ++nt) {
                     float f[2];
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
@@ -512,13 +574,13 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                     for (int k = 0; k < 4; ++k) {
                         ones[nt][k] *= f[k & 1];
 #pragma unroll
-                        for (int d = 0; d < 2 * G; ++d) o[nt][d][k] *= f[k & 1];
+                        for (int d = 0; d < 2 * SETS; ++d) o[nt][d][k] *= f[k & 1];
                     }
                 }
             }
             // (times 2^48)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+            for (int nt = 0; nt < T; ++nt) {
                 const float back[2] = {(m[nt][0] == -INFINITY ? 0.f : m[nt][0]) - 48.f, (m[nt][1] == -INFINITY ? 0.f : m[nt][1]) - 48.f};
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt) {
@@ -542,6 +604,27 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                     take<S::V_BYTES>(v[k], tile + V_AT + (mt * 16 + 4 * k + t4) * RB + g4 * S::V_BYTES);
                     take<SB>(f[k], tile + VS_AT + (mt * 16 + 4 * k + t4) * SB);
                 }
+                if constexpr (FOUR) {
+                    // a key's weight in the low half for the first group's columns, in the high half for the second's
+                    const uint32_t even = g4 < 4 ? 0x4410 : 0x1044, odd = g4 < 4 ? 0x4432 : 0x3244;
+                    const uint32_t one_key[4] = {__byte_perm(w[0][mt][0], 0u, even), __byte_perm(w[0][mt][0], 0u, odd),
+                                                 __byte_perm(w[0][mt][1], 0u, even), __byte_perm(w[0][mt][1], 0u, odd)};
+#pragma unroll
+                    for (int k = 0; k < PAIRS; ++k) {
+                        const uint32_t one = g4 == k ? 0x3f803f80u : 0u;
+#pragma unroll
+                        for (int n = 0; n < 4; n += 2) {
+                            uint32_t x0[4], x1[4];
+                            spread_word(x0, v[n][k]);
+                            spread_word(x1, v[n + 1][k]);
+                            const uint32_t b0 = times2(one_key[n], f[n][k]), b1 = times2(one_key[n + 1], f[n + 1][k]);
+                            mma(o[0][2 * k], x0[0], x0[1], x1[0], x1[1], b0, b1);
+                            mma(o[0][2 * k + 1], x0[2], x0[3], x1[2], x1[3], b0, b1);
+                            mma(ones[0], one, 0u, one, 0u, b0, b1);
+                        }
+                    }
+                    continue;
+                }
 #pragma unroll
                 for (int gi = 0; gi < G; ++gi) {
                     uint32_t x0[4], x1[4];                             // keys of the first and the second half of the rows
@@ -552,7 +635,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                     const uint32_t f1 = __byte_perm(f[2][gi >> 1], f[3][gi >> 1], gi & 1 ? 0x7632 : 0x5410);
                     const uint32_t one = g4 == gi ? 0x3f803f80u : 0u;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
+                    for (int nt = 0; nt < T; ++nt) {
                         const uint32_t b0 = times2(w[nt][mt][0], f0), b1 = times2(w[nt][mt][1], f1);
                         mma(o[nt][2 * gi], x0[0], x0[1], x1[0], x1[1], b0, b1);
                         mma(o[nt][2 * gi + 1], x0[2], x0[3], x1[2], x1[3], b0, b1);
@@ -587,21 +670,21 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
         float* w_l = w_m + WARPS * COLS;                               // [WARPS][COLS]
         float* w_o = w_l + WARPS * COLS;                               // [WARPS][COLS][WO]
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int nt = 0; nt < T; ++nt) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float sum = l[nt][c];
                 sum += __shfl_xor_sync(0xffffffffu, sum, 4);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 8);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-                const int col = nt * 8 + 2 * t4 + c;
+                const int col = FOUR ? (2 * t4 + c) & 3 : nt * 8 + 2 * t4 + c;
                 if (g4 == 0) {
                     w_m[warp * COLS + col] = m[nt][c];
                     w_l[warp * COLS + col] = sum * 0x1p-48f;
                 }
             }
 #pragma unroll
-            for (int gi = 0; gi < G; ++gi) {
+            for (int gi = 0; gi < SETS; ++gi) {
                 // (row gi of the product with ones lies with lane 4 gi + t)
                 const float less[2] = {__shfl_sync(0xffffffffu, ones[nt][0], 4 * gi + t4) * (S::L * 0x1p-48f),
                                        __shfl_sync(0xffffffffu, ones[nt][1], 4 * gi + t4) * (S::L * 0x1p-48f)};
@@ -613,7 +696,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
                     r.y = fmaf(o[nt][2 * gi][2 + c], ODD, -less[c]);
                     r.z = fmaf(o[nt][2 * gi + 1][c], EVEN, -less[c]);
                     r.w = fmaf(o[nt][2 * gi + 1][2 + c], ODD, -less[c]);
-                    *reinterpret_cast<float4*>(w_o + (size_t)(warp * COLS + nt * 8 + 2 * t4 + c) * WO + g4 * (D / 8) + 4 * gi) = r;
+                    const int col = FOUR ? (2 * t4 + c) & 3 : nt * 8 + 2 * t4 + c, run = FOUR ? 2 * gi + (t4 >> 1) : gi;
+                    *reinterpret_cast<float4*>(w_o + (size_t)(warp * COLS + col) * WO + g4 * (D / 8) + 4 * run) = r;
                 }
             }
         }
@@ -710,7 +794,7 @@ template <int D> __device__ __forceinline__ bf16* result_of(const Params& p, int
 constexpr int JOIN_WARPS = 4;
 template <int D, int NT>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_quant_join_kernel(const Params p) {
-    constexpr int COLS = 8 * NT;
+    constexpr int COLS = columns_of_tiles(NT);
     pdl_wait();
     const int4 row = p.shared[blockIdx.x], cut = p.shared[p.ctas];
     const int e = row.x, lane = threadIdx.x & 31;
@@ -736,7 +820,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_quant_join_kernel(const 
 // 26.5 with the kernel above; 64 of 2,048, 512 rows on 444 CTAs: 46.7 and 44.9.)
 template <int D, int NT, int MERGE_WARPS>
 __global__ void __launch_bounds__(MERGE_WARPS * 32) attn_quant_merge_kernel(const Params p) {
-    constexpr int COLS = 8 * NT;
+    constexpr int COLS = columns_of_tiles(NT);
     __shared__ float sh_o[MERGE_WARPS][D], sh_l[MERGE_WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y, e = blockIdx.x / p.most_blocks, block = blockIdx.x - e * p.most_blocks;
     // (every warp for itself, from the step's lists)
@@ -776,7 +860,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) attn_quant_merge_kernel(cons
 
 template <int D, int BITS, int NT> constexpr size_t smem_bytes() {
     using S = Shape<D, BITS>;
-    constexpr size_t ring = (size_t)WARPS * S::STAGES * S::WARP_STAGE, merge = (size_t)WARPS * 8 * NT * (D + 4 + 2) * 4;
+    constexpr size_t ring = (size_t)WARPS * S::STAGES * S::WARP_STAGE, merge = (size_t)WARPS * columns_of_tiles(NT) * (D + 4 + 2) * 4;
     constexpr size_t all = ring + (q_in_ring<D, BITS, NT>() ? 0 : q_bytes<D, NT>());
     return all > merge ? all : merge;
 }
@@ -797,7 +881,7 @@ template <int D, int BITS, int NT, bool TILES> int wave() {
 }
 template <int D, int BITS, int NT, bool TILES> int launch(Params p, long long steps_of_row, cudaStream_t s) {
     constexpr size_t smem = smem_bytes<D, BITS, NT>();
-    constexpr int COLS = 8 * NT;
+    constexpr int COLS = columns_of_tiles(NT);
     const int wave_ctas = wave<D, BITS, NT, TILES>();
     const long long rows = (long long)p.entries * p.most_blocks, units = rows * (steps_of_row + ROW_COST);
     p.ctas = (int)(units < wave_ctas ? units : wave_ctas);
@@ -815,9 +899,10 @@ template <int D, int BITS, int NT, bool TILES> int launch(Params p, long long st
     return kipp_launch(attn_quant_merge_kernel<D, NT, 4>, grid, dim3(128), 0, s, 1, p);
 }
 
-// 8 columns where they hold every query of a kv head (8 tokens behind 8,100 keys, 4 queries each: 25.2 us, 31.7 with 16), else 16 (12
+// 4 columns where they hold every query of a kv head in 4 bits (8 tokens behind 8,100 keys, 4 queries each: 23.2 us, with 8 columns 24.9, with
+// 16 31.7), 8 where those do, else 16 (12
 // queries: 35.5 us, 42.3 with 8); heads of 256 have no room for their sums: always 8
-int columns_of(int head_dim, long long queries) { return head_dim == 256 || queries <= 8 ? 8 : 16; }
+int columns_of(int bits, int head_dim, long long queries) { return bits == 4 && queries <= 4 ? 4 : head_dim == 256 || queries <= 8 ? 8 : 16; }
 }  // namespace
 
 // Whether the kernel takes these heads.
@@ -855,7 +940,7 @@ extern "C" int kipp_attn_quant(const KippAttnQuant* a) {
           (uintptr_t)a->scratch) & 15) != 0)
         return -3;
     // (row numbers of pages and steps of all rows are 32-bit)
-    const long long cols = columns_of(head_dim, (long long)most * (n_q / n_kv));
+    const long long cols = columns_of(bits, head_dim, (long long)most * (n_q / n_kv));
     const long long room = (long long)a->table_width * page_size, steps = (room + STEP - 1) / STEP;
     const long long blocks = n_kv * (((long long)most * (n_q / n_kv) + cols - 1) / cols);
     if ((long long)a->n_pages * n_kv * page_size > 0x7fffffffLL || room > 0x7fffffffLL ||
@@ -881,6 +966,8 @@ extern "C" int kipp_attn_quant(const KippAttnQuant* a) {
     cudaStream_t s = (cudaStream_t)a->stream;
 #define KIPP_CASE(d, b)                                                                                            \
     if (head_dim == d && bits == b) {                                                                              \
+        if constexpr (b == 4)                                                                                      \
+            if (cols == 4) return page_size % 16 == 0 ? launch<d, b, 0, true>(p, steps, s) : launch<d, b, 0, false>(p, steps, s);    \
         if (cols == 8) return page_size % 16 == 0 ? launch<d, b, 1, true>(p, steps, s) : launch<d, b, 1, false>(p, steps, s);        \
         if constexpr (d != 256) return page_size % 16 == 0 ? launch<d, b, 2, true>(p, steps, s) : launch<d, b, 2, false>(p, steps, s); \
     }
