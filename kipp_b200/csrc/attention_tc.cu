@@ -1014,7 +1014,8 @@ int pool_map(CUtensorMap* out, const void* ptr, long long rows, int cols, int bo
 int pool_map4(CUtensorMap* out, const void* ptr, int n_pages, int n_kv, int page_size, int cols, int pages_per_box) {
     static std::unordered_map<MapKey, CUtensorMap, MapHash> cache;
     static std::mutex mu;
-    MapKey key{ptr, (long long)n_pages * n_kv, cols, page_size * 1024 + pages_per_box};
+    // (pages and kv heads apart: pools of one address and as many rows may differ in both)
+    MapKey key{ptr, (long long)n_pages << 32 | n_kv, cols, page_size * 1024 + pages_per_box};
     std::lock_guard<std::mutex> lock(mu);
     auto it = cache.find(key);
     if (it != cache.end()) { *out = it->second; return 0; }

@@ -250,6 +250,29 @@ def test_a_captured_prompt():
         assert torch.equal(out, want) and st.tolist() == [0] * 4
 
 
+def test_portions_of_pools_of_one_size(monkeypatch):
+    """Pages read back for 4 heads of 4 pages, 2 of 8 and 1 of 16 are as many bytes, and may come to lie in the same memory (as here): how
+    they are fetched must not be that of another step."""
+    from kipp_b200.kernels import cache_quant
+    D, page = 128, 16
+    memory, read = torch.empty(2, 16 * page * D, dtype=BF16, device=DEV), cache_quant._read_entries
+
+    def read_there(*args):
+        pages = read(*args)
+        for there, got in zip(memory, pages):
+            there.copy_(got.flatten())
+        return tuple(there.view(got.shape) for there, got in zip(memory, pages))
+    monkeypatch.setattr(cache_quant, "_read_entries", read_there)
+    for nkv, slots in ((4, 4), (1, 16), (2, 8), (4, 4)):
+        layout = [(slots * page - 64, 64)]
+        meta, table, n_pages = step(layout, page, slots, spare=0)
+        pages, k, v = random_pages(n_pages, nkv, page, D, 8, slots)
+        q = queries(meta, 4, D, slots)
+        for _ in range(2):
+            out, st = attend(pages, meta, q, 4, D ** -0.5, impl="portion")
+            check(out, q, meta, table, k, v, layout, nkv, page, None, D ** -0.5, lambda e: False)
+
+
 def test_long_portions_choose_the_prompt_kernel():
     """Where reading back pays, portions go that way by themselves; a few tokens and small steps stay on the codes."""
     from kipp_b200.kernels.cache_quant import _plan
