@@ -104,7 +104,8 @@ def qk_norm_rope_write_quantized(qkv: torch.Tensor, q_out: torch.Tensor, pages: 
                                  cos_sin: Optional[torch.Tensor] = None) -> None:
     """Per-head RMSNorm of q and k, rotation, q to ``q_out`` [T, n_q, D], k and v as codes into ``pages`` through
     ``block_table`` [entries, width].  ``cos_sin`` is the step's ``rope_table``; without it the table is made here.
-    A position whose page is not mapped is not written: status word 0 becomes 2."""
+    A position whose page is not mapped is not written: status word 0 becomes 2.  Two tokens of a step must not have one place in the
+    cache."""
     what, D, n_kv = "qk_norm_rope_write_quantized", pages.head_dim, pages.n_kv
     shape, dtype, q_norm, k_norm, table, norm_dtype = qkv.shape, qkv.dtype, 0, 0, 0, 0
     if len(shape) != 2 or shape[1] != (n_q + 2 * n_kv) * D or shape[0] < tokens:
