@@ -98,6 +98,21 @@ def test_rows_that_blocks_share(D, nq, nkv, bits, entries, longest, window):
         check(out, q, meta, table, k, v, layout, nkv, page, window, D ** -0.5, lambda e: False)
 
 
+@pytest.mark.parametrize("page", [16, 6])
+@pytest.mark.parametrize("window", [None, 3, 130])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("group,tokens", [(1, 4), (1, 3), (2, 2), (3, 1), (4, 1), (5, 1), (1, 5)])
+def test_columns_of_several_tokens(group, tokens, D, window, page):
+    """Four columns and five of a kv head, of one token or of several, each with its own limits."""
+    nkv, layout = 2, [(126, tokens), (0, tokens), (1000, 1), (255, tokens), (31, 0)]
+    meta, table, n_pages = step(layout, page, 1)
+    pages, k, v = random_pages(n_pages, nkv, page, D, 4, 1)
+    q = queries(meta, nkv * group, D, 1)
+    out, st = attend(pages, meta, q, nkv * group, D ** -0.5, window, impl="direct")
+    assert st.tolist() == [0] * 4
+    check(out, q, meta, table, k, v, layout, nkv, page, window, D ** -0.5, lambda e: False)
+
+
 # ------------------------------------------------------------------ what no token sees
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("impl,page", [("direct", 16), ("direct", 5), ("read", 16), ("read", 5), ("portion", 16)])
