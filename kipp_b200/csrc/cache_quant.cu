@@ -529,8 +529,10 @@ template <bool ENTRIES> int launch_read(const ReadParams& p, int bits, int out_d
     const bool many = units >= 4 * READ_THREADS && units * p.n > 32LL * READ_THREADS * kipp_sm_count();
     const int per = READ_THREADS * (many ? 4 : 1);
     const unsigned x = (unsigned)((units + per - 1) / per);
-    auto kernel = out_dtype == KIPP_DT_F32 ? (bits == 4 ? read_kernel<float, 4, ENTRIES>(p.head_dim, many) : read_kernel<float, 8, ENTRIES>(p.head_dim, many))
-                                           : (bits == 4 ? read_kernel<bf16, 4, ENTRIES>(p.head_dim, many) : read_kernel<bf16, 8, ENTRIES>(p.head_dim, many));
+    // (the kernels of one head size take two scales as a word: scales at odd multiples of two bytes go to the one for any size)
+    const int dim = (((uintptr_t)p.pages.k_scales | (uintptr_t)p.pages.v_scales) & 3) == 0 ? p.head_dim : 0;
+    auto kernel = out_dtype == KIPP_DT_F32 ? (bits == 4 ? read_kernel<float, 4, ENTRIES>(dim, many) : read_kernel<float, 8, ENTRIES>(dim, many))
+                                           : (bits == 4 ? read_kernel<bf16, 4, ENTRIES>(dim, many) : read_kernel<bf16, 8, ENTRIES>(dim, many));
     if constexpr (ENTRIES) {
         if (p.factors != nullptr) {
             const bool wide = p.head_dim == 128;
