@@ -602,6 +602,7 @@ extern "C" int kipp_quant_cache_write(const KippQuantWrite* a) {
         a->rotary_dim > a->head_dim || (a->rotary_dim & 1) || a->table_width <= 0 || a->status == nullptr ||
         a->ld_qkv < (long long)(a->n_q + 2 * a->n_kv) * a->head_dim)
         return KIPP_ERR_ARG;
+    if (a->rotary_dim > 0 && ((uintptr_t)a->cos_sin & 7) != 0) return -3;              // (an angle's two numbers are one load)
     if ((a->dtype != KIPP_DT_F32 && a->dtype != KIPP_DT_BF16) || (a->norm_dtype != KIPP_DT_F32 && a->norm_dtype != KIPP_DT_BF16)) return KIPP_ERR_DTYPE;
     const WriteParams p = {a->qkv, a->ld_qkv, a->q_out, pages, a->q_norm_w, a->k_norm_w, a->norm_dtype, a->eps,
                            a->rotary_dim > 0 ? (const float2*)a->cos_sin : nullptr, a->rotary_dim, a->positions, a->entry_of_token,
