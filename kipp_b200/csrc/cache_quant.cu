@@ -458,8 +458,8 @@ template <int BITS> __device__ __forceinline__ void put_unit(float* p, const Uni
 }
 
 // One block per (share of a page, page); DIM is the head size, or 0 for any.  Every thread has UNROLL units of eight channels of keys
-// and of values on their way at once.  A page whose number is negative (unmapped) or past the pool becomes zeros; past the
-// pool is also reported.  Bound by HBM, three quarters and more of it writes (8 x 8,100 tokens of 8 heads of 128 from 4 bits: 62 us, 5.5 TB/s).
+// and of values on their way at once.  A listed page whose number is negative (unmapped) or past the pool becomes zeros; past the
+// pool is also reported, and of an entry's pages whatever is not there and some token sees.  Bound by HBM, three quarters and more of it writes (8 x 8,100 tokens of 8 heads of 128 from 4 bits: 62 us, 5.5 TB/s).
 constexpr int READ_THREADS = 256;
 template <typename T> struct IsHalf { static constexpr bool value = false; };
 template <> struct IsHalf<__half> { static constexpr bool value = true; };
@@ -474,8 +474,13 @@ __global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const ReadPara
     if constexpr (ENTRIES) {
         const int e = p.first_entry + i / p.table_width, slot = i % p.table_width;
         const int2 seen = seen_keys(p, e);
-        const bool used = page >= 0 && (long long)slot * p.pages.page_size < seen.y && (long long)(slot + 1) * p.pages.page_size > seen.x;
-        if (blockIdx.x == 0 && threadIdx.x == 0) p.table_out[(size_t)e * p.table_width + slot] = used ? i : -1;
+        const bool needed = (long long)slot * p.pages.page_size < seen.y && (long long)(slot + 1) * p.pages.page_size > seen.x, used = needed && page >= 0;
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            p.table_out[(size_t)e * p.table_width + slot] = used ? i : -1;
+            // (a page that a token sees and that is not mapped, and a table that ends before the last token: the prompt kernel
+            // takes both for zeros without a word)
+            if ((needed && !used) || (slot == 0 && seen.y > (long long)p.table_width * p.pages.page_size)) atomicExch(p.status, 3);
+        }
         if (!used) return;
         from = max(0, seen.x - slot * p.pages.page_size);
         to = min(p.pages.page_size, seen.y - slot * p.pages.page_size);
