@@ -321,12 +321,13 @@ struct ReadParams {
     int table_width, first_entry, window;
     int at;                         // what the launch begins with, a page's place in the list or among the entries'
     float2* factors;                // float16: [entries][n_kv], what keys and values are multiplied by
+    int least;                      // the entries of fewer tokens are left out
 };
 
-// The keys of entry e that its tokens see, [first, end): none where it brings no token.
+// The keys of entry e that its tokens see, [first, end): none where it is left out.
 __device__ __forceinline__ int2 seen_keys(const ReadParams& p, int e) {
     const int tokens = p.q_start[e + 1] - p.q_start[e], first = p.context_len[e];
-    if (tokens <= 0) return make_int2(0, 0);
+    if (tokens < p.least) return make_int2(0, 0);
     return make_int2(p.window > 0 ? max(0, first - p.window + 1) : 0, first + tokens);
 }
 
@@ -630,7 +631,7 @@ extern "C" int kipp_quant_cache_read(const KippQuantRead* a) {
         return KIPP_ERR_ARG;
     if (a->out_dtype != KIPP_DT_F32 && a->out_dtype != KIPP_DT_BF16) return KIPP_ERR_DTYPE;
     if (!read_aligned(pages, a->k_out, a->v_out)) return -3;
-    ReadParams p = {a->k_out, a->v_out, pages, a->list, a->n, a->head_dim, a->status, nullptr, nullptr, nullptr, 0, 0, 0, 0, nullptr};
+    ReadParams p = {a->k_out, a->v_out, pages, a->list, a->n, a->head_dim, a->status, nullptr, nullptr, nullptr, 0, 0, 0, 0, nullptr, 1};
     return launch_read<false>(p, a->bits, a->out_dtype, (cudaStream_t)a->stream);
 }
 
@@ -639,7 +640,8 @@ extern "C" int kipp_quant_cache_read(const KippQuantRead* a) {
 // step's shape and only those entries' rows are written.  The pages no token sees are neither read nor
 // written; their table entries are -1.  The slots that no token sees, of pages that some are seen of, become zeros: they may hold
 // anything, and the attention over the pages multiplies them by weights of 0.
-// With `factors` (heads of 64 and 128) the pages are float16, multiplied by the powers of two that it makes there.
+// With `factors` (heads of 64 and 128) the pages are float16, multiplied by the powers of two that it makes there, and the entries of one
+// token, which the kernel over codes serves, count as bringing none.
 extern "C" int kipp_quant_cache_read_entries(const KippQuantReadEntries* a) {
     if (a->entries <= 0) return 0;
     const QuantPages pages = {(uint8_t*)a->k_codes, (bf16*)a->k_scales, (uint8_t*)a->v_codes, (bf16*)a->v_scales, a->n_pages, a->page_size, a->n_kv};
@@ -652,6 +654,6 @@ extern "C" int kipp_quant_cache_read_entries(const KippQuantReadEntries* a) {
         (a->factors != nullptr && (((uintptr_t)a->k_scales | (uintptr_t)a->v_scales) & 3) != 0))
         return -3;
     ReadParams p = {a->k_out, a->v_out, pages, a->block_table, a->entries * a->table_width, a->head_dim, a->status, a->table_out, a->q_start,
-                    a->context_len, a->table_width, a->first_entry, a->window, 0, (float2*)a->factors};
+                    a->context_len, a->table_width, a->first_entry, a->window, 0, (float2*)a->factors, a->factors != nullptr ? 2 : 1};
     return launch_read<true>(p, a->bits, a->out_dtype, (cudaStream_t)a->stream);
 }

@@ -1099,7 +1099,7 @@ public:
         run(f(&a), "quant_cache_write");
     }
     // What entries first .. first + entries - 1 see, read back into pages of their own: the view of those.  With `factors` (two numbers
-    // an entry of the step and kv head, made here) the pages are float16, multiplied by those.
+    // an entry of the step and kv head, made here) the pages are float16, multiplied by those, and entries of one token are left out.
     PagedCacheView quant_read_entries(const PagedCacheView& cache, int dtype, const int* q_start, const int* context_len, int first,
                                       int entries, int all_entries, int n_kv, int head_dim, int window, float* factors = nullptr) {
         using Fn = int (*)(const QuantReadEntriesArgs*);

@@ -170,7 +170,7 @@ def read_quantized_pages(k_out: torch.Tensor, v_out: torch.Tensor, pages: Quanti
 def _read_entries(pages: QuantizedPages, dtype: torch.dtype, meta, block_table: torch.Tensor, first: int, entries: int, window: int,
                   status: torch.Tensor, table: torch.Tensor, stream: int, factors: Optional[torch.Tensor] = None):
     """Pages of what ``entries`` entries from ``first`` on see, in ``dtype``, and their rows of ``table``.  With ``factors`` (float32
-    [entries of the step, n_kv, 2], made here) the pages' 16 bits are float16, multiplied by those."""
+    [entries of the step, n_kv, 2], made here) the pages' 16 bits are float16, multiplied by those, and entries of one token are left out."""
     width = block_table.shape[1]
     k = torch.empty((entries * width, pages.n_kv, pages.page_size, pages.head_dim), dtype=dtype, device=table.device)
     v = torch.empty_like(k)

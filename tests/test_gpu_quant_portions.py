@@ -59,3 +59,24 @@ def test_a_table_that_is_too_short_is_reported(impl):
         assert st.tolist() == [want, 0, 0, 0], width
         check(out, q, meta, table, k, v, layout[:1], nkv, page, None, D ** -0.5, lambda e: impl == "read")
         check(out[170:], q[170:], meta, table[2:], k, v, layout[2:], nkv, page, None, D ** -0.5, lambda e: impl == "read")
+
+
+# ------------------------------------------------------------------ mixed steps
+@pytest.mark.parametrize("window", [None, 90])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_single_tokens_between_portions_are_not_read_back(bits, window):
+    """What they see is neither read nor written for the prompt kernel: the kernel over codes serves them."""
+    layout, nq, nkv, D, page = [(30, 100), (400, 1), (0, 0), (700, 1), (0, 130), (5, 2), (900, 1)], 32, 2, 128, 16
+    meta, table, n_pages = step(layout, page, 3)
+    pages, k, v = random_pages(n_pages, nkv, page, D, bits, 3)
+    q = queries(meta, nq, D, 3)
+    out, st = attend(pages, meta, q, nq, D ** -0.5, window, impl="portion")
+    assert st.tolist() == [0] * 4
+    check(out, q, meta, table, k, v, layout, nkv, page, window, D ** -0.5, lambda e: False)
+    made, factors = torch.full_like(meta.block_tables[0], -7), torch.zeros(len(layout), nkv, 2, device=DEV)
+    cache_quant._read_entries(pages, BF16, meta, meta.block_tables[0], 0, 6, window or 0, st, made, torch.cuda.current_stream().cuda_stream, factors)
+    for e, (c, n) in enumerate(layout):
+        lo = max(0, c - (window or 10 ** 6) + 1) // page
+        needed = -(-(c + n) // page) - lo if n > 1 else 0
+        assert int((made[e] >= 0).sum()) == needed and (e == 6) == bool((made[e] == -7).all()), e
+    assert st.tolist() == [0] * 4
