@@ -298,7 +298,9 @@ struct Params {
     const float* sink;          // [n_q] or null
     const bf16* gate; long long ld_gate; int gate_dims;
     float out_scale;
-    const float2* factors;      // the H form: [entries][n_kv], what keys and values are multiplied by
+    // the H form: [entries][n_kv], what keys and values are multiplied by; and the entries it works on, whatever the list holds beside them
+    const float2* factors;
+    int first_entry, end_entry;
 };
 
 // D, DV: columns of the query / key tiles (64, 128, and in the X form 192) and of the value tile (64, 128, and in the X
@@ -357,6 +359,12 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     if constexpr (X) pdl_wait();
     const int item = gridDim.y - 1 - blockIdx.y;
     const int entry = p.work[2 * item], tile_tok = p.work[2 * item + 1];
+    if constexpr (H) {
+        if (entry < p.first_entry || entry >= p.end_entry) {           // (the whole CTA; it ends no earlier than the grid before it)
+            pdl_wait();
+            return;
+        }
+    }
     const int h = blockIdx.x, g = h / (p.n_q / p.n_kv);
     const int qs = p.q_start[entry], q_len = p.q_start[entry + 1] - qs;
     const int ctx = p.context_len[entry];
@@ -1081,7 +1089,7 @@ extern "C" int kipp_attn_prefill_tc_ex_supported(int head_dim, int v_dim, int n_
 static int prefill_tc(void* out, const void* q, int tokens, const void* k_pages, const void* v_pages, int n_pages,
                       const int* q_start, const int* context_len, const int* block_table, int table_width, int page_size,
                       const int* work, int items, int n_q, int n_kv, int head_dim, int v_dim, float scale, int window,
-                      float out_scale, const MixExtras* ex, const float2* factors, int* status, void* stream) {
+                      float out_scale, const MixExtras* ex, const float2* factors, int first_entry, int entries, int* status, void* stream) {
     if (items <= 0) return 0;
     if (items > 65535) return KIPP_ERR_ARG;
     if (!kipp_attn_prefill_tc_page_ok(page_size) || n_pages <= 0 || window < 0 || status == nullptr || tokens <= 0)
@@ -1124,7 +1132,7 @@ static int prefill_tc(void* out, const void* q, int tokens, const void* k_pages,
     rc = pool_map(&mo, out, tokens, n_q * v_dim, 32);
     if (rc) return rc;
     cudaStream_t s = (cudaStream_t)stream;
-    p.factors = factors;
+    p.factors = factors; p.first_entry = first_entry; p.end_entry = first_entry + entries;
     if (factors != nullptr)
         return head_dim == 64 ? launch<64, 64, false, true>(mk, mv, mk4, mv4, mq, mo, p, items, s)
                               : launch<128, 128, false, true>(mk, mv, mk4, mv4, mq, mo, p, items, s);
@@ -1162,21 +1170,24 @@ extern "C" int kipp_attn_prefill_tc(void* out, const void* q, int tokens, const 
                                     int* status, void* stream) {
     if (items > 0 && !kipp_attn_prefill_tc_supported(head_dim, n_q, n_kv)) return KIPP_ERR_ARG;
     return prefill_tc(out, q, tokens, k_pages, v_pages, n_pages, q_start, context_len, block_table, table_width, page_size, work,
-                      items, n_q, n_kv, head_dim, head_dim, scale, window, 1.f, nullptr, nullptr, status, stream);
+                      items, n_q, n_kv, head_dim, head_dim, scale, window, 1.f, nullptr, nullptr, 0, 0, status, stream);
 }
 
 // The H form: k_pages and v_pages float16, entry e's keys and values of kv head g multiplied by factors[e * n_kv + g] (two
-// numbers, powers of two).  q and out are bfloat16; scale > 0.
+// numbers, powers of two).  q and out are bfloat16; scale > 0.  The tiles of entries first_entry .. first_entry + entries - 1 are
+// worked on, wherever in the list they are.
 extern "C" int kipp_attn_prefill_tc_half(void* out, const void* q, int tokens, const void* k_pages, const void* v_pages,
                                          int n_pages, const int* q_start, const int* context_len,
                                          const int* block_table, int table_width, int page_size, const int* work,
                                          int items, int n_q, int n_kv, int head_dim, float scale, int window,
-                                         const void* factors, int* status, void* stream) {
-    if (items <= 0) return 0;
-    if (!kipp_attn_prefill_tc_supported(head_dim, n_q, n_kv) || factors == nullptr || !(scale > 0.f)) return KIPP_ERR_ARG;
+                                         const void* factors, int first_entry, int entries, int* status, void* stream) {
+    if (items <= 0 || entries <= 0) return 0;
+    if (!kipp_attn_prefill_tc_supported(head_dim, n_q, n_kv) || factors == nullptr || !(scale > 0.f) || first_entry < 0 ||
+        entries > 0x7fffffff - first_entry)
+        return KIPP_ERR_ARG;
     if ((uintptr_t)factors & 7) return -3;
     return prefill_tc(out, q, tokens, k_pages, v_pages, n_pages, q_start, context_len, block_table, table_width, page_size, work,
-                      items, n_q, n_kv, head_dim, head_dim, scale, window, 1.f, nullptr, static_cast<const float2*>(factors), status, stream);
+                      items, n_q, n_kv, head_dim, head_dim, scale, window, 1.f, nullptr, static_cast<const float2*>(factors), first_entry, entries, status, stream);
 }
 
 extern "C" int kipp_attn_prefill_tc_ex(void* out, const void* q, int tokens, const void* k_pages, const void* v_pages,
@@ -1192,7 +1203,7 @@ extern "C" int kipp_attn_prefill_tc_ex(void* out, const void* q, int tokens, con
     // a gate per element is read 16 bytes at a time
     if (ex->gate != nullptr && ex->gate_dims && ((((uintptr_t)ex->gate + 2 * (size_t)ex->gate_off) & 15) || (ex->ld_gate & 7))) return -3;
     return prefill_tc(out, q, tokens, k_pages, v_pages, n_pages, q_start, context_len, block_table, table_width, page_size, work,
-                      items, n_q, n_kv, head_dim, v_dim, scale, window, out_scale, ex, nullptr, status, stream);
+                      items, n_q, n_kv, head_dim, v_dim, scale, window, out_scale, ex, nullptr, 0, 0, status, stream);
 }
 
 // Whether kipp_latent_expand_tc takes the pages and is the faster form for `keys` cached tokens, new ones among them.  Its

@@ -8,6 +8,8 @@
 #pragma once
 #include <algorithm>
 #include <cmath>
+#include <tuple>
+#include <vector>
 
 #include "runtime.hpp"
 
@@ -1098,6 +1100,12 @@ public:
                                   head_dim, write_cache ? 1 : 0, eps};
         run(f(&a), "quant_cache_write");
     }
+    // Room for the pages of `entries` entries, keys' and values'.
+    std::pair<void*, void*> quant_read_back_room(const PagedCacheView& cache, int dtype, int entries, int n_kv, int head_dim) {
+        const size_t bytes = (size_t)entries * cache.table_width * n_kv * cache.page_size * head_dim * dtype_size(dtype);
+        void* keys = workspace->buffer("quant_keys", bytes);
+        return {keys, workspace->buffer("quant_values", bytes)};
+    }
     // What entries first .. first + entries - 1 see, read back into pages of their own: the view of those.  With `factors` (two numbers
     // an entry of the step and kv head, made here) the pages are float16, multiplied by those, and entries of one token are left out.
     PagedCacheView quant_read_entries(const PagedCacheView& cache, int dtype, const int* q_start, const int* context_len, int first,
@@ -1108,9 +1116,7 @@ public:
         v.bits = 0;
         v.k_scales = v.v_scales = nullptr;
         v.n_pages = entries * cache.table_width;
-        const size_t bytes = (size_t)v.n_pages * n_kv * cache.page_size * head_dim * dtype_size(dtype);
-        v.k_pages = workspace->buffer("quant_keys", bytes);
-        v.v_pages = workspace->buffer("quant_values", bytes);
+        std::tie(v.k_pages, v.v_pages) = quant_read_back_room(cache, dtype, entries, n_kv, head_dim);
         int* table = workspace->get<int>("quant_table", (size_t)all_entries * cache.table_width);
         v.block_table = table;
         const QuantReadEntriesArgs a = {v.k_pages, v.v_pages, table, cache.k_pages, cache.k_scales, cache.v_pages, cache.v_scales, q_start,
@@ -1140,8 +1146,8 @@ public:
     }
     // Causal grouped-query attention over a quantised cache.  bfloat16 heads of 64, 128 and 256 run on the codes; where portions of
     // PREFILL_TC_MIN_TOKENS and more are among the entries and it pays, those of more than one token read their pages back for the
-    // tcgen05 prompt kernel, as long as the pages have room in EXPAND_MAX_BYTES; other heads and 32-bit read back always, as many entries at
-    // a time as have room there.  Which it is depends on the step's shape only.
+    // tcgen05 prompt kernel; other heads and 32-bit read back always.  As many entries at a time are read back as have room in
+    // EXPAND_MAX_BYTES, one at least.  Which form it is depends on the step's shape only.
     void attention_quantized(void* out, const void* q, const PagedCacheView& cache, int dtype, const AttentionWork& work,
                              const std::vector<int>& q_lens, const int* positions, const int* entry_of_token, const int* q_start,
                              const int* context_len, int n_q, int n_kv, int head_dim, float scale, int window) {
@@ -1149,16 +1155,20 @@ public:
         const long long page_bytes = 2LL * n_kv * cache.page_size * head_dim * (long long)dtype_size(dtype);
         const long long at_once = std::max(1LL, EXPAND_MAX_BYTES / (page_bytes * cache.table_width));
         if (dtype == BF16 && attention_quant_supported(cache.bits, head_dim, n_q, n_kv)) {
-            int first = -1, last = -1, longest = 1;
+            int longest = 1;
             long long several = 0, tokens = 0, tiles = 0;
             bool single = false;
+            struct Chunk { int first, entries; };           // a run of entries that are read back together
+            std::vector<Chunk> chunks;
+            int largest = 0;
             for (int e = 0; e < entries; ++e) {
                 const int n = q_lens[(size_t)e];
                 longest = std::max(longest, n);
                 if (n == 1) single = true;
                 if (n <= 1) continue;
-                if (first < 0) first = e;
-                last = e;
+                if (!chunks.empty() && e - chunks.back().first < at_once) chunks.back().entries = e + 1 - chunks.back().first;
+                else chunks.push_back({e, 1});
+                largest = std::max(largest, chunks.back().entries);
                 ++several;
                 tokens += n;
                 tiles += (n + 127) / 128;
@@ -1169,18 +1179,21 @@ public:
             // bits 50 and 75, 62 and 62.)
             const bool pays = n_q * tokens > 4096 * ((n_q * tiles + 295) / 296) + 64 * n_kv * several;
             const bool portions = prefill_tensor_core && pays && scale > 0.f && longest >= PREFILL_TC_MIN_TOKENS && work.n_prefill_items128 > 0 &&
-                                  last - first + 1 <= at_once && attention_tc_supported(head_dim, n_q, n_kv, cache.page_size);
+                                  attention_tc_supported(head_dim, n_q, n_kv, cache.page_size);
             if (!portions || single)
                 attention_quant_direct(out, q, cache, q_start, context_len, entries, portions ? 1 : longest, n_q, n_kv, head_dim, scale, window);
-            if (portions) {
-                float* factors = workspace->get<float>("quant_factors", 2 * (size_t)entries * n_kv);
-                const PagedCacheView v = quant_read_entries(cache, dtype, q_start, context_len, first, last - first + 1, entries, n_kv, head_dim,
+            if (!portions) return;
+            float* factors = workspace->get<float>("quant_factors", 2 * (size_t)entries * n_kv);
+            quant_read_back_room(cache, dtype, largest, n_kv, head_dim);           // (no buffer moves between two chunks)
+            for (const Chunk& c : chunks) {
+                const PagedCacheView v = quant_read_entries(cache, dtype, q_start, context_len, c.first, c.entries, entries, n_kv, head_dim,
                                                             window, factors);
                 using Fn = int (*)(void*, const void*, int, const void*, const void*, int, const int*, const int*, const int*, int, int,
-                                   const int*, int, int, int, int, float, int, const void*, int*, void*);
+                                   const int*, int, int, int, int, float, int, const void*, int, int, int*, void*);
                 static Fn f = kernel_symbol<Fn>("attention_tc", "kipp_attn_prefill_tc_half");
                 run(f(out, q, work.tokens, v.k_pages, v.v_pages, v.n_pages, q_start, context_len, v.block_table, v.table_width, v.page_size,
-                      work.prefill_work128, work.n_prefill_items128, n_q, n_kv, head_dim, scale, window, factors, status, stream),
+                      work.prefill_work128, work.n_prefill_items128, n_q, n_kv, head_dim, scale, window, factors, c.first, c.entries, status,
+                      stream),
                     "attn_prefill_tc");
                 ++tc_prefill_launches;
             }

@@ -211,8 +211,9 @@ def _direct_ok(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPages, n_q: i
     return q.dtype == torch.bfloat16 and _supported[key] and pages.aligned and (q.data_ptr() | out.data_ptr()) % 16 == 0
 
 
-def _portion_span(q, pages, meta, block_table, n_q, scale):
-    """The entries of more than one token from the first to the last, where the prompt kernel takes them, or None."""
+def _portion_chunks(q, pages, meta, block_table, n_q, scale):
+    """The entries of more than one token as (first, number) of runs whose pages may be read back together, where the prompt kernel
+    takes them, or None.  (Entries of one token may lie between; they count as room, and are left out.)"""
     if not scale > 0 or getattr(meta, "prefill_work128", None) is None:
         return None
     several = [e for e, n in enumerate(meta.q_lens) if n > 1]
@@ -221,19 +222,25 @@ def _portion_span(q, pages, meta, block_table, n_q, scale):
     from . import attention_bf16
     if not attention_bf16.prefill_tc_supported(pages.head_dim, n_q, pages.n_kv, pages.page_size):
         return None
-    return several[0], several[-1] + 1
+    most, chunks = _entries_at_once(pages, q.dtype, block_table.shape[1]), []
+    for e in several:
+        if chunks and e - chunks[-1][0] < most:
+            chunks[-1] = (chunks[-1][0], e + 1 - chunks[-1][0])
+        else:
+            chunks.append((e, 1))
+    return chunks
 
 
 def _plan(out, q, pages, meta, block_table, n_q, scale=1.0):
-    """(form of the entries of one token, form of the others, the entries of more than one token from the first to the last):
+    """(form of the entries of one token, form of the others, the runs of entries that portions are read back in):
     forms "direct" (the kernel over codes), "portion" (read back, tcgen05 prompt kernel, for positive scales) and "read" (read back, CUDA cores).
     The prompt kernel reads a key and a value once for 128 tokens, the kernel over codes once for 8 or 16 columns."""
     if not _direct_ok(out, q, pages, n_q):
         return "read", "read", None
     if max(meta.q_lens) >= PORTION_MIN and _portions_pay(meta.q_lens, n_q, pages.n_kv):
-        span = _portion_span(q, pages, meta, block_table, n_q, scale)
-        if span is not None and span[1] - span[0] <= _entries_at_once(pages, q.dtype, block_table.shape[1]):
-            return "direct", "portion", span
+        chunks = _portion_chunks(q, pages, meta, block_table, n_q, scale)
+        if chunks is not None:
+            return "direct", "portion", chunks
     return "direct", "direct", None
 
 
@@ -272,14 +279,14 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
     if tokens == 0:
         return
     if impl is None:
-        single, several, span = _plan(out, q, pages, meta, block_table, n_q, scale)
+        single, several, chunks = _plan(out, q, pages, meta, block_table, n_q, scale)
     elif impl == "portion":
-        single, several, span = "direct", "portion", _portion_span(q, pages, meta, block_table, n_q, scale)
-        if span is None or not _direct_ok(out, q, pages, n_q):
+        single, several, chunks = "direct", "portion", _portion_chunks(q, pages, meta, block_table, n_q, scale)
+        if chunks is None or not _direct_ok(out, q, pages, n_q):
             raise KernelError(f"{what}: portions are read back for bfloat16 heads of 64 or 128, 16-byte aligned, a positive scale and a "
                               "list of their 128-token tiles")
     elif impl in ("direct", "read"):
-        single, several, span = impl, impl, None
+        single, several, chunks = impl, impl, None
         if impl == "direct" and not _direct_ok(out, q, pages, n_q):
             raise KernelError(f"{what}: the kernel over codes takes bfloat16 heads of 64, 128 or 256, 16-byte aligned")
     else:
@@ -292,7 +299,9 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
         return
     if 1 in q_lens:
         _direct(out, q, pages, meta, block_table, n_q, scale, window, status, 1, stream)
-    _portions(out, q, pages, meta, block_table, n_q, scale, window, status, span, stream)
+    table = torch.empty_like(block_table)
+    for first, entries in chunks:
+        _portions(out, q, pages, meta, block_table, n_q, scale, window, status, first, entries, table, stream)
 
 
 def _direct(out, q, pages, meta, block_table, n_q, scale, window, status, most: int, stream: int) -> None:
@@ -310,18 +319,18 @@ def _direct(out, q, pages, meta, block_table, n_q, scale, window, status, most: 
                        pages.page_size, width, len(meta.q_lens), most, n_q, pages.n_kv, D, window, scale), "attn_quant")
 
 
-def _portions(out, q, pages, meta, block_table, n_q, scale, window, status, span, stream: int) -> None:
-    """The entries of more than one token: their pages read back as float16, and the prompt kernel over those."""
-    table = torch.empty_like(block_table)
+def _portions(out, q, pages, meta, block_table, n_q, scale, window, status, first: int, entries: int, table, stream: int) -> None:
+    """Those of ``entries`` entries from ``first`` on that bring more than one token: their pages read back as float16, and the prompt
+    kernel over those."""
     factors = torch.empty((len(meta.q_lens), pages.n_kv, 2), dtype=torch.float32, device=q.device)
-    k, v = _read_entries(pages, q.dtype, meta, block_table, span[0], span[1] - span[0], window, status, table, stream, factors)
+    k, v = _read_entries(pages, q.dtype, meta, block_table, first, entries, window, status, table, stream, factors)
     f = _fn("attention_tc", "kipp_attn_prefill_tc_half",
             [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
-             c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_void_p])
+             c_void_p, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p])
     _check(f(out.data_ptr(), q.data_ptr(), q.shape[0], k.data_ptr(), v.data_ptr(), k.shape[0], meta.q_start.data_ptr(),
              meta.context_len.data_ptr(), table.data_ptr(), table.shape[1], pages.page_size, _ptr(meta.prefill_work128),
-             meta.n_prefill_items128, n_q, pages.n_kv, pages.head_dim, scale, window, factors.data_ptr(), status.data_ptr(), stream),
-           "attn_prefill_tc")
+             meta.n_prefill_items128, n_q, pages.n_kv, pages.head_dim, scale, window, factors.data_ptr(), first, entries, status.data_ptr(),
+             stream), "attn_prefill_tc")
 
 
 def _by_reading(out, q, pages, meta, block_table, n_q, scale, window, status, stream: int) -> None:

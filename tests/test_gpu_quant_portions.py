@@ -80,3 +80,52 @@ def test_single_tokens_between_portions_are_not_read_back(bits, window):
         needed = -(-(c + n) // page) - lo if n > 1 else 0
         assert int((made[e] >= 0).sum()) == needed and (e == 6) == bool((made[e] == -7).all()), e
     assert st.tolist() == [0] * 4
+
+
+@pytest.mark.parametrize("at_once", [1, 2, 3])
+@pytest.mark.parametrize("D,nkv", [(128, 2), (64, 3)])
+def test_portions_that_do_not_fit_together(D, nkv, at_once, monkeypatch):
+    """Room for a few entries' pages only: they go several at a time, and each has what it has when all go at once, bit for bit, wherever
+    the list has its tiles."""
+    layout, nq, page = [(30, 100), (400, 1), (0, 0), (700, 1), (0, 130), (5, 2), (900, 1), (333, 260)], 16 * nkv, 16
+    meta, table, n_pages = step(layout, page, 3)
+    pages, k, v = random_pages(n_pages, nkv, page, D, 4, 3)
+    q = queries(meta, nq, D, 3, spare=3)
+    want, st = attend(pages, meta, q, nq, D ** -0.5, impl="portion")
+    check(want, q, meta, table, k, v, layout, nkv, page, None, D ** -0.5, lambda e: False)
+    monkeypatch.setattr(cache_quant, "READ_BYTES", at_once * 2 * nkv * page * D * 2 * table.shape[1])
+    assert chosen(q, q, pages, meta, nq) == "portion"
+    chunks = cache_quant._plan(q, q, pages, meta, meta.block_tables[0], nq)[2]
+    assert chunks == {1: [(0, 1), (4, 1), (5, 1), (7, 1)], 2: [(0, 1), (4, 2), (7, 1)], 3: [(0, 1), (4, 2), (7, 1)]}[at_once]
+    order = torch.randperm(meta.n_prefill_items128, generator=torch.Generator().manual_seed(1)).to(DEV)
+    for tiles in (meta.prefill_work128, meta.prefill_work128.flip(0).contiguous(), meta.prefill_work128[order].contiguous()):
+        meta.prefill_work128 = tiles
+        for impl in (None, "portion"):
+            out, st = attend(pages, meta, q, nq, D ** -0.5, impl=impl)
+            assert st.tolist() == [0] * 4 and torch.equal(out, want) and (out[meta.tokens:] == 7).all()
+
+
+def test_an_engine_whose_portions_do_not_fit_together():
+    """320 key heads of 128: two portions behind 3,900 tokens would take 1.3 GB read back, more than goes at a time."""
+    from gpu_util import part_engine
+    from kipp_b200.engine import StepEntry
+    from kipp_b200.parts import AttentionMixer, NoPositionEncoding, PreNormBlock, RMSNorm, SwiGLUFeedForward
+    from tiny import nmse
+    heads, long = 320, 3900
+    block = PreNormBlock(RMSNorm(64, 1e-5), AttentionMixer(64, heads, heads, 128, NoPositionEncoding()), RMSNorm(64, 1e-5),
+                         SwiGLUFeedForward(64, 16))
+    eng, _ = part_engine("bfloat16", 64, block=block, kv_quant="int4", page_size=16, n_pages=640, max_requests=5)
+    g = torch.Generator().manual_seed(5)
+    text = {r: torch.randint(0, 32, (n,), generator=g).tolist() for r, n in (("a", long + 100), ("b", 40), ("c", 150))}
+    text["a2"], text["c2"] = text["a"], text["c"]
+    for r in ("a", "a2"):
+        for at in range(0, long, 500):
+            eng.step([StepEntry(r, text[r][at:min(at + 500, long)], [])], check=True)
+    eng.step([StepEntry("b", text["b"][:-1], [])], check=True)
+    eng.profile_start()
+    got = eng.step([StepEntry("a", text["a"][long:], list(range(100))), StepEntry("b", text["b"][-1:], [0]),
+                    StepEntry("c", text["c"], list(range(150)))], check=True).double().cpu()
+    assert "attn_prefill_tc" in eng.profile_stop()
+    for rows, r, new in ((got[:100], "a2", text["a"][long:]), (got[101:], "c2", text["c"])):
+        want = eng.step([StepEntry(r, new, list(range(len(new))))], check=True).double().cpu()
+        assert nmse(rows, want) <= 1e-4, r
