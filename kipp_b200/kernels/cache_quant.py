@@ -211,13 +211,22 @@ def _direct_ok(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPages, n_q: i
     return q.dtype == torch.bfloat16 and _supported[key] and pages.aligned and (q.data_ptr() | out.data_ptr()) % 16 == 0
 
 
+def _tiles_ok(meta, device: int) -> bool:
+    """Whether the step has a list of 128-token tiles that can be that of every entry of more than one token."""
+    work = getattr(meta, "prefill_work128", None)
+    if work is None or work.dtype is not _I32 or not work.is_contiguous() or work.get_device() != device:
+        return False
+    tiles = sum((n + 127) // 128 for n in meta.q_lens if n > 1)
+    return getattr(meta, "n_prefill_items128", 0) == tiles and work.numel() >= 2 * tiles
+
+
 def _portion_chunks(q, pages, meta, block_table, n_q, scale):
     """The entries of more than one token as (first, number) of runs whose pages may be read back together, where the prompt kernel
-    takes them, or None.  (Entries of one token may lie between; they count as room, and are left out.)"""
-    if not scale > 0 or getattr(meta, "prefill_work128", None) is None:
+    takes them and the step's list of tiles is theirs, or None.  (Entries of one token may lie between; they count as room, and are left out.)"""
+    if not scale > 0:
         return None
     several = [e for e, n in enumerate(meta.q_lens) if n > 1]
-    if not several:
+    if not several or not _tiles_ok(meta, pages.device_index):
         return None
     from . import attention_bf16
     if not attention_bf16.prefill_tc_supported(pages.head_dim, n_q, pages.n_kv, pages.page_size):
@@ -249,8 +258,9 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
     """Causal grouped-query attention of the step's tokens over a quantised cache.
 
     ``meta`` is the step's metadata as for ``attention`` (``tokens``, ``q_lens``, ``positions``, ``entry_of_token``,
-    ``q_start``, ``context_len``, and where entries bring 64 tokens or more the list of their 128-token tiles,
-    ``prefill_work128`` and ``n_prefill_items128``).  bfloat16 with heads of 64, 128 or 256 runs on the codes themselves; long
+    ``q_start``, ``context_len``, and for steps with entries of 64 tokens or more the list of the 128-token tiles of every entry of more
+    than one token, ``prefill_work128`` int32 [tiles, (entry, first token)] in any order, and ``n_prefill_items128``; a step without
+    that list, or with one of another length, stays on the codes).  bfloat16 with heads of 64, 128 or 256 runs on the codes themselves; long
     portions of prompts, other heads and float32 on pages that are read back.  A page that is not mapped, or past the pool, sets
     status word 0 to 3.  On the codes a result is off by up to 2^-64 a key beside its roundings (values of 2^-40 and less feel it), and
     queries of 2^80 and more count as infinite.  ``impl`` forces a form:
@@ -284,7 +294,7 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
         single, several, chunks = "direct", "portion", _portion_chunks(q, pages, meta, block_table, n_q, scale)
         if chunks is None or not _direct_ok(out, q, pages, n_q):
             raise KernelError(f"{what}: portions are read back for bfloat16 heads of 64 or 128, 16-byte aligned, a positive scale and a "
-                              "list of their 128-token tiles")
+                              "list of the 128-token tiles of every entry of more than one token")
     elif impl in ("direct", "read"):
         single, several, chunks = impl, impl, None
         if impl == "direct" and not _direct_ok(out, q, pages, n_q):

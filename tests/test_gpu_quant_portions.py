@@ -129,3 +129,25 @@ def test_an_engine_whose_portions_do_not_fit_together():
     for rows, r, new in ((got[:100], "a2", text["a"][long:]), (got[101:], "c2", text["c"])):
         want = eng.step([StepEntry(r, new, list(range(len(new))))], check=True).double().cpu()
         assert nmse(rows, want) <= 1e-4, r
+
+
+@pytest.mark.parametrize("wrong", ["none", "long portions only", "empty", "more", "short", "int64", "strided", "elsewhere"])
+def test_lists_of_tiles_that_are_not_the_step_s(wrong):
+    """A list that cannot hold the tiles of every entry of more than one token: refused where portions are asked for, and otherwise the
+    step stays on the codes; no row is left unwritten."""
+    layout, nq, nkv, D, page = [(30, 300), (400, 1), (5, 40), (60, 2), (0, 130)], 32, 2, 128, 16
+    meta, table, n_pages = step(layout, page, 3)
+    pages, k, v = random_pages(n_pages, nkv, page, D, 4, 3)
+    q = queries(meta, nq, D, 3)
+    assert chosen(q, q, pages, meta, nq) == "portion"
+    whole, n = meta.prefill_work128, meta.n_prefill_items128
+    assert n == 3 + 1 + 1 + 2
+    meta.prefill_work128, meta.n_prefill_items128 = {
+        "none": (None, 0), "long portions only": (whole[[0, 1, 2, 5, 6]].contiguous(), 5), "empty": (whole, 0), "more": (whole, n + 1),
+        "short": (whole[:-1], n), "int64": (whole.long(), n), "strided": (whole.repeat(1, 2)[:, :2], n), "elsewhere": (whole.cpu(), n)}[wrong]
+    with pytest.raises(K.KernelError, match="list of the 128-token tiles"):
+        attend(pages, meta, q, nq, D ** -0.5, impl="portion")
+    assert chosen(q, q, pages, meta, nq) == "direct"
+    out, st = attend(pages, meta, q, nq, D ** -0.5)
+    assert st.tolist() == [0] * 4
+    check(out, q, meta, table, k, v, layout, nkv, page, None, D ** -0.5, lambda e: False)
