@@ -915,6 +915,20 @@ template <int D, int BITS, int NT, bool TILES> int launch(Params p, long long st
 // 16 31.7), 8 where those do, else 16 (12
 // queries: 35.5 us, 42.3 with 8); heads of 256 have no room for their sums: always 8
 int columns_of(int bits, int head_dim, long long queries) { return bits == 4 && queries <= 4 ? 4 : head_dim == 256 || queries <= 8 ? 8 : 16; }
+// The kernel of these heads and columns.
+int launch_columns(const Params& p, int bits, int head_dim, long long cols, long long steps, cudaStream_t s) {
+    const bool tiles = p.page_size % 16 == 0;
+#define KIPP_CASE(d, b)                                                                                            \
+    if (head_dim == d && bits == b) {                                                                              \
+        if constexpr (b == 4)                                                                                      \
+            if (cols == 4) return tiles ? launch<d, b, 0, true>(p, steps, s) : launch<d, b, 0, false>(p, steps, s);                  \
+        if (cols == 8) return tiles ? launch<d, b, 1, true>(p, steps, s) : launch<d, b, 1, false>(p, steps, s);                      \
+        if constexpr (d != 256) return tiles ? launch<d, b, 2, true>(p, steps, s) : launch<d, b, 2, false>(p, steps, s);             \
+    }
+    KIPP_CASE(64, 4) KIPP_CASE(64, 8) KIPP_CASE(128, 4) KIPP_CASE(128, 8) KIPP_CASE(256, 4) KIPP_CASE(256, 8)
+#undef KIPP_CASE
+    return KIPP_ERR_ARG;
+}
 }  // namespace
 
 // Whether the kernel takes these heads.
@@ -954,16 +968,17 @@ extern "C" int kipp_attn_quant(const KippAttnQuant* a) {
     // (row numbers of pages and steps of all rows are 32-bit)
     const long long cols = columns_of(bits, head_dim, (long long)most * (n_q / n_kv));
     const long long room = (long long)a->table_width * page_size, steps = (room + STEP - 1) / STEP;
-    const long long blocks = n_kv * (((long long)most * (n_q / n_kv) + cols - 1) / cols);
-    if ((long long)a->n_pages * n_kv * page_size > 0x7fffffffLL || room > 0x7fffffffLL ||
-        blocks > 0x3fffffffLL / entries / (steps + ROW_COST) || (long long)most * n_q > 0x3fffffffLL)
+    const long long blocks = n_kv * (((long long)most * (n_q / n_kv) + cols - 1) / cols), entry_units = blocks * (steps + ROW_COST);
+    if ((long long)a->n_pages * n_kv * page_size > 0x7fffffffLL || room > 0x7fffffffLL || (long long)most * n_q > 0x3fffffffLL ||
+        entry_units > 0x3fffffffLL)
         return KIPP_ERR_ARG;
+    // (what every entry may have: a step of many, one of them with many tokens and one with a long table, goes in several launches)
+    const int at_once = (int)(0x3fffffffLL / entry_units);
     Params p = {};
     p.out = (bf16*)a->out; p.q = (const bf16*)a->q;
     p.k_codes = (const uint8_t*)a->k_codes; p.k_scales = (const uint8_t*)a->k_scales;
     p.v_codes = (const uint8_t*)a->v_codes; p.v_scales = (const uint8_t*)a->v_scales;
-    p.q_start = a->q_start; p.context_len = a->context_len; p.block_table = a->block_table;
-    p.entries = entries; p.table_width = a->table_width; p.page_size = page_size; p.n_pages = a->n_pages; p.most = most;
+    p.table_width = a->table_width; p.page_size = page_size; p.n_pages = a->n_pages; p.most = most;
     p.page_shift = -1;
     for (int i = 0; i < 31; ++i) if (page_size == 1 << i) p.page_shift = i;
     p.n_q = n_q; p.n_kv = n_kv; p.group = n_q / n_kv; p.window = a->window;
@@ -975,15 +990,11 @@ extern "C" int kipp_attn_quant(const KippAttnQuant* a) {
     p.shared = (int4*)(p.part_ml + 2LL * MOST_CTAS * MOST_COLUMNS * 2);
     p.most_blocks = (int)blocks;
     p.status = a->status;
-    cudaStream_t s = (cudaStream_t)a->stream;
-#define KIPP_CASE(d, b)                                                                                            \
-    if (head_dim == d && bits == b) {                                                                              \
-        if constexpr (b == 4)                                                                                      \
-            if (cols == 4) return page_size % 16 == 0 ? launch<d, b, 0, true>(p, steps, s) : launch<d, b, 0, false>(p, steps, s);    \
-        if (cols == 8) return page_size % 16 == 0 ? launch<d, b, 1, true>(p, steps, s) : launch<d, b, 1, false>(p, steps, s);        \
-        if constexpr (d != 256) return page_size % 16 == 0 ? launch<d, b, 2, true>(p, steps, s) : launch<d, b, 2, false>(p, steps, s); \
+    for (int first = 0; first < entries; first += at_once) {
+        p.entries = entries - first < at_once ? entries - first : at_once;
+        p.q_start = a->q_start + first; p.context_len = a->context_len + first; p.block_table = a->block_table + (size_t)first * a->table_width;
+        if (const int e = launch_columns(p, bits, head_dim, cols, steps, (cudaStream_t)a->stream)) return e;
+        if (at_once >= entries - first) break;
     }
-    KIPP_CASE(64, 4) KIPP_CASE(64, 8) KIPP_CASE(128, 4) KIPP_CASE(128, 8) KIPP_CASE(256, 4) KIPP_CASE(256, 8)
-#undef KIPP_CASE
-    return KIPP_ERR_ARG;
+    return 0;
 }
