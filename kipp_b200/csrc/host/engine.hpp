@@ -613,8 +613,16 @@ inline size_t Engine::workspace_estimate() const {
     // slack stand for them), and the logits rows
     const size_t es = dtype_size(dtype_);
     const size_t per_token = (size_t)plan_->hidden_size * (4 * (size_t)(plan_->streams + (plan_->streams > 1 ? 2 : 0)) + es * 12);
-    // a quantised cache: the pages that a step reads back, and the parts of rows of its attention
-    const size_t read_back = opt_.kv_bits ? (size_t)Ops::EXPAND_MAX_BYTES + (40u << 20) : 0;
+    // a quantised cache: the pages that a step reads back, of one entry at least, and the parts of rows of its attention
+    size_t read_back = 0;
+    if (opt_.kv_bits) {
+        const long long longest = plan_->max_positions > 0 ? plan_->max_positions : opt_.cache_tokens > 0 ? opt_.cache_tokens : 8192;
+        size_t row = 0;
+        for (auto& run : plan_->order)
+            for (Mixer* mixer : plan_->layers[(size_t)run.layer].second->mixers())
+                if (auto cs = mixer->cache_spec()) row = std::max(row, (size_t)cs->kv_heads * (cs->head_dim + cs->stored_v_dim()) * es);
+        read_back = std::max((size_t)Ops::EXPAND_MAX_BYTES, row * (size_t)(longest + opt_.page_size)) + (40u << 20);
+    }
     return per_token * (size_t)opt_.max_batch_tokens + (size_t)opt_.max_logit_rows * plan_->vocab_size * 4 + (64u << 20) + read_back;
 }
 

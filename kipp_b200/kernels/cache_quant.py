@@ -13,7 +13,7 @@ import torch
 from .ops import KernelError, _check, _fn, _ptr, c_float, c_int, c_void_p, dtype_code, rope_table
 
 c_ll, c_char_p = ctypes.c_longlong, ctypes.c_char_p
-READ_BYTES = 1 << 30          # most bytes of keys and values that attention reads back at a time
+READ_BYTES = 1 << 30          # most bytes of keys and values that attention reads back at a time (one entry's, where those are more)
 
 
 class QuantizedPages:

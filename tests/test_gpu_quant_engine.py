@@ -162,3 +162,22 @@ def test_command_line(capsys):
         assert main(["--model", model_folder("E"), "--prompt-ids", "5,17,3,9,100,7", "--decode", "8", "--kv-quant", kv]) == 0
         lines[kv] = [x for x in capsys.readouterr().out.splitlines() if x.startswith("generated")]
         assert len(lines[kv]) == 1 and len(lines[kv][0].split("\t")[1].split()) == 8
+
+
+@pytest.mark.parametrize("dtype,size", [("float32", 4), ("bfloat16", 2)])
+def test_the_workspace_has_room_for_an_entry_read_back(dtype, size):
+    """What an engine reserves, by the message of one that is too large: beside what the plain cache's does, a whole entry of the longest
+    text, where that is more than is read back at a time."""
+    import re
+
+    from kipp_b200.parts import AttentionMixer, NoPositionEncoding, PreNormBlock, RMSNorm, SwiGLUFeedForward
+    reserved = {}
+    for heads in (8, 640):
+        for kv_quant in (None, "int8"):
+            block = PreNormBlock(RMSNorm(64, 1e-5), AttentionMixer(64, heads, heads, 128, NoPositionEncoding()), RMSNorm(64, 1e-5),
+                                 SwiGLUFeedForward(64, 16))
+            with pytest.raises(Exception, match="of workspace") as e:
+                part_engine(dtype, 64, block=block, kv_quant=kv_quant, n_pages=2 ** 27)
+            reserved[heads, kv_quant] = int(re.search(r"(\d+) of workspace", str(e.value)).group(1))
+    assert reserved[8, "int8"] - reserved[8, None] >= 2 ** 30
+    assert reserved[640, "int8"] - reserved[640, None] >= 2 * 640 * 128 * size * 4096     # (4,096 positions)
