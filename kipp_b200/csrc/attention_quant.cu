@@ -80,7 +80,7 @@ struct Entry {
 template <int COLS> __device__ __forceinline__ Entry entry_of(const Params& p, int e) {
     Entry r;
     r.q_len = p.q_start[e + 1] - p.q_start[e];
-    r.context = p.context_len[e];
+    r.context = min(p.context_len[e], 0x7fffffff - max(r.q_len, 0));          // (far behind any table: reported, as all that is)
     if (r.q_len <= 0 || r.q_len > p.most || r.context < 0) { r.blocks = r.n_steps = r.column_blocks = 0; return r; }
     const int room = p.table_width * p.page_size;
     const int hi = min(r.context + r.q_len, room) - 1;
@@ -965,11 +965,11 @@ extern "C" int kipp_attn_quant(const KippAttnQuant* a) {
     if ((((uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->k_codes | (uintptr_t)a->v_codes | (uintptr_t)a->k_scales | (uintptr_t)a->v_scales |
           (uintptr_t)a->scratch) & 15) != 0)
         return -3;
-    // (row numbers of pages and steps of all rows are 32-bit)
+    // (row numbers of pages, keys, those of steps that are looked up ahead too, and steps of all rows are 32-bit)
     const long long cols = columns_of(bits, head_dim, (long long)most * (n_q / n_kv));
     const long long room = (long long)a->table_width * page_size, steps = (room + STEP - 1) / STEP;
     const long long blocks = n_kv * (((long long)most * (n_q / n_kv) + cols - 1) / cols), entry_units = blocks * (steps + ROW_COST);
-    if ((long long)a->n_pages * n_kv * page_size > 0x7fffffffLL || room > 0x7fffffffLL || (long long)most * n_q > 0x3fffffffLL ||
+    if ((long long)a->n_pages * n_kv * page_size > 0x7fffffffLL || room > 0x7fffffffLL - 32 * STEP || (long long)most * n_q > 0x3fffffffLL ||
         entry_units > 0x3fffffffLL)
         return KIPP_ERR_ARG;
     // (what every entry may have: a step of many, one of them with many tokens and one with a long table, goes in several launches)

@@ -367,10 +367,12 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     }
     const int h = blockIdx.x, g = h / (p.n_q / p.n_kv);
     const int qs = p.q_start[entry], q_len = p.q_start[entry + 1] - qs;
-    const int ctx = p.context_len[entry];
+    // (H: a length far behind the table, which is reported with the pages, must not become a loop over as many keys)
+    const int ctx = H ? min(max(p.context_len[entry], 0), 0x7fffffff - q_len - BM) : p.context_len[entry];
     // keys the tile may see: from the first token's window start to the last token
     const int tile_first = ctx + tile_tok, tile_last = ctx + min(tile_tok + BM - 1, q_len - 1);
-    const int lo = first_visible(tile_first, p.window, X ? p.chunk : 0), hi = tile_last;
+    const int hi = H ? min(tile_last, p.table_width * p.page_size - 1) : tile_last;
+    const int lo = H ? min(first_visible(tile_first, p.window, 0), hi) : first_visible(tile_first, p.window, X ? p.chunk : 0);
     const int first_tile = lo / BN, last_tile = hi / BN;
     const int n_tiles = last_tile - first_tile + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

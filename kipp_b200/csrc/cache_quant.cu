@@ -326,8 +326,9 @@ struct ReadParams {
 
 // The keys of entry e that its tokens see, [first, end): none where it is left out.
 __device__ __forceinline__ int2 seen_keys(const ReadParams& p, int e) {
-    const int tokens = p.q_start[e + 1] - p.q_start[e], first = p.context_len[e];
+    const int tokens = p.q_start[e + 1] - p.q_start[e];
     if (tokens < p.least) return make_int2(0, 0);
+    const int first = min(max(p.context_len[e], 0), 0x7fffffff - tokens);
     return make_int2(p.window > 0 ? max(0, first - p.window + 1) : 0, first + tokens);
 }
 
@@ -345,8 +346,9 @@ __global__ void __launch_bounds__(FACTOR_THREADS) quant_factor_kernel(const Read
     const int2 seen = seen_keys(p, e);
     const int* table = p.list + (size_t)e * p.table_width;
     const int end = min((long long)seen.y, (long long)p.table_width * p.pages.page_size);
+    const int begin = min(seen.x, end);           // (a window behind the table's end has nothing, and its keys' numbers may end at 2^31)
     uint32_t most[2] = {0u, 0u};                  // pairs of bfloat16 without signs
-    for (int base = seen.x + threadIdx.x; base < end; base += 4 * FACTOR_THREADS) {
+    for (int base = begin + threadIdx.x; base < end; base += 4 * FACTOR_THREADS) {
         uint32_t k[4][G / 2], v[4][G / 2];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

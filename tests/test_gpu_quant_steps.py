@@ -21,3 +21,26 @@ def test_many_entries_of_a_long_table(window):
     out, st = attend(pages, meta, q, nq, D ** -0.5, window, impl="direct")
     assert st.tolist() == [0] * 4
     check(out, q, meta, table, k, v, layout, nkv, page, window, D ** -0.5, lambda e: False)
+
+
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 70, 10 ** 9, -5])
+@pytest.mark.parametrize("window", [None, 40])
+@pytest.mark.parametrize("impl", ["direct", "portion"])
+def test_lengths_far_behind_the_table(impl, window, length):
+    """An entry said to have more cached than any table holds is reported, one below nothing has no result or any; the others are not
+    touched by it."""
+    layout, nq, nkv, D, page = [(301, 70), (90, 80), (40, 1), (77, 1)], 8, 2, 128, 16
+    meta, table, n_pages = step(layout, page, 3)
+    pages, k, v = random_pages(n_pages, nkv, page, D, 4, 3)
+    q = queries(meta, nq, D, 3)
+    for entry in (1, 3):
+        meta.context_len[entry] = length
+        got, st = attend(pages, meta, q, nq, D ** -0.5, window, impl=impl)
+        meta.context_len[entry] = layout[entry][0]
+        assert length < 0 or st.tolist() == [3, 0, 0, 0]
+        assert st.tolist()[1:] == [0, 0, 0] and torch.isfinite(got).all()
+        at = 0
+        for e, (_, n) in enumerate(layout):                 # (how a row is cut into parts depends on all lengths)
+            if e != entry:
+                check(got[at:], q[at:], meta, table[e:], k, v, layout[e:e + 1], nkv, page, window, D ** -0.5, lambda e: False)
+            at += n
