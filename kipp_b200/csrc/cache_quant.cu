@@ -348,12 +348,16 @@ __global__ void __launch_bounds__(FACTOR_THREADS) quant_factor_kernel(const Read
     const int end = min((long long)seen.y, (long long)p.table_width * p.pages.page_size);
     const int begin = min(seen.x, end);           // (a window behind the table's end has nothing, and its keys' numbers may end at 2^31)
     uint32_t most[2] = {0u, 0u};                  // pairs of bfloat16 without signs
+    // (what is not there of an entry's keys, behind the table's end too: the prompt kernel takes zeros for both without a word, and a
+    // page past the pool is reported by the kernel that reads it; the report made there took 59 registers instead of 48 and 3 % of the time)
+    bool missing = seen.y > end;
     for (int base = begin + threadIdx.x; base < end; base += 4 * FACTOR_THREADS) {
         uint32_t k[4][G / 2], v[4][G / 2];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int j = base + i * FACTOR_THREADS, slot = j / p.pages.page_size;
             const int page = j < end ? table[slot] : -1;
+            if (page < 0 && j < end) missing = true;
 #pragma unroll
             for (int w = 0; w < G / 2; ++w) k[i][w] = v[i][w] = 0u;
             if (page >= 0 && page < p.pages.n_pages) {
@@ -378,6 +382,7 @@ __global__ void __launch_bounds__(FACTOR_THREADS) quant_factor_kernel(const Read
         if (lane == 0) sh[i][warp] = one;
     }
     __syncthreads();
+    if (missing) atomicExch(p.status, 3);
     if (warp == 0) {
         float f[2];
 #pragma unroll
@@ -461,8 +466,8 @@ template <int BITS> __device__ __forceinline__ void put_unit(float* p, const Uni
 }
 
 // One block per (share of a page, page); DIM is the head size, or 0 for any.  Every thread has UNROLL units of eight channels of keys
-// and of values on their way at once.  A listed page whose number is negative (unmapped) or past the pool becomes zeros; past the
-// pool is also reported, and of an entry's pages whatever is not there and some token sees.  Bound by HBM, three quarters and more of it writes (8 x 8,100 tokens of 8 heads of 128 from 4 bits: 62 us, 5.5 TB/s).
+// and of values on their way at once.  A page whose number is negative (unmapped) or past the pool becomes zeros; past the
+// pool is also reported.  Bound by HBM, three quarters and more of it writes (8 x 8,100 tokens of 8 heads of 128 from 4 bits: 62 us, 5.5 TB/s).
 constexpr int READ_THREADS = 256;
 template <typename T> struct IsHalf { static constexpr bool value = false; };
 template <> struct IsHalf<__half> { static constexpr bool value = true; };
@@ -477,13 +482,8 @@ __global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const ReadPara
     if constexpr (ENTRIES) {
         const int e = p.first_entry + i / p.table_width, slot = i % p.table_width;
         const int2 seen = seen_keys(p, e);
-        const bool needed = (long long)slot * p.pages.page_size < seen.y && (long long)(slot + 1) * p.pages.page_size > seen.x, used = needed && page >= 0;
-        if (blockIdx.x == 0 && threadIdx.x == 0) {
-            p.table_out[(size_t)e * p.table_width + slot] = used ? i : -1;
-            // (a page that a token sees and that is not mapped, and a table that ends before the last token: the prompt kernel
-            // takes both for zeros without a word)
-            if ((needed && !used) || (slot == 0 && seen.y > (long long)p.table_width * p.pages.page_size)) atomicExch(p.status, 3);
-        }
+        const bool used = page >= 0 && (long long)slot * p.pages.page_size < seen.y && (long long)(slot + 1) * p.pages.page_size > seen.x;
+        if (blockIdx.x == 0 && threadIdx.x == 0) p.table_out[(size_t)e * p.table_width + slot] = used ? i : -1;
         if (!used) return;
         from = max(0, seen.x - slot * p.pages.page_size);
         to = min(p.pages.page_size, seen.y - slot * p.pages.page_size);
