@@ -717,7 +717,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
             }
             if (whole) {
 #pragma unroll
-                for (int w = 0; w < WARPS; ++w) part_f[w][col] = sum > 0.f ? part_f[w][col] / sum : 0.f;
+                for (int w = 0; w < WARPS; ++w) part_f[w][col] = sum == 0.f ? 0.f : part_f[w][col] / sum;
             } else if (col < live) {
                 *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * COLS + col) * 2) = make_float2(mx, sum);
             }
@@ -747,7 +747,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm<D, BITS, NT>()) attn_quan
 }
 
 // One warp adds the parts first, first + step, .. of a column: D / 32 values a lane and the weights' sum, both of the parts' largest
-// maximum `mx`.  `index` gives the place of a part.  (A batch of parts is on its way at once.  One token behind 60,000 keys, 2 rows of 222
+// maximum `mx`.  A sum of 0 is a row that sees nothing, and gives zeros; one that is no number stays that.  `index` gives the place of a part.  (A batch of parts is on its way at once.  One token behind 60,000 keys, 2 rows of 222
 // parts: 11.6 us in all; with a scan of all maxima before them 14.4.)
 template <int D, typename Index>
 __device__ __forceinline__ void add_parts(const Params& p, int first, int step, int parts, Index index, float (&acc)[D / 32], float& sum, float& mx) {
@@ -816,7 +816,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_quant_join_kernel(const 
         add_parts<D>(p, 0, 1, parts, index, acc, sum, mx);
         bf16* out = result_of<D>(p, e, row.y, (row.z >> 1) + col);
 #pragma unroll
-        for (int k = 0; k < D / 32; ++k) out[k * 32 + lane] = __float2bfloat16_rn(sum > 0.f ? acc[k] / sum : 0.f);
+        for (int k = 0; k < D / 32; ++k) out[k * 32 + lane] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc[k] / sum);
     }
 }
 
@@ -866,7 +866,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) attn_quant_merge_kernel(cons
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < MERGE_WARPS; ++w) v = fmaf(sh_o[w][d], f[w], v);
-        out[d] = __float2bfloat16_rn(sum > 0.f ? v / sum : 0.f);
+        out[d] = __float2bfloat16_rn(sum == 0.f ? 0.f : v / sum);
     }
 }
 

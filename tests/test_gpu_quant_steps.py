@@ -44,3 +44,25 @@ def test_lengths_far_behind_the_table(impl, window, length):
             if e != entry:
                 check(got[at:], q[at:], meta, table[e:], k, v, layout[e:e + 1], nkv, page, window, D ** -0.5, lambda e: False)
             at += n
+
+
+@pytest.mark.parametrize("impl,bad", [("direct", float("nan")), ("direct", float("inf")), ("direct", -float("inf")), ("portion", float("nan")),
+                                      (None, float("nan"))])
+@pytest.mark.parametrize("layout", [[(40, 1), (3000, 1)], [(300, 1)] * 90 + [(40, 2), (900, 1)], [(0, 70), (9000, 1), (400, 130), (5000, 3)]])
+def test_queries_that_are_no_numbers(impl, bad, layout):
+    """Their results are no numbers either, in however many parts their keys are; the other queries have their results.  (The prompt kernel
+    takes an infinite query as it is: a row whose keys all have the other sign there scores -inf everywhere, as one that sees nothing.
+    The kernel of CUDA cores behind "read" leaves out scores that are no numbers, here as over the plain cache.)"""
+    nq, nkv, D, page = 32, 8, 128, 16
+    meta, table, n_pages = step(layout, page, 3)
+    if impl == "portion" and meta.n_prefill_items128 == 0:
+        return
+    pages, k, v = random_pages(n_pages, nkv, page, D, 4, 3)
+    q = queries(meta, nq, D, 3)
+    clean, _ = attend(pages, meta, q, nq, D ** -0.5, impl=impl)
+    hit = torch.zeros(meta.tokens, nq, dtype=torch.bool, device=DEV)
+    hit[::3, 5] = hit[-1, 31] = hit[0, 0] = True
+    q[:, :, 7] = torch.where(hit, torch.tensor(bad, dtype=BF16, device=DEV), q[:, :, 7])
+    got, st = attend(pages, meta, q, nq, D ** -0.5, impl=impl)
+    assert st.tolist() == [0] * 4
+    assert torch.equal(got[~hit], clean[~hit]) and torch.isnan(got[hit]).all()
