@@ -262,8 +262,9 @@ def attention_quantized(out: torch.Tensor, q: torch.Tensor, pages: QuantizedPage
     than one token, ``prefill_work128`` int32 [tiles, (entry, first token)] in any order, and ``n_prefill_items128``; a step without
     that list, or with one of another length, stays on the codes).  bfloat16 with heads of 64, 128 or 256 runs on the codes themselves; long
     portions of prompts, other heads and float32 on pages that are read back.  A page that is not mapped, or past the pool, sets
-    status word 0 to 3.  On the codes a result is off by up to 2^-64 a key beside its roundings (values of 2^-40 and less feel it), and
-    queries of 2^80 and more count as infinite.  ``impl`` forces a form:
+    status word 0 to 3.  On the codes a weight is rounded to bfloat16 with its value's scale, in portions to float16, and the result
+    to bfloat16; beside that a result is off by up to 2^-64 a key on the codes (values of 2^-40 and less feel it), and queries of 2^80 and
+    more count as infinite there.  ``impl`` forces a form:
     "direct" or "read" for the whole step, "portion" (long portions') for every entry of more than one token."""
     what, D, n_kv, q_lens, tokens = "attention_quantized", pages.head_dim, pages.n_kv, meta.q_lens, meta.tokens
     window = int(window or 0)
