@@ -19,7 +19,7 @@
 //
 // A weight is rounded once, to bfloat16 with its value's scale, as the tensor cores take it: it comes there as two bfloat16 words, its upper
 // 16 bits and the upper 16 of what they leave, 2^-14 of it at most going lost, and one fused multiply-add rounds the sum of both products.  The
-// normaliser sums the weights themselves.  (Rounded by itself first too, a word less: 3 to 5 % faster at 4 bits, 1 at 8; 8 tokens behind 8,100 keys at 4 bits
+// normaliser sums the weights themselves.  (Rounded by itself first too, a word less: 2 to 3 % faster at 4 bits, level at 8; 8 tokens behind 8,100 keys at 4 bits
 // then were off by 0.31 % of the result's norm, now 0.21, 0.16 of it the rounding of the result.)
 //
 // Products are made the other way round from the kernels of attention_mma.cu, keys (then channels) as
@@ -33,10 +33,10 @@
 // second's in the other, zeros elsewhere: a word is used as it is, both groups' sums come out of one product, and the accumulators
 // are half as many.
 //
-// What bounds it: at 4 bits a warp executes some 500 instructions for 32 keys of 128 channels, 230 of them on the integer
-// pipe (which takes a warp's in two cycles), and a lone warp needs over 2,000 cycles for them; with three warps a scheduler issue is
-// half busy and the integer pipe too, and keys and values come at some 5 TB/s (8 tokens behind 8,100 keys, 32 query and 8 key
-// heads: 23.2 us with the joining of the parts, 75 MB).  At 8 bits it is the memory, 6.0 TB/s (64 tokens behind 2,048: 57.4 us, 287 MB).
+// What bounds it: at 4 bits a warp executes some 600 instructions for 32 keys of 128 channels (what surrounds its steps counted in), and a
+// lone warp needs over 2,000 cycles for them; with three warps a scheduler issue is half busy and the integer pipe 45 % of the time.  8 tokens
+// behind 8,100 to 64,800 keys (32 query and 8 key heads) lie on a line of 8 us, the way in and out and the joining of the parts, and 5.3 TB/s: 23.0 us
+// and 75 MB behind 8,100.  At 8 bits it is the memory (64 tokens behind 2,048: 55 us, 287 MB).
 // Each warp works on its own 32 keys of a step of 128 with its own maximum, fetches its own rows, and meets the other three
 // warps only at the end of a piece.  A maximum is raised only when a score passes it by 2^8.
 //
@@ -206,9 +206,9 @@ template <int D, int BITS> struct Shape {
     static constexpr int CHUNKS = RB / 16;
     static constexpr int K_BYTES = RB / 4, V_BYTES = RB / 8; // a lane's stretch of a key's row and of a value's
     static constexpr int WARP_STAGE = WARP_KEYS * 2 * (RB + SB);
-    // Steps in the ring, and CTAs an SM (ctas_per_sm).  Heads of 128: three CTAs of 168 registers a thread and four steps (4 bits,
-    // 8 tokens of 8,100 keys in 8 columns 26.1 us, in 4 23.2; four CTAs of 128 registers and three steps 28.5 and 23.5).  A step's scores made beside the one before's
-    // values, two streams of instructions, gave nothing (26.1).
+    // Steps in the ring, and CTAs an SM (ctas_per_sm).  Heads of 128: three CTAs of 168 registers a thread and four steps (at 4 bits four CTAs
+    // of 128 registers and three steps took 9 % longer in 8 columns, 1 % in 4).  A step's scores made beside the one before's values, two
+    // streams of instructions, gave nothing.
     static constexpr int STAGES = RB == 128 && D == 128 ? 2 : D == 256 ? 3 : 4;
     static constexpr float L = BITS == 4 ? 8.f : 128.f;
 };
@@ -834,8 +834,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_quant_join_kernel(const 
 }
 
 // The same where there are no more rows than CTAs: a block a row and column, MERGE_WARPS warps that share the parts.  What a block
-// is to do it finds from the step's lists before the wait.  (Eight tokens of 8,100 keys, 64 rows of some 7 parts: 25.5 us in all,
-// 26.5 with the kernel above; 64 of 2,048, 512 rows on 444 CTAs: 46.7 and 44.9.)
+// is to do it finds from the step's lists before the wait.  (Eight tokens of 8,100 keys, 64 rows of some 7 parts: 1 us less than
+// with the kernel above; 64 of 2,048, 512 rows on 444 CTAs: 1.8 us more.)
 template <int D, int NT, int MERGE_WARPS>
 __global__ void __launch_bounds__(MERGE_WARPS * 32) attn_quant_merge_kernel(const Params p) {
     constexpr int COLS = columns_of_tiles(NT);
@@ -924,8 +924,8 @@ template <int D, int BITS, int NT, bool TILES> int launch(Params p, long long st
     return kipp_launch(attn_quant_merge_kernel<D, NT, 4>, grid, dim3(128), 0, s, 1, p);
 }
 
-// 4 columns where they hold every query of a kv head in 4 bits (8 tokens behind 8,100 keys, 4 queries each: 23.2 us, with 8 columns 24.9, with
-// 16 31.7), 8 where those do, else 16 (12
+// 4 columns where they hold every query of a kv head in 4 bits (8 tokens behind 8,100 keys, 4 queries each: 23.0 us, with 8 columns 25.0, with
+// 16 32.7), 8 where those do, else 16 (12
 // queries: 35.5 us, 42.3 with 8); heads of 256 have no room for their sums: always 8
 int columns_of(int bits, int head_dim, long long queries) { return bits == 4 && queries <= 4 ? 4 : head_dim == 256 || queries <= 8 ? 8 : 16; }
 // The kernel of these heads and columns.

@@ -133,8 +133,9 @@ template <int BITS> __device__ __forceinline__ void put_codes(uint8_t* p, uint32
 // four runs of two groups; the four lanes whose numbers agree modulo HEAD_DIM / 64 hold the same two groups, so a
 // group's extremes are two exchanges away.  The 64-bit sum of squares (16 conversions a lane on a pipe of 16 lanes) is
 // formed for keys only: queries get no codes, and four in five heads are theirs.
-// Bound by its instructions (some 220 a warp and four query heads, three times as many where there are codes to make) and their
-// latencies, at 20 to 24 warps an SM, not by memory: 2,048 tokens of 32 and 2 x 8 bfloat16 heads of 128 to 8 bits take 17.4 us
+// Bound by its instructions (some 220 a warp and four query heads, three times as many where there are codes to make), at an issue rate of a
+// half, and by what its 19 warps an SM wait for between them, their rows first (long scoreboard 2.6 of 9 warps an issue), fixed latencies next
+// (1.6), not by memory's rate: 2,048 tokens of 32 and 2 x 8 bfloat16 heads of 128 to 8 bits take 17.4 us
 // (46 MB, 2.7 TB/s), 2,513 of 12 and 2 x 2 float32 heads of 64 to 4 bits 8.0 us (18 MB, 2.3 TB/s), eight tokens 2.6 us.  A block is no
 // larger than a token's heads need (those float32 heads: 15.8 us with 128 threads of which half are idle, 11.0 with 64); blocks of
 // 64, 192 and 384 threads were slower than 128, 8 blocks an SM of 64 registers a thread no faster than 6 of 80.
