@@ -113,6 +113,8 @@ def qk_norm_rope_write_quantized(qkv: torch.Tensor, q_out: torch.Tensor, pages: 
     ld, one = qkv.stride()
     if one != 1:
         raise KernelError(f"{what}: qkv's rows must be contiguous")
+    if shape[0] == 1:             # (the stride of a lone row says nothing)
+        ld = shape[1]
     if q_out.dtype != dtype or not q_out.is_contiguous() or q_out.numel() < tokens * n_q * D:
         raise KernelError(f"{what}: q_out must be contiguous, of qkv's dtype and hold every query")
     _lists(what, "positions, entry_of_token and block_table", positions, entry_of_token, block_table)

@@ -66,3 +66,22 @@ def test_queries_that_are_no_numbers(impl, bad, layout):
     got, st = attend(pages, meta, q, nq, D ** -0.5, impl=impl)
     assert st.tolist() == [0] * 4
     assert torch.equal(got[~hit], clean[~hit]) and torch.isnan(got[hit]).all()
+
+
+@pytest.mark.parametrize("D", [128, 96])
+def test_a_lone_row_of_any_stride(D):
+    """One token's projection as a transposed column, whose first stride is 1: what the same row gives as it is."""
+    nq, nkv, page = 4, 2, 16
+    meta, table, n_pages = step([(20, 1)], page, 1)
+    column = torch.randn((nq + 2 * nkv) * D, 1, generator=torch.Generator().manual_seed(1)).to(BF16).to(DEV)
+    row = column.t()
+    assert row.shape[0] == 1 and row.stride() == (1, 1)
+    results = []
+    for qkv in (row, column.flatten()[None].contiguous()):
+        pages, st = K.QuantizedPages.zeros(n_pages, nkv, page, D, 8, DEV), status()
+        q = torch.zeros(1, nq, D, dtype=BF16, device=DEV)
+        K.qk_norm_rope_write_quantized(qkv, q, pages, None, None, 1e-6, None, 0, meta.positions, meta.entry_of_token, meta.block_tables[0], 1, nq,
+                                       True, st)
+        assert st.tolist() == [0] * 4 and bool(pages.k_codes.any())
+        results.append((q, pages.k_codes, pages.k_scales, pages.v_codes, pages.v_scales))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
