@@ -18,7 +18,8 @@ READ_BYTES = 1 << 30          # most bytes of keys and values that attention rea
 
 class QuantizedPages:
     """One run's cache: codes uint8 ``[pages, n_kv, page_size, D * bits / 8]`` and scales bfloat16
-    ``[pages, n_kv, page_size, D / 32]`` of keys and of values.  D is a multiple of 32, at most 512."""
+    ``[pages, n_kv, page_size, D / 32]`` of keys and of values.  D is a multiple of 32, at most 512.  Launches go by the addresses
+    that the tensors have when the object is made: they may be written to, but not exchanged, moved or resized."""
 
     def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor, bits: int):
         if bits != 4 and bits != 8:
